@@ -526,6 +526,67 @@ int pccnn_conv_backward_bf16(const pccnn_basis *basis, const float *pts, const f
                              float *d_param_b, float *d_pdf, float *d_pts, float *d_samples,
                              void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- attention between levels --------------------------------------------
+ * Three operators with no counterpart in the reference, which moves features between levels with local convolutions only:
+ * layer norm of features, rotary positions over the point coordinates, and softmax attention of the points of one level
+ * to those of another.  Features are f32 or bf16 (bit patterns), `type` one of PCCNN_TYPE_*; everything is computed in
+ * f32 and a bf16 result is rounded once.  Strides are in elements and not negative; features of a row (of a head) lie
+ * one behind the other; results are dense. */
+#define PCCNN_TYPE_F32 0
+#define PCCNN_TYPE_BF16 1
+
+/* out[n,channels] = (x - mean) rstd gamma + beta per row of feats, mean and variance over the row's channels,
+ * rstd = 1 / sqrt(variance + eps).  gamma, beta [channels] of weight_type.  stats_out (nullable) f32[n,2] = (mean, rstd),
+ * which the backward call takes.  Backward: d_feats (nullable) [n,channels]; d_gamma, d_beta (both or neither)
+ * [channels] of weight_type, summed in a fixed order; the workspace is only needed for these two. */
+size_t pccnn_layer_norm_workspace_bytes(int64_t n, int64_t channels);
+int pccnn_layer_norm_forward(const void *feats, int type, int64_t row_stride, const void *gamma, const void *beta,
+                             int weight_type, float eps, int64_t n, int64_t channels, void *out, float *stats_out,
+                             void *stream);
+int pccnn_layer_norm_backward(const void *feats, int type, int64_t row_stride, const void *gamma, int weight_type,
+                              const float *stats, const void *in_grads, int64_t grads_stride, int64_t n,
+                              int64_t channels, void *d_feats, void *d_gamma, void *d_beta, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* Rotary positions: out[n,heads,width]; pair p of a head's features (p and p + pairs, or 2p and 2p + 1 with `adjacent`)
+ * turned by pts[n, axes[p]] * freqs[p] (by its negative with `backwards`, which is the gradient); features from 2 * pairs
+ * on are copied.  pts f32[n,num_axes] (1 to 6 axes), freqs f32[pairs], axes i32[pairs] in [0,num_axes); pairs <= 4096.
+ * pccnn_rotary_points_backward: d_pts f32[n,num_axes] from the features that were turned and the gradient of the result. */
+int pccnn_rotary(const void *feats, int type, int64_t stride_n, int64_t stride_h, const float *pts, const float *freqs,
+                 const int32_t *axes, int64_t n, int heads, int width, int pairs, int num_axes, int adjacent,
+                 int backwards, void *out, void *stream);
+int pccnn_rotary_points_backward(const void *feats, int type, int64_t stride_n, int64_t stride_h, const float *pts,
+                                 const float *freqs, const int32_t *axes, const void *in_grads, int64_t grads_stride_n,
+                                 int64_t grads_stride_h, int64_t n, int heads, int width, int pairs, int num_axes,
+                                 int adjacent, float *d_pts, void *stream);
+
+/* Softmax attention, cloud by cloud.  queries [m,heads,width], keys and values [n,key_heads,width] (width <= 128, heads
+ * a multiple of key_heads: query head h reads key head h / (heads / key_heads)).  Cloud c has the queries
+ * query_starts[c] .. query_starts[c+1] and the keys key_starts[c] .. key_starts[c+1]: i32[clouds+1], ascending, from 0 to
+ * m and n, either side of any length, zero included; max_queries / max_keys are the largest of these lengths (rows past
+ * them are not computed).  key_mask (nullable) u8[n]: a zero switches the key off for all queries; what its rows hold
+ * (infinities and NaN included) then has no effect, and its gradients are zero.  A query without any key gets zeros and
+ * lse -inf.  scale: positive, finite.
+ * forward: out [m,heads,width]; lse_out (nullable) f32[m,heads] = log of the sum of exp(scale q.k), for the backward call.
+ * backward: d_queries (nullable) [m,heads,width], d_keys and d_values (both or neither) [n,key_heads,width]; results do
+ * not depend on the order of anything (no atomics).  f32 products keep f32 accuracy; infinities in f32 features that are
+ * not switched off give NaN. */
+typedef struct pccnn_attention {
+    const void *queries, *keys, *values;
+    int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+    const int32_t *query_starts, *key_starts;
+    const uint8_t *key_mask;
+    int64_t m, n, max_queries, max_keys;
+    int type, clouds, heads, key_heads, width;
+    float scale;
+} pccnn_attention;
+size_t pccnn_attention_workspace_bytes(const pccnn_attention *problem, int backward);
+int pccnn_attention_forward(const pccnn_attention *problem, void *out, float *lse_out, void *workspace,
+                            size_t workspace_bytes, void *stream);
+int pccnn_attention_backward(const pccnn_attention *problem, const void *out, const float *lse, const void *in_grads,
+                             int64_t grads_stride_n, int64_t grads_stride_h, void *d_queries, void *d_keys,
+                             void *d_values, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- per-kernel timing ---------------------------------------------------
  * Measurement hooks with no counterpart in the reference (it has no profiler hooks).  While
  * enabled, the entry points above bracket their main kernels with HIP events on the launch

@@ -26,6 +26,17 @@ class Basis(ctypes.Structure):
 
 BP = ctypes.POINTER(Basis)
 
+class Attention(ctypes.Structure):
+    """struct pccnn_attention of include/pccnn_hip.h."""
+    _fields_ = [("queries", P), ("keys", P), ("values", P), ("q_stride_n", I64), ("q_stride_h", I64),
+                ("k_stride_n", I64), ("k_stride_h", I64), ("v_stride_n", I64), ("v_stride_h", I64),
+                ("query_starts", P), ("key_starts", P), ("key_mask", P), ("m", I64), ("n", I64), ("max_queries", I64),
+                ("max_keys", I64), ("type", ctypes.c_int), ("clouds", ctypes.c_int), ("heads", ctypes.c_int),
+                ("key_heads", ctypes.c_int), ("width", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+AP = ctypes.POINTER(Attention)
+
 # name -> (restype, argtypes); mirrors include/pccnn_hip.h declaration by declaration.
 SIGNATURES = {
     "pccnn_last_error": (ctypes.c_char_p, []),
@@ -91,6 +102,14 @@ SIGNATURES = {
     "pccnn_linear_basis_forward": (I32, [P, P, P, P, P, P, I64, I64, I64, I32, I32, P, P]),
     "pccnn_linear_basis_workspace_bytes": (SZ, [I64]),
     "pccnn_linear_basis_backward": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I32, I32, P, P, P, P, P, SZ, P]),
+    "pccnn_layer_norm_workspace_bytes": (SZ, [I64, I64]),
+    "pccnn_layer_norm_forward": (I32, [P, I32, I64, P, P, I32, F32, I64, I64, P, P, P]),
+    "pccnn_layer_norm_backward": (I32, [P, I32, I64, P, I32, P, P, I64, I64, I64, P, P, P, P, SZ, P]),
+    "pccnn_rotary": (I32, [P, I32, I64, I64, P, P, P, I64, I32, I32, I32, I32, I32, I32, P, P]),
+    "pccnn_rotary_points_backward": (I32, [P, I32, I64, I64, P, P, P, P, I64, I64, I64, I32, I32, I32, I32, I32, P, P]),
+    "pccnn_attention_workspace_bytes": (SZ, [AP, I32]),
+    "pccnn_attention_forward": (I32, [AP, P, P, P, SZ, P]),
+    "pccnn_attention_backward": (I32, [AP, P, P, P, I64, I64, P, P, P, P, SZ, P]),
     "pccnn_timing_enable": (I32, [I32]),
     "pccnn_timing_reset": (I32, []),
     "pccnn_timing_count": (I32, []),

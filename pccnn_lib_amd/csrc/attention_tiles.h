@@ -1,0 +1,167 @@
+// Tiles of the attention kernels: 32 x 32 products on v_mfma_f32_32x32x16_bf16, operands in LDS or registers.
+//
+// A product C = A B has C's column in the lane (lane & 31) and C's rows 8 (i / 4) + 4 (lane / 32) + i % 4 in its sixteen
+// registers i.  A lane's operand of A is eight consecutive k of one row (row = lane & 31, k from 8 (lane / 32)), of B
+// eight consecutive k of one column.  Registers 8 g .. 8 g + 7 of C are then, per lane half, the rows
+// 16 g + 4 half + {0..3} and 16 g + 8 + 4 half + {0..3}: taken as they are they serve as a B operand of a following product
+// over C's rows, if the A operand takes its k in the same order.  The transposing LDS read fetches exactly that order from
+// a tile stored row by row, so neither the probabilities nor the tiles are ever moved between lanes.
+//
+// f32 features are carried as three bf16 terms each (x = x0 + x1 + x2 holds all 24 bits) and a product as the six
+// partial products whose terms' indices add up to at most 2; what is left out is below one f32 rounding.
+#pragma once
+#include "elements.h"
+
+#ifdef __HIPCC__
+typedef short pccnn_i16x4 __attribute__((ext_vector_type(4)));
+typedef short pccnn_i16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct AttnTerms { static constexpr int value = 3; };
+template <> struct AttnTerms<uint16_t> { static constexpr int value = 1; };
+
+// One operand: eight values, as one or three bf16 terms.
+template <int TERMS> struct AttnFrag {
+    pccnn_bf16x8 t[TERMS];
+};
+
+template <int TERMS> __device__ __forceinline__ void attn_mma(pccnn_f32x16 &c, const AttnFrag<TERMS> &a,
+                                                             const AttnFrag<TERMS> &b)
+{
+    if constexpr (TERMS == 3) {                         // smallest products first
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[2], b.t[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], c, 0, 0, 0);
+    }
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], c, 0, 0, 0);
+}
+
+// Eight f32 values as terms, each rounded to nearest even from what the terms before it leave.
+template <int TERMS> __device__ __forceinline__ AttnFrag<TERMS> attn_split(const float (&x)[8])
+{
+    AttnFrag<TERMS> f;
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+        pccnn_u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = pccnn_bf16_pair(rest[2 * i], rest[2 * i + 1]);
+            if (t + 1 < TERMS) {
+                rest[2 * i] -= __uint_as_float(w[i] << 16);
+                rest[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+        f.t[t] = __builtin_bit_cast(pccnn_bf16x8, w);
+    }
+    return f;
+}
+
+// Eight consecutive features of one row, as they lie in memory.
+template <typename T> struct AttnChunk;
+template <> struct AttnChunk<uint16_t> { pccnn_u32x4 v; };
+template <> struct AttnChunk<float> { float v[8]; };
+
+__device__ __forceinline__ void attn_clear(AttnChunk<uint16_t> &c) { c.v = (pccnn_u32x4){0u, 0u, 0u, 0u}; }
+__device__ __forceinline__ void attn_clear(AttnChunk<float> &c)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c.v[i] = 0.0f;
+}
+
+// Features col .. col + 7 of a row of `width`, zeros past its end.  `wide`: 2 when width is a multiple of 8 and every row
+// starts at a multiple of 16 bytes, 1 when width is a multiple of 4 and rows start at multiples of four elements, else 0.
+__device__ __forceinline__ void attn_load(AttnChunk<uint16_t> &c, const uint16_t *row, int col, int width, int wide)
+{
+    attn_clear(c);
+    if (col >= width) return;
+    if (wide == 2) {
+        c.v = *(const pccnn_u32x4 *)(row + col);
+    } else if (wide == 1) {
+        const pccnn_u32x2 lo = *(const pccnn_u32x2 *)(row + col);
+        c.v[0] = lo[0]; c.v[1] = lo[1];
+        if (col + 4 < width) {
+            const pccnn_u32x2 hi = *(const pccnn_u32x2 *)(row + col + 4);
+            c.v[2] = hi[0]; c.v[3] = hi[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < width) c.v[i / 2] |= (uint32_t)row[col + i] << (16 * (i % 2));
+    }
+}
+__device__ __forceinline__ void attn_load(AttnChunk<float> &c, const float *row, int col, int width, int wide)
+{
+    attn_clear(c);
+    if (col >= width) return;
+    if (wide >= 1) {
+        const float4 lo = *(const float4 *)(row + col);
+        c.v[0] = lo.x; c.v[1] = lo.y; c.v[2] = lo.z; c.v[3] = lo.w;
+        if (col + 4 < width) {
+            const float4 hi = *(const float4 *)(row + col + 4);
+            c.v[4] = hi.x; c.v[5] = hi.y; c.v[6] = hi.z; c.v[7] = hi.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < width) c.v[i] = row[col + i];
+    }
+}
+__device__ __forceinline__ AttnFrag<1> attn_frag(const AttnChunk<uint16_t> &c)
+{
+    AttnFrag<1> f;
+    f.t[0] = __builtin_bit_cast(pccnn_bf16x8, c.v);
+    return f;
+}
+__device__ __forceinline__ AttnFrag<3> attn_frag(const AttnChunk<float> &c) { return attn_split<3>(c.v); }
+
+// A tile of ROWS rows in LDS, bf16, one plane per term; a row is DP features and 16 bytes of padding.
+template <int TERMS, int ROWS, int DP> struct AttnTile {
+    static constexpr int STRIDE = DP + 8;
+    static constexpr int PLANE = ROWS * STRIDE;                       // elements
+    static constexpr int BYTES = TERMS * PLANE * 2;
+    uint16_t *base;
+    __device__ __forceinline__ void put(int row, int col, const AttnFrag<TERMS> &f) const
+    {
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+            *(pccnn_u32x4 *)(base + t * PLANE + row * STRIDE + col) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
+    }
+    // Operand with the tile's rows as C's rows: eight features from `col` of row `row`.
+    __device__ __forceinline__ AttnFrag<TERMS> rows(int row, int col) const
+    {
+        AttnFrag<TERMS> f;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+            f.t[t] = __builtin_bit_cast(pccnn_bf16x8, *(const pccnn_u32x4 *)(base + t * PLANE + row * STRIDE + col));
+        return f;
+    }
+    // Operand with the tile's features as C's rows (feature col + (lane & 31)) and as k the sixteen tile rows from `row`,
+    // in the order of C's registers: row + 4 half + {0..3}, row + 8 + 4 half + {0..3}.  The read exchanges a 4 x 16 block
+    // among sixteen lanes: lane i brings four features of row i / 4 and gets feature i of all four rows.
+    __device__ __forceinline__ AttnFrag<TERMS> columns(int row, int col, int lane) const
+    {
+        const int r = row + 4 * (lane >> 5) + ((lane & 15) >> 2), c = col + (lane & 16) + 4 * (lane & 3);
+        AttnFrag<TERMS> f;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            uint16_t *p = base + t * PLANE + r * STRIDE + c;
+            typedef __attribute__((address_space(3))) pccnn_i16x4 *lds_ptr;
+            const pccnn_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+            const pccnn_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * STRIDE));
+            f.t[t] = __builtin_bit_cast(pccnn_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        return f;
+    }
+};
+
+// max(v, v of the lane 32 away)
+__device__ __forceinline__ float attn_max_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+#endif

@@ -1428,6 +1428,214 @@ def point_conv_weight_var(basis, feats, neigh, ends):
     return _generic_weight_var(name, desc, k, None, feats, None, neigh, ends, None, False)
 
 
+# ----------------------------------------------------------------------------- attention between levels
+#
+# Layer norm, rotary positions and attention: operators the reference does not have.  Features are float32 or bfloat16
+# (computed in fp32, rounded once); beside contiguous tensors they may be views whose last dimension is dense.
+
+_FEATURE_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+GRAD_QUERIES, GRAD_KEYS = 64, 128
+
+
+def _chk_features(t, name, ndim, dtype=None, device=None):
+    """A GPU tensor of float32 or bfloat16 (or exactly ``dtype``) with a dense last dimension and no negative strides."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError("%s: expected a torch.Tensor, got %s" % (name, type(t).__name__))
+    if not t.is_cuda:
+        raise RuntimeError("%s: expected a GPU tensor, got device %s" % (name, t.device))
+    if t.dtype not in _FEATURE_TYPES or (dtype is not None and t.dtype != dtype):
+        raise RuntimeError("%s: expected dtype %s, got %s" % (name, "torch.float32 or torch.bfloat16" if dtype is None
+                                                              else dtype, t.dtype))
+    if t.dim() != ndim:
+        raise RuntimeError("%s: expected %d dimensions, got shape %s" % (name, ndim, tuple(t.shape)))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError("%s: expected a dense last dimension, got strides %s" % (name, tuple(t.stride())))
+    if device is not None:
+        if t.device != device:
+            raise RuntimeError("%s: on %s but other arguments are on %s" % (name, t.device, device))
+    elif t.device.index != torch.cuda.current_device():
+        raise RuntimeError("%s: on %s, but the current device is cuda:%d; run the call under "
+                           "`with torch.cuda.device(tensor.device):`" % (name, t.device, torch.cuda.current_device()))
+    return t
+
+
+def _norm_args(name, feats, weights):
+    _chk_features(feats, name + ": features", 2)
+    for label, w in weights:
+        _chk_features(w, name + ": " + label, 1, weights[0][1].dtype if isinstance(weights[0][1], torch.Tensor) else None,
+                      feats.device)
+        if w.shape[0] != feats.shape[1]:
+            raise RuntimeError("%s: %s has %d values for %d channels" % (name, label, w.shape[0], feats.shape[1]))
+        if w.dtype not in (torch.float32, feats.dtype):
+            raise RuntimeError("%s: %s: expected float32 or the features' dtype, got %s" % (name, label, w.dtype))
+    if feats.shape[1] < 1:
+        raise RuntimeError(name + ": features without channels")
+
+
+def layer_norm(feats, gamma, beta, eps=1e-5, return_stats=False):
+    """Layer norm of every row: (x - mean) / sqrt(variance + eps) * gamma + beta over the row's channels.  feats [N, C]
+    float32 or bfloat16 (rows may be a view's); gamma, beta [C], float32 or of the features' dtype.  -> out [N, C], and
+    with ``return_stats`` also f32 [N, 2] = (mean, 1 / sqrt(variance + eps)), which ``layer_norm_grads`` takes."""
+    name = "layer_norm"
+    _norm_args(name, feats, (("gamma", gamma), ("beta", beta)))
+    n, c = feats.shape
+    out = torch.empty((n, c), dtype=feats.dtype, device=feats.device)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=feats.device) if return_stats else None
+    _lib.call("pccnn_layer_norm_forward", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), _ptr(gamma),
+              _ptr(beta), _FEATURE_TYPES[gamma.dtype], float(eps), n, c, _ptr(out), _optr(stats), _stream())
+    return (out, stats) if return_stats else out
+
+
+def layer_norm_grads(feats, gamma, stats, in_grads, grad_mask=GRAD_ALL):
+    """Gradients of ``layer_norm`` -> (d_feats [N, C], d_gamma [C], d_beta [C]), the last two in gamma's dtype and summed
+    over the rows in a fixed order; None for a group that ``grad_mask`` (GRAD_FEATS, GRAD_WEIGHTS) does not name."""
+    name = "layer_norm_grads"
+    _norm_args(name, feats, (("gamma", gamma),))
+    n, c = feats.shape
+    _chk(stats, name + ": stats", torch.float32, 2, feats.device)
+    _chk_features(in_grads, name + ": in_grads", 2, feats.dtype, feats.device)
+    if tuple(stats.shape) != (n, 2) or in_grads.shape != feats.shape:
+        raise RuntimeError(name + ": inconsistent shapes")
+    d_feats = torch.empty((n, c), dtype=feats.dtype, device=feats.device) if grad_mask & GRAD_FEATS else None
+    d_gamma = d_beta = ws = None
+    if grad_mask & GRAD_WEIGHTS:
+        d_gamma, d_beta = torch.empty_like(gamma), torch.empty_like(gamma)
+        ws = _workspace(_lib.load().pccnn_layer_norm_workspace_bytes(n, c), feats.device)
+    _lib.call("pccnn_layer_norm_backward", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), _ptr(gamma),
+              _FEATURE_TYPES[gamma.dtype], _ptr(stats), _ptr(in_grads), in_grads.stride(0), n, c, _optr(d_feats),
+              _optr(d_gamma), _optr(d_beta), _optr(ws), 0 if ws is None else ws.numel(), _stream())
+    return d_feats, d_gamma, d_beta
+
+
+def _rotary_args(name, feats, pts, freqs, axes):
+    _chk_features(feats, name + ": features", 3)
+    dev = feats.device
+    _chk(pts, name + ": pts", torch.float32, 2, dev)
+    _chk(freqs, name + ": freqs", torch.float32, 1, dev)
+    _chk(axes, name + ": axes", torch.int32, 1, dev)
+    n, heads, width = feats.shape
+    if pts.shape[0] != n or axes.shape[0] != freqs.shape[0] or 2 * freqs.shape[0] > width:
+        raise RuntimeError("%s: %d points for %d rows, %d frequencies and %d axes for heads of %d features"
+                           % (name, pts.shape[0], n, freqs.shape[0], axes.shape[0], width))
+    if not 1 <= pts.shape[1] <= MAX_DIMS:
+        raise RuntimeError("%s: %d-dimensional positions are not supported (1 to %d)" % (name, pts.shape[1], MAX_DIMS))
+    return (n, heads, width, freqs.shape[0], pts.shape[1])
+
+
+def _turned(feats, pts, freqs, axes, dims, adjacent, backwards):
+    out = torch.empty(feats.shape, dtype=feats.dtype, device=feats.device)
+    _lib.call("pccnn_rotary", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), feats.stride(1), _ptr(pts),
+              _ptr(freqs), _ptr(axes), *dims, 1 if adjacent else 0, 1 if backwards else 0, _ptr(out), _stream())
+    return out
+
+
+def rotary(feats, pts, freqs, axes, adjacent=False):
+    """Rotary positions over several axes: pair p of every head's features is turned by the angle
+    pts[n, axes[p]] * freqs[p].  feats [N, H, W] float32 or bfloat16, pts f32 [N, A] (A = 1 to 6), freqs f32 [P], axes
+    i32 [P] with values in [0, A), 2 P <= W.  Pair p is (p, p + P), with ``adjacent`` (2p, 2p + 1); features from 2 P on
+    are copied.  -> [N, H, W]."""
+    dims = _rotary_args("rotary", feats, pts, freqs, axes)
+    return _turned(feats, pts, freqs, axes, dims, adjacent, False)
+
+
+def rotary_grads(feats, pts, freqs, axes, in_grads, adjacent=False, grad_mask=GRAD_FEATS):
+    """Gradients of ``rotary`` -> (d_feats [N, H, W], d_pts f32 [N, A]); None for one that ``grad_mask`` (GRAD_FEATS,
+    GRAD_PTS) does not name."""
+    name = "rotary_grads"
+    dims = _rotary_args(name, feats, pts, freqs, axes)
+    _chk_features(in_grads, name + ": in_grads", 3, feats.dtype, feats.device)
+    if in_grads.shape != feats.shape:
+        raise RuntimeError(name + ": inconsistent shapes")
+    d_feats = _turned(in_grads, pts, freqs, axes, dims, adjacent, True) if grad_mask & GRAD_FEATS else None
+    d_pts = None
+    if grad_mask & GRAD_PTS:
+        d_pts = torch.empty_like(pts)
+        _lib.call("pccnn_rotary_points_backward", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0),
+                  feats.stride(1), _ptr(pts), _ptr(freqs), _ptr(axes), _ptr(in_grads), in_grads.stride(0),
+                  in_grads.stride(1), *dims, 1 if adjacent else 0, _ptr(d_pts), _stream())
+    return d_feats, d_pts
+
+
+def _attention_args(name, queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask, scale):
+    """The call's problem as the struct the library takes."""
+    _chk_features(queries, name + ": queries", 3)
+    dtype, dev = queries.dtype, queries.device
+    _chk_features(keys, name + ": keys", 3, dtype, dev)
+    _chk_features(values, name + ": values", 3, dtype, dev)
+    _chk(query_starts, name + ": query_starts", torch.int32, 1, dev)
+    _chk(key_starts, name + ": key_starts", torch.int32, 1, dev)
+    m, heads, width = queries.shape
+    n, key_heads = keys.shape[:2]
+    if keys.shape[2] != width or values.shape != keys.shape:
+        raise RuntimeError("%s: queries %s, keys %s, values %s: expected [M, H, W], [N, G, W], [N, G, W]"
+                           % (name, tuple(queries.shape), tuple(keys.shape), tuple(values.shape)))
+    if key_heads < 1 or heads < 1 or heads % key_heads != 0:
+        raise RuntimeError("%s: %d heads over %d key heads" % (name, heads, key_heads))
+    if query_starts.shape != key_starts.shape or query_starts.shape[0] < 1:
+        raise RuntimeError("%s: query_starts %s and key_starts %s: expected [clouds + 1] both"
+                           % (name, tuple(query_starts.shape), tuple(key_starts.shape)))
+    if key_mask is not None:
+        _chk(key_mask, name + ": key_mask", torch.bool, 1, dev)
+        if key_mask.shape[0] != n:
+            raise RuntimeError("%s: key_mask of %d values for %d keys" % (name, key_mask.shape[0], n))
+    p = _lib.Attention()
+    p.queries, p.keys, p.values = queries.data_ptr(), keys.data_ptr(), values.data_ptr()
+    p.q_stride_n, p.q_stride_h = queries.stride(0), queries.stride(1)
+    p.k_stride_n, p.k_stride_h = keys.stride(0), keys.stride(1)
+    p.v_stride_n, p.v_stride_h = values.stride(0), values.stride(1)
+    p.query_starts, p.key_starts = query_starts.data_ptr(), key_starts.data_ptr()
+    p.key_mask = None if key_mask is None else key_mask.data_ptr()
+    p.m, p.n, p.max_queries, p.max_keys = m, n, int(max_queries), int(max_keys)
+    p.type, p.clouds, p.heads, p.key_heads, p.width = (_FEATURE_TYPES[dtype], query_starts.shape[0] - 1, heads,
+                                                       key_heads, width)
+    p.scale = width ** -0.5 if scale is None else float(scale)
+    return p
+
+
+def cross_attention(queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask=None, scale=None,
+                    return_lse=False):
+    """Softmax attention of every cloud's queries to the same cloud's keys.  queries [M, H, W], keys and values [N, G, W]
+    (float32 or bfloat16, W <= 128; H a multiple of G: query head h reads key head h // (H // G)).  The clouds lie one
+    behind the other: query_starts, key_starts i32 [clouds + 1] from 0 to M and N; max_queries, max_keys: the largest
+    number of a cloud's queries and keys (rows past them are not computed).  ``key_mask`` bool [N]: False switches a key
+    off, whatever its features hold; ``scale`` (positive; default W ** -0.5) multiplies the scores.  -> out [M, H, W] (zeros
+    for a query without any key), and with ``return_lse`` also f32 [M, H], the log of the sum of the exponentials, which
+    ``cross_attention_grads`` takes.  Few queries over many keys (one token per cloud) are split over the keys and joined."""
+    p = _attention_args("cross_attention", queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask,
+                        scale)
+    dev = queries.device
+    out = torch.empty(queries.shape, dtype=queries.dtype, device=dev)
+    lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    ws = _workspace(_lib.load().pccnn_attention_workspace_bytes(ctypes.byref(p), 0), dev)
+    _lib.call("pccnn_attention_forward", ctypes.byref(p), _ptr(out), _optr(lse), _ptr(ws), ws.numel(), _stream())
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_grads(queries, keys, values, query_starts, key_starts, max_queries, max_keys, out, lse, in_grads,
+                          key_mask=None, scale=None, grad_mask=GRAD_QUERIES | GRAD_KEYS):
+    """Gradients of ``cross_attention`` from its result and ``lse`` -> (d_queries [M, H, W], d_keys [N, G, W],
+    d_values [N, G, W]); None for a group that ``grad_mask`` (GRAD_QUERIES; GRAD_KEYS: keys and values) does not name.  No
+    float atomics: the same bits from run to run."""
+    name = "cross_attention_grads"
+    p = _attention_args(name, queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask, scale)
+    dev = queries.device
+    _chk(out, name + ": out", queries.dtype, 3, dev)
+    _chk(lse, name + ": lse", torch.float32, 2, dev)
+    _chk_features(in_grads, name + ": in_grads", 3, queries.dtype, dev)
+    if out.shape != queries.shape or in_grads.shape != queries.shape or lse.shape != queries.shape[:2]:
+        raise RuntimeError(name + ": inconsistent shapes")
+    d_queries = d_keys = d_values = None
+    if grad_mask & GRAD_QUERIES:
+        d_queries = torch.empty(queries.shape, dtype=queries.dtype, device=dev)
+    if grad_mask & GRAD_KEYS:
+        d_keys = torch.empty(keys.shape, dtype=queries.dtype, device=dev)
+        d_values = torch.empty(keys.shape, dtype=queries.dtype, device=dev)
+    ws = _workspace(_lib.load().pccnn_attention_workspace_bytes(ctypes.byref(p), 1), dev)
+    _lib.call("pccnn_attention_backward", ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(in_grads), in_grads.stride(0),
+              in_grads.stride(1), _optr(d_queries), _optr(d_keys), _optr(d_values), _ptr(ws), ws.numel(), _stream())
+    return d_queries, d_keys, d_values
+
+
 REFERENCE_NAMES = (
     "build_grid_ds", "compute_keys", "find_neighbors", "compute_pdf", "compute_pdf_grads", "poisson_disk_sampling",
     "mc_conv", "mc_conv_grads", "mc_conv_weight_var", "point_conv_basis", "point_conv_basis_grads", "point_conv",
