@@ -20,6 +20,10 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument", "-Wno-ignored-optimization-argument",
 ]
 
+# Flags of single sources.  attention.hip: matrix results in ordinary registers, where the softmax works on them; the
+# compiler's own choice puts them into accumulation registers and moves every value out and in again.
+EXTRA_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
@@ -44,7 +48,7 @@ def build(verbose=True, jobs=8, incremental=False):
         batch = []
         for src in srcs[i:i + jobs]:
             obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
-            cmd = [hipcc] + HIPCC_FLAGS + ["-c", src, "-o", obj]
+            cmd = [hipcc] + HIPCC_FLAGS + EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             batch.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

@@ -22,22 +22,38 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
 constexpr int kOwn = 32 * kWaves;            // rows (forward, dq) or keys (dk, dv) of a workgroup
-constexpr int kTile = 64;                    // the other side's rows in LDS at a time
 constexpr int kMaxWidth = 128;
 constexpr float kLog2e = 1.44269504088896341f;
 
+// Rows of the other side that are in LDS at a time, twice (one tile is brought in while the other is worked on).  Three
+// terms of wide heads take half as many (64 or 128 features: 48 and 96 KiB of a CU's 160; 96 features do not divide evenly).
+template <typename T, int DP> constexpr int attn_tile_rows()
+{
+    return AttnTerms<T>::value == 3 && (DP == 64 || DP == 128) ? 32 : 64;
+}
+
+// The side that is walked: rows `n` elements apart, heads `h`.  Either as the caller has it (`wide`: attn_load), or - bf16
+// features whose rows are whole 16-byte units - as planes that go to LDS without passing through registers.
+struct AttnStream {
+    const void *p;
+    int64_t n, h, plane;
+    int wide, units;
+};
+
 struct AttnArgs {
-    const void *q, *k, *v, *g;               // queries, keys, values, gradient of the output
+    const void *q, *k, *v, *g;               // a workgroup's own side: queries, keys, values, gradient of the output
     int64_t q_n, q_h, k_n, k_h, v_n, v_h, g_n, g_h;
+    int wide_q, wide_k, wide_v, wide_g, wide_o;
+    AttnStream one, two;                     // the walked side: keys and values, or queries and output gradients
     const int32_t *q_starts, *k_starts;
     const uint8_t *mask;
     int64_t m, n;
     int clouds, heads, key_heads, group, width;
     float scale;
-    int wide_q, wide_k, wide_v, wide_g;
     int tiles, splits, per_split;            // own tiles per cloud and head; parts of the other side and tiles in each
     void *out;                               // forward: O; backward: dq
-    float *lse, *delta;                      // [m, heads]
+    float *lse;                              // [m, heads]
+    float *shift, *delta;                    // [key_heads][m * group]: a row's L in units of log 2 (+inf: no keys), and D
     void *d_k, *d_v;
     float *part, *part_v;                    // [split][rows or keys][heads][width] f32, when splits > 1
     float2 *part_ml;                         // [split][m][heads] (maximum in units of log 2, sum)
@@ -64,60 +80,105 @@ struct AttnBlock {
         rows = (int)min((q1 - q0) * a.group, (int64_t)INT32_MAX - 2 * kOwn);
         keys = (int)(k1 - k0);
     }
-    // Token (query * heads + head) of a row.
     __device__ __forceinline__ int64_t query(const AttnArgs &a, int row) const { return q0 + row / a.group; }
     __device__ __forceinline__ int head_of(const AttnArgs &a, int row) const { return head * a.group + row % a.group; }
+    // Where a row's shift and delta are.
+    __device__ __forceinline__ int64_t stat(const AttnArgs &a, int row) const
+    {
+        return head * (a.m * a.group) + q0 * a.group + row;
+    }
 };
 
-// Which of the 64 keys from `key` on take part: within the cloud and not switched off.
-__device__ __forceinline__ uint64_t live_keys(const AttnArgs &a, const AttnBlock &b, int key, int lane)
+// One bit per row of a tile: the first `count` of `rows`.
+__device__ __forceinline__ uint64_t first_bits(int count, int rows)
 {
-    const int mine = key + lane;
-    return __ballot(mine < b.keys && (a.mask == nullptr || a.mask[b.k0 + mine] != 0));
+    return count <= 0 ? 0 : count >= rows ? (rows == 64 ? ~0ull : (1ull << rows) - 1) : (1ull << count) - 1;
 }
 
-// The part of a 64-row tile (DP features each) that a thread carries from memory to LDS.
-template <typename T, int DP> struct Carrier {
+// Which of the `rows` keys from `key` on take part: within the cloud and not switched off.  `flag` holds the lane's mask
+// byte, loaded ahead of its use.
+__device__ __forceinline__ uint8_t key_flag(const AttnArgs &a, const AttnBlock &b, int key, int lane)
+{
+    if (a.mask == nullptr) return 1;
+    return key + lane < b.keys ? a.mask[b.k0 + key + lane] : 0;
+}
+__device__ __forceinline__ uint64_t live_keys(const AttnArgs &a, const AttnBlock &b, int key, uint8_t flag, int rows)
+{
+    const uint64_t all = first_bits(b.keys - key, rows);
+    return a.mask == nullptr ? all : all & __ballot(flag != 0);
+}
+
+// Brings tile after tile of a stream into LDS.  GROUPED: a stream row is a row of the problem (query * group + head in
+// group), else a key.
+template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
     static constexpr int TERMS = AttnTerms<T>::value;
-    static constexpr int PER_ROW = DP / 8;
-    static constexpr int COUNT = kTile * PER_ROW / kThreads;
-    AttnChunk<T> c[COUNT];
-    // rows from `row` on of `limit`, at base + (row of the tile) * stride
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int row, int limit, int width, int wide)
+    static constexpr int ROWS = attn_tile_rows<T, DP>();
+    typedef AttnTile<TERMS, ROWS, DP> Tile;
+    static constexpr int COUNT = ROWS * Tile::UNITS / kThreads;
+    static_assert(COUNT >= 1 && COUNT * kThreads == ROWS * Tile::UNITS, "every thread carries whole units");
+    const uint16_t *from[DIRECT ? COUNT : 1];
+    int64_t step;
+    AttnChunk<T> held[DIRECT ? 1 : COUNT];
+
+    static __device__ __forceinline__ int row_of(int j) { return (threadIdx.x + j * kThreads) / Tile::UNITS; }
+    static __device__ __forceinline__ int unit_of(int j) { return (threadIdx.x + j * kThreads) % Tile::UNITS; }
+    static __device__ __forceinline__ int64_t offset(const AttnStream &s, int group, int row)
     {
-#pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const int i = threadIdx.x + j * kThreads, r = row + i / PER_ROW, col = 8 * (i % PER_ROW);
-            if (r < limit)
-                attn_load(c[j], base + r * stride, col, width, wide);
-            else
-                attn_clear(c[j]);
+        if constexpr (GROUPED) {
+            const int query = group == 1 ? row : row / group;
+            return query * s.n + (row - query * group) * s.h;
+        } else {
+            return row * s.n;
         }
     }
-    // rows of the problem: row -> (query, head of the group)
-    __device__ __forceinline__ void load_rows(const T *base, int64_t stride_n, int64_t stride_h, int row, int limit,
-                                              int group, int width, int wide)
+    // `base`: the cloud's and head's first element
+    __device__ __forceinline__ void start(const AttnStream &s, int64_t base, int group, int row)
+    {
+        if constexpr (DIRECT) {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j)
+                from[j] = (const uint16_t *)s.p + base + offset(s, group, row + row_of(j)) +
+                          8 * Tile::unit_at(row_of(j), unit_of(j));
+            step = !GROUPED || group == 1 ? ROWS * s.n : ROWS / group * s.n;
+        }
+    }
+    // Starts bringing the tile of rows `row` .. into `tile` (DIRECT), or into registers.  Rows without a bit in `live`
+    // become zeros; `limit`: rows that exist.
+    __device__ __forceinline__ void fetch(const AttnStream &s, int64_t base, int group, int row, int limit, uint64_t live,
+                                          int width, const Tile &tile)
     {
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
-            const int i = threadIdx.x + j * kThreads, r = row + i / PER_ROW, col = 8 * (i % PER_ROW);
-            if (r < limit) {
-                const int query = group == 1 ? r : r / group;
-                attn_load(c[j], base + query * stride_n + (r - query * group) * stride_h, col, width, wide);
+            if constexpr (DIRECT) {
+                const int r = row_of(j), unit = Tile::unit_at(r, unit_of(j));
+                const bool mine = ((live >> r) & 1) && unit < s.units;
+                if constexpr (GROUPED) {
+                    if (group > 1 && ROWS % group != 0)
+                        from[j] = (const uint16_t *)s.p + base + offset(s, group, row + r) + 8 * unit;
+                }
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t)
+                    attn_bring<16>(mine ? (const void *)(from[j] + t * s.plane) : (const void *)attn_fill,
+                                   tile.base + t * Tile::PLANE + 8 * (j * kThreads + (threadIdx.x & ~(PCCNN_WAVE - 1))));
+                from[j] += step;
             } else {
-                attn_clear(c[j]);
+                attn_clear(held[j]);
+                if (row + row_of(j) < limit)
+                    attn_load(held[j], (const T *)s.p + base + offset(s, group, row + row_of(j)), 8 * unit_of(j), width,
+                              s.wide);
             }
         }
     }
-    // a row whose bit is not set becomes zeros, whatever was loaded
-    __device__ __forceinline__ void put(const AttnTile<TERMS, kTile, DP> &tile, uint64_t live) const
+    // Not DIRECT: what was fetched goes to LDS.
+    __device__ __forceinline__ void put(const Tile &tile, uint64_t live) const
     {
+        if constexpr (!DIRECT) {
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const int i = threadIdx.x + j * kThreads, r = i / PER_ROW, col = 8 * (i % PER_ROW);
-            AttnChunk<T> chunk = c[j];
-            if (!((live >> r) & 1)) attn_clear(chunk);
-            tile.put(r, col, attn_frag(chunk));
+            for (int j = 0; j < COUNT; ++j) {
+                AttnChunk<T> chunk = held[j];
+                if (!((live >> row_of(j)) & 1)) attn_clear(chunk);
+                tile.put(row_of(j), unit_of(j), attn_frag(chunk));
+            }
         }
     }
 };
@@ -128,7 +189,7 @@ __device__ __forceinline__ void hide(pccnn_f32x16 &s, uint32_t live, int half)
     const uint32_t mine = live >> (4 * half);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (!((mine >> (8 * (i / 4) + i % 4)) & 1)) s[i] = -INFINITY;
+        s[i] = (mine >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : -INFINITY;
 }
 
 __device__ __forceinline__ void clear(pccnn_f32x16 &c)
@@ -144,6 +205,20 @@ template <int TERMS> __device__ __forceinline__ AttnFrag<TERMS> half_of(const pc
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = s[8 * g + i];
     return attn_split<TERMS>(x);
+}
+
+// A lane's operand of its own side: DP features of one row in steps of sixteen, zeros where there is no row.
+template <typename T, int DP>
+__device__ __forceinline__ void own_side(AttnFrag<AttnTerms<T>::value> (&f)[DP / 16], const void *p, int64_t at, bool live,
+                                         int half, int width, int wide)
+{
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        AttnChunk<T> c;
+        attn_clear(c);
+        if (live) attn_load(c, (const T *)p + at, 16 * kk + 8 * half, width, wide);
+        f[kk] = attn_frag(c);
+    }
 }
 
 // Writes a lane's column of a transposed result (features 32 dt + 8 (i / 4) + 4 half + i % 4 in register i) to a dense row.
@@ -172,85 +247,103 @@ __device__ __forceinline__ void write_column(T *row, const pccnn_f32x16 (&acc)[D
 
 // ------------------------------------------------------------------------------------------------- forward
 
-template <typename T, int DP>
+// The running maximum is only raised when a tile exceeds it by more than this many powers of two: P then stays below
+// 2^8 in f32 and bf16 (exponents to spare in both), and the accumulators are rarely scaled.
+constexpr float kSlack = 8.0f;
+
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
 {
     constexpr int TERMS = AttnTerms<T>::value;
+    typedef Feeder<T, DP, DIRECT, false> Feed;
+    typedef typename Feed::Tile Tile;
+    constexpr int ROWS = Feed::ROWS;
     extern __shared__ __align__(16) uint16_t lds[];
-    const AttnTile<TERMS, kTile, DP> tile_k = {lds}, tile_v = {lds + TERMS * AttnTile<TERMS, kTile, DP>::PLANE};
     const AttnBlock b(a, blockIdx.x);
     if (b.tile * kOwn >= b.rows) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int row = b.tile * kOwn + wave * 32 + (lane & 31);
     const bool working = b.tile * kOwn + wave * 32 < b.rows;         // any row of this wavefront exists
-    const T *k = (const T *)a.k + b.k0 * a.k_n + b.head * a.k_h;
-    const T *v = (const T *)a.v + b.k0 * a.v_n + b.head * a.v_h;
+    const int64_t k_at = b.k0 * a.one.n + b.head * a.one.h, v_at = b.k0 * a.two.n + b.head * a.two.h;
 
-    AttnFrag<TERMS> q[DP / 16];
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        AttnChunk<T> c;
-        attn_clear(c);
-        if (row < b.rows)
-            attn_load(c, (const T *)a.q + b.query(a, row) * a.q_n + b.head_of(a, row) * a.q_h, 16 * kk + 8 * half, a.width,
-                      a.wide_q);
-        q[kk] = attn_frag(c);
+    int key = b.split * a.per_split * ROWS;
+    const int end = min(b.keys, key + a.per_split * ROWS);
+    Feed k, v;
+    uint64_t live = 0;
+    uint8_t flag = 0;
+    k.start(a.one, k_at, 1, key);
+    v.start(a.two, v_at, 1, key);
+    if (key < end) {
+        flag = key_flag(a, b, key, lane);
+        live = live_keys(a, b, key, flag, ROWS);
+        k.fetch(a.one, k_at, 1, key, b.keys, live, a.width, Tile{lds});
+        v.fetch(a.two, v_at, 1, key, b.keys, live, a.width, Tile{lds + Tile::ELEMENTS});
+        flag = key_flag(a, b, key + ROWS, lane);
     }
+    AttnFrag<TERMS> q[DP / 16];
+    own_side<T, DP>(q, a.q, row < b.rows ? b.query(a, row) * a.q_n + b.head_of(a, row) * a.q_h : 0, row < b.rows, half,
+                    a.width, a.wide_q);
     pccnn_f32x16 acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
     float top = -INFINITY, sum = 0.0f;                               // of the lane's row; the sum over the lane's keys only
     const float c2 = a.scale * kLog2e;
 
-    int key = b.split * a.per_split * kTile;
-    const int end = min(b.keys, key + a.per_split * kTile);
-    Carrier<T, DP> next_k, next_v;
-    uint64_t next_live = 0;
-    if (key < end) {
-        next_k.load(k, a.k_n, key, b.keys, a.width, a.wide_k);
-        next_v.load(v, a.v_n, key, b.keys, a.width, a.wide_v);
-        next_live = live_keys(a, b, key, lane);
-    }
-    for (; key < end; key += kTile) {
-        const uint64_t live = next_live;
-        __syncthreads();
-        next_k.put(tile_k, live);
-        next_v.put(tile_v, live);
-        __syncthreads();
-        if (key + kTile < end) {
-            next_k.load(k, a.k_n, key + kTile, b.keys, a.width, a.wide_k);
-            next_v.load(v, a.v_n, key + kTile, b.keys, a.width, a.wide_v);
-            next_live = live_keys(a, b, key + kTile, lane);
+    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
+        const Tile tile_k = {lds + stage * 2 * Tile::ELEMENTS}, tile_v = {tile_k.base + Tile::ELEMENTS};
+        const Tile next_k = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_v = {next_k.base + Tile::ELEMENTS};
+        const uint64_t now = live;
+        if constexpr (DIRECT) {
+            attn_landed();
+        } else {
+            k.put(tile_k, now);
+            v.put(tile_v, now);
+            __syncthreads();
         }
-        if (!working || live == 0) continue;
-        pccnn_f32x16 s[2];
+        if (key + ROWS < end) {
+            live = live_keys(a, b, key + ROWS, flag, ROWS);
+            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.width, next_k);
+            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.width, next_v);
+            flag = key_flag(a, b, key + 2 * ROWS, lane);
+        }
+        if (!working || now == 0) continue;
+        pccnn_f32x16 s[ROWS / 32];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < ROWS / 32; ++t) {
             clear(s[t]);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk)
-                attn_mma<TERMS>(s[t], tile_k.rows(32 * t + (lane & 31), 16 * kk + 8 * half), q[kk]);
-            if (live != ~0ull) hide(s[t], (uint32_t)(live >> (32 * t)), half);
+                attn_mma<TERMS>(s[t], tile_k.rows(32 * t + (lane & 31), 2 * kk + half), q[kk]);
         }
+        if (now != first_bits(ROWS, ROWS))
+#pragma unroll
+            for (int t = 0; t < ROWS / 32; ++t) hide(s[t], (uint32_t)(now >> (32 * t)), half);
         float high = s[0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) high = fmaxf(high, fmaxf(s[0][i], s[1][i]));
-        high = fmaxf(top, attn_max_halves(high) * c2);
-        const float shift = high == -INFINITY ? 0.0f : high;
-        const float shrink = __builtin_amdgcn_exp2f(top - shift);
-        top = high;
-        sum *= shrink;
+        for (int t = 0; t < ROWS / 32; ++t)
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
+            for (int i = 0; i < 16; ++i) high = fmaxf(high, s[t][i]);
+        high = attn_max_halves(high) * c2;
+        if (__any(high > top + kSlack)) {
+            const float raised = fmaxf(top, high);
+            const float shrink = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - raised);
+            top = raised;
+            sum *= shrink;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
+            for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+                for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int t = 0; t < ROWS / 32; ++t) {
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c2, -shift));
-                sum += s[t][i];
+                sums[i % 4] += s[t][i];
             }
+            sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const AttnFrag<TERMS> p = half_of<TERMS>(s[t], g);
@@ -274,118 +367,161 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     }
 }
 
-// Joins the parts of a forward pass that was split over the keys: one thread per feature.
-template <typename T> __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttnArgs a)
+// Joins the parts of a forward pass that was split over the keys: THREADS threads to a (query, head), LANES of them side by
+// side over its features (four each), the groups over the parts, added up in a fixed order.
+template <typename T, int THREADS> __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttnArgs a, int lanes)
 {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, tokens = a.m * a.heads;
-    if (i >= tokens * a.width) return;
-    const int64_t token = i / a.width;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * tokens + token].x);
-    const float shift = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, value = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * tokens + token];
-        const float w = __builtin_amdgcn_exp2f(ml.x - shift);
-        sum = fmaf(ml.y, w, sum);
-        value = fmaf(a.part[s * tokens * a.width + i], w, value);
+    __shared__ float sums[kThreads][5];
+    const int mine = threadIdx.x % THREADS, first = threadIdx.x - mine;
+    const int64_t tokens = a.m * a.heads, token = (int64_t)blockIdx.x * (kThreads / THREADS) + threadIdx.x / THREADS;
+    const int group = mine / lanes, groups = THREADS / lanes, col = mine % lanes * 4;
+    float value[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f, top = -INFINITY;
+    if (token < tokens) {
+        for (int s = mine; s < a.splits; s += THREADS) top = fmaxf(top, a.part_ml[s * tokens + token].x);
     }
-    const float one[1] = {top == -INFINITY ? 0.0f : value / sum};
-    pccnn_store<1>((T *)a.out + i, one);
-    if (a.lse != nullptr && i % a.width == 0)
-        a.lse[token] = top == -INFINITY ? -INFINITY : top * (1.0f / kLog2e) + logf(sum);
+    sums[threadIdx.x][0] = top;
+    __syncthreads();
+    for (int i = 0; i < min(THREADS, a.splits); ++i) top = fmaxf(top, sums[first + i][0]);
+    __syncthreads();
+    const float shift = top == -INFINITY ? 0.0f : top;
+    if (token < tokens) {
+#pragma unroll 4
+        for (int s = group; s < a.splits; s += groups) {
+            const float2 ml = a.part_ml[s * tokens + token];
+            const float w = __builtin_amdgcn_exp2f(ml.x - shift);
+            const float *p = a.part + (s * tokens + token) * a.width + col;
+            sum = fmaf(ml.y, w, sum);
+            if (a.width % 4 == 0) {
+                if (col < a.width) {
+                    const float4 x = *(const float4 *)p;
+                    value[0] = fmaf(x.x, w, value[0]); value[1] = fmaf(x.y, w, value[1]);
+                    value[2] = fmaf(x.z, w, value[2]); value[3] = fmaf(x.w, w, value[3]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < a.width) value[i] = fmaf(p[i], w, value[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[threadIdx.x][i] = value[i];
+    sums[threadIdx.x][4] = sum;
+    __syncthreads();
+    if (group != 0 || token >= tokens) return;
+    for (int g = 1; g < groups; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) value[i] += sums[threadIdx.x + g * lanes][i];
+        sum += sums[threadIdx.x + g * lanes][4];
+    }
+    const bool none = top == -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float one[1] = {none ? 0.0f : value[i] / sum};
+        if (col + i < a.width) pccnn_store<1>((T *)a.out + token * a.width + col + i, one);
+    }
+    if (a.lse != nullptr && col == 0) a.lse[token] = none ? -INFINITY : top * (1.0f / kLog2e) + logf(sum);
 }
 
 // ------------------------------------------------------------------------------------------------- backward
 
-// delta[m, heads] = dO . O, eight lanes to a row.
+// What the backward kernels need of a row: D = dO . O, and L in units of log 2 (+inf for a row without keys: every P is
+// zero).  Eight lanes to a row, eight features each at a time.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_delta_kernel(AttnArgs a, const T *__restrict__ out)
+__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a, const T *__restrict__ out)
 {
     const int64_t token = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 8;
     const bool live = token < a.m * a.heads;
     const int64_t query = token / a.heads;
+    const int head = (int)(token - query * a.heads);
     float sum = 0.0f;
     if (live)
-        for (int col = threadIdx.x % 8; col < a.width; col += 8) {
-            float x[1], g[1];
-            pccnn_load<1>(out + token * a.width + col, x);
-            pccnn_load<1>((const T *)a.g + query * a.g_n + (token - query * a.heads) * a.g_h + col, g);
-            sum = fmaf(x[0], g[0], sum);
+        for (int col = 8 * (threadIdx.x % 8); col < a.width; col += 64) {
+            AttnChunk<T> x, g;
+            attn_load(x, out + token * a.width, col, a.width, a.wide_o);
+            attn_load(g, (const T *)a.g + query * a.g_n + head * a.g_h, col, a.width, a.wide_g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(attn_value(x, i), attn_value(g, i), sum);
         }
     sum = pccnn_group_sum<8>(sum);
-    if (live && threadIdx.x % 8 == 0) a.delta[token] = sum;
+    if (live && threadIdx.x % 8 == 0) {
+        const int64_t at = head / a.group * (a.m * a.group) + query * a.group + head % a.group;
+        const float lse = a.lse[token];
+        a.shift[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+        a.delta[at] = lse == -INFINITY ? 0.0f : sum;
+    }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
 {
     constexpr int TERMS = AttnTerms<T>::value;
+    typedef Feeder<T, DP, DIRECT, false> Feed;
+    typedef typename Feed::Tile Tile;
+    constexpr int ROWS = Feed::ROWS;
     extern __shared__ __align__(16) uint16_t lds[];
-    const AttnTile<TERMS, kTile, DP> tile_k = {lds}, tile_v = {lds + TERMS * AttnTile<TERMS, kTile, DP>::PLANE};
     const AttnBlock b(a, blockIdx.x);
     if (b.tile * kOwn >= b.rows) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int row = b.tile * kOwn + wave * 32 + (lane & 31);
     const bool working = b.tile * kOwn + wave * 32 < b.rows;
-    const T *k = (const T *)a.k + b.k0 * a.k_n + b.head * a.k_h;
-    const T *v = (const T *)a.v + b.k0 * a.v_n + b.head * a.v_h;
-    const int64_t query = b.query(a, row < b.rows ? row : 0);
-    const int head = b.head_of(a, row < b.rows ? row : 0);
-    const int64_t token = query * a.heads + head;
+    const int64_t k_at = b.k0 * a.one.n + b.head * a.one.h, v_at = b.k0 * a.two.n + b.head * a.two.h;
 
-    AttnFrag<TERMS> q[DP / 16], g[DP / 16];
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        AttnChunk<T> c;
-        attn_clear(c);
-        if (row < b.rows)
-            attn_load(c, (const T *)a.q + query * a.q_n + head * a.q_h, 16 * kk + 8 * half, a.width, a.wide_q);
-        q[kk] = attn_frag(c);
-        attn_clear(c);
-        if (row < b.rows)
-            attn_load(c, (const T *)a.g + query * a.g_n + head * a.g_h, 16 * kk + 8 * half, a.width, a.wide_g);
-        g[kk] = attn_frag(c);
+    int key = b.split * a.per_split * ROWS;
+    const int end = min(b.keys, key + a.per_split * ROWS);
+    Feed k, v;
+    uint64_t live = 0;
+    uint8_t flag = 0;
+    k.start(a.one, k_at, 1, key);
+    v.start(a.two, v_at, 1, key);
+    if (key < end) {
+        flag = key_flag(a, b, key, lane);
+        live = live_keys(a, b, key, flag, ROWS);
+        k.fetch(a.one, k_at, 1, key, b.keys, live, a.width, Tile{lds});
+        v.fetch(a.two, v_at, 1, key, b.keys, live, a.width, Tile{lds + Tile::ELEMENTS});
+        flag = key_flag(a, b, key + ROWS, lane);
     }
-    const float lse = row < b.rows ? a.lse[token] : -INFINITY, delta = row < b.rows ? a.delta[token] : 0.0f;
-    const float shift = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys: every P is zero
+    const bool real = row < b.rows;
+    const int64_t query = b.query(a, real ? row : 0);
+    const int head = b.head_of(a, real ? row : 0);
+    AttnFrag<TERMS> q[DP / 16], g[DP / 16];
+    own_side<T, DP>(q, a.q, query * a.q_n + head * a.q_h, real, half, a.width, a.wide_q);
+    own_side<T, DP>(g, a.g, query * a.g_n + head * a.g_h, real, half, a.width, a.wide_g);
+    const float shift = real ? a.shift[b.stat(a, row)] : INFINITY, delta = real ? a.delta[b.stat(a, row)] : 0.0f;
     const float c2 = a.scale * kLog2e;
     pccnn_f32x16 acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
 
-    int key = b.split * a.per_split * kTile;
-    const int end = min(b.keys, key + a.per_split * kTile);
-    Carrier<T, DP> next_k, next_v;
-    uint64_t next_live = 0;
-    if (key < end) {
-        next_k.load(k, a.k_n, key, b.keys, a.width, a.wide_k);
-        next_v.load(v, a.v_n, key, b.keys, a.width, a.wide_v);
-        next_live = live_keys(a, b, key, lane);
-    }
-    for (; key < end; key += kTile) {
-        const uint64_t live = next_live;
-        __syncthreads();
-        next_k.put(tile_k, live);
-        next_v.put(tile_v, live);
-        __syncthreads();
-        if (key + kTile < end) {
-            next_k.load(k, a.k_n, key + kTile, b.keys, a.width, a.wide_k);
-            next_v.load(v, a.v_n, key + kTile, b.keys, a.width, a.wide_v);
-            next_live = live_keys(a, b, key + kTile, lane);
+    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
+        const Tile tile_k = {lds + stage * 2 * Tile::ELEMENTS}, tile_v = {tile_k.base + Tile::ELEMENTS};
+        const Tile next_k = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_v = {next_k.base + Tile::ELEMENTS};
+        const uint64_t now = live;
+        if constexpr (DIRECT) {
+            attn_landed();
+        } else {
+            k.put(tile_k, now);
+            v.put(tile_v, now);
+            __syncthreads();
         }
-        if (!working || live == 0) continue;
+        if (key + ROWS < end) {
+            live = live_keys(a, b, key + ROWS, flag, ROWS);
+            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.width, next_k);
+            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.width, next_v);
+            flag = key_flag(a, b, key + 2 * ROWS, lane);
+        }
+        if (!working || now == 0) continue;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < ROWS / 32; ++t) {
             pccnn_f32x16 s, dp;
             clear(s);
             clear(dp);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
-                attn_mma<TERMS>(s, tile_k.rows(32 * t + (lane & 31), 16 * kk + 8 * half), q[kk]);
-                attn_mma<TERMS>(dp, tile_v.rows(32 * t + (lane & 31), 16 * kk + 8 * half), g[kk]);
+                attn_mma<TERMS>(s, tile_k.rows(32 * t + (lane & 31), 2 * kk + half), q[kk]);
+                attn_mma<TERMS>(dp, tile_v.rows(32 * t + (lane & 31), 2 * kk + half), g[kk]);
             }
-            if (live != ~0ull) hide(s, (uint32_t)(live >> (32 * t)), half);
+            if (now != first_bits(ROWS, ROWS)) hide(s, (uint32_t)(now >> (32 * t)), half);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -shift)) * (dp[i] - delta);
@@ -398,45 +534,57 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
             }
         }
     }
-    if (row >= b.rows) return;
-    if (lse == -INFINITY) {                                          // whatever its gradient holds (0 times NaN)
+    if (!real) return;
+    if (shift == INFINITY) {                                         // whatever its gradient holds (0 times NaN)
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
     }
+    const int64_t token = query * a.heads + head;
     if (a.splits > 1)
         write_column<float, DP>(a.part + ((int64_t)b.split * a.m * a.heads + token) * a.width, acc, a.scale, half, a.width);
     else
         write_column<T, DP>((T *)a.out + token * a.width, acc, a.scale, half, a.width);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
 {
     constexpr int TERMS = AttnTerms<T>::value;
-    constexpr int PLANES = TERMS * AttnTile<TERMS, kTile, DP>::PLANE;
+    typedef Feeder<T, DP, DIRECT, true> Feed;
+    typedef typename Feed::Tile Tile;
+    constexpr int ROWS = Feed::ROWS;
     extern __shared__ __align__(16) uint16_t lds[];
-    const AttnTile<TERMS, kTile, DP> tile_q = {lds}, tile_g = {lds + PLANES};
-    float *row_shift = (float *)(lds + 2 * PLANES), *row_delta = row_shift + kTile;
+    float *const stats = (float *)(lds + 4 * Tile::ELEMENTS);        // [stage][shift, delta][64]
     const AttnBlock b(a, blockIdx.x);
     if (b.tile * kOwn >= b.keys) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int key = b.tile * kOwn + wave * 32 + (lane & 31);
     const bool working = b.tile * kOwn + wave * 32 < b.keys;
     const bool live = key < b.keys && (a.mask == nullptr || a.mask[b.k0 + key] != 0);
-    const T *q = (const T *)a.q + b.q0 * a.q_n + b.head * a.group * a.q_h;
-    const T *g = (const T *)a.g + b.q0 * a.g_n + b.head * a.group * a.g_h;
+    const int64_t q_at = b.q0 * a.one.n + b.head * a.group * a.one.h, g_at = b.q0 * a.two.n + b.head * a.group * a.two.h;
 
-    AttnFrag<TERMS> k[DP / 16], v[DP / 16];
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        AttnChunk<T> c;
-        attn_clear(c);
-        if (live) attn_load(c, (const T *)a.k + (b.k0 + key) * a.k_n + b.head * a.k_h, 16 * kk + 8 * half, a.width, a.wide_k);
-        k[kk] = attn_frag(c);
-        attn_clear(c);
-        if (live) attn_load(c, (const T *)a.v + (b.k0 + key) * a.v_n + b.head * a.v_h, 16 * kk + 8 * half, a.width, a.wide_v);
-        v[kk] = attn_frag(c);
+    int row = (int)min((int64_t)b.split * a.per_split * ROWS, (int64_t)b.rows);
+    const int end = (int)min((int64_t)b.rows, row + (int64_t)a.per_split * ROWS);
+    Feed q, g;
+    q.start(a.one, q_at, a.group, row);
+    g.start(a.two, g_at, a.group, row);
+    // shifts and deltas of the tile's rows go to LDS the same way, one wavefront each
+    auto fetch_stats = [&](int from, int stage) {
+        if (wave < 2) {
+            const float *src = (wave == 0 ? a.shift : a.delta) + b.stat(a, from + lane);
+            attn_bring<4>(from + lane < b.rows ? (const void *)src : (const void *)(attn_fill + (wave == 0 ? 4 : 0)),
+                          stats + (stage * 2 + wave) * 64);
+        }
+    };
+    if (row < end) {
+        const uint64_t bits = first_bits(b.rows - row, ROWS);
+        q.fetch(a.one, q_at, a.group, row, b.rows, bits, a.width, Tile{lds});
+        g.fetch(a.two, g_at, a.group, row, b.rows, bits, a.width, Tile{lds + Tile::ELEMENTS});
+        fetch_stats(row, 0);
     }
+    AttnFrag<TERMS> k[DP / 16], v[DP / 16];
+    own_side<T, DP>(k, a.k, (b.k0 + key) * a.k_n + b.head * a.k_h, live, half, a.width, a.wide_k);
+    own_side<T, DP>(v, a.v, (b.k0 + key) * a.v_n + b.head * a.v_h, live, half, a.width, a.wide_v);
     pccnn_f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) {
@@ -444,54 +592,42 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
         clear(dv[dt]);
     }
     const float c2 = a.scale * kLog2e;
-    int row = (int)min((int64_t)b.split * a.per_split * kTile, (int64_t)b.rows);
-    const int end = (int)min((int64_t)b.rows, row + (int64_t)a.per_split * kTile);
-    Carrier<T, DP> next_q, next_g;
-    float next_shift = INFINITY, next_delta = 0.0f;                  // of row threadIdx.x of the tile
-    auto fetch = [&](int from) {
-        next_q.load_rows(q, a.q_n, a.q_h, from, b.rows, a.group, a.width, a.wide_q);
-        next_g.load_rows(g, a.g_n, a.g_h, from, b.rows, a.group, a.width, a.wide_g);
-        if (threadIdx.x < kTile) {
-            const int r = from + (int)threadIdx.x;
-            next_shift = INFINITY;                                   // no such row, or one without keys: every P is zero
-            next_delta = 0.0f;
-            if (r < b.rows) {
-                const int64_t token = b.query(a, r) * a.heads + b.head_of(a, r);
-                const float lse = a.lse[token];
-                if (lse != -INFINITY) {
-                    next_shift = lse * kLog2e;
-                    next_delta = a.delta[token];
-                }
-            }
+    for (int stage = 0; row < end; row += ROWS, stage ^= 1) {
+        const Tile tile_q = {lds + stage * 2 * Tile::ELEMENTS}, tile_g = {tile_q.base + Tile::ELEMENTS};
+        const Tile next_q = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_g = {next_q.base + Tile::ELEMENTS};
+        if constexpr (!DIRECT) {
+            const uint64_t bits = first_bits(b.rows - row, ROWS);
+            q.put(tile_q, bits);
+            g.put(tile_g, bits);
         }
-    };
-    if (row < end) fetch(row);
-    for (; row < end; row += kTile) {
-        __syncthreads();
-        next_q.put(tile_q, ~0ull);
-        next_g.put(tile_g, ~0ull);
-        if (threadIdx.x < kTile) {
-            row_shift[threadIdx.x] = next_shift;
-            row_delta[threadIdx.x] = next_delta;
+        attn_landed();
+        if (row + ROWS < end) {
+            const uint64_t bits = first_bits(b.rows - row - ROWS, ROWS);
+            q.fetch(a.one, q_at, a.group, row + ROWS, b.rows, bits, a.width, next_q);
+            g.fetch(a.two, g_at, a.group, row + ROWS, b.rows, bits, a.width, next_g);
+            fetch_stats(row + ROWS, stage ^ 1);
         }
-        __syncthreads();
-        if (row + kTile < end) fetch(row + kTile);
         if (!working) continue;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < ROWS / 32; ++t) {
             pccnn_f32x16 s, dp;
             clear(s);
             clear(dp);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
-                attn_mma<TERMS>(s, tile_q.rows(32 * t + (lane & 31), 16 * kk + 8 * half), k[kk]);
-                attn_mma<TERMS>(dp, tile_g.rows(32 * t + (lane & 31), 16 * kk + 8 * half), v[kk]);
+                attn_mma<TERMS>(s, tile_q.rows(32 * t + (lane & 31), 2 * kk + half), k[kk]);
+                attn_mma<TERMS>(dp, tile_g.rows(32 * t + (lane & 31), 2 * kk + half), v[kk]);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = 32 * t + 8 * (i / 4) + 4 * half + i % 4;
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -row_shift[r]));
-                dp[i] = s[i] * (dp[i] - row_delta[r]);
+            for (int i = 0; i < 4; ++i) {
+                const float4 shift = *(const float4 *)(stats + stage * 128 + 32 * t + 8 * i + 4 * half);
+                const float4 delta = *(const float4 *)(stats + stage * 128 + 64 + 32 * t + 8 * i + 4 * half);
+                const float sh[4] = {shift.x, shift.y, shift.z, shift.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + j], c2, -sh[j]));
+                    dp[4 * i + j] = s[4 * i + j] * (dp[4 * i + j] - de[j]);
+                }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -523,16 +659,23 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
     }
 }
 
-// Sum of the parts of a gradient, in order.
-template <typename T>
+// Sum of the parts of a gradient, in order; VEC values per thread (4 when the count is a multiple of 4).
+template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void attention_sum_kernel(const float *__restrict__ part, int splits, int64_t count,
                                                                 T *__restrict__ out)
 {
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
-        float sum[1] = {0.0f};
-        for (int s = 0; s < splits; ++s) sum[0] += part[s * count + i];
-        pccnn_store<1>(out + i, sum);
+    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VEC;
+    if (i >= count) return;
+    float sum[VEC], x[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        pccnn_load<VEC>(part + s * count + i, x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum[j] += x[j];
     }
+    pccnn_store<VEC>(out + i, sum);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -589,24 +732,53 @@ AttnArgs attn_args(const pccnn_attention *p)
     a.wide_q = attn_wide(a.q, a.q_n, a.q_h, p->type, a.width);
     a.wide_k = attn_wide(a.k, a.k_n, a.k_h, p->type, a.width);
     a.wide_v = attn_wide(a.v, a.v_n, a.v_h, p->type, a.width);
+    a.one = a.two = AttnStream{};
     a.splits = 1;
     return a;
+}
+
+// Whether a tensor's rows go to LDS as they are: bf16, whole 16-byte units, 16-byte rows.
+bool attn_direct(int type, int wide_one, int wide_two) { return type == PCCNN_TYPE_BF16 && wide_one == 2 && wide_two == 2; }
+
+// Calls f(type, padded width) for the instantiation that serves this type and head width.
+template <typename F> int attn_dispatch(int type, int width, F f)
+{
+    auto by_width = [&](auto zero) {
+        if (width <= 32) return f(zero, std::integral_constant<int, 32>());
+        if (width <= 64) return f(zero, std::integral_constant<int, 64>());
+        if (width <= 96) return f(zero, std::integral_constant<int, 96>());
+        return f(zero, std::integral_constant<int, 128>());
+    };
+    return type == PCCNN_TYPE_F32 ? by_width(0.0f) : by_width((uint16_t)0);
 }
 
 constexpr int64_t kWantedBlocks = 1024;      // workgroups that fill the chip (four per CU)
 constexpr int kLeastTiles = 4;               // tiles below which a part is not worth its join
 
 // Tiles of the own side, and the parts the other side is cut into so that few own tiles still fill the chip.
-void attn_plan(AttnArgs &a, int64_t own, int64_t other)
+void attn_plan(AttnArgs &a, int type, int64_t own, int64_t other)
 {
+    const int rows = attn_dispatch(type, a.width, [](auto zero, auto dp) -> int {
+        return attn_tile_rows<decltype(zero), decltype(dp)::value>();
+    });
     a.tiles = (int)std::max<int64_t>(1, pccnn_ceil_div(own, kOwn));
-    const int64_t base = (int64_t)a.tiles * a.key_heads * a.clouds, tiles = std::max<int64_t>(1, pccnn_ceil_div(other, kTile));
+    const int64_t base = (int64_t)a.tiles * a.key_heads * a.clouds, tiles = std::max<int64_t>(1, pccnn_ceil_div(other, rows));
     int64_t splits = std::max<int64_t>(1, std::min(kWantedBlocks / base, tiles / kLeastTiles));
     a.per_split = (int)pccnn_ceil_div(tiles, splits);
     a.splits = (int)pccnn_ceil_div(tiles, a.per_split);
 }
-void attn_plan_rows(AttnArgs &a, const pccnn_attention *p) { attn_plan(a, p->max_queries * a.group, p->max_keys); }
-void attn_plan_keys(AttnArgs &a, const pccnn_attention *p) { attn_plan(a, p->max_keys, p->max_queries * a.group); }
+void attn_plan_rows(AttnArgs &a, const pccnn_attention *p) 
+{
+    attn_plan(a, p->type, p->max_queries * a.group, p->max_keys);
+    a.one = {a.k, a.k_n, a.k_h, 0, a.wide_k, a.width / 8};
+    a.two = {a.v, a.v_n, a.v_h, 0, a.wide_v, a.width / 8};
+}
+void attn_plan_keys(AttnArgs &a, const pccnn_attention *p) 
+{
+    attn_plan(a, p->type, p->max_keys, p->max_queries * a.group);
+    a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
+    a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
+}
 
 int64_t attn_blocks(const AttnArgs &a) { return (int64_t)a.tiles * a.splits * a.key_heads * a.clouds; }
 
@@ -621,18 +793,10 @@ template <typename KERNEL> int attn_launch(const char *name, KERNEL kernel, cons
     return PCCNN_OK;
 }
 
-template <typename T, int DP> constexpr size_t tile_bytes() { return AttnTile<AttnTerms<T>::value, kTile, DP>::BYTES; }
-
-// Calls f(type, padded width) for the instantiation that serves this type and head width.
-template <typename F> int attn_dispatch(int type, int width, F f)
+// LDS of the kernels: two tiles of two tensors.
+template <typename T, int DP> constexpr size_t tiles_bytes()
 {
-    auto by_width = [&](auto zero) {
-        if (width <= 32) return f(zero, std::integral_constant<int, 32>());
-        if (width <= 64) return f(zero, std::integral_constant<int, 64>());
-        if (width <= 96) return f(zero, std::integral_constant<int, 96>());
-        return f(zero, std::integral_constant<int, 128>());
-    };
-    return type == PCCNN_TYPE_F32 ? by_width(0.0f) : by_width((uint16_t)0);
+    return 4 * 2 * (size_t)AttnTile<AttnTerms<T>::value, attn_tile_rows<T, DP>(), DP>::ELEMENTS;
 }
 
 size_t forward_bytes(const AttnArgs &a)
@@ -653,7 +817,7 @@ extern "C" size_t pccnn_attention_workspace_bytes(const pccnn_attention *p, int 
     size_t rows = a.splits > 1 ? pccnn_align((size_t)a.splits * a.m * a.heads * a.width * sizeof(float)) : 0;
     attn_plan_keys(a, p);
     size_t keys = a.splits > 1 ? 2 * pccnn_align((size_t)a.splits * a.n * a.key_heads * a.width * sizeof(float)) : 0;
-    return 256 + pccnn_align((size_t)a.m * a.heads * sizeof(float)) + std::max(rows, keys);
+    return 256 + 2 * pccnn_align((size_t)a.m * a.heads * sizeof(float)) + std::max(rows, keys);
 }
 
 extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, float *lse_out, void *workspace,
@@ -678,9 +842,21 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
     return attn_dispatch(p->type, p->width, [&](auto zero, auto dp) -> int {
         using T = decltype(zero);
         constexpr int DP = decltype(dp)::value;
-        const int rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP>, a, 2 * tile_bytes<T, DP>(), s);
+        int rc;
+        if (attn_direct(p->type, a.wide_k, a.wide_v)) {
+            if constexpr (sizeof(T) == 2)
+                rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
+        } else {
+            rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP, false>, a, tiles_bytes<T, DP>(), s);
+        }
         if (rc != PCCNN_OK || a.splits == 1) return rc;
-        attention_join_kernel<T><<<(unsigned)pccnn_ceil_div(a.m * a.heads * a.width, kThreads), kThreads, 0, s>>>(a);
+        // a wavefront to a result up to 32 parts, a workgroup beyond
+        int lanes = 1;
+        while (4 * lanes < a.width) lanes *= 2;
+        if (a.splits <= 32)
+            attention_join_kernel<T, 64><<<(unsigned)pccnn_ceil_div(a.m * a.heads, 4), kThreads, 0, s>>>(a, lanes);
+        else
+            attention_join_kernel<T, 256><<<(unsigned)(a.m * a.heads), kThreads, 0, s>>>(a, lanes);
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
     });
@@ -705,6 +881,8 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
     a.wide_g = attn_wide(a.g, a.g_n, a.g_h, p->type, a.width);
     a.lse = (float *)lse;
     PccnnArena arena(workspace, workspace_bytes);
+    a.wide_o = attn_wide(out, a.width, a.width, p->type, a.width);
+    a.shift = arena.take<float>((size_t)p->m * p->heads);
     a.delta = arena.take<float>((size_t)p->m * p->heads);
     const size_t after = arena.used;
     return attn_dispatch(p->type, p->width, [&](auto zero, auto dp) -> int {
@@ -712,14 +890,18 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         constexpr int DP = decltype(dp)::value;
         int rc = PCCNN_OK;
         auto sum_parts = [&](const float *part, int64_t count, void *to) {
-            const unsigned blocks = (unsigned)std::min<int64_t>(pccnn_ceil_div(count, kThreads), 8192);
-            attention_sum_kernel<T><<<blocks, kThreads, 0, s>>>(part, a.splits, count, (T *)to);
+            if (count % 4 == 0)
+                attention_sum_kernel<T, 4><<<(unsigned)pccnn_ceil_div(count, 4 * kThreads), kThreads, 0, s>>>(part, a.splits,
+                                                                                                          count, (T *)to);
+            else
+                attention_sum_kernel<T, 1><<<(unsigned)pccnn_ceil_div(count, kThreads), kThreads, 0, s>>>(part, a.splits,
+                                                                                                      count, (T *)to);
         };
         if (p->m > 0) {
             PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention_grads: workspace of %zu bytes is too small",
                           workspace_bytes);
             const int64_t threads = a.m * a.heads * 8;
-            attention_delta_kernel<T><<<(unsigned)pccnn_ceil_div(threads, kThreads), kThreads, 0, s>>>(a, (const T *)out);
+            attention_rows_kernel<T><<<(unsigned)pccnn_ceil_div(threads, kThreads), kThreads, 0, s>>>(a, (const T *)out);
             PCCNN_LAUNCH_CHECK();
         }
         if (d_queries != nullptr && p->m > 0) {
@@ -732,7 +914,12 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
                 PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE,
                               "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
             }
-            rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP>, a, 2 * tile_bytes<T, DP>(), s);
+            if (attn_direct(p->type, a.wide_k, a.wide_v)) {
+                if constexpr (sizeof(T) == 2)
+                    rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
+            } else {
+                rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP, false>, a, tiles_bytes<T, DP>(), s);
+            }
             if (rc != PCCNN_OK) return rc;
             if (a.splits > 1) sum_parts(a.part, count, d_queries);
             PCCNN_LAUNCH_CHECK();
@@ -749,8 +936,13 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
                 PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE,
                               "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
             }
-            rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP>, a,
-                             2 * tile_bytes<T, DP>() + 2 * kTile * sizeof(float), s);
+            const size_t bytes = tiles_bytes<T, DP>() + 4 * 64 * sizeof(float);
+            if (attn_direct(p->type, a.wide_q, a.wide_g)) {
+                if constexpr (sizeof(T) == 2)
+                    rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP, true>, a, bytes, s);
+            } else {
+                rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP, false>, a, bytes, s);
+            }
             if (rc != PCCNN_OK) return rc;
             if (a.splits > 1) {
                 sum_parts(a.part, count, d_keys);

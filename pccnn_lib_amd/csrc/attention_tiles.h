@@ -110,6 +110,13 @@ __device__ __forceinline__ void attn_load(AttnChunk<float> &c, const float *row,
             if (col + i < width) c.v[i] = row[col + i];
     }
 }
+// The i-th of a chunk's values.
+__device__ __forceinline__ float attn_value(const AttnChunk<uint16_t> &c, int i)
+{
+    return __uint_as_float(i % 2 ? c.v[i / 2] & 0xffff0000u : c.v[i / 2] << 16);
+}
+__device__ __forceinline__ float attn_value(const AttnChunk<float> &c, int i) { return c.v[i]; }
+
 __device__ __forceinline__ AttnFrag<1> attn_frag(const AttnChunk<uint16_t> &c)
 {
     AttnFrag<1> f;
@@ -118,25 +125,44 @@ __device__ __forceinline__ AttnFrag<1> attn_frag(const AttnChunk<uint16_t> &c)
 }
 __device__ __forceinline__ AttnFrag<3> attn_frag(const AttnChunk<float> &c) { return attn_split<3>(c.v); }
 
-// A tile of ROWS rows in LDS, bf16, one plane per term; a row is DP features and 16 bytes of padding.
+// A tile of ROWS rows in LDS, bf16, one plane per term, rows of DP features without padding.  The 16-byte units of a row
+// are exchanged among themselves by a rule on the row, chosen so that the two reads below touch every group of four banks
+// once: sixteen rows at one unit (an operand's rows), and four rows at four neighboring units (its columns).
 template <int TERMS, int ROWS, int DP> struct AttnTile {
-    static constexpr int STRIDE = DP + 8;
-    static constexpr int PLANE = ROWS * STRIDE;                       // elements
-    static constexpr int BYTES = TERMS * PLANE * 2;
+    static constexpr int UNITS = DP / 8;                              // 16-byte units of a row: 4, 8, 12 or 16
+    static constexpr int PLANE = ROWS * DP;                           // elements
+    static constexpr int ELEMENTS = TERMS * PLANE;
     uint16_t *base;
-    __device__ __forceinline__ void put(int row, int col, const AttnFrag<TERMS> &f) const
+    // Where unit `unit` of row `row` lies within the row (its own inverse, except for twelve units).
+    static __device__ __forceinline__ int place(int row, int unit)
+    {
+        if constexpr (UNITS == 4) return unit ^ ((row >> 2) & 3);
+        if constexpr (UNITS == 8) return unit ^ (((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1));
+        if constexpr (UNITS == 16) return unit ^ ((row & 3) << 2 | ((row >> 2) & 3));
+        const int moved = unit + ((row >> 2) & 3);
+        return moved >= UNITS ? moved - UNITS : moved;
+    }
+    // Which unit of the row lies there.
+    static __device__ __forceinline__ int unit_at(int row, int placed)
+    {
+        if constexpr (UNITS != 12) return place(row, placed);
+        const int moved = placed - ((row >> 2) & 3);
+        return moved < 0 ? moved + UNITS : moved;
+    }
+    __device__ __forceinline__ void put(int row, int unit, const AttnFrag<TERMS> &f) const
     {
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
-            *(pccnn_u32x4 *)(base + t * PLANE + row * STRIDE + col) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
+            *(pccnn_u32x4 *)(base + t * PLANE + row * DP + 8 * place(row, unit)) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
     }
-    // Operand with the tile's rows as C's rows: eight features from `col` of row `row`.
-    __device__ __forceinline__ AttnFrag<TERMS> rows(int row, int col) const
+    // Operand with the tile's rows as C's rows: the eight features of unit `unit` of row `row`.
+    __device__ __forceinline__ AttnFrag<TERMS> rows(int row, int unit) const
     {
         AttnFrag<TERMS> f;
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
-            f.t[t] = __builtin_bit_cast(pccnn_bf16x8, *(const pccnn_u32x4 *)(base + t * PLANE + row * STRIDE + col));
+            f.t[t] = __builtin_bit_cast(pccnn_bf16x8,
+                                        *(const pccnn_u32x4 *)(base + t * PLANE + row * DP + 8 * place(row, unit)));
         return f;
     }
     // Operand with the tile's features as C's rows (feature col + (lane & 31)) and as k the sixteen tile rows from `row`,
@@ -144,19 +170,42 @@ template <int TERMS, int ROWS, int DP> struct AttnTile {
     // among sixteen lanes: lane i brings four features of row i / 4 and gets feature i of all four rows.
     __device__ __forceinline__ AttnFrag<TERMS> columns(int row, int col, int lane) const
     {
-        const int r = row + 4 * (lane >> 5) + ((lane & 15) >> 2), c = col + (lane & 16) + 4 * (lane & 3);
+        const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), unit = (col + (lane & 16)) / 8 + ((lane & 3) >> 1);
+        const int lo_at = r * DP + 8 * place(r, unit) + 4 * (lane & 1);
+        const int hi_at = (r + 8) * DP + 8 * place(r + 8, unit) + 4 * (lane & 1);
         AttnFrag<TERMS> f;
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) {
-            uint16_t *p = base + t * PLANE + r * STRIDE + c;
             typedef __attribute__((address_space(3))) pccnn_i16x4 *lds_ptr;
-            const pccnn_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-            const pccnn_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * STRIDE));
+            uint16_t *p = base + t * PLANE + row * DP;                // row: a multiple of 16, so place() sees r alone
+            const pccnn_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + lo_at));
+            const pccnn_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + hi_at));
             f.t[t] = __builtin_bit_cast(pccnn_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
         return f;
     }
 };
+
+// What lanes without a row of their own bring into LDS: zeros, and for a row's shift plus infinity.
+__device__ const uint32_t attn_fill[8] = {0u, 0u, 0u, 0u, 0x7f800000u, 0u, 0u, 0u};
+
+// Memory to LDS without a register between: lane i's `bytes` (4 or 16) from its own address to `lds` + i * bytes, `lds`
+// the same in all lanes.  Lands by the next wait for vector memory (attn_landed).
+template <int BYTES> __device__ __forceinline__ void attn_bring(const void *from, void *lds)
+{
+    typedef const __attribute__((address_space(1))) uint32_t *global_ptr;
+    typedef __attribute__((address_space(3))) uint32_t *lds_ptr;
+    if constexpr (BYTES == 16)
+        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)lds, 16, 0, 0);
+    else
+        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)lds, 4, 0, 0);
+}
+// Everything this wavefront brought has landed; with the barrier behind it, everything the workgroup brought.
+__device__ __forceinline__ void attn_landed()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0)
+    __syncthreads();
+}
 
 // max(v, v of the lane 32 away)
 __device__ __forceinline__ float attn_max_halves(float v)
