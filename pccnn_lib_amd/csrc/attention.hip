@@ -116,7 +116,8 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
     typedef AttnTile<TERMS, ROWS, DP> Tile;
     static constexpr int COUNT = ROWS * Tile::UNITS / kThreads;
     static_assert(COUNT >= 1 && COUNT * kThreads == ROWS * Tile::UNITS, "every thread carries whole units");
-    const uint16_t *from[DIRECT ? COUNT : 1];
+    const char *base;                        // DIRECT: the tile's first row (the same in all lanes)
+    uint32_t off[DIRECT ? COUNT : 1];        // and from there the lane's units, in bytes
     int64_t step;
     AttnChunk<T> held[DIRECT ? 1 : COUNT];
 
@@ -131,40 +132,59 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
             return row * s.n;
         }
     }
-    // `base`: the cloud's and head's first element
-    __device__ __forceinline__ void start(const AttnStream &s, int64_t base, int group, int row)
+    // Tiles start at multiples of ROWS: where the group divides them, every tile has the same offsets within it.
+    static __device__ __forceinline__ bool regular(int group) { return !GROUPED || ROWS % group == 0; }
+    // `at`: the cloud's and head's first element.  Units past the heads' width lie nowhere, which reads zeros.
+    __device__ __forceinline__ void start(const AttnStream &s, int64_t at, int group, int row)
     {
         if constexpr (DIRECT) {
+            base = (const char *)s.p + 2 * (at + offset(s, group, row));
+            step = 2 * (!GROUPED || group == 1 ? ROWS * s.n : ROWS / group * s.n);
 #pragma unroll
-            for (int j = 0; j < COUNT; ++j)
-                from[j] = (const uint16_t *)s.p + base + offset(s, group, row + row_of(j)) +
-                          8 * Tile::unit_at(row_of(j), unit_of(j));
-            step = !GROUPED || group == 1 ? ROWS * s.n : ROWS / group * s.n;
+            for (int j = 0; j < COUNT; ++j) {
+                const int r = row_of(j), unit = Tile::unit_at(r, unit_of(j));
+                off[j] = unit < s.units ? 2 * (uint32_t)(offset(s, group, r) + 8 * unit) : kAttnNowhere;
+            }
         }
     }
     // Starts bringing the tile of rows `row` .. into `tile` (DIRECT), or into registers.  Rows without a bit in `live`
-    // become zeros; `limit`: rows that exist.
-    __device__ __forceinline__ void fetch(const AttnStream &s, int64_t base, int group, int row, int limit, uint64_t live,
-                                          int width, const Tile &tile)
+    // become zeros; `limit`: rows that exist; `masked`: other rows than the last ones may lack their bits.
+    __device__ __forceinline__ void fetch(const AttnStream &s, int64_t at, int group, int row, int limit, uint64_t live,
+                                          bool masked, int width, const Tile &tile)
     {
+        if constexpr (DIRECT) {
+            if (!regular(group)) {                       // the tile's first row may lie inside a group
+                base = (const char *)s.p + 2 * (at + row / group * s.n);
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            if constexpr (DIRECT) {
-                const int r = row_of(j), unit = Tile::unit_at(r, unit_of(j));
-                const bool mine = ((live >> r) & 1) && unit < s.units;
-                if constexpr (GROUPED) {
-                    if (group > 1 && ROWS % group != 0)
-                        from[j] = (const uint16_t *)s.p + base + offset(s, group, row + r) + 8 * unit;
+                for (int j = 0; j < COUNT; ++j) {
+                    const int r = row_of(j), unit = Tile::unit_at(r, unit_of(j));
+                    const int query = (row + r) / group, head = row + r - query * group;
+                    if (unit < s.units) off[j] = 2 * (uint32_t)((query - row / group) * s.n + head * s.h + 8 * unit);
                 }
+            }
+            uint32_t at_unit[COUNT];
+            if (masked) {
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t)
-                    attn_bring<16>(mine ? (const void *)(from[j] + t * s.plane) : (const void *)attn_fill,
-                                   tile.base + t * Tile::PLANE + 8 * (j * kThreads + (threadIdx.x & ~(PCCNN_WAVE - 1))));
-                from[j] += step;
+                for (int j = 0; j < COUNT; ++j) at_unit[j] = (live >> row_of(j)) & 1 ? off[j] : kAttnNowhere;
             } else {
+#pragma unroll
+                for (int j = 0; j < COUNT; ++j) at_unit[j] = row_of(j) < limit - row ? off[j] : kAttnNowhere;
+            }
+            const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+                const __amdgpu_buffer_rsrc_t window = attn_window(base + 2 * t * s.plane);
+#pragma unroll
+                for (int j = 0; j < COUNT; ++j)
+                    attn_bring(window, at_unit[j], tile.base + t * Tile::PLANE + 8 * (j * kThreads + wave_unit));
+            }
+            base += step;
+        } else {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j) {
                 attn_clear(held[j]);
                 if (row + row_of(j) < limit)
-                    attn_load(held[j], (const T *)s.p + base + offset(s, group, row + row_of(j)), 8 * unit_of(j), width,
+                    attn_load(held[j], (const T *)s.p + at + offset(s, group, row + row_of(j)), 8 * unit_of(j), width,
                               s.wide);
             }
         }
@@ -276,8 +296,8 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     if (key < end) {
         flag = key_flag(a, b, key, lane);
         live = live_keys(a, b, key, flag, ROWS);
-        k.fetch(a.one, k_at, 1, key, b.keys, live, a.width, Tile{lds});
-        v.fetch(a.two, v_at, 1, key, b.keys, live, a.width, Tile{lds + Tile::ELEMENTS});
+        k.fetch(a.one, k_at, 1, key, b.keys, live, a.mask != nullptr, a.width, Tile{lds});
+        v.fetch(a.two, v_at, 1, key, b.keys, live, a.mask != nullptr, a.width, Tile{lds + Tile::ELEMENTS});
         flag = key_flag(a, b, key + ROWS, lane);
     }
     AttnFrag<TERMS> q[DP / 16];
@@ -302,8 +322,8 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
         }
         if (key + ROWS < end) {
             live = live_keys(a, b, key + ROWS, flag, ROWS);
-            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.width, next_k);
-            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.width, next_v);
+            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_k);
+            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_v);
             flag = key_flag(a, b, key + 2 * ROWS, lane);
         }
         if (!working || now == 0) continue;
@@ -477,8 +497,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     if (key < end) {
         flag = key_flag(a, b, key, lane);
         live = live_keys(a, b, key, flag, ROWS);
-        k.fetch(a.one, k_at, 1, key, b.keys, live, a.width, Tile{lds});
-        v.fetch(a.two, v_at, 1, key, b.keys, live, a.width, Tile{lds + Tile::ELEMENTS});
+        k.fetch(a.one, k_at, 1, key, b.keys, live, a.mask != nullptr, a.width, Tile{lds});
+        v.fetch(a.two, v_at, 1, key, b.keys, live, a.mask != nullptr, a.width, Tile{lds + Tile::ELEMENTS});
         flag = key_flag(a, b, key + ROWS, lane);
     }
     const bool real = row < b.rows;
@@ -506,8 +526,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
         }
         if (key + ROWS < end) {
             live = live_keys(a, b, key + ROWS, flag, ROWS);
-            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.width, next_k);
-            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.width, next_v);
+            k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_k);
+            v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_v);
             flag = key_flag(a, b, key + 2 * ROWS, lane);
         }
         if (!working || now == 0) continue;
@@ -568,19 +588,20 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
     Feed q, g;
     q.start(a.one, q_at, a.group, row);
     g.start(a.two, g_at, a.group, row);
-    // shifts and deltas of the tile's rows go to LDS the same way, one wavefront each
-    auto fetch_stats = [&](int from, int stage) {
+    // shifts and deltas of the tile's rows, one wavefront each; they pass through a register, since LDS that the compiler
+    // knows to be filled behind its back would make it wait for all that is on its way
+    float stat = 0.0f;
+    auto fetch_stats = [&](int from) {
         if (wave < 2) {
-            const float *src = (wave == 0 ? a.shift : a.delta) + b.stat(a, from + lane);
-            attn_bring<4>(from + lane < b.rows ? (const void *)src : (const void *)(attn_fill + (wave == 0 ? 4 : 0)),
-                          stats + (stage * 2 + wave) * 64);
+            stat = wave == 0 ? INFINITY : 0.0f;
+            if (from + lane < b.rows) stat = (wave == 0 ? a.shift : a.delta)[b.stat(a, from + lane)];
         }
     };
     if (row < end) {
         const uint64_t bits = first_bits(b.rows - row, ROWS);
-        q.fetch(a.one, q_at, a.group, row, b.rows, bits, a.width, Tile{lds});
-        g.fetch(a.two, g_at, a.group, row, b.rows, bits, a.width, Tile{lds + Tile::ELEMENTS});
-        fetch_stats(row, 0);
+        q.fetch(a.one, q_at, a.group, row, b.rows, bits, false, a.width, Tile{lds});
+        g.fetch(a.two, g_at, a.group, row, b.rows, bits, false, a.width, Tile{lds + Tile::ELEMENTS});
+        fetch_stats(row);
     }
     AttnFrag<TERMS> k[DP / 16], v[DP / 16];
     own_side<T, DP>(k, a.k, (b.k0 + key) * a.k_n + b.head * a.k_h, live, half, a.width, a.wide_k);
@@ -600,12 +621,13 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
             q.put(tile_q, bits);
             g.put(tile_g, bits);
         }
+        if (wave < 2) stats[(stage * 2 + wave) * 64 + lane] = stat;
         attn_landed();
         if (row + ROWS < end) {
             const uint64_t bits = first_bits(b.rows - row - ROWS, ROWS);
-            q.fetch(a.one, q_at, a.group, row + ROWS, b.rows, bits, a.width, next_q);
-            g.fetch(a.two, g_at, a.group, row + ROWS, b.rows, bits, a.width, next_g);
-            fetch_stats(row + ROWS, stage ^ 1);
+            fetch_stats(row + ROWS);
+            q.fetch(a.one, q_at, a.group, row + ROWS, b.rows, bits, false, a.width, next_q);
+            g.fetch(a.two, g_at, a.group, row + ROWS, b.rows, bits, false, a.width, next_g);
         }
         if (!working) continue;
 #pragma unroll
@@ -737,8 +759,12 @@ AttnArgs attn_args(const pccnn_attention *p)
     return a;
 }
 
-// Whether a tensor's rows go to LDS as they are: bf16, whole 16-byte units, 16-byte rows.
-bool attn_direct(int type, int wide_one, int wide_two) { return type == PCCNN_TYPE_BF16 && wide_one == 2 && wide_two == 2; }
+// Whether the walked side goes to LDS as it is: bf16, whole 16-byte units, 16-byte rows, 32-bit offsets within a tile.
+bool attn_direct(int type, const AttnStream &one, const AttnStream &two)
+{
+    const int64_t reach = 64 * (std::max(one.n, two.n) + std::max(one.h, two.h)) + kMaxWidth;     // offsets within a tile
+    return type == PCCNN_TYPE_BF16 && one.wide == 2 && two.wide == 2 && reach < (1ll << 30);
+}
 
 // Calls f(type, padded width) for the instantiation that serves this type and head width.
 template <typename F> int attn_dispatch(int type, int width, F f)
@@ -843,7 +869,7 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
         using T = decltype(zero);
         constexpr int DP = decltype(dp)::value;
         int rc;
-        if (attn_direct(p->type, a.wide_k, a.wide_v)) {
+        if (attn_direct(p->type, a.one, a.two)) {
             if constexpr (sizeof(T) == 2)
                 rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
         } else {
@@ -914,7 +940,7 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
                 PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE,
                               "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
             }
-            if (attn_direct(p->type, a.wide_k, a.wide_v)) {
+            if (attn_direct(p->type, a.one, a.two)) {
                 if constexpr (sizeof(T) == 2)
                     rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
             } else {
@@ -937,7 +963,7 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
                               "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
             }
             const size_t bytes = tiles_bytes<T, DP>() + 4 * 64 * sizeof(float);
-            if (attn_direct(p->type, a.wide_q, a.wide_g)) {
+            if (attn_direct(p->type, a.one, a.two)) {
                 if constexpr (sizeof(T) == 2)
                     rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP, true>, a, bytes, s);
             } else {

@@ -186,19 +186,18 @@ template <int TERMS, int ROWS, int DP> struct AttnTile {
     }
 };
 
-// What lanes without a row of their own bring into LDS: zeros, and for a row's shift plus infinity.
-__device__ const uint32_t attn_fill[8] = {0u, 0u, 0u, 0u, 0x7f800000u, 0u, 0u, 0u};
-
-// Memory to LDS without a register between: lane i's `bytes` (4 or 16) from its own address to `lds` + i * bytes, `lds`
-// the same in all lanes.  Lands by the next wait for vector memory (attn_landed).
-template <int BYTES> __device__ __forceinline__ void attn_bring(const void *from, void *lds)
+// A window on memory from `base` (the same in all lanes) for range-checked loads: an offset past 2^31 bytes reads zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_window(const void *base)
 {
-    typedef const __attribute__((address_space(1))) uint32_t *global_ptr;
-    typedef __attribute__((address_space(3))) uint32_t *lds_ptr;
-    if constexpr (BYTES == 16)
-        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)lds, 16, 0, 0);
-    else
-        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)lds, 4, 0, 0);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, 0x00027000);
+}
+constexpr uint32_t kAttnNowhere = 0xfffffff0u;       // an offset past every window
+// Memory to LDS without a register between: 16 bytes per lane, from its own offset in the window to `lds` + 16 * lane,
+// `lds` the same in all lanes.  Lands by the next wait for vector memory (attn_landed).
+__device__ __forceinline__ void attn_bring(__amdgpu_buffer_rsrc_t window, uint32_t offset, void *lds)
+{
+    typedef __attribute__((address_space(3))) void *lds_ptr;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(window, (lds_ptr)lds, 16, offset, 0, 0, 0);
 }
 // Everything this wavefront brought has landed; with the barrier behind it, everything the workgroup brought.
 __device__ __forceinline__ void attn_landed()
