@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     constexpr int TERMS = AttnTerms<T>::value;
     typedef Feeder<T, DP, DIRECT, false> Feed;
     typedef typename Feed::Tile Tile;
-    constexpr int ROWS = Feed::ROWS;
+    constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
     const AttnBlock b(a, blockIdx.x);
     if (b.tile * kOwn >= b.rows) return;
@@ -329,12 +329,15 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
         if (!working || now == 0) continue;
         pccnn_f32x16 s[ROWS / 32];
 #pragma unroll
-        for (int t = 0; t < ROWS / 32; ++t) {
-            clear(s[t]);
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk)
-                attn_mma<TERMS>(s[t], tile_k.rows(32 * t + (lane & 31), 2 * kk + half), q[kk]);
-        }
+        for (int t = 0; t < ROWS / 32; ++t) clear(s[t]);
+        AttnAhead<TERMS> ahead;
+        auto key_rows = [&](int i) { return tile_k.rows(32 * (i / STEPS) + (lane & 31), 2 * (i % STEPS) + half); };
+        ahead.template prime<ROWS / 32 * STEPS>(key_rows);
+        ahead.template run<ROWS / 32 * STEPS>(key_rows, [&](int i, const AttnFrag<TERMS> &f) {
+            attn_mma<TERMS>(s[i / STEPS], f, q[i % STEPS]);
+        });
+        auto value_columns = [&](int i) { return tile_v.columns(16 * (i / BLOCKS), 32 * (i % BLOCKS), lane); };
+        ahead.template prime<ROWS / 16 * BLOCKS>(value_columns);
         if (now != first_bits(ROWS, ROWS))
 #pragma unroll
             for (int t = 0; t < ROWS / 32; ++t) hide(s[t], (uint32_t)(now >> (32 * t)), half);
@@ -355,23 +358,22 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
                 for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
         }
         const float shift = top == -INFINITY ? 0.0f : top;
+        AttnFrag<TERMS> p;
+        ahead.template run<ROWS / 16 * BLOCKS>(value_columns, [&](int i, const AttnFrag<TERMS> &f) {
+            if (i % BLOCKS == 0) {                                   // the next sixteen keys' probabilities
+                pccnn_f32x16 &x = s[i / BLOCKS / 2];
+                const int from = 8 * (i / BLOCKS % 2);
+                float sums[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < ROWS / 32; ++t) {
-            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c2, -shift));
-                sums[i % 4] += s[t][i];
+                for (int j = from; j < from + 8; ++j) {
+                    x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c2, -shift));
+                    sums[j % 2] += x[j];
+                }
+                sum += sums[0] + sums[1];
+                p = half_of<TERMS>(x, i / BLOCKS % 2);
             }
-            sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const AttnFrag<TERMS> p = half_of<TERMS>(s[t], g);
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt)
-                    attn_mma<TERMS>(acc[dt], tile_v.columns(32 * t + 16 * g, 32 * dt, lane), p);
-            }
-        }
+            attn_mma<TERMS>(acc[i % BLOCKS], f, p);
+        });
     }
     sum = pccnn_add_row_xor32(sum);
     if (row >= b.rows) return;
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     constexpr int TERMS = AttnTerms<T>::value;
     typedef Feeder<T, DP, DIRECT, false> Feed;
     typedef typename Feed::Tile Tile;
-    constexpr int ROWS = Feed::ROWS;
+    constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
     const AttnBlock b(a, blockIdx.x);
     if (b.tile * kOwn >= b.rows) return;
@@ -536,22 +538,29 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
             pccnn_f32x16 s, dp;
             clear(s);
             clear(dp);
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-                attn_mma<TERMS>(s, tile_k.rows(32 * t + (lane & 31), 2 * kk + half), q[kk]);
-                attn_mma<TERMS>(dp, tile_v.rows(32 * t + (lane & 31), 2 * kk + half), g[kk]);
-            }
+            AttnAhead<TERMS> ahead;
+            auto rows = [&](int i) { return (i < STEPS ? tile_k : tile_v).rows(32 * t + (lane & 31), 2 * (i % STEPS) + half); };
+            ahead.template prime<2 * STEPS>(rows);
+            ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
+                if (i < STEPS)
+                    attn_mma<TERMS>(s, f, q[i]);
+                else
+                    attn_mma<TERMS>(dp, f, g[i - STEPS]);
+            });
+            auto columns = [&](int i) { return tile_k.columns(32 * t + 16 * (i / BLOCKS), 32 * (i % BLOCKS), lane); };
+            ahead.template prime<2 * BLOCKS>(columns);
             if (now != first_bits(ROWS, ROWS)) hide(s, (uint32_t)(now >> (32 * t)), half);
+            AttnFrag<TERMS> ds;
+            ahead.template run<2 * BLOCKS>(columns, [&](int i, const AttnFrag<TERMS> &f) {
+                if (i % BLOCKS == 0) {
+                    const int from = 8 * (i / BLOCKS);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -shift)) * (dp[i] - delta);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const AttnFrag<TERMS> ds = half_of<TERMS>(s, h);
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt)
-                    attn_mma<TERMS>(acc[dt], tile_k.columns(32 * t + 16 * h, 32 * dt, lane), ds);
-            }
+                    for (int j = from; j < from + 8; ++j)
+                        s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -shift)) * (dp[j] - delta);
+                    ds = half_of<TERMS>(s, i / BLOCKS);
+                }
+                attn_mma<TERMS>(acc[i % BLOCKS], f, ds);
+            });
         }
     }
     if (!real) return;
@@ -572,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
     constexpr int TERMS = AttnTerms<T>::value;
     typedef Feeder<T, DP, DIRECT, true> Feed;
     typedef typename Feed::Tile Tile;
-    constexpr int ROWS = Feed::ROWS;
+    constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
     float *const stats = (float *)(lds + 4 * Tile::ELEMENTS);        // [stage][shift, delta][64]
     const AttnBlock b(a, blockIdx.x);
@@ -635,31 +644,43 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
             pccnn_f32x16 s, dp;
             clear(s);
             clear(dp);
+            AttnAhead<TERMS> ahead;
+            auto rows = [&](int i) { return (i < STEPS ? tile_q : tile_g).rows(32 * t + (lane & 31), 2 * (i % STEPS) + half); };
+            ahead.template prime<2 * STEPS>(rows);
+            ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
+                if (i < STEPS)
+                    attn_mma<TERMS>(s, f, k[i]);
+                else
+                    attn_mma<TERMS>(dp, f, v[i - STEPS]);
+            });
+            // sixteen rows at a time: first the output gradients' columns (dv), then the queries' (dk)
+            auto columns = [&](int i) {
+                return (i / BLOCKS % 2 == 0 ? tile_g : tile_q).columns(32 * t + 16 * (i / BLOCKS / 2), 32 * (i % BLOCKS), lane);
+            };
+            ahead.template prime<4 * BLOCKS>(columns);
+            AttnFrag<TERMS> p, ds;
+            ahead.template run<4 * BLOCKS>(columns, [&](int i, const AttnFrag<TERMS> &f) {
+                if (i % (2 * BLOCKS) == 0) {
+                    const int h = i / BLOCKS / 2;
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-                attn_mma<TERMS>(s, tile_q.rows(32 * t + (lane & 31), 2 * kk + half), k[kk]);
-                attn_mma<TERMS>(dp, tile_g.rows(32 * t + (lane & 31), 2 * kk + half), v[kk]);
-            }
+                    for (int n = 2 * h; n < 2 * h + 2; ++n) {
+                        const float4 shift = *(const float4 *)(stats + stage * 128 + 32 * t + 8 * n + 4 * half);
+                        const float4 delta = *(const float4 *)(stats + stage * 128 + 64 + 32 * t + 8 * n + 4 * half);
+                        const float sh[4] = {shift.x, shift.y, shift.z, shift.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 shift = *(const float4 *)(stats + stage * 128 + 32 * t + 8 * i + 4 * half);
-                const float4 delta = *(const float4 *)(stats + stage * 128 + 64 + 32 * t + 8 * i + 4 * half);
-                const float sh[4] = {shift.x, shift.y, shift.z, shift.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + j], c2, -sh[j]));
-                    dp[4 * i + j] = s[4 * i + j] * (dp[4 * i + j] - de[j]);
+                        for (int j = 0; j < 4; ++j) {
+                            s[4 * n + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * n + j], c2, -sh[j]));
+                            dp[4 * n + j] = s[4 * n + j] * (dp[4 * n + j] - de[j]);
+                        }
+                    }
+                    p = half_of<TERMS>(s, h);
+                    ds = half_of<TERMS>(dp, h);
                 }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const AttnFrag<TERMS> p = half_of<TERMS>(s, h), ds = half_of<TERMS>(dp, h);
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) {
-                    attn_mma<TERMS>(dv[dt], tile_g.columns(32 * t + 16 * h, 32 * dt, lane), p);
-                    attn_mma<TERMS>(dk[dt], tile_q.columns(32 * t + 16 * h, 32 * dt, lane), ds);
-                }
-            }
+                if (i / BLOCKS % 2 == 0)
+                    attn_mma<TERMS>(dv[i % BLOCKS], f, p);
+                else
+                    attn_mma<TERMS>(dk[i % BLOCKS], f, ds);
+            });
         }
     }
     if (key >= b.keys) return;
@@ -767,7 +788,7 @@ bool attn_direct(int type, const AttnStream &one, const AttnStream &two)
 }
 
 // Calls f(type, padded width) for the instantiation that serves this type and head width.
-template <typename F> int attn_dispatch(int type, int width, F f)
+template <typename F> auto attn_dispatch(int type, int width, F f)
 {
     auto by_width = [&](auto zero) {
         if (width <= 32) return f(zero, std::integral_constant<int, 32>());
@@ -778,51 +799,114 @@ template <typename F> int attn_dispatch(int type, int width, F f)
     return type == PCCNN_TYPE_F32 ? by_width(0.0f) : by_width((uint16_t)0);
 }
 
-constexpr int64_t kWantedBlocks = 1024;      // workgroups that fill the chip (four per CU)
-constexpr int kLeastTiles = 4;               // tiles below which a part is not worth its join
-
-// Tiles of the own side, and the parts the other side is cut into so that few own tiles still fill the chip.
-void attn_plan(AttnArgs &a, int type, int64_t own, int64_t other)
+// Workgroups of a kernel that are on the chip at once.
+template <typename KERNEL> int attn_slots(KERNEL kernel, size_t lds)
 {
-    const int rows = attn_dispatch(type, a.width, [](auto zero, auto dp) -> int {
-        return attn_tile_rows<decltype(zero), decltype(dp)::value>();
-    });
-    a.tiles = (int)std::max<int64_t>(1, pccnn_ceil_div(own, kOwn));
-    const int64_t base = (int64_t)a.tiles * a.key_heads * a.clouds, tiles = std::max<int64_t>(1, pccnn_ceil_div(other, rows));
-    int64_t splits = std::max<int64_t>(1, std::min(kWantedBlocks / base, tiles / kLeastTiles));
-    a.per_split = (int)pccnn_ceil_div(tiles, splits);
-    a.splits = (int)pccnn_ceil_div(tiles, a.per_split);
+    int device = 0, cus = 0, per_cu = 0;
+    if (hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, (const void *)kernel, kThreads, lds) != hipSuccess ||
+        cus < 1 || per_cu < 1) {
+        (void)hipGetLastError();
+        return 512;                          // no device to ask: two per CU
+    }
+    return cus * per_cu;
 }
-void attn_plan_rows(AttnArgs &a, const pccnn_attention *p) 
+enum AttnPass { ATTN_FORWARD, ATTN_QUERIES, ATTN_KEYS };
+
+// The kernel of a pass, its LDS and the workgroups that are resident at once (asked once).
+struct AttnKernel {
+    void (*run)(AttnArgs);
+    size_t lds;
+    int slots, rows;
+};
+template <typename T, int DP, bool DIRECT, AttnPass PASS> AttnKernel attn_kernel()
 {
-    attn_plan(a, p->type, p->max_queries * a.group, p->max_keys);
+    AttnKernel k;
+    if constexpr (PASS == ATTN_FORWARD) k.run = attention_fwd_kernel<T, DP, DIRECT>;
+    if constexpr (PASS == ATTN_QUERIES) k.run = attention_dq_kernel<T, DP, DIRECT>;
+    if constexpr (PASS == ATTN_KEYS) k.run = attention_dkv_kernel<T, DP, DIRECT>;
+    k.rows = attn_tile_rows<T, DP>();
+    // two tiles of two tensors, and the backward rows' statistics
+    k.lds = 4 * 2 * (size_t)AttnTile<AttnTerms<T>::value, attn_tile_rows<T, DP>(), DP>::ELEMENTS +
+            (PASS == ATTN_KEYS ? 4 * 64 * sizeof(float) : 0);
+    static const int slots = attn_slots(k.run, k.lds);
+    k.slots = slots;
+    return k;
+}
+template <AttnPass PASS> AttnKernel attn_kernel_of(int type, int width, bool direct)
+{
+    return attn_dispatch(type, width, [&](auto zero, auto dp) -> AttnKernel {
+        using T = decltype(zero);
+        constexpr int DP = decltype(dp)::value;
+        if constexpr (sizeof(T) == 2)
+            if (direct) return attn_kernel<T, DP, true, PASS>();
+        return attn_kernel<T, DP, false, PASS>();
+    });
+}
+
+// Into how many parts the other side is cut.  More parts even out the last round of workgroups (1068 tiles on 512 places
+// take three rounds where 2.1 would do) and fill the chip when there are few tiles, but each part writes its sums in f32
+// and they are read again by the join.  The estimate below (microseconds) weighs the two: a tile of the other side costs a
+// place its share of 900 TFLOP/s of bf16 products (six per product in f32) or of 5 TB/s, whichever is longer; parts cost
+// their bytes at 4 TB/s and a launch.
+void attn_plan(AttnArgs &a, const AttnKernel &kernel, int type, int products, int64_t own, int64_t own_all, int64_t other,
+               int64_t other_all)
+{
+    const double terms = type == PCCNN_TYPE_F32 ? 6.0 : 1.0, padded = (a.width + 31) / 32 * 32.0;
+    const double unit = kernel.slots * std::max(2.0 * products * kOwn * kernel.rows * padded * terms / 900e6,
+                                                2.0 * kernel.rows * a.width * pccnn_type_bytes(type) / 5e6);
+    const double result = (double)own_all * a.key_heads * a.width * 4 * (products == 4 ? 2 : 1);     // bytes of one part
+    a.tiles = (int)std::max<int64_t>(1, pccnn_ceil_div(own, kOwn));
+    const int64_t tiles = std::max<int64_t>(1, pccnn_ceil_div(other, kernel.rows));
+    // workgroups that have work, and the tiles a mean one walks (clouds differ in size)
+    const double mean_own = (double)own_all / a.clouds, mean_other = (double)other_all / a.clouds;
+    const double groups = a.key_heads * (double)a.clouds * std::min<double>(a.tiles, mean_own / kOwn + 0.5);
+    const double mean_tiles = std::min<double>((double)tiles, mean_other / kernel.rows + 0.5);
+    double best = 1e300;
+    for (int64_t s = 1; s <= tiles; s += s < 8 ? 1 : s / 4) {
+        const int64_t per = pccnn_ceil_div(tiles, s), parts = pccnn_ceil_div(tiles, per);
+        const double work = groups * (mean_tiles + 2.0 * std::min<double>((double)parts, mean_tiles / per + 1.0));
+        const double rounds = std::ceil(groups * parts / kernel.slots - 0.01) * (std::min<double>((double)per, mean_tiles) + 2.0);
+        const double cost = unit * std::max(rounds, work / kernel.slots + 0.5 * per) +
+                            (parts > 1 ? 6.0 + 2.0 * parts * result / 4e6 : 0.0);
+        if (cost < best) {
+            best = cost;
+            a.per_split = (int)per;
+            a.splits = (int)parts;
+        }
+    }
+}
+// The three passes: which side is walked, by which kernel, in how many parts.
+AttnKernel attn_plan_rows(AttnArgs &a, const pccnn_attention *p, bool forward)
+{
     a.one = {a.k, a.k_n, a.k_h, 0, a.wide_k, a.width / 8};
     a.two = {a.v, a.v_n, a.v_h, 0, a.wide_v, a.width / 8};
+    const bool direct = attn_direct(p->type, a.one, a.two);
+    const AttnKernel kernel = forward ? attn_kernel_of<ATTN_FORWARD>(p->type, a.width, direct)
+                                      : attn_kernel_of<ATTN_QUERIES>(p->type, a.width, direct);
+    attn_plan(a, kernel, p->type, forward ? 2 : 3, p->max_queries * a.group, p->m * a.group, p->max_keys, p->n);
+    return kernel;
 }
-void attn_plan_keys(AttnArgs &a, const pccnn_attention *p) 
+AttnKernel attn_plan_keys(AttnArgs &a, const pccnn_attention *p, bool direct)
 {
-    attn_plan(a, p->type, p->max_keys, p->max_queries * a.group);
-    a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
-    a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
+    const AttnKernel kernel = attn_kernel_of<ATTN_KEYS>(p->type, a.width, direct);
+    attn_plan(a, kernel, p->type, 4, p->max_keys, p->n, p->max_queries * a.group, p->m * a.group);
+    return kernel;
 }
 
 int64_t attn_blocks(const AttnArgs &a) { return (int64_t)a.tiles * a.splits * a.key_heads * a.clouds; }
 
-template <typename KERNEL> int attn_launch(const char *name, KERNEL kernel, const AttnArgs &a, size_t lds, hipStream_t s)
+int attn_launch(const char *name, const AttnKernel &kernel, const AttnArgs &a, hipStream_t s)
 {
     const int64_t blocks = attn_blocks(a);
     PCCNN_REQUIRE(blocks <= INT32_MAX, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
-    if (lds > 65536)
-        PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    kernel<<<(unsigned)blocks, kThreads, lds, s>>>(a);
+    if (kernel.lds > 65536)
+        PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel.run, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)kernel.lds));
+    kernel.run<<<(unsigned)blocks, kThreads, kernel.lds, s>>>(a);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
-}
-
-// LDS of the kernels: two tiles of two tensors.
-template <typename T, int DP> constexpr size_t tiles_bytes()
-{
-    return 4 * 2 * (size_t)AttnTile<AttnTerms<T>::value, attn_tile_rows<T, DP>(), DP>::ELEMENTS;
 }
 
 size_t forward_bytes(const AttnArgs &a)
@@ -838,18 +922,22 @@ extern "C" size_t pccnn_attention_workspace_bytes(const pccnn_attention *p, int 
 {
     if (p == nullptr || p->heads < 1 || p->key_heads < 1 || p->clouds < 1 || p->m < 0 || p->n < 0) return 256;
     AttnArgs a = attn_args(p);
-    attn_plan_rows(a, p);
+    attn_plan_rows(a, p, !backward);
     if (!backward) return std::max<size_t>(256, forward_bytes(a));
-    size_t rows = a.splits > 1 ? pccnn_align((size_t)a.splits * a.m * a.heads * a.width * sizeof(float)) : 0;
-    attn_plan_keys(a, p);
-    size_t keys = a.splits > 1 ? 2 * pccnn_align((size_t)a.splits * a.n * a.key_heads * a.width * sizeof(float)) : 0;
+    const size_t rows = a.splits > 1 ? pccnn_align((size_t)a.splits * a.m * a.heads * a.width * sizeof(float)) : 0;
+    size_t keys = 0;
+    for (bool direct : {false, true}) {              // which one the gradient's layout allows is not known here
+        attn_plan_keys(a, p, direct);
+        if (a.splits > 1)
+            keys = std::max(keys, 2 * pccnn_align((size_t)a.splits * a.n * a.key_heads * a.width * sizeof(float)));
+    }
     return 256 + 2 * pccnn_align((size_t)a.m * a.heads * sizeof(float)) + std::max(rows, keys);
 }
 
 extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, float *lse_out, void *workspace,
                                        size_t workspace_bytes, void *stream)
 {
-    const int rc = attn_check("cross_attention", p);
+    int rc = attn_check("cross_attention", p);
     if (rc != PCCNN_OK) return rc;
     if (p->m == 0 || p->clouds == 0) return PCCNN_OK;
     PCCNN_REQUIRE(out != nullptr, PCCNN_ERR_INVALID, "cross_attention: null pointer");
@@ -857,7 +945,7 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
     AttnArgs a = attn_args(p);
     a.out = out;
     a.lse = lse_out;
-    attn_plan_rows(a, p);
+    const AttnKernel kernel = attn_plan_rows(a, p, true);
     if (a.splits > 1) {
         PccnnArena arena(workspace, workspace_bytes);
         a.part = arena.take<float>((size_t)a.splits * a.m * a.heads * a.width);
@@ -865,117 +953,109 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention: workspace of %zu bytes is too small",
                       workspace_bytes);
     }
-    return attn_dispatch(p->type, p->width, [&](auto zero, auto dp) -> int {
+    rc = attn_launch("cross_attention", kernel, a, s);
+    if (rc != PCCNN_OK || a.splits == 1) return rc;
+    // a wavefront to a result up to 32 parts, a workgroup beyond
+    int lanes = 1;
+    while (4 * lanes < a.width) lanes *= 2;
+    auto join = [&](auto zero) {
         using T = decltype(zero);
-        constexpr int DP = decltype(dp)::value;
-        int rc;
-        if (attn_direct(p->type, a.one, a.two)) {
-            if constexpr (sizeof(T) == 2)
-                rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
-        } else {
-            rc = attn_launch("cross_attention", attention_fwd_kernel<T, DP, false>, a, tiles_bytes<T, DP>(), s);
-        }
-        if (rc != PCCNN_OK || a.splits == 1) return rc;
-        // a wavefront to a result up to 32 parts, a workgroup beyond
-        int lanes = 1;
-        while (4 * lanes < a.width) lanes *= 2;
         if (a.splits <= 32)
             attention_join_kernel<T, 64><<<(unsigned)pccnn_ceil_div(a.m * a.heads, 4), kThreads, 0, s>>>(a, lanes);
         else
             attention_join_kernel<T, 256><<<(unsigned)(a.m * a.heads), kThreads, 0, s>>>(a, lanes);
-        PCCNN_LAUNCH_CHECK();
-        return PCCNN_OK;
-    });
+    };
+    if (p->type == PCCNN_TYPE_F32)
+        join(0.0f);
+    else
+        join((uint16_t)0);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
 }
 
 extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *out, const float *lse, const void *in_grads,
                                         int64_t grads_stride_n, int64_t grads_stride_h, void *d_queries, void *d_keys,
                                         void *d_values, void *workspace, size_t workspace_bytes, void *stream)
 {
-    int rc = attn_check("cross_attention_grads", p);
+    const char *name = "cross_attention_grads";
+    int rc = attn_check(name, p);
     if (rc != PCCNN_OK) return rc;
-    PCCNN_REQUIRE(grads_stride_n >= 0 && grads_stride_h >= 0, PCCNN_ERR_INVALID, "cross_attention_grads: a negative stride");
+    PCCNN_REQUIRE(grads_stride_n >= 0 && grads_stride_h >= 0, PCCNN_ERR_INVALID, "%s: a negative stride", name);
     PCCNN_REQUIRE((d_keys != nullptr) == (d_values != nullptr), PCCNN_ERR_INVALID,
-                  "cross_attention_grads: the gradients of keys and values come together");
+                  "%s: the gradients of keys and values come together", name);
     if (p->clouds == 0 || (d_queries == nullptr && d_keys == nullptr)) return PCCNN_OK;
-    PCCNN_REQUIRE(p->m == 0 || (out && lse && in_grads), PCCNN_ERR_INVALID, "cross_attention_grads: null pointer");
+    PCCNN_REQUIRE(p->m == 0 || (out && lse && in_grads), PCCNN_ERR_INVALID, "%s: null pointer", name);
     const hipStream_t s = (hipStream_t)stream;
     AttnArgs a = attn_args(p);
     a.g = in_grads;
     a.g_n = grads_stride_n;
     a.g_h = grads_stride_h;
     a.wide_g = attn_wide(a.g, a.g_n, a.g_h, p->type, a.width);
+    a.wide_o = attn_wide(out, a.width, a.width, p->type, a.width);
     a.lse = (float *)lse;
     PccnnArena arena(workspace, workspace_bytes);
-    a.wide_o = attn_wide(out, a.width, a.width, p->type, a.width);
-    a.shift = arena.take<float>((size_t)p->m * p->heads);
-    a.delta = arena.take<float>((size_t)p->m * p->heads);
-    const size_t after = arena.used;
-    return attn_dispatch(p->type, p->width, [&](auto zero, auto dp) -> int {
-        using T = decltype(zero);
-        constexpr int DP = decltype(dp)::value;
-        int rc = PCCNN_OK;
-        auto sum_parts = [&](const float *part, int64_t count, void *to) {
-            if (count % 4 == 0)
-                attention_sum_kernel<T, 4><<<(unsigned)pccnn_ceil_div(count, 4 * kThreads), kThreads, 0, s>>>(part, a.splits,
-                                                                                                          count, (T *)to);
-            else
-                attention_sum_kernel<T, 1><<<(unsigned)pccnn_ceil_div(count, kThreads), kThreads, 0, s>>>(part, a.splits,
-                                                                                                      count, (T *)to);
-        };
-        if (p->m > 0) {
-            PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention_grads: workspace of %zu bytes is too small",
-                          workspace_bytes);
-            const int64_t threads = a.m * a.heads * 8;
-            attention_rows_kernel<T><<<(unsigned)pccnn_ceil_div(threads, kThreads), kThreads, 0, s>>>(a, (const T *)out);
-            PCCNN_LAUNCH_CHECK();
-        }
-        if (d_queries != nullptr && p->m > 0) {
-            attn_plan_rows(a, p);
-            a.out = d_queries;
-            const int64_t count = a.m * a.heads * a.width;
-            arena.used = after;
-            if (a.splits > 1) {
-                a.part = arena.take<float>((size_t)a.splits * count);
-                PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE,
-                              "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
-            }
-            if (attn_direct(p->type, a.one, a.two)) {
-                if constexpr (sizeof(T) == 2)
-                    rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP, true>, a, tiles_bytes<T, DP>(), s);
-            } else {
-                rc = attn_launch("cross_attention_grads", attention_dq_kernel<T, DP, false>, a, tiles_bytes<T, DP>(), s);
-            }
-            if (rc != PCCNN_OK) return rc;
-            if (a.splits > 1) sum_parts(a.part, count, d_queries);
-            PCCNN_LAUNCH_CHECK();
-        }
-        if (d_keys != nullptr && p->n > 0) {
-            attn_plan_keys(a, p);
-            a.d_k = d_keys;
-            a.d_v = d_values;
-            const int64_t count = a.n * a.key_heads * a.width;
-            arena.used = after;
-            if (a.splits > 1) {
-                a.part = arena.take<float>((size_t)a.splits * count);
-                a.part_v = arena.take<float>((size_t)a.splits * count);
-                PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE,
-                              "cross_attention_grads: workspace of %zu bytes is too small", workspace_bytes);
-            }
-            const size_t bytes = tiles_bytes<T, DP>() + 4 * 64 * sizeof(float);
-            if (attn_direct(p->type, a.one, a.two)) {
-                if constexpr (sizeof(T) == 2)
-                    rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP, true>, a, bytes, s);
-            } else {
-                rc = attn_launch("cross_attention_grads", attention_dkv_kernel<T, DP, false>, a, bytes, s);
-            }
-            if (rc != PCCNN_OK) return rc;
-            if (a.splits > 1) {
-                sum_parts(a.part, count, d_keys);
-                sum_parts(a.part_v, count, d_values);
-            }
-            PCCNN_LAUNCH_CHECK();
-        }
+    auto in_workspace = [&]() -> int {
+        PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
         return PCCNN_OK;
-    });
+    };
+    auto sum_parts = [&](const float *part, int64_t count, void *to) {
+        auto sum = [&](auto zero) {
+            using T = decltype(zero);
+            if (count % 4 == 0)
+                attention_sum_kernel<T, 4><<<(unsigned)pccnn_ceil_div(count, 4 * kThreads), kThreads, 0, s>>>(
+                    part, a.splits, count, (T *)to);
+            else
+                attention_sum_kernel<T, 1><<<(unsigned)pccnn_ceil_div(count, kThreads), kThreads, 0, s>>>(
+                    part, a.splits, count, (T *)to);
+        };
+        if (p->type == PCCNN_TYPE_F32)
+            sum(0.0f);
+        else
+            sum((uint16_t)0);
+    };
+    if (p->m > 0) {
+        a.shift = arena.take<float>((size_t)p->m * p->heads);
+        a.delta = arena.take<float>((size_t)p->m * p->heads);
+        if ((rc = in_workspace()) != PCCNN_OK) return rc;
+        const unsigned blocks = (unsigned)pccnn_ceil_div(a.m * a.heads * 8, kThreads);
+        if (p->type == PCCNN_TYPE_F32)
+            attention_rows_kernel<float><<<blocks, kThreads, 0, s>>>(a, (const float *)out);
+        else
+            attention_rows_kernel<uint16_t><<<blocks, kThreads, 0, s>>>(a, (const uint16_t *)out);
+        PCCNN_LAUNCH_CHECK();
+    }
+    const size_t after = arena.used;
+    if (d_queries != nullptr && p->m > 0) {
+        const AttnKernel kernel = attn_plan_rows(a, p, false);
+        const int64_t count = a.m * a.heads * a.width;
+        a.out = d_queries;
+        if (a.splits > 1) a.part = arena.take<float>((size_t)a.splits * count);
+        if ((rc = in_workspace()) != PCCNN_OK) return rc;
+        rc = attn_launch(name, kernel, a, s);
+        if (rc != PCCNN_OK) return rc;
+        if (a.splits > 1) sum_parts(a.part, count, d_queries);
+        PCCNN_LAUNCH_CHECK();
+    }
+    if (d_keys != nullptr && p->n > 0) {
+        a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
+        a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
+        const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(p->type, a.one, a.two));
+        const int64_t count = a.n * a.key_heads * a.width;
+        a.d_k = d_keys;
+        a.d_v = d_values;
+        arena.used = after;
+        if (a.splits > 1) {
+            a.part = arena.take<float>((size_t)a.splits * count);
+            a.part_v = arena.take<float>((size_t)a.splits * count);
+        }
+        if ((rc = in_workspace()) != PCCNN_OK) return rc;
+        rc = attn_launch(name, kernel, a, s);
+        if (rc != PCCNN_OK) return rc;
+        if (a.splits > 1) {
+            sum_parts(a.part, count, d_keys);
+            sum_parts(a.part_v, count, d_values);
+        }
+        PCCNN_LAUNCH_CHECK();
+    }
+    return PCCNN_OK;
 }

@@ -206,6 +206,31 @@ __device__ __forceinline__ void attn_landed()
     __syncthreads();
 }
 
+// Operands are read from LDS a few products ahead of their use: a read takes as long as four products of 32 cycles, and the
+// compiler, left alone, reads each one just before.  `load(i)` is the operand of the i-th of COUNT products, `use(i, f)` the
+// product; the order of reads and products is kept, other instructions may move between them.
+template <int TERMS> struct AttnAhead {
+    static constexpr int DEPTH = TERMS == 3 ? 1 : 4;      // (three terms: six products to an operand)
+    AttnFrag<TERMS> f[DEPTH];
+    template <int COUNT, typename LOAD> __device__ __forceinline__ void prime(LOAD load)
+    {
+#pragma unroll
+        for (int i = 0; i < DEPTH && i < COUNT; ++i) f[i] = load(i);
+        __builtin_amdgcn_sched_barrier(0x6);              // VALU and SALU may cross
+    }
+    template <int COUNT, typename LOAD, typename USE> __device__ __forceinline__ void run(LOAD load, USE use)
+    {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const AttnFrag<TERMS> now = f[i % DEPTH];
+            if (i + DEPTH < COUNT) f[i % DEPTH] = load(i + DEPTH);
+            __builtin_amdgcn_sched_barrier(0x6);
+            use(i, now);
+            __builtin_amdgcn_sched_barrier(0x6);
+        }
+    }
+};
+
 // max(v, v of the lane 32 away)
 __device__ __forceinline__ float attn_max_halves(float v)
 {
