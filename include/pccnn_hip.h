@@ -532,6 +532,8 @@ int pccnn_conv_backward_bf16(const pccnn_basis *basis, const float *pts, const f
  * to those of another.  Features are f32 or bf16 (bit patterns), `type` one of PCCNN_TYPE_*; everything is computed in
  * f32 and a bf16 result is rounded once.  Strides are in elements and not negative; features of a row (of a head) lie
  * one behind the other; results are dense. */
+#define PCCNN_GRAD_QUERIES 64
+#define PCCNN_GRAD_KEYS 128 /* keys and values */
 #define PCCNN_TYPE_F32 0
 #define PCCNN_TYPE_BF16 1
 

@@ -17,6 +17,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
 constexpr int kMaxBlocks = 1024;             // workgroups of the persistent kernels: four per CU, sixteen wavefronts
+// The backward pass has as many wavefronts in half as many workgroups: every one leaves a row of column sums.
+constexpr int kBackThreads = 512, kBackWaves = kBackThreads / PCCNN_WAVE, kBackBlocks = 512;
 constexpr int kRegisterColumns = 2048;       // the longest row that one wavefront holds (32 values per lane)
 
 // ------------------------------------------------------------------------------------ rows in registers
@@ -86,20 +88,23 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const T *__restrict_
     }
 }
 
-// partial: [workgroup][2][c] column sums (dgamma, dbeta), or null when nobody wants them; d_feats null likewise.
+// partial: [workgroup][2][c] column sums (dgamma, dbeta), or null when nobody wants them; d_feats null likewise.  Short rows
+// are worked on two at a time, so that a lane has four loads on their way.
 template <typename T, int VEC, int LANES, int CHUNKS>
-__global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T *__restrict__ feats, int64_t stride,
-                                                           const void *__restrict__ gamma, int weight_type,
-                                                           const float2 *__restrict__ stats,
-                                                           const T *__restrict__ grads, int64_t grads_stride, int64_t n,
-                                                           int c, T *__restrict__ d_feats, float *__restrict__ partial)
+__global__ __launch_bounds__(kBackThreads) void norm_bwd_kernel(const T *__restrict__ feats, int64_t stride,
+                                                               const void *__restrict__ gamma, int weight_type,
+                                                               const float2 *__restrict__ stats,
+                                                               const T *__restrict__ grads, int64_t grads_stride,
+                                                               int64_t n, int c, T *__restrict__ d_feats,
+                                                               float *__restrict__ partial)
 {
     constexpr int ROWS = PCCNN_WAVE / LANES;
     constexpr int COLUMNS = LANES * CHUNKS * VEC;
-    __shared__ float sums[kWaves][COLUMNS];
+    constexpr int PAIR = CHUNKS * VEC <= 8 ? 2 : 1;
+    __shared__ float sums[kBackWaves][COLUMNS];
     const int lane = threadIdx.x % LANES, slot = (threadIdx.x % PCCNN_WAVE) / LANES, wave = threadIdx.x / PCCNN_WAVE;
-    const int64_t first = ((int64_t)blockIdx.x * kWaves + wave) * ROWS;
-    const int64_t step = (int64_t)gridDim.x * kWaves * ROWS;
+    const int64_t first = ((int64_t)blockIdx.x * kBackWaves + wave) * ROWS;
+    const int64_t step = (int64_t)gridDim.x * kBackWaves * ROWS;
     const float inv_c = 1.0f / (float)c;
     float w[CHUNKS][VEC], dg[CHUNKS][VEC], db[CHUNKS][VEC];
 #pragma unroll
@@ -110,46 +115,54 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T *__restrict_
             w[k][i] = col < c ? pccnn_element(gamma, weight_type, col) : 0.0f;
             dg[k][i] = db[k][i] = 0.0f;
         }
-    for (int64_t base = first; base < n; base += step) {
-        const int64_t row = base + slot;
-        const bool live = row < n;
-        const float2 stat = live ? stats[row] : make_float2(0.0f, 0.0f);
-        float x[CHUNKS][VEC], g[CHUNKS][VEC];
+    for (int64_t base = first; base < n; base += PAIR * step) {
+        float x[PAIR][CHUNKS][VEC], g[PAIR][CHUNKS][VEC];
+        float2 stat[PAIR];
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            const int col = (k * LANES + lane) * VEC;
-            if (live && col < c) {
-                pccnn_load<VEC>(feats + row * stride + col, x[k]);
-                pccnn_load<VEC>(grads + row * grads_stride + col, g[k]);
-            } else {
+        for (int u = 0; u < PAIR; ++u) {
+            const int64_t row = base + u * step + slot;
+            const bool live = row < n;
+            stat[u] = live ? stats[row] : make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) { x[k][i] = stat.x; g[k][i] = 0.0f; }
+            for (int k = 0; k < CHUNKS; ++k) {
+                const int col = (k * LANES + lane) * VEC;
+                if (live && col < c) {
+                    pccnn_load<VEC>(feats + row * stride + col, x[u][k]);
+                    pccnn_load<VEC>(grads + row * grads_stride + col, g[u][k]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) { x[u][k][i] = stat[u].x; g[u][k][i] = 0.0f; }
+                }
             }
         }
-        float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
+        for (int u = 0; u < PAIR; ++u) {
+            const int64_t row = base + u * step + slot;
+            float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                x[k][i] = (x[k][i] - stat.x) * stat.y;
-                dg[k][i] = fmaf(g[k][i], x[k][i], dg[k][i]);
-                db[k][i] += g[k][i];
-                g[k][i] *= w[k][i];
-                sum += g[k][i];
-                dot = fmaf(g[k][i], x[k][i], dot);
-            }
-        if (d_feats == nullptr) continue;
-        sum = pccnn_group_sum<LANES>(sum) * inv_c;
-        dot = pccnn_group_sum<LANES>(dot) * inv_c;
-        if (!live) continue;
+            for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            const int col = (k * LANES + lane) * VEC;
-            if (col < c) {
-                float d[VEC];
+                for (int i = 0; i < VEC; ++i) {
+                    x[u][k][i] = (x[u][k][i] - stat[u].x) * stat[u].y;
+                    dg[k][i] = fmaf(g[u][k][i], x[u][k][i], dg[k][i]);
+                    db[k][i] += g[u][k][i];
+                    g[u][k][i] *= w[k][i];
+                    sum += g[u][k][i];
+                    dot = fmaf(g[u][k][i], x[u][k][i], dot);
+                }
+            if (d_feats == nullptr) continue;
+            sum = pccnn_group_sum<LANES>(sum) * inv_c;
+            dot = pccnn_group_sum<LANES>(dot) * inv_c;
+            if (row >= n) continue;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) d[i] = stat.y * (g[k][i] - sum - x[k][i] * dot);
-                pccnn_store<VEC>(d_feats + row * c + col, d);
+            for (int k = 0; k < CHUNKS; ++k) {
+                const int col = (k * LANES + lane) * VEC;
+                if (col < c) {
+                    float d[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) d[i] = stat[u].y * (g[u][k][i] - sum - x[u][k][i] * dot);
+                    pccnn_store<VEC>(d_feats + row * c + col, d);
+                }
             }
         }
     }
@@ -166,10 +179,10 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const T *__restrict_
                 if (slot == 0) sums[wave][(k * LANES + lane) * VEC + i] = total;
             }
         __syncthreads();
-        for (int col = threadIdx.x; col < c; col += kThreads) {
+        for (int col = threadIdx.x; col < c; col += kBackThreads) {
             float total = 0.0f;
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) total += sums[v][col];
+            for (int v = 0; v < kBackWaves; ++v) total += sums[v][col];
             mine[which * c + col] = total;
         }
     }
@@ -283,8 +296,17 @@ __global__ __launch_bounds__(kReduceThreads) void norm_reduce_kernel(const float
     const int64_t col = (int64_t)blockIdx.x * kReduceColumns + threadIdx.x % kReduceColumns;
     const int group = threadIdx.x / kReduceColumns;
     float total = 0.0f;
-    if (col < 2 * c)
-        for (int p = group; p < parts; p += GROUPS) total += partial[(int64_t)p * 2 * c + col];
+    if (col < 2 * c) {
+        float x[8];
+        int p = group;
+        for (; p + 7 * GROUPS < parts; p += 8 * GROUPS) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = partial[(int64_t)(p + i * GROUPS) * 2 * c + col];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) total += x[i];
+        }
+        for (; p < parts; p += GROUPS) total += partial[(int64_t)p * 2 * c + col];
+    }
     sums[group][threadIdx.x % kReduceColumns] = total;
     __syncthreads();
     if (threadIdx.x >= kReduceColumns || col >= 2 * c) return;
@@ -325,10 +347,10 @@ int norm_align(int64_t c, int type, const void *a, int64_t a_stride, const void 
 // Rows that fit a wavefront's registers at their load width.
 bool norm_in_registers(const NormShape &s) { return s.vec * s.chunks <= kRegisterColumns / PCCNN_WAVE && s.chunks <= 16; }
 
-unsigned norm_blocks(int64_t n, int lanes)
+unsigned norm_blocks(int64_t n, int lanes, int waves, int most)
 {
-    const int64_t rows = (int64_t)kWaves * (PCCNN_WAVE / lanes);
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(kMaxBlocks, pccnn_ceil_div(n, rows)));
+    const int64_t rows = (int64_t)waves * (PCCNN_WAVE / lanes);
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, pccnn_ceil_div(n, rows)));
 }
 
 struct NormForward {
@@ -343,7 +365,7 @@ struct NormForward {
     hipStream_t stream;
     template <typename T, int VEC, int LANES, int CHUNKS> void launch() const
     {
-        norm_fwd_kernel<T, VEC, LANES, CHUNKS><<<norm_blocks(n, LANES), kThreads, 0, stream>>>(
+        norm_fwd_kernel<T, VEC, LANES, CHUNKS><<<norm_blocks(n, LANES, kWaves, kMaxBlocks), kThreads, 0, stream>>>(
             (const T *)feats, stride, gamma, beta, weight_type, eps, n, (int)c, (T *)out, (float2 *)stats);
     }
 };
@@ -360,7 +382,7 @@ struct NormBackward {
     hipStream_t stream;
     template <typename T, int VEC, int LANES, int CHUNKS> void launch() const
     {
-        norm_bwd_kernel<T, VEC, LANES, CHUNKS><<<norm_blocks(n, LANES), kThreads, 0, stream>>>(
+        norm_bwd_kernel<T, VEC, LANES, CHUNKS><<<norm_blocks(n, LANES, kBackWaves, kBackBlocks), kBackThreads, 0, stream>>>(
             (const T *)feats, stride, gamma, weight_type, (const float2 *)stats, (const T *)grads, grads_stride, n, (int)c,
             (T *)d_feats, partial);
     }
@@ -461,7 +483,7 @@ extern "C" int pccnn_layer_norm_backward(const void *feats, int type, int64_t ro
         const int align = norm_align(channels, type, feats, row_stride, in_grads, grads_stride, written);
         const NormShape s = norm_shape(channels, type, align);
         if (norm_in_registers(s)) {
-            parts = (int)norm_blocks(n, s.lanes);
+            parts = (int)norm_blocks(n, s.lanes, kBackWaves, kBackBlocks);
             norm_launch(s, type, NormBackward{feats, row_stride, gamma, weight_type, stats, in_grads, grads_stride, n,
                                               channels, d_feats, partial, str});
         } else {

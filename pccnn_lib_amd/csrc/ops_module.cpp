@@ -9,6 +9,8 @@
 
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -791,6 +793,237 @@ Tensor point_conv_weight_var(const Tensor &basis, const Tensor &feats, const Ten
     return generic_weight_var(explicit_args("point_conv_weight_var", basis, feats, neigh, ends));
 }
 
+// ------------------------------------------------------------------ attention between levels
+//
+// Operators the reference does not have: layer norm, rotary positions, attention.  Features are float32 or bfloat16 and
+// may be views whose last dimension is dense.
+
+int feature_type(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? PCCNN_TYPE_BF16 : PCCNN_TYPE_F32; }
+
+const Tensor &chk_features(const Tensor &t, const char *op, const char *what, int ndim, const Tensor *first = nullptr,
+                           bool same_dtype = true)
+{
+    TORCH_CHECK(t.defined(), op, ": ", what, ": expected a torch.Tensor");
+    TORCH_CHECK(t.is_cuda(), op, ": ", what, ": expected a GPU tensor, got device ", t.device());
+    const at::ScalarType type = t.scalar_type();
+    TORCH_CHECK(type == at::kFloat || type == at::kBFloat16, op, ": ", what,
+                ": expected dtype torch.float32 or torch.bfloat16, got ", type);
+    TORCH_CHECK(!first || !same_dtype || type == first->scalar_type(), op, ": ", what, ": expected dtype ",
+                first->scalar_type(), ", got ", type);
+    TORCH_CHECK(t.dim() == ndim, op, ": ", what, ": expected ", ndim, " dimensions, got shape ", t.sizes());
+    TORCH_CHECK(t.size(ndim - 1) <= 1 || t.stride(ndim - 1) == 1, op, ": ", what,
+                ": expected a dense last dimension, got strides ", t.strides());
+    if (first) {
+        TORCH_CHECK(t.device() == first->device(), op, ": ", what, ": on ", t.device(), " but other arguments are on ",
+                    first->device());
+    } else {
+        TORCH_CHECK(t.device().index() == c10::hip::current_device(), op, ": ", what, ": on ", t.device(),
+                    ", but the current device is cuda:", (int)c10::hip::current_device(),
+                    "; run the call under `with torch.cuda.device(tensor.device):`");
+    }
+    return t;
+}
+
+void *optr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
+Tensor feature_result(const Tensor &like) { return at::empty(like.sizes(), like.options()); }
+
+void norm_weight(const char *op, const char *what, const Tensor &w, const Tensor &feats)
+{
+    chk_features(w, op, what, 1, &feats, false);
+    TORCH_CHECK(w.size(0) == feats.size(1), op, ": ", what, " has ", w.size(0), " values for ", feats.size(1), " channels");
+    TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == feats.scalar_type(), op, ": ", what,
+                ": expected dtype float32 or the features' dtype, got ", w.scalar_type());
+    TORCH_CHECK(feats.size(1) >= 1, op, ": features without channels");
+}
+
+py::object layer_norm(const Tensor &feats, const Tensor &gamma, const Tensor &beta, double eps, bool return_stats)
+{
+    const char *op = "layer_norm";
+    chk_features(feats, op, "features", 2);
+    norm_weight(op, "gamma", gamma, feats);
+    norm_weight(op, "beta", beta, feats);
+    TORCH_CHECK(beta.scalar_type() == gamma.scalar_type(), op, ": beta: expected dtype ", gamma.scalar_type(), ", got ",
+                beta.scalar_type());
+    Tensor out = feature_result(feats);
+    OptTensor stats;
+    if (return_stats) stats = at::empty({feats.size(0), 2}, feats.options().dtype(at::kFloat));
+    rc_check(pccnn_layer_norm_forward(feats.data_ptr(), feature_type(feats), feats.stride(0), gamma.data_ptr(),
+                                      beta.data_ptr(), feature_type(gamma), (float)eps, feats.size(0), feats.size(1),
+                                      out.data_ptr(), ofptr(stats), cur_stream()),
+             "pccnn_layer_norm_forward");
+    return return_stats ? py::object(py::make_tuple(out, *stats)) : py::cast(out);
+}
+
+py::tuple layer_norm_grads(const Tensor &feats, const Tensor &gamma, const Tensor &stats, const Tensor &in_grads,
+                           int64_t grad_mask)
+{
+    const char *op = "layer_norm_grads";
+    chk_features(feats, op, "features", 2);
+    norm_weight(op, "gamma", gamma, feats);
+    chk(stats, "layer_norm_grads: stats", at::kFloat, 2, &feats);
+    chk_features(in_grads, op, "in_grads", 2, &feats);
+    const int64_t n = feats.size(0), c = feats.size(1);
+    TORCH_CHECK(stats.size(0) == n && stats.size(1) == 2 && in_grads.sizes() == feats.sizes(), op, ": inconsistent shapes");
+    OptTensor d_feats, d_gamma, d_beta, ws;
+    if (grad_mask & PCCNN_GRAD_FEATS) d_feats = feature_result(feats);
+    if (grad_mask & PCCNN_GRAD_WEIGHTS) {
+        d_gamma = at::empty({c}, gamma.options());
+        d_beta = at::empty({c}, gamma.options());
+        ws = workspace(pccnn_layer_norm_workspace_bytes(n, c), feats);
+    }
+    rc_check(pccnn_layer_norm_backward(feats.data_ptr(), feature_type(feats), feats.stride(0), gamma.data_ptr(),
+                                       feature_type(gamma), fptr(stats), in_grads.data_ptr(), in_grads.stride(0), n, c,
+                                       optr(d_feats), optr(d_gamma), optr(d_beta), optr(ws),
+                                       ws.has_value() ? (size_t)ws->numel() : 0, cur_stream()),
+             "pccnn_layer_norm_backward");
+    return py::make_tuple(opt(d_feats), opt(d_gamma), opt(d_beta));
+}
+
+void rotary_args(const char *op, const Tensor &feats, const Tensor &pts, const Tensor &freqs, const Tensor &axes)
+{
+    const std::string name = op;
+    chk_features(feats, op, "features", 3);
+    chk(pts, name + ": pts", at::kFloat, 2, &feats);
+    chk(freqs, name + ": freqs", at::kFloat, 1, &feats);
+    chk(axes, name + ": axes", at::kInt, 1, &feats);
+    TORCH_CHECK(pts.size(0) == feats.size(0) && axes.size(0) == freqs.size(0) && 2 * freqs.size(0) <= feats.size(2), op, ": ",
+                pts.size(0), " points for ", feats.size(0), " rows, ", freqs.size(0), " frequencies and ", axes.size(0),
+                " axes for heads of ", feats.size(2), " features");
+    TORCH_CHECK(pts.size(1) >= 1 && pts.size(1) <= kMaxDims, op, ": ", pts.size(1),
+                "-dimensional positions are not supported (1 to ", kMaxDims, ")");
+    TORCH_CHECK(feats.size(1) <= INT32_MAX && feats.size(2) <= INT32_MAX, op, ": ", feats.size(1), " heads of ",
+                feats.size(2), " features");
+}
+
+Tensor turned(const char *op, const Tensor &feats, const Tensor &pts, const Tensor &freqs, const Tensor &axes, bool adjacent,
+              bool backwards)
+{
+    Tensor out = feature_result(feats);
+    rc_check(pccnn_rotary(feats.data_ptr(), feature_type(feats), feats.stride(0), feats.stride(1), fptr(pts), fptr(freqs),
+                          iptr(axes), feats.size(0), (int)feats.size(1), (int)feats.size(2), (int)freqs.size(0),
+                          (int)pts.size(1), adjacent, backwards, out.data_ptr(), cur_stream()),
+             op);
+    return out;
+}
+
+Tensor rotary(const Tensor &feats, const Tensor &pts, const Tensor &freqs, const Tensor &axes, bool adjacent)
+{
+    rotary_args("rotary", feats, pts, freqs, axes);
+    return turned("pccnn_rotary", feats, pts, freqs, axes, adjacent, false);
+}
+
+py::tuple rotary_grads(const Tensor &feats, const Tensor &pts, const Tensor &freqs, const Tensor &axes,
+                       const Tensor &in_grads, bool adjacent, int64_t grad_mask)
+{
+    const char *op = "rotary_grads";
+    rotary_args(op, feats, pts, freqs, axes);
+    chk_features(in_grads, op, "in_grads", 3, &feats);
+    TORCH_CHECK(in_grads.sizes() == feats.sizes(), op, ": inconsistent shapes");
+    OptTensor d_feats, d_pts;
+    if (grad_mask & PCCNN_GRAD_FEATS) d_feats = turned("pccnn_rotary", in_grads, pts, freqs, axes, adjacent, true);
+    if (grad_mask & PCCNN_GRAD_PTS) {
+        d_pts = at::empty(pts.sizes(), pts.options());
+        rc_check(pccnn_rotary_points_backward(feats.data_ptr(), feature_type(feats), feats.stride(0), feats.stride(1),
+                                              fptr(pts), fptr(freqs), iptr(axes), in_grads.data_ptr(), in_grads.stride(0),
+                                              in_grads.stride(1), feats.size(0), (int)feats.size(1), (int)feats.size(2),
+                                              (int)freqs.size(0), (int)pts.size(1), adjacent, ofptr(d_pts), cur_stream()),
+                 "pccnn_rotary_points_backward");
+    }
+    return py::make_tuple(opt(d_feats), opt(d_pts));
+}
+
+pccnn_attention attention_args(const char *op, const Tensor &queries, const Tensor &keys, const Tensor &values,
+                               const Tensor &query_starts, const Tensor &key_starts, int64_t max_queries, int64_t max_keys,
+                               const OptTensor &key_mask, const c10::optional<double> &scale)
+{
+    const std::string name = op;
+    chk_features(queries, op, "queries", 3);
+    chk_features(keys, op, "keys", 3, &queries);
+    chk_features(values, op, "values", 3, &queries);
+    chk(query_starts, name + ": query_starts", at::kInt, 1, &queries);
+    chk(key_starts, name + ": key_starts", at::kInt, 1, &queries);
+    const int64_t heads = queries.size(1), key_heads = keys.size(1), width = queries.size(2);
+    TORCH_CHECK(keys.size(2) == width && values.sizes() == keys.sizes(), op, ": queries ", queries.sizes(), ", keys ",
+                keys.sizes(), ", values ", values.sizes(), ": expected [M, H, W], [N, G, W], [N, G, W]");
+    TORCH_CHECK(key_heads >= 1 && heads >= 1 && heads % key_heads == 0 && heads <= INT32_MAX, op, ": ", heads,
+                " heads over ", key_heads, " key heads");
+    TORCH_CHECK(query_starts.size(0) == key_starts.size(0) && query_starts.size(0) >= 1 && query_starts.size(0) <= INT32_MAX,
+                op, ": query_starts ", query_starts.sizes(), " and key_starts ", key_starts.sizes(),
+                ": expected [clouds + 1] both");
+    if (key_mask.has_value()) {
+        chk(*key_mask, name + ": key_mask", at::kBool, 1, &queries);
+        TORCH_CHECK(key_mask->size(0) == keys.size(0), op, ": key_mask of ", key_mask->size(0), " values for ", keys.size(0),
+                    " keys");
+    }
+    pccnn_attention p = {};
+    p.queries = queries.data_ptr();
+    p.keys = keys.data_ptr();
+    p.values = values.data_ptr();
+    p.q_stride_n = queries.stride(0);
+    p.q_stride_h = queries.stride(1);
+    p.k_stride_n = keys.stride(0);
+    p.k_stride_h = keys.stride(1);
+    p.v_stride_n = values.stride(0);
+    p.v_stride_h = values.stride(1);
+    p.query_starts = iptr(query_starts);
+    p.key_starts = iptr(key_starts);
+    p.key_mask = key_mask.has_value() ? (const uint8_t *)key_mask->data_ptr() : nullptr;
+    p.m = queries.size(0);
+    p.n = keys.size(0);
+    p.max_queries = max_queries;
+    p.max_keys = max_keys;
+    p.type = feature_type(queries);
+    p.clouds = (int)(query_starts.size(0) - 1);
+    p.heads = (int)heads;
+    p.key_heads = (int)key_heads;
+    p.width = (int)std::min<int64_t>(width, INT32_MAX);
+    p.scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(width, 1)));
+    return p;
+}
+
+py::object cross_attention(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &query_starts,
+                           const Tensor &key_starts, int64_t max_queries, int64_t max_keys, const OptTensor &key_mask,
+                           const c10::optional<double> &scale, bool return_lse)
+{
+    const pccnn_attention p = attention_args("cross_attention", queries, keys, values, query_starts, key_starts, max_queries,
+                                             max_keys, key_mask, scale);
+    Tensor out = feature_result(queries);
+    OptTensor lse;
+    if (return_lse) lse = at::empty({p.m, p.heads}, queries.options().dtype(at::kFloat));
+    Tensor ws = workspace(pccnn_attention_workspace_bytes(&p, 0), queries);
+    rc_check(pccnn_attention_forward(&p, out.data_ptr(), ofptr(lse), ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
+             "pccnn_attention_forward");
+    return return_lse ? py::object(py::make_tuple(out, *lse)) : py::cast(out);
+}
+
+py::tuple cross_attention_grads(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &query_starts,
+                                const Tensor &key_starts, int64_t max_queries, int64_t max_keys, const Tensor &out,
+                                const Tensor &lse, const Tensor &in_grads, const OptTensor &key_mask,
+                                const c10::optional<double> &scale, int64_t grad_mask)
+{
+    const char *op = "cross_attention_grads";
+    const pccnn_attention p = attention_args(op, queries, keys, values, query_starts, key_starts, max_queries, max_keys,
+                                             key_mask, scale);
+    chk(out, "cross_attention_grads: out", queries.scalar_type(), 3, &queries);
+    chk(lse, "cross_attention_grads: lse", at::kFloat, 2, &queries);
+    chk_features(in_grads, op, "in_grads", 3, &queries);
+    TORCH_CHECK(out.sizes() == queries.sizes() && in_grads.sizes() == queries.sizes() && lse.size(0) == p.m &&
+                    lse.size(1) == p.heads,
+                op, ": inconsistent shapes");
+    OptTensor d_queries, d_keys, d_values;
+    if (grad_mask & PCCNN_GRAD_QUERIES) d_queries = feature_result(queries);
+    if (grad_mask & PCCNN_GRAD_KEYS) {
+        d_keys = feature_result(keys);
+        d_values = feature_result(keys);
+    }
+    Tensor ws = workspace(pccnn_attention_workspace_bytes(&p, 1), queries);
+    rc_check(pccnn_attention_backward(&p, out.data_ptr(), fptr(lse), in_grads.data_ptr(), in_grads.stride(0),
+                                      in_grads.stride(1), optr(d_queries), optr(d_keys), optr(d_values), ws.data_ptr(),
+                                      (size_t)ws.numel(), cur_stream()),
+             "pccnn_attention_backward");
+    return py::make_tuple(opt(d_queries), opt(d_keys), opt(d_values));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(pccnn_lib_ops, mod)
@@ -917,6 +1150,21 @@ PYBIND11_MODULE(pccnn_lib_ops, mod)
                 return kp_family_weight_var("pccnn_weight_variance", PCCNN_BASIS_GAUSS, pts, pdf, feats, samples, neigh,
                                             ends, radii, kernel_pts, sigma);
             });
+
+    // attention between levels (no counterpart in the reference)
+    mod.def("layer_norm", &layer_norm, "feats"_a, "gamma"_a, "beta"_a, "eps"_a = 1e-5, "return_stats"_a = false);
+    mod.def("layer_norm_grads", &layer_norm_grads, "feats"_a, "gamma"_a, "stats"_a, "in_grads"_a, "grad_mask"_a = all);
+    mod.def("rotary", &rotary, "feats"_a, "pts"_a, "freqs"_a, "axes"_a, "adjacent"_a = false);
+    mod.def("rotary_grads", &rotary_grads, "feats"_a, "pts"_a, "freqs"_a, "axes"_a, "in_grads"_a, "adjacent"_a = false,
+            "grad_mask"_a = (int)PCCNN_GRAD_FEATS);
+    const c10::optional<double> by_width;
+    mod.def("cross_attention", &cross_attention, "queries"_a, "keys"_a, "values"_a, "query_starts"_a, "key_starts"_a,
+            "max_queries"_a, "max_keys"_a, "key_mask"_a = none, "scale"_a = by_width, "return_lse"_a = false);
+    mod.def("cross_attention_grads", &cross_attention_grads, "queries"_a, "keys"_a, "values"_a, "query_starts"_a,
+            "key_starts"_a, "max_queries"_a, "max_keys"_a, "out"_a, "lse"_a, "in_grads"_a, "key_mask"_a = none,
+            "scale"_a = by_width, "grad_mask"_a = (int)(PCCNN_GRAD_QUERIES | PCCNN_GRAD_KEYS));
+    mod.attr("ADDED_NAMES") = py::make_tuple("layer_norm", "layer_norm_grads", "rotary", "rotary_grads", "cross_attention",
+                                             "cross_attention_grads");
 
     mod.attr("GRAD_WEIGHTS") = PCCNN_GRAD_WEIGHTS;
     mod.attr("GRAD_FEATS") = PCCNN_GRAD_FEATS;

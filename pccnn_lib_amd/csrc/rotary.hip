@@ -33,7 +33,13 @@ struct RotaryShape {
     int heads, width, pairs, axes;
     int tile;                                // points per workgroup
     int turned, units;                       // units of work per head: of 2 PV turned features, and with the rest
+    uint32_t by_units, by_heads, by_pairs;   // ceil(2^32 / divisor): a quotient by one multiplication (0: divide)
 };
+
+__device__ __forceinline__ int quotient(int value, int divisor, uint32_t inverse)
+{
+    return inverse != 0 ? (int)__umulhi((uint32_t)value, inverse) : value / divisor;
+}
 
 template <typename T, int PV, bool ADJACENT>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const T *__restrict__ in, const float *__restrict__ pts,
@@ -44,17 +50,18 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const T *__restrict__ 
     const int64_t first = (int64_t)blockIdx.x * s.tile;
     const int points = (int)min((int64_t)s.tile, s.n - first);
     for (int i = threadIdx.x; i < points * s.pairs; i += kThreads) {
-        const int point = i / s.pairs, p = i - point * s.pairs;
+        const int point = quotient(i, s.pairs, s.by_pairs), p = i - point * s.pairs;
         const int axis = max(0, min(axis_of[p], s.axes - 1));
         float2 t = turn_of(pts[(first + point) * s.axes + axis], freqs[p]);
         t.y *= sign;
         turns[i] = t;
     }
     __syncthreads();
-    const int per_point = s.heads * s.units;
-    for (int u = threadIdx.x; u < points * per_point; u += kThreads) {
-        const int point = u / per_point, rest = u - point * per_point;
-        const int head = rest / s.units, unit = rest - head * s.units;
+    const int total = points * s.heads * s.units;
+#pragma unroll 2
+    for (int u = threadIdx.x; u < total; u += kThreads) {
+        const int row = quotient(u, s.units, s.by_units), unit = u - row * s.units;
+        const int point = quotient(row, s.heads, s.by_heads), head = row - point * s.heads;
         const T *src = in + (first + point) * s.stride_n + head * s.stride_h;
         T *dst = out + ((first + point) * s.heads + head) * (int64_t)s.width;
         if (unit < s.turned) {
@@ -153,12 +160,20 @@ template <typename T, int PV> void rotary_launch(const RotaryShape &shape, const
     RotaryShape s = shape;
     s.turned = s.pairs / PV;
     s.units = s.turned + (int)pccnn_ceil_div(s.width - 2 * s.pairs, PV);
-    // a workgroup's points: up to about 4096 units of work and 32 KiB of angles, fewer while that leaves CUs without work
+    // a workgroup's points: about 1024 units of work (four per thread, so that the angles of some workgroups are formed
+    // while others stream) and up to 32 KiB of angles, fewer while that leaves CUs without work
     const int64_t per_point = (int64_t)s.heads * s.units;
-    int64_t tile = std::max<int64_t>(1, 4096 / per_point);
+    int64_t tile = std::max<int64_t>(1, 1024 / per_point);
     tile = std::min<int64_t>(tile, std::max(1, kMaxPairs / std::max(1, s.pairs)));
     tile = std::min<int64_t>(tile, std::max<int64_t>(1, pccnn_ceil_div(s.n, 1024)));
     s.tile = (int)tile;
+    // value * inverse / 2^32 is the quotient while value * divisor < 2^32 (the inverse is less than one too large)
+    auto inverse = [&](int64_t largest, int64_t divisor) -> uint32_t {
+        return divisor > 1 && largest * divisor < (1ll << 32) ? (uint32_t)pccnn_ceil_div(1ll << 32, divisor) : 0;
+    };
+    s.by_units = inverse(tile * per_point, s.units);
+    s.by_heads = inverse(tile * s.heads, s.heads);
+    s.by_pairs = inverse(tile * s.pairs, s.pairs);
     const unsigned blocks = (unsigned)pccnn_ceil_div(s.n, tile);
     const size_t lds = (size_t)tile * s.pairs * sizeof(float2);
     if (adjacent)
@@ -198,7 +213,7 @@ extern "C" int pccnn_rotary(const void *feats, int type, int64_t stride_n, int64
     if (n == 0) return PCCNN_OK;
     PCCNN_REQUIRE(feats && pts && out && (pairs == 0 || (freqs && axes)), PCCNN_ERR_INVALID, "rotary: null pointer");
     PCCNN_REQUIRE(n <= (int64_t)INT32_MAX, PCCNN_ERR_UNSUPPORTED, "rotary: n=%lld (up to 2^31 - 1)", (long long)n);
-    const RotaryShape s = {n, stride_n, stride_h, heads, width, pairs, num_axes, 0, 0, 0};
+    const RotaryShape s = {n, stride_n, stride_h, heads, width, pairs, num_axes, 0, 0, 0, 0, 0, 0};
     const float sign = backwards ? -1.0f : 1.0f;
     const hipStream_t str = (hipStream_t)stream;
     if (type == PCCNN_TYPE_F32) return rotary_run<float>(s, type, feats, pts, freqs, axes, adjacent, sign, out, str);
@@ -218,7 +233,7 @@ extern "C" int pccnn_rotary_points_backward(const void *feats, int type, int64_t
     PCCNN_REQUIRE(feats && pts && in_grads && d_pts && (pairs == 0 || (freqs && axes)), PCCNN_ERR_INVALID,
                   "rotary_grads: null pointer");
     PCCNN_REQUIRE(n <= (int64_t)INT32_MAX, PCCNN_ERR_UNSUPPORTED, "rotary_grads: n=%lld (up to 2^31 - 1)", (long long)n);
-    const RotaryShape s = {n, stride_n, stride_h, heads, width, pairs, num_axes, 0, 0, 0};
+    const RotaryShape s = {n, stride_n, stride_h, heads, width, pairs, num_axes, 0, 0, 0, 0, 0, 0};
     const unsigned blocks = (unsigned)pccnn_ceil_div(n, kThreads / PCCNN_WAVE);
     const hipStream_t str = (hipStream_t)stream;
     auto run = [&](auto zero) {

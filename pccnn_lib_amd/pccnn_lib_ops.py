@@ -1642,6 +1642,9 @@ REFERENCE_NAMES = (
     "point_conv_grads", "point_conv_weight_var", "kp_conv", "kp_conv_grads", "kp_conv_weight_var", "kp_conv_n",
     "kp_conv_n_grads", "kp_conv_n_weight_var", "sph_conv", "sph_conv_grads", "sph_conv_weight_var", "pccnn",
     "pccnn_grads", "pccnn_weight_variance")
+# Operators the reference does not have that the compiled module serves too (a Python call through ctypes costs about
+# ten microseconds, more than the smallest of them run).
+ADDED_NAMES = ("layer_norm", "layer_norm_grads", "rotary", "rotary_grads", "cross_attention", "cross_attention_grads")
 
 
 # ----------------------------------------------------------------------------- bindings
@@ -1649,9 +1652,10 @@ REFERENCE_NAMES = (
 # Two bindings of the same C ABI serve the 26 reference names: the compiled extension module ``pccnn_lib_ops`` (what
 # the reference builds from setup.py:7-31; csrc/ops_module.cpp here: pybind11, TORCH_CHECK contracts, at::empty
 # outputs, torch's current HIP stream) and the ctypes functions above, which need no compiler.  The compiled one is
-# used when it has been built; ``use_binding`` switches.  Functions beyond the 26 names exist only in this module.
+# used when it has been built; ``use_binding`` switches.  Both also serve ``ADDED_NAMES``; other functions beyond the 26
+# names exist only in this module.
 
-BINDINGS = {"ctypes": {name: globals()[name] for name in REFERENCE_NAMES}}
+BINDINGS = {"ctypes": {name: globals()[name] for name in REFERENCE_NAMES + ADDED_NAMES}}
 binding = "ctypes"
 
 
@@ -1675,7 +1679,7 @@ def _load_compiled():
 
 
 def use_binding(which):
-    """Route the 26 reference names through the "compiled" extension or through "ctypes"; returns the name of the
+    """Route the 26 reference names and ``ADDED_NAMES`` through the "compiled" extension or through "ctypes"; returns the name of the
     binding in use before the call.  Raises if the compiled module has not been built."""
     global binding
     if which not in BINDINGS:
@@ -1685,7 +1689,11 @@ def use_binding(which):
         if mod is None:
             raise RuntimeError("use_binding: the compiled pccnn_lib_ops extension has not been built "
                                "(python -m pccnn_lib_amd.build)")
-        BINDINGS["compiled"] = {name: getattr(mod, name) for name in REFERENCE_NAMES}
+        missing = [name for name in ADDED_NAMES if not hasattr(mod, name)]
+        if missing:
+            raise RuntimeError("use_binding: the compiled pccnn_lib_ops extension was built from older sources (it has no "
+                               "%s); rebuild it with `python -m pccnn_lib_amd.build`" % missing[0])
+        BINDINGS["compiled"] = {name: getattr(mod, name) for name in REFERENCE_NAMES + ADDED_NAMES}
     before, binding = binding, which
     globals().update(BINDINGS[which])
     return before
