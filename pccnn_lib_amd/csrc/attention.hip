@@ -51,6 +51,7 @@ struct AttnArgs {
     int clouds, heads, key_heads, group, width;
     float scale;
     int tiles, splits, per_split;            // own tiles per cloud and head; parts of the other side and tiles in each
+    int longest_first;                       // clouds in the order of what a workgroup has to walk
     void *out;                               // forward: O; backward: dq
     float *lse;                              // [m, heads]
     float *shift, *delta;                    // [key_heads][m * group]: a row's L in units of log 2 (+inf: no keys), and D
@@ -64,14 +65,28 @@ struct AttnBlock {
     int64_t q0, k0;                          // first query and key of the cloud
     int rows, keys;                          // rows = queries * group
     int head, split, tile;
-    __device__ __forceinline__ AttnBlock(const AttnArgs &a, int64_t block)
+    // The cloud with the r-th longest other side (`starts`), for up to 64 clouds: workgroups start in the order of their
+    // numbers, and the long ones shall not be the last.
+    static __device__ __forceinline__ int longest(const int32_t *starts, int clouds, int r)
+    {
+        const int lane = threadIdx.x % PCCNN_WAVE;
+        const int mine = lane < clouds ? starts[lane + 1] - starts[lane] : -1;
+        int before = 0;
+        for (int j = 0; j < clouds; ++j) {
+            const int other = __builtin_amdgcn_readlane(mine, j);
+            before += other > mine || (other == mine && j < lane);
+        }
+        return __builtin_ctzll(__ballot(lane < clouds && before == r) | 1ull << 63);
+    }
+    __device__ __forceinline__ AttnBlock(const AttnArgs &a, int64_t block, const int32_t *walked)
     {
         tile = (int)(block % a.tiles);
         block /= a.tiles;
         split = (int)(block % a.splits);
         block /= a.splits;
         head = (int)(block % a.key_heads);
-        const int cloud = (int)(block / a.key_heads);
+        int cloud = (int)(block / a.key_heads);
+        if (a.longest_first) cloud = min(longest(walked, a.clouds, cloud), a.clouds - 1);
         // starts outside the tensors are a caller's mistake, but never an access outside them
         const int64_t q1 = min(max((int64_t)a.q_starts[cloud + 1], (int64_t)0), a.m);
         const int64_t k1 = min(max((int64_t)a.k_starts[cloud + 1], (int64_t)0), a.n);
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     typedef typename Feed::Tile Tile;
     constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
-    const AttnBlock b(a, blockIdx.x);
+    const AttnBlock b(a, blockIdx.x, a.k_starts);
     if (b.tile * kOwn >= b.rows) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int row = b.tile * kOwn + wave * 32 + (lane & 31);
@@ -380,7 +395,8 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     const int64_t token = b.query(a, row) * a.heads + b.head_of(a, row);
     if (a.splits > 1) {
         const int64_t at = (int64_t)b.split * a.m * a.heads + token;
-        write_column<float, DP>(a.part + at * a.width, acc, 1.0f, half, a.width);
+        const int padded = (a.width + 3) / 4 * 4;
+        write_column<float, DP>(a.part + at * padded, acc, 1.0f, half, padded);
         if (half == 0) a.part_ml[at] = make_float2(top, sum);
     } else {
         const bool none = top == -INFINITY;                          // no live key at all: zeros
@@ -391,51 +407,70 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
 
 // Joins the parts of a forward pass that was split over the keys: THREADS threads to a (query, head), LANES of them side by
 // side over its features (four each), the groups over the parts, added up in a fixed order.
-template <typename T, int THREADS> __global__ __launch_bounds__(kThreads) void attention_join_kernel(AttnArgs a, int lanes)
+template <typename T, int THREADS, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void attention_join_kernel(AttnArgs a, int lanes)
 {
-    __shared__ float sums[kThreads][5];
+    __shared__ float sums[BLOCK][5];
     const int mine = threadIdx.x % THREADS, first = threadIdx.x - mine;
-    const int64_t tokens = a.m * a.heads, token = (int64_t)blockIdx.x * (kThreads / THREADS) + threadIdx.x / THREADS;
+    const int64_t tokens = a.m * a.heads, token = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
     const int group = mine / lanes, groups = THREADS / lanes, col = mine % lanes * 4;
     float value[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f, top = -INFINITY;
     if (token < tokens) {
         for (int s = mine; s < a.splits; s += THREADS) top = fmaxf(top, a.part_ml[s * tokens + token].x);
     }
-    sums[threadIdx.x][0] = top;
-    __syncthreads();
-    for (int i = 0; i < min(THREADS, a.splits); ++i) top = fmaxf(top, sums[first + i][0]);
-    __syncthreads();
+    top = pccnn_wave_minmax<true>(top);
+    if (THREADS > PCCNN_WAVE) {
+        sums[threadIdx.x][0] = top;
+        __syncthreads();
+        for (int i = 0; i < THREADS; i += PCCNN_WAVE) top = fmaxf(top, sums[first + i][0]);
+        __syncthreads();
+    }
     const float shift = top == -INFINITY ? 0.0f : top;
-    if (token < tokens) {
-#pragma unroll 4
-        for (int s = group; s < a.splits; s += groups) {
-            const float2 ml = a.part_ml[s * tokens + token];
-            const float w = __builtin_amdgcn_exp2f(ml.x - shift);
-            const float *p = a.part + (s * tokens + token) * a.width + col;
-            sum = fmaf(ml.y, w, sum);
-            if (a.width % 4 == 0) {
-                if (col < a.width) {
-                    const float4 x = *(const float4 *)p;
-                    value[0] = fmaf(x.x, w, value[0]); value[1] = fmaf(x.y, w, value[1]);
-                    value[2] = fmaf(x.z, w, value[2]); value[3] = fmaf(x.w, w, value[3]);
-                }
-            } else {
+    const int padded = (a.width + 3) / 4 * 4;                        // a part's rows are whole units of four
+    if (token < tokens && col < padded) {
+        constexpr int BATCH = THREADS > PCCNN_WAVE ? 8 : 2;          // parts whose loads are on their way together
+        for (int s = group; s < a.splits; s += BATCH * groups) {
+            float2 ml[BATCH];
+            float4 x[BATCH];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (col + i < a.width) value[i] = fmaf(p[i], w, value[i]);
+            for (int u = 0; u < BATCH; ++u) {
+                const int64_t at = min(s + u * groups, a.splits - 1) * tokens + token;
+                ml[u] = a.part_ml[at];
+                x[u] = *(const float4 *)(a.part + at * padded + col);
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const float w = s + u * groups < a.splits ? __builtin_amdgcn_exp2f(ml[u].x - shift) : 0.0f;
+                sum = fmaf(ml[u].y, w, sum);
+                value[0] = fmaf(x[u].x, w, value[0]); value[1] = fmaf(x[u].y, w, value[1]);
+                value[2] = fmaf(x[u].z, w, value[2]); value[3] = fmaf(x[u].w, w, value[3]);
             }
         }
     }
+    // the groups of a wavefront first, then the wavefronts of the result
+    for (int o = lanes; o < PCCNN_WAVE; o *= 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[threadIdx.x][i] = value[i];
-    sums[threadIdx.x][4] = sum;
-    __syncthreads();
-    if (group != 0 || token >= tokens) return;
-    for (int g = 1; g < groups; ++g) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) value[i] += sums[threadIdx.x + g * lanes][i];
-        sum += sums[threadIdx.x + g * lanes][4];
+        for (int i = 0; i < 4; ++i) value[i] += __shfl_xor(value[i], o);
+        sum += __shfl_xor(sum, o);
     }
+    if (THREADS > PCCNN_WAVE) {
+        const int wave = mine / PCCNN_WAVE;
+        if (mine % PCCNN_WAVE < lanes) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[first + wave * 32 + mine % PCCNN_WAVE][i] = value[i];
+            sums[first + wave * 32 + mine % PCCNN_WAVE][4] = sum;
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int w = 1; w < THREADS / PCCNN_WAVE; ++w) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) value[i] += sums[first + w * 32 + mine][i];
+                sum += sums[first + w * 32 + mine][4];
+            }
+        }
+    }
+    if (group != 0 || token >= tokens) return;
     const bool none = top == -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -482,7 +517,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     typedef typename Feed::Tile Tile;
     constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
-    const AttnBlock b(a, blockIdx.x);
+    const AttnBlock b(a, blockIdx.x, a.k_starts);
     if (b.tile * kOwn >= b.rows) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int row = b.tile * kOwn + wave * 32 + (lane & 31);
@@ -584,7 +619,7 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
     constexpr int ROWS = Feed::ROWS, STEPS = DP / 16, BLOCKS = DP / 32;
     extern __shared__ __align__(16) uint16_t lds[];
     float *const stats = (float *)(lds + 4 * Tile::ELEMENTS);        // [stage][shift, delta][64]
-    const AttnBlock b(a, blockIdx.x);
+    const AttnBlock b(a, blockIdx.x, a.q_starts);
     if (b.tile * kOwn >= b.keys) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int key = b.tile * kOwn + wave * 32 + (lane & 31);
@@ -861,21 +896,23 @@ void attn_plan(AttnArgs &a, const AttnKernel &kernel, int type, int products, in
     const int64_t tiles = std::max<int64_t>(1, pccnn_ceil_div(other, kernel.rows));
     // workgroups that have work, and the tiles a mean one walks (clouds differ in size)
     const double mean_own = (double)own_all / a.clouds, mean_other = (double)other_all / a.clouds;
-    const double groups = a.key_heads * (double)a.clouds * std::min<double>(a.tiles, mean_own / kOwn + 0.5);
-    const double mean_tiles = std::min<double>((double)tiles, mean_other / kernel.rows + 0.5);
+    const double groups = a.key_heads * (double)a.clouds * std::min<double>(a.tiles, std::max(1.0, mean_own / kOwn + 0.5));
+    const double mean_tiles = std::min<double>((double)tiles, std::max(1.0, mean_other / kernel.rows + 0.5));
     double best = 1e300;
     for (int64_t s = 1; s <= tiles; s += s < 8 ? 1 : s / 4) {
         const int64_t per = pccnn_ceil_div(tiles, s), parts = pccnn_ceil_div(tiles, per);
         const double work = groups * (mean_tiles + 2.0 * std::min<double>((double)parts, mean_tiles / per + 1.0));
         const double rounds = std::ceil(groups * parts / kernel.slots - 0.01) * (std::min<double>((double)per, mean_tiles) + 2.0);
         const double cost = unit * std::max(rounds, work / kernel.slots + 0.5 * per) +
-                            (parts > 1 ? 6.0 + 2.0 * parts * result / 4e6 : 0.0);
+                            (parts > 1 ? 6.0 + 0.01 * parts + 2.0 * parts * result / 4e6 : 0.0);
         if (cost < best) {
             best = cost;
             a.per_split = (int)per;
             a.splits = (int)parts;
         }
     }
+    a.longest_first = a.clouds > 1 && a.clouds <= PCCNN_WAVE && other * a.clouds > other_all &&
+                      (double)a.tiles * a.splits * a.key_heads * a.clouds > kernel.slots;
 }
 // The three passes: which side is walked, by which kernel, in how many parts.
 AttnKernel attn_plan_rows(AttnArgs &a, const pccnn_attention *p, bool forward)
@@ -913,7 +950,7 @@ size_t forward_bytes(const AttnArgs &a)
 {
     if (a.splits == 1) return 0;
     const size_t tokens = (size_t)a.splits * a.m * a.heads;
-    return pccnn_align(tokens * a.width * sizeof(float)) + pccnn_align(tokens * sizeof(float2));
+    return pccnn_align(tokens * ((a.width + 3) / 4 * 4) * sizeof(float)) + pccnn_align(tokens * sizeof(float2));
 }
 
 } // namespace
@@ -948,22 +985,22 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
     const AttnKernel kernel = attn_plan_rows(a, p, true);
     if (a.splits > 1) {
         PccnnArena arena(workspace, workspace_bytes);
-        a.part = arena.take<float>((size_t)a.splits * a.m * a.heads * a.width);
+        a.part = arena.take<float>((size_t)a.splits * a.m * a.heads * ((a.width + 3) / 4 * 4));
         a.part_ml = arena.take<float2>((size_t)a.splits * a.m * a.heads);
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention: workspace of %zu bytes is too small",
                       workspace_bytes);
     }
     rc = attn_launch("cross_attention", kernel, a, s);
     if (rc != PCCNN_OK || a.splits == 1) return rc;
-    // a wavefront to a result up to 32 parts, a workgroup beyond
+    // a wavefront to a result up to 32 parts, a workgroup of sixteen beyond
     int lanes = 1;
     while (4 * lanes < a.width) lanes *= 2;
     auto join = [&](auto zero) {
         using T = decltype(zero);
         if (a.splits <= 32)
-            attention_join_kernel<T, 64><<<(unsigned)pccnn_ceil_div(a.m * a.heads, 4), kThreads, 0, s>>>(a, lanes);
+            attention_join_kernel<T, 64, 256><<<(unsigned)pccnn_ceil_div(a.m * a.heads, 4), 256, 0, s>>>(a, lanes);
         else
-            attention_join_kernel<T, 256><<<(unsigned)(a.m * a.heads), kThreads, 0, s>>>(a, lanes);
+            attention_join_kernel<T, 1024, 1024><<<(unsigned)(a.m * a.heads), 1024, 0, s>>>(a, lanes);
     };
     if (p->type == PCCNN_TYPE_F32)
         join(0.0f);
