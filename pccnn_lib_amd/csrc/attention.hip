@@ -321,27 +321,20 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     pccnn_f32x16 acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
-    float top = -INFINITY, sum = 0.0f;                               // of the lane's row; the sum over the lane's keys only
+    float top = -INFINITY, sums[2] = {0.0f, 0.0f};                   // of the lane's row; the sum over the lane's keys only
     const float c2 = a.scale * kLog2e;
 
-    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
-        const Tile tile_k = {lds + stage * 2 * Tile::ELEMENTS}, tile_v = {tile_k.base + Tile::ELEMENTS};
-        const Tile next_k = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_v = {next_k.base + Tile::ELEMENTS};
-        const uint64_t now = live;
-        if constexpr (DIRECT) {
-            attn_landed();
-        } else {
-            k.put(tile_k, now);
-            v.put(tile_v, now);
-            __syncthreads();
-        }
+    // One tile: `here` holds it, `there` is where the next one goes.  That the two do not overlap is what lets the operands'
+    // reads go on while the next tile is on its way.
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, const uint64_t now) {
+        const Tile tile_k = {here}, tile_v = {here + Tile::ELEMENTS}, next_k = {there}, next_v = {there + Tile::ELEMENTS};
         if (key + ROWS < end) {
             live = live_keys(a, b, key + ROWS, flag, ROWS);
             k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_k);
             v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_v);
             flag = key_flag(a, b, key + 2 * ROWS, lane);
         }
-        if (!working || now == 0) continue;
+        if (!working || now == 0) return;
         pccnn_f32x16 s[ROWS / 32];
 #pragma unroll
         for (int t = 0; t < ROWS / 32; ++t) clear(s[t]);
@@ -366,7 +359,8 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
             const float raised = fmaxf(top, high);
             const float shrink = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - raised);
             top = raised;
-            sum *= shrink;
+            sums[0] *= shrink;
+            sums[1] *= shrink;
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -378,19 +372,29 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
             if (i % BLOCKS == 0) {                                   // the next sixteen keys' probabilities
                 pccnn_f32x16 &x = s[i / BLOCKS / 2];
                 const int from = 8 * (i / BLOCKS % 2);
-                float sums[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int j = from; j < from + 8; ++j) {
                     x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c2, -shift));
                     sums[j % 2] += x[j];
                 }
-                sum += sums[0] + sums[1];
                 p = half_of<TERMS>(x, i / BLOCKS % 2);
             }
             attn_mma<TERMS>(acc[i % BLOCKS], f, p);
         });
+    };
+    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
+        uint16_t *const here = lds + stage * 2 * Tile::ELEMENTS, *const there = lds + (stage ^ 1) * 2 * Tile::ELEMENTS;
+        const uint64_t now = live;
+        if constexpr (DIRECT) {
+            attn_landed();
+        } else {
+            k.put(Tile{here}, now);
+            v.put(Tile{here + Tile::ELEMENTS}, now);
+            __syncthreads();
+        }
+        walk(here, there, now);
     }
-    sum = pccnn_add_row_xor32(sum);
+    const float sum = pccnn_add_row_xor32(sums[0] + sums[1]);
     if (row >= b.rows) return;
     const int64_t token = b.query(a, row) * a.heads + b.head_of(a, row);
     if (a.splits > 1) {
@@ -550,24 +554,17 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
 
-    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
-        const Tile tile_k = {lds + stage * 2 * Tile::ELEMENTS}, tile_v = {tile_k.base + Tile::ELEMENTS};
-        const Tile next_k = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_v = {next_k.base + Tile::ELEMENTS};
-        const uint64_t now = live;
-        if constexpr (DIRECT) {
-            attn_landed();
-        } else {
-            k.put(tile_k, now);
-            v.put(tile_v, now);
-            __syncthreads();
-        }
+    // One tile: `here` holds it, `there` is where the next one goes.  That the two do not overlap is what lets the operands'
+    // reads go on while the next tile is on its way.
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, const uint64_t now) {
+        const Tile tile_k = {here}, tile_v = {here + Tile::ELEMENTS}, next_k = {there}, next_v = {there + Tile::ELEMENTS};
         if (key + ROWS < end) {
             live = live_keys(a, b, key + ROWS, flag, ROWS);
             k.fetch(a.one, k_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_k);
             v.fetch(a.two, v_at, 1, key + ROWS, b.keys, live, a.mask != nullptr, a.width, next_v);
             flag = key_flag(a, b, key + 2 * ROWS, lane);
         }
-        if (!working || now == 0) continue;
+        if (!working || now == 0) return;
 #pragma unroll
         for (int t = 0; t < ROWS / 32; ++t) {
             pccnn_f32x16 s, dp;
@@ -597,6 +594,18 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
                 attn_mma<TERMS>(acc[i % BLOCKS], f, ds);
             });
         }
+    };
+    for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
+        uint16_t *const here = lds + stage * 2 * Tile::ELEMENTS, *const there = lds + (stage ^ 1) * 2 * Tile::ELEMENTS;
+        const uint64_t now = live;
+        if constexpr (DIRECT) {
+            attn_landed();
+        } else {
+            k.put(Tile{here}, now);
+            v.put(Tile{here + Tile::ELEMENTS}, now);
+            __syncthreads();
+        }
+        walk(here, there, now);
     }
     if (!real) return;
     if (shift == INFINITY) {                                         // whatever its gradient holds (0 times NaN)
@@ -657,23 +666,15 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
         clear(dv[dt]);
     }
     const float c2 = a.scale * kLog2e;
-    for (int stage = 0; row < end; row += ROWS, stage ^= 1) {
-        const Tile tile_q = {lds + stage * 2 * Tile::ELEMENTS}, tile_g = {tile_q.base + Tile::ELEMENTS};
-        const Tile next_q = {lds + (stage ^ 1) * 2 * Tile::ELEMENTS}, next_g = {next_q.base + Tile::ELEMENTS};
-        if constexpr (!DIRECT) {
-            const uint64_t bits = first_bits(b.rows - row, ROWS);
-            q.put(tile_q, bits);
-            g.put(tile_g, bits);
-        }
-        if (wave < 2) stats[(stage * 2 + wave) * 64 + lane] = stat;
-        attn_landed();
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, const float *__restrict__ stat_here) {
+        const Tile tile_q = {here}, tile_g = {here + Tile::ELEMENTS}, next_q = {there}, next_g = {there + Tile::ELEMENTS};
         if (row + ROWS < end) {
             const uint64_t bits = first_bits(b.rows - row - ROWS, ROWS);
             fetch_stats(row + ROWS);
             q.fetch(a.one, q_at, a.group, row + ROWS, b.rows, bits, false, a.width, next_q);
             g.fetch(a.two, g_at, a.group, row + ROWS, b.rows, bits, false, a.width, next_g);
         }
-        if (!working) continue;
+        if (!working) return;
 #pragma unroll
         for (int t = 0; t < ROWS / 32; ++t) {
             pccnn_f32x16 s, dp;
@@ -699,8 +700,8 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
                     const int h = i / BLOCKS / 2;
 #pragma unroll
                     for (int n = 2 * h; n < 2 * h + 2; ++n) {
-                        const float4 shift = *(const float4 *)(stats + stage * 128 + 32 * t + 8 * n + 4 * half);
-                        const float4 delta = *(const float4 *)(stats + stage * 128 + 64 + 32 * t + 8 * n + 4 * half);
+                        const float4 shift = *(const float4 *)(stat_here + 32 * t + 8 * n + 4 * half);
+                        const float4 delta = *(const float4 *)(stat_here + 64 + 32 * t + 8 * n + 4 * half);
                         const float sh[4] = {shift.x, shift.y, shift.z, shift.w}, de[4] = {delta.x, delta.y, delta.z, delta.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -717,6 +718,17 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
                     attn_mma<TERMS>(dk[i % BLOCKS], f, ds);
             });
         }
+    };
+    for (int stage = 0; row < end; row += ROWS, stage ^= 1) {
+        uint16_t *const here = lds + stage * 2 * Tile::ELEMENTS, *const there = lds + (stage ^ 1) * 2 * Tile::ELEMENTS;
+        if constexpr (!DIRECT) {
+            const uint64_t bits = first_bits(b.rows - row, ROWS);
+            q.put(Tile{here}, bits);
+            g.put(Tile{here + Tile::ELEMENTS}, bits);
+        }
+        if (wave < 2) stats[(stage * 2 + wave) * 64 + lane] = stat;
+        attn_landed();
+        walk(here, there, stats + stage * 128);
     }
     if (key >= b.keys) return;
     if (!live) {
