@@ -6,9 +6,10 @@ from .convolutions import (ComputeKPConv, ComputeKPConvWeightVar, ComputeMCConv,
                            ComputePointConvBasis, ComputePointConv, ComputePointConvWeightVar, ComputeKPConvN,
                            ComputeKPConvNWeightVar, ComputeSPHConv, ComputeSPHConvWeightVar, ComputePCCNN,
                            ComputePCCNNWeightVar)
+from .attention import ComputeCrossAttention, ComputeLayerNorm, ComputeRotary
 
 __all__ = ["BuildGridDS", "ComputeKeys", "FindNeighbors", "PoissonDiskSamlping", "ComputePDF",
            "ComputeKPConv", "ComputeKPConvWeightVar", "ComputeMCConv", "ComputeMCConvWeightVar",
            "ComputePointConvBasis", "ComputePointConv", "ComputePointConvWeightVar",
            "ComputeKPConvN", "ComputeKPConvNWeightVar", "ComputeSPHConv", "ComputeSPHConvWeightVar",
-           "ComputePCCNN", "ComputePCCNNWeightVar"]
+           "ComputePCCNN", "ComputePCCNNWeightVar", "ComputeLayerNorm", "ComputeRotary", "ComputeCrossAttention"]

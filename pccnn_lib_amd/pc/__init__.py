@@ -4,10 +4,12 @@ from .bounding_box import BoundingBox
 from .grid import Grid
 from .neighborhood import Neighborhood
 from .point_pooling import PointPooling
+from .cloud_ranges import CloudRanges
 from . import layers
 from .layers import *  # noqa: F401,F403
 from .layers import __all__ as _layer_names
 from . import models
 from .models import IModel
 
-__all__ = ["Pointcloud", "BoundingBox", "Grid", "Neighborhood", "PointPooling", "layers", "models", "IModel"] + list(_layer_names)
+__all__ = ["Pointcloud", "BoundingBox", "Grid", "Neighborhood", "PointPooling", "CloudRanges", "layers", "models",
+           "IModel"] + list(_layer_names)

@@ -1,14 +1,15 @@
 """The layer classes and their factories under the reference's names (pccnn_lib/pc/layers/__init__.py:1-10); several of
-them share a module here."""
+them share a module here.  ``LayerNormalization``, ``RotaryPositions`` and ``CrossAttention`` have no counterpart there."""
 import importlib
 
 _HOMES = {
-    "norm": ("Bias", "GroupNormalization"),
+    "norm": ("Bias", "GroupNormalization", "LayerNormalization"),
     "conv_base": ("IConvLayer", "IConvLayerFactory"),
     "mcconv": ("MCConv", "MCConvFactory"),
     "pointconv": ("PointConv", "PointConvFactory"),
     "kpconv": ("KPConv", "KPConvFactory", "KPConvN", "KPConvNFactory", "PCCNN", "PCCNNFactory"),
     "sphconv": ("SPHConv", "SPHConvFactory"),
+    "attention": ("RotaryPositions", "CrossAttention"),
 }
 
 __all__ = []

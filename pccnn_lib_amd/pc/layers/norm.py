@@ -1,5 +1,7 @@
 import torch
 
+from ...op_wrappers import ComputeLayerNorm
+
 
 class Bias(torch.nn.Module):
     """Learned per-feature offset, parameter ``bias_`` [1, F] (pccnn_lib/pc/layers/Bias.py:3-29)."""
@@ -41,3 +43,17 @@ class GroupNormalization(torch.nn.Module):
         spread = cloud_mean(centred * centred)[cloud_of].unsqueeze(1)
         normed = centred / torch.sqrt(spread + 1e-8)
         return normed.reshape(-1, self.num_features_) * self.gamma_ + self.betas_
+
+
+class LayerNormalization(torch.nn.Module):
+    """Layer norm of every point's features, parameters ``gamma_`` and ``betas_`` [1, F] (no counterpart in the reference;
+    named like ``GroupNormalization``'s).  Features float32, or bfloat16 under parameters of either type."""
+
+    def __init__(self, p_num_features, p_eps=1e-5):
+        super(LayerNormalization, self).__init__()
+        self.num_features_, self.eps_ = p_num_features, p_eps
+        self.gamma_ = torch.nn.Parameter(torch.ones(1, p_num_features))
+        self.betas_ = torch.nn.Parameter(torch.zeros(1, p_num_features))
+
+    def forward(self, p_feats):
+        return ComputeLayerNorm.apply(p_feats, self.gamma_.reshape(-1), self.betas_.reshape(-1), self.eps_)
