@@ -23,6 +23,9 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
 constexpr int kOwn = 32 * kWaves;            // rows (forward, dq) or keys (dk, dv) of a workgroup
 constexpr int kMaxWidth = 128;
+// Own tiles per cloud from which on f32 is turned into planes of terms first.  Measured with and without: 6 tiles over
+// 1201 keys 51 and 47 us, 32 over 600 keys 162 and 176, 50 tiles 603 and 755, 5 over 4096 rows (backward) 313 and 302.
+constexpr int kPlanesFrom = 7;
 constexpr float kLog2e = 1.44269504088896341f;
 
 // Rows of the other side that are in LDS at a time, twice (one tile is brought in while the other is worked on).  Three
@@ -278,6 +281,27 @@ __device__ __forceinline__ void write_column(T *row, const pccnn_f32x16 (&acc)[D
                 }
             }
         }
+}
+
+// f32 features as planes of their bf16 terms, [plane][token][head][DP], zeros past the width: what a walked side that
+// several workgroups walk is turned into once, so that its tiles go to LDS as they are.  Two tensors (blockIdx.y), one
+// unit of eight features per thread.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void attention_planes_kernel(AttnStream one, AttnStream two, int64_t tokens,
+                                                                   int heads, int width, uint16_t *__restrict__ planes_one,
+                                                                   uint16_t *__restrict__ planes_two)
+{
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = i / (DP / 8);
+    if (row >= tokens * heads) return;
+    const AttnStream &s = blockIdx.y == 0 ? one : two;
+    uint16_t *to = (blockIdx.y == 0 ? planes_one : planes_two) + 8 * i;
+    const int64_t token = row / heads;
+    AttnChunk<float> c;
+    attn_load(c, (const float *)s.p + token * s.n + (row - token * heads) * s.h, 8 * (int)(i % (DP / 8)), width, s.wide);
+    const AttnFrag<3> f = attn_frag(c);
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+        *(pccnn_u32x4 *)(to + t * tokens * heads * DP) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
 }
 
 // ------------------------------------------------------------------------------------------------- forward
@@ -827,11 +851,14 @@ AttnArgs attn_args(const pccnn_attention *p)
     return a;
 }
 
-// Whether the walked side goes to LDS as it is: bf16, whole 16-byte units, 16-byte rows, 32-bit offsets within a tile.
-bool attn_direct(int type, const AttnStream &one, const AttnStream &two)
+// Whether the walked side goes to LDS without passing registers.  bf16: where rows are whole 16-byte units with 32-bit
+// offsets within a tile.  f32: where it is worth turning into planes of terms first, that is where each cloud has several
+// own tiles (`own`: rows of all clouds) to walk it.
+bool attn_direct(const AttnArgs &a, int type, const AttnStream &one, const AttnStream &two, int64_t own)
 {
-    const int64_t reach = 64 * (std::max(one.n, two.n) + std::max(one.h, two.h)) + kMaxWidth;     // offsets within a tile
-    return type == PCCNN_TYPE_BF16 && one.wide == 2 && two.wide == 2 && reach < (1ll << 30);
+    if (type == PCCNN_TYPE_F32) return own >= (int64_t)kPlanesFrom * kOwn * a.clouds;
+    const int64_t reach = 64 * (std::max(one.n, two.n) + std::max(one.h, two.h)) + kMaxWidth;
+    return one.wide == 2 && two.wide == 2 && reach < (1ll << 30);
 }
 
 // Calls f(type, padded width) for the instantiation that serves this type and head width.
@@ -866,6 +893,7 @@ struct AttnKernel {
     void (*run)(AttnArgs);
     size_t lds;
     int slots, rows;
+    bool direct;
 };
 template <typename T, int DP, bool DIRECT, AttnPass PASS> AttnKernel attn_kernel()
 {
@@ -874,6 +902,7 @@ template <typename T, int DP, bool DIRECT, AttnPass PASS> AttnKernel attn_kernel
     if constexpr (PASS == ATTN_QUERIES) k.run = attention_dq_kernel<T, DP, DIRECT>;
     if constexpr (PASS == ATTN_KEYS) k.run = attention_dkv_kernel<T, DP, DIRECT>;
     k.rows = attn_tile_rows<T, DP>();
+    k.direct = DIRECT;
     // two tiles of two tensors, and the backward rows' statistics
     k.lds = 4 * 2 * (size_t)AttnTile<AttnTerms<T>::value, attn_tile_rows<T, DP>(), DP>::ELEMENTS +
             (PASS == ATTN_KEYS ? 4 * 64 * sizeof(float) : 0);
@@ -886,9 +915,7 @@ template <AttnPass PASS> AttnKernel attn_kernel_of(int type, int width, bool dir
     return attn_dispatch(type, width, [&](auto zero, auto dp) -> AttnKernel {
         using T = decltype(zero);
         constexpr int DP = decltype(dp)::value;
-        if constexpr (sizeof(T) == 2)
-            if (direct) return attn_kernel<T, DP, true, PASS>();
-        return attn_kernel<T, DP, false, PASS>();
+        return direct ? attn_kernel<T, DP, true, PASS>() : attn_kernel<T, DP, false, PASS>();
     });
 }
 
@@ -931,7 +958,7 @@ AttnKernel attn_plan_rows(AttnArgs &a, const pccnn_attention *p, bool forward)
 {
     a.one = {a.k, a.k_n, a.k_h, 0, a.wide_k, a.width / 8};
     a.two = {a.v, a.v_n, a.v_h, 0, a.wide_v, a.width / 8};
-    const bool direct = attn_direct(p->type, a.one, a.two);
+    const bool direct = attn_direct(a, p->type, a.one, a.two, p->m * a.group);
     const AttnKernel kernel = forward ? attn_kernel_of<ATTN_FORWARD>(p->type, a.width, direct)
                                       : attn_kernel_of<ATTN_QUERIES>(p->type, a.width, direct);
     attn_plan(a, kernel, p->type, forward ? 2 : 3, p->max_queries * a.group, p->m * a.group, p->max_keys, p->n);
@@ -942,6 +969,29 @@ AttnKernel attn_plan_keys(AttnArgs &a, const pccnn_attention *p, bool direct)
     const AttnKernel kernel = attn_kernel_of<ATTN_KEYS>(p->type, a.width, direct);
     attn_plan(a, kernel, p->type, 4, p->max_keys, p->n, p->max_queries * a.group, p->m * a.group);
     return kernel;
+}
+// Bytes of the two tensors' planes, when the pass works on planes.
+size_t planes_bytes(const AttnArgs &a, int type, const AttnKernel &kernel, int64_t tokens, int heads)
+{
+    if (type != PCCNN_TYPE_F32 || !kernel.direct) return 0;
+    return 2 * pccnn_align((size_t)3 * tokens * heads * ((a.width + 31) / 32 * 32) * sizeof(uint16_t));
+}
+// Turns the walked side into planes and lets the pass walk those.
+int attn_planes(AttnArgs &a, int type, const AttnKernel &kernel, int64_t tokens, int heads, PccnnArena &arena, hipStream_t s)
+{
+    if (type != PCCNN_TYPE_F32 || !kernel.direct) return PCCNN_OK;
+    return attn_dispatch(type, a.width, [&](auto, auto dp) -> int {
+        constexpr int DP = decltype(dp)::value;
+        const size_t count = (size_t)tokens * heads * DP;
+        uint16_t *one = arena.take<uint16_t>(3 * count), *two = arena.take<uint16_t>(3 * count);
+        PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention: workspace of %zu bytes is too small", arena.size);
+        const dim3 grid((unsigned)pccnn_ceil_div((int64_t)count / 8, kThreads), 2);
+        attention_planes_kernel<DP><<<grid, kThreads, 0, s>>>(a.one, a.two, tokens, heads, a.width, one, two);
+        PCCNN_LAUNCH_CHECK();
+        a.one = {one, (int64_t)heads * DP, DP, (int64_t)count, 2, DP / 8};
+        a.two = {two, (int64_t)heads * DP, DP, (int64_t)count, 2, DP / 8};
+        return PCCNN_OK;
+    });
 }
 
 int64_t attn_blocks(const AttnArgs &a) { return (int64_t)a.tiles * a.splits * a.key_heads * a.clouds; }
@@ -969,16 +1019,20 @@ size_t forward_bytes(const AttnArgs &a)
 
 extern "C" size_t pccnn_attention_workspace_bytes(const pccnn_attention *p, int backward)
 {
-    if (p == nullptr || p->heads < 1 || p->key_heads < 1 || p->clouds < 1 || p->m < 0 || p->n < 0) return 256;
+    if (p == nullptr || !pccnn_type_ok(p->type) || p->heads < 1 || p->key_heads < 1 || p->clouds < 1 || p->m < 0 || p->n < 0 ||
+        p->width < 1 || p->width > kMaxWidth)
+        return 256;
     AttnArgs a = attn_args(p);
-    attn_plan_rows(a, p, !backward);
-    if (!backward) return std::max<size_t>(256, forward_bytes(a));
-    const size_t rows = a.splits > 1 ? pccnn_align((size_t)a.splits * a.m * a.heads * a.width * sizeof(float)) : 0;
+    AttnKernel kernel = attn_plan_rows(a, p, !backward);
+    size_t rows = planes_bytes(a, p->type, kernel, p->n, a.key_heads);
+    if (!backward) return 256 + rows + forward_bytes(a);
+    if (a.splits > 1) rows += pccnn_align((size_t)a.splits * a.m * a.heads * a.width * sizeof(float));
     size_t keys = 0;
     for (bool direct : {false, true}) {              // which one the gradient's layout allows is not known here
-        attn_plan_keys(a, p, direct);
-        if (a.splits > 1)
-            keys = std::max(keys, 2 * pccnn_align((size_t)a.splits * a.n * a.key_heads * a.width * sizeof(float)));
+        kernel = attn_plan_keys(a, p, direct);
+        const size_t parts = a.splits > 1
+                                 ? 2 * pccnn_align((size_t)a.splits * a.n * a.key_heads * a.width * sizeof(float)) : 0;
+        keys = std::max(keys, parts + planes_bytes(a, p->type, kernel, p->m, a.heads));
     }
     return 256 + 2 * pccnn_align((size_t)a.m * a.heads * sizeof(float)) + std::max(rows, keys);
 }
@@ -995,8 +1049,10 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
     a.out = out;
     a.lse = lse_out;
     const AttnKernel kernel = attn_plan_rows(a, p, true);
+    PccnnArena arena(workspace, workspace_bytes);
+    rc = attn_planes(a, p->type, kernel, p->n, a.key_heads, arena, s);
+    if (rc != PCCNN_OK) return rc;
     if (a.splits > 1) {
-        PccnnArena arena(workspace, workspace_bytes);
         a.part = arena.take<float>((size_t)a.splits * a.m * a.heads * ((a.width + 3) / 4 * 4));
         a.part_ml = arena.take<float2>((size_t)a.splits * a.m * a.heads);
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "cross_attention: workspace of %zu bytes is too small",
@@ -1078,6 +1134,7 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         const AttnKernel kernel = attn_plan_rows(a, p, false);
         const int64_t count = a.m * a.heads * a.width;
         a.out = d_queries;
+        if ((rc = attn_planes(a, p->type, kernel, p->n, a.key_heads, arena, s)) != PCCNN_OK) return rc;
         if (a.splits > 1) a.part = arena.take<float>((size_t)a.splits * count);
         if ((rc = in_workspace()) != PCCNN_OK) return rc;
         rc = attn_launch(name, kernel, a, s);
@@ -1088,11 +1145,12 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
     if (d_keys != nullptr && p->n > 0) {
         a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
         a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
-        const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(p->type, a.one, a.two));
+        const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(a, p->type, a.one, a.two, p->n));
         const int64_t count = a.n * a.key_heads * a.width;
         a.d_k = d_keys;
         a.d_v = d_values;
         arena.used = after;
+        if ((rc = attn_planes(a, p->type, kernel, p->m, a.heads, arena, s)) != PCCNN_OK) return rc;
         if (a.splits > 1) {
             a.part = arena.take<float>((size_t)a.splits * count);
             a.part_v = arena.take<float>((size_t)a.splits * count);
