@@ -531,7 +531,7 @@ int pccnn_conv_backward_bf16(const pccnn_basis *basis, const float *pts, const f
  * layer norm of features, rotary positions over the point coordinates, and softmax attention of the points of one level
  * to those of another.  Features are f32 or bf16 (bit patterns), `type` one of PCCNN_TYPE_*; everything is computed in
  * f32 and a bf16 result is rounded once.  Strides are in elements and not negative; features of a row (of a head) lie
- * one behind the other; results are dense. */
+ * one behind the other; results are dense and start at multiples of 16 bytes. */
 #define PCCNN_GRAD_QUERIES 64
 #define PCCNN_GRAD_KEYS 128 /* keys and values */
 #define PCCNN_TYPE_F32 0

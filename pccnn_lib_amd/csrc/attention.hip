@@ -23,6 +23,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
 constexpr int kOwn = 32 * kWaves;            // rows (forward, dq) or keys (dk, dv) of a workgroup
 constexpr int kMaxWidth = 128;
+constexpr int64_t kMostTokens = 1ll << 32;   // queries x heads, keys x key heads
 // Own tiles per cloud from which on f32 is turned into planes of terms first.  Measured with and without: 6 tiles over
 // 1201 keys 51 and 47 us, 32 over 600 keys 162 and 176, 50 tiles 603 and 755, 5 over 4096 rows (backward) 313 and 302.
 constexpr int kPlanesFrom = 7;
@@ -329,8 +330,8 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     const bool working = b.tile * kOwn + wave * 32 < b.rows;         // any row of this wavefront exists
     const int64_t k_at = b.k0 * a.one.n + b.head * a.one.h, v_at = b.k0 * a.two.n + b.head * a.two.h;
 
-    int key = b.split * a.per_split * ROWS;
-    const int end = min(b.keys, key + a.per_split * ROWS);
+    int key = (int)min((int64_t)b.split * a.per_split * ROWS, (int64_t)b.keys);
+    const int end = (int)min((int64_t)b.keys, key + (int64_t)a.per_split * ROWS);
     Feed k, v;
     uint64_t live = 0;
     uint8_t flag = 0;
@@ -558,8 +559,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     const bool working = b.tile * kOwn + wave * 32 < b.rows;
     const int64_t k_at = b.k0 * a.one.n + b.head * a.one.h, v_at = b.k0 * a.two.n + b.head * a.two.h;
 
-    int key = b.split * a.per_split * ROWS;
-    const int end = min(b.keys, key + a.per_split * ROWS);
+    int key = (int)min((int64_t)b.split * a.per_split * ROWS, (int64_t)b.keys);
+    const int end = (int)min((int64_t)b.keys, key + (int64_t)a.per_split * ROWS);
     Feed k, v;
     uint64_t live = 0;
     uint8_t flag = 0;
@@ -819,6 +820,9 @@ int attn_check(const char *name, const pccnn_attention *p)
                   PCCNN_ERR_UNSUPPORTED, "%s: m=%lld, n=%lld: starts are 32-bit", name, (long long)p->m, (long long)p->n);
     PCCNN_REQUIRE(p->scale > 0.0f && p->scale <= 3.0e38f, PCCNN_ERR_INVALID, "%s: scale=%g (positive and finite)", name,
                   (double)p->scale);
+    PCCNN_REQUIRE(p->m * p->heads <= kMostTokens && p->n * p->key_heads <= kMostTokens, PCCNN_ERR_UNSUPPORTED,
+                  "%s: %lld queries of %d heads, %lld keys of %d (up to 2^32 of both)", name, (long long)p->m, p->heads,
+                  (long long)p->n, p->key_heads);
     const int64_t strides[] = {p->q_stride_n, p->q_stride_h, p->k_stride_n, p->k_stride_h, p->v_stride_n, p->v_stride_h};
     for (int64_t s : strides)
         PCCNN_REQUIRE(s >= 0, PCCNN_ERR_INVALID, "%s: a stride of %lld elements", name, (long long)s);
@@ -865,7 +869,7 @@ AttnArgs attn_args(const pccnn_attention *p)
 bool attn_direct(const AttnArgs &a, int type, const AttnStream &one, const AttnStream &two, int64_t own)
 {
     if (type == PCCNN_TYPE_F32) return own >= (int64_t)kPlanesFrom * kOwn * a.clouds;
-    const int64_t reach = 64 * (std::max(one.n, two.n) + std::max(one.h, two.h)) + kMaxWidth;
+    const int64_t reach = 64 * std::max(one.n, two.n) + std::max(64, a.group) * std::max(one.h, two.h) + kMaxWidth;
     return one.wide == 2 && two.wide == 2 && reach < (1ll << 30);
 }
 
@@ -994,7 +998,7 @@ size_t planes_bytes(const AttnArgs &a, int type, const AttnKernel &kernel, int64
 // Turns the walked side into planes and lets the pass walk those.
 int attn_planes(AttnArgs &a, int type, const AttnKernel &kernel, int64_t tokens, int heads, PccnnArena &arena, hipStream_t s)
 {
-    if (type != PCCNN_TYPE_F32 || !kernel.direct) return PCCNN_OK;
+    if (type != PCCNN_TYPE_F32 || !kernel.direct || tokens == 0) return PCCNN_OK;      // (no tokens: nothing is walked)
     return attn_dispatch(type, a.width, [&](auto, auto dp) -> int {
         constexpr int DP = decltype(dp)::value;
         const size_t count = (size_t)tokens * heads * DP;
@@ -1060,6 +1064,7 @@ extern "C" int pccnn_attention_forward(const pccnn_attention *p, void *out, floa
     if (rc != PCCNN_OK) return rc;
     if (p->m == 0 || p->clouds == 0) return PCCNN_OK;
     PCCNN_REQUIRE(out != nullptr, PCCNN_ERR_INVALID, "cross_attention: null pointer");
+    PCCNN_REQUIRE((uintptr_t)out % 16 == 0, PCCNN_ERR_INVALID, "cross_attention: a result that is not 16-byte aligned");
     const hipStream_t s = (hipStream_t)stream;
     AttnArgs a = attn_args(p);
     a.out = out;
@@ -1106,6 +1111,8 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
                   "%s: the gradients of keys and values come together", name);
     if (p->clouds == 0 || (d_queries == nullptr && d_keys == nullptr)) return PCCNN_OK;
     PCCNN_REQUIRE(p->m == 0 || (out && lse && in_grads), PCCNN_ERR_INVALID, "%s: null pointer", name);
+    PCCNN_REQUIRE(((uintptr_t)d_queries | (uintptr_t)d_keys | (uintptr_t)d_values) % 16 == 0, PCCNN_ERR_INVALID,
+                  "%s: a result that is not 16-byte aligned", name);
     const hipStream_t s = (hipStream_t)stream;
     AttnArgs a = attn_args(p);
     a.g = in_grads;

@@ -72,6 +72,8 @@ def test_attention_entry_points_refuse_bad_arguments(lib):
         assert forward(scale=scale) == -1 and b"scale" in lib.pccnn_last_error()
     assert forward(k_stride_n=-1) == -1 and forward(keys=None) == -1 and forward(query_starts=None) == -1
     assert forward(out=None) == -1 and b"null" in lib.pccnn_last_error()
+    assert forward(out=20) == -1 and b"aligned" in lib.pccnn_last_error()
+    assert forward(m=1 << 30, heads=8, key_heads=2) == -2
     assert forward(m=0, max_queries=0, out=None) == 0 and forward(clouds=0, out=None) == 0
     # one query over many keys is split over the keys, which takes a workspace
     long = dict(m=1, max_queries=1, n=1000000, max_keys=1000000, k_stride_n=32)

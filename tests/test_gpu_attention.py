@@ -3,7 +3,7 @@
 Tolerances follow from the roundings.  u is the relative error that one rounding of the type may bring: 2^-8 for bf16
 (nearest even, 8 significant bits: half of a spacing of 2^-7), and for f32, whose sums run over at most a few thousand terms of 2^-24 each, 2^-16 of the
 sum of the terms' magnitudes.  A bf16 attention rounds the probabilities, the score gradients and the results: the bound of
-every element is formed in 64 bits from exactly these roundings (``_attention_bounds``).
+every element is formed in 64 bits from exactly these roundings (``_attention_exact``).
 """
 import math
 
@@ -340,6 +340,60 @@ def test_attention_of_views(ops, type, views, width):
 def test_attention_split_over_the_long_side(ops, type, q_sizes, k_sizes, heads, key_heads, width):
     _attention_check(ops, type, q_sizes, k_sizes, heads, key_heads, width, seed=11)
     _attention_check(ops, type, q_sizes, k_sizes, heads, key_heads, width, seed=12, off=0.5)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("q_sizes,k_sizes,heads,key_heads,width,off", [
+    ([1000, 900], [300, 41], 2, 2, 24, 0.3),       # several own tiles per cloud: f32 keys become planes of terms
+    ([1000], [0], 2, 1, 32, 0.0), ([0], [1000], 2, 1, 32, 0.0),
+    ([33, 20], [1000, 2000], 3, 1, 48, 0.2),       # groups of three: a tile's rows start inside a group (backward)
+    ([40], [950], 6, 1, 64, 0.0), ([700, 2100], [950, 1000], 5, 1, 33, 0.1), ([900], [900], 2, 2, 128, 0.0),
+    ([5, 0, 900], [1, 900, 900], 2, 2, 1, 0.0), ([7], [1000], 70, 1, 5, 0.0)])
+def test_attention_of_many_own_tiles_and_odd_groups(ops, type, q_sizes, k_sizes, heads, key_heads, width, off):
+    _attention_check(ops, type, q_sizes, k_sizes, heads, key_heads, width, off=off, seed=15)
+
+
+def test_attention_of_more_clouds_than_a_wavefront_orders(ops):
+    # up to 64 uneven clouds are worked on longest first, more in their own order; one head and eight (runs of tiles)
+    gen = _gen(16)
+    for clouds in (63, 64, 65, 130):
+        q_sizes = torch.randint(0, 300, (clouds,), generator=gen).tolist()
+        k_sizes = torch.randint(0, 200, (clouds,), generator=gen).tolist()
+        for heads in (1, 8):
+            _attention_check(ops, "bf16", q_sizes, k_sizes, heads, heads, 16, seed=clouds)
+
+
+def test_the_operators_in_a_graph(ops):
+    # captured once, replayed with eager work between the replays, on new inputs each time
+    gen = _gen(17)
+    x = _normal(gen, 700, 64).to(torch.bfloat16).to(DEV)
+    gamma, beta = torch.rand(64, generator=gen).to(DEV), torch.rand(64, generator=gen).to(DEV)
+    pts, freqs, of_axis = [t.to(DEV) for t in _rotary_plan(gen, 700, 3, 8)]
+    starts, sizes = _starts([300, 400]).to(DEV), 400
+
+    def block():
+        y, stats = ops.layer_norm(x, gamma, beta, return_stats=True)
+        q = ops.rotary(y.reshape(700, 4, 16), pts, freqs, of_axis)
+        out, lse = ops.cross_attention(q, q, q, starts, starts, sizes, sizes, return_lse=True)
+        grads = ops.cross_attention_grads(q, q, q, starts, starts, sizes, sizes, out, lse, q)
+        back = ops.rotary_grads(q, pts, freqs, of_axis, grads[0])[0]
+        return [y, q, out, lse, *grads, *ops.layer_norm_grads(x, gamma, stats, back.reshape(700, 64))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = block()
+    for i in range(4):
+        x.copy_(_normal(gen, 700, 64).to(torch.bfloat16).to(DEV))
+        want = block()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), i
 
 
 @pytest.mark.parametrize("type", ["f32", "bf16"])
