@@ -8,6 +8,11 @@
 // gamma, beta and the two column sums of the backward pass stay in registers over the whole loop, and one small second
 // kernel adds the workgroups' sums in a fixed order (no atomics: the same bits from run to run).  Rows longer than a
 // wavefront's registers hold (2048 values) take a workgroup each and are read again from the caches instead.
+//
+// Bound by HBM.  800000 rows of 64 bf16 values: forward 37 us = 5.5 TB/s, backward 65 us = 4.7 TB/s (three streams, the
+// column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 16
+// and 2.4 us (both passes fit the 256 MB cache).  One row: 2 us, the launch.  Two rows at a time in the backward pass and
+// half as many rows of sums took the last kernel from 6.6 to 3.9 us and left the first one as it was.
 #include "elements.h"
 
 #include <algorithm>
