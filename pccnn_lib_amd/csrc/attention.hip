@@ -56,7 +56,7 @@ struct AttnStream {
 };
 
 struct AttnArgs {
-    const void *q, *k, *v, *g;               // a workgroup's own side: queries, keys, values, gradient of the output
+    const void *q, *k, *v, *g, *o;           // a workgroup's own side: queries, keys, values, gradient of the output, O
     int64_t q_n, q_h, k_n, k_h, v_n, v_h, g_n, g_h;
     int wide_q, wide_k, wide_v, wide_g, wide_o;
     AttnStream one, two;                     // the walked side: keys and values, or queries and output gradients
@@ -527,30 +527,30 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(AttnArgs a, int l
 
 // ------------------------------------------------------------------------------------------------- backward
 
-// What the backward kernels need of a row: D = dO . O, and L in units of log 2 (+inf for a row without keys: every P is
-// zero).  Eight lanes to a row, eight features each at a time; 96 MB in 19 us.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a, const T *__restrict__ out)
+// What the kernel of dk and dv needs of a row, for a call that wants no dq (whose kernel leaves it on the way): D = dO . O,
+// and L in units of log 2 (+inf for a row without keys: every P is zero).  Two lanes to a row, which add in the order of
+// the halves of a wavefront there: the same bits.
+template <typename T> __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a)
 {
-    const int64_t token = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 8;
+    const int64_t token = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 2;
     const bool live = token < a.m * a.heads;
     const int64_t query = token / a.heads;
     const int head = (int)(token - query * a.heads);
-    float sum = 0.0f;
+    float delta = 0.0f;
     if (live)
-        for (int col = 8 * (threadIdx.x % 8); col < a.width; col += 64) {
-            AttnChunk<T> x, g;
-            attn_load(x, out + token * a.width, col, a.width, a.wide_o);
-            attn_load(g, (const T *)a.g + query * a.g_n + head * a.g_h, col, a.width, a.wide_g);
+        for (int col = 8 * (threadIdx.x % 2); col < a.width; col += 16) {
+            AttnChunk<T> o, d;
+            attn_load(o, (const T *)a.o + token * a.width, col, a.width, a.wide_o);
+            attn_load(d, (const T *)a.g + query * a.g_n + head * a.g_h, col, a.width, a.wide_g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(attn_value(x, i), attn_value(g, i), sum);
+            for (int i = 0; i < 8; ++i) delta = fmaf(attn_value(o, i), attn_value(d, i), delta);
         }
-    sum = pccnn_group_sum<8>(sum);
-    if (live && threadIdx.x % 8 == 0) {
+    delta = pccnn_group_sum<2>(delta);
+    if (live && threadIdx.x % 2 == 0) {
         const int64_t at = head / a.group * (a.m * a.group) + query * a.group + head % a.group;
         const float lse = a.lse[token];
         a.shift[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-        a.delta[at] = lse == -INFINITY ? 0.0f : sum;
+        a.delta[at] = lse == -INFINITY ? 0.0f : delta;
     }
 }
 
@@ -591,7 +591,29 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     AttnFrag<TERMS> q[DP / 16], g[DP / 16];
     own_side<T, DP>(q, a.q, query * a.q_n + head * a.q_h, real, half, a.width, a.wide_q);
     own_side<T, DP>(g, a.g, query * a.g_n + head * a.g_h, real, half, a.width, a.wide_g);
-    const float shift = real ? a.shift[b.stat(a, row)] : INFINITY, delta = real ? a.delta[b.stat(a, row)] : 0.0f;
+    // D = dO . O and L of the row, left for the other kernel by the first part
+    const int64_t token = query * a.heads + head;
+    float delta = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        AttnChunk<T> o, d;
+        attn_clear(o);
+        attn_clear(d);
+        if (real) {
+            attn_load(o, (const T *)a.o + token * a.width, 16 * kk + 8 * half, a.width, a.wide_o);
+            attn_load(d, (const T *)a.g + query * a.g_n + head * a.g_h, 16 * kk + 8 * half, a.width, a.wide_g);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = fmaf(attn_value(o, i), attn_value(d, i), delta);
+    }
+    delta = pccnn_add_row_xor32(delta);
+    const float lse = real ? a.lse[token] : -INFINITY;
+    const float shift = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys: every P is zero
+    if (lse == -INFINITY) delta = 0.0f;
+    if (real && half == 0 && b.split == 0) {
+        a.shift[b.stat(a, row)] = shift;
+        a.delta[b.stat(a, row)] = delta;
+    }
     const float c2 = a.scale * kLog2e;
     pccnn_f32x16 acc[DP / 32];
 #pragma unroll
@@ -655,7 +677,6 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
     }
-    const int64_t token = query * a.heads + head;
     if (a.splits > 1)
         write_column<float, DP>(a.part + ((int64_t)b.split * a.m * a.heads + token) * a.width, acc, a.scale, half, a.width);
     else
@@ -794,13 +815,16 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
     }
 }
 
-// Sum of the parts of a gradient, in order; VEC values per thread (4 when the count is a multiple of 4).
+// Sum of the parts of one or two gradients (blockIdx.y), in order; VEC values per thread (4 when the count is a multiple
+// of 4).
 template <typename T, int VEC>
-__global__ __launch_bounds__(kThreads) void attention_sum_kernel(const float *__restrict__ part, int splits, int64_t count,
-                                                                T *__restrict__ out)
+__global__ __launch_bounds__(kThreads) void attention_sum_kernel(const float *__restrict__ part_one,
+                                                                const float *__restrict__ part_two, int splits,
+                                                                int64_t count, T *__restrict__ one, T *__restrict__ two)
 {
     const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (i >= count) return;
+    const float *part = blockIdx.y == 0 ? part_one : part_two;
     float sum[VEC], x[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
@@ -810,7 +834,7 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(const float *__
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum[j] += x[j];
     }
-    pccnn_store<VEC>(out + i, sum);
+    pccnn_store<VEC>((blockIdx.y == 0 ? one : two) + i, sum);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -1133,20 +1157,22 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
     a.wide_g = attn_wide(a.g, a.g_n, a.g_h, p->type, a.width);
     a.wide_o = attn_wide(out, a.width, a.width, p->type, a.width);
     a.lse = (float *)lse;
+    a.o = out;
     PccnnArena arena(workspace, workspace_bytes);
     auto in_workspace = [&]() -> int {
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
         return PCCNN_OK;
     };
-    auto sum_parts = [&](const float *part, int64_t count, void *to) {
+    auto sum_parts = [&](const float *part_one, const float *part_two, int64_t count, void *one, void *two) {
         auto sum = [&](auto zero) {
             using T = decltype(zero);
+            const unsigned tensors = two != nullptr ? 2 : 1;
             if (count % 4 == 0)
-                attention_sum_kernel<T, 4><<<(unsigned)pccnn_ceil_div(count, 4 * kThreads), kThreads, 0, s>>>(
-                    part, a.splits, count, (T *)to);
+                attention_sum_kernel<T, 4><<<dim3((unsigned)pccnn_ceil_div(count, 4 * kThreads), tensors), kThreads, 0, s>>>(
+                    part_one, part_two, a.splits, count, (T *)one, (T *)two);
             else
-                attention_sum_kernel<T, 1><<<(unsigned)pccnn_ceil_div(count, kThreads), kThreads, 0, s>>>(
-                    part, a.splits, count, (T *)to);
+                attention_sum_kernel<T, 1><<<dim3((unsigned)pccnn_ceil_div(count, kThreads), tensors), kThreads, 0, s>>>(
+                    part_one, part_two, a.splits, count, (T *)one, (T *)two);
         };
         if (p->type == PCCNN_TYPE_F32)
             sum(0.0f);
@@ -1157,12 +1183,6 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         a.shift = arena.take<float>((size_t)p->m * p->heads);
         a.delta = arena.take<float>((size_t)p->m * p->heads);
         if ((rc = in_workspace()) != PCCNN_OK) return rc;
-        const unsigned blocks = (unsigned)pccnn_ceil_div(a.m * a.heads * 8, kThreads);
-        if (p->type == PCCNN_TYPE_F32)
-            attention_rows_kernel<float><<<blocks, kThreads, 0, s>>>(a, (const float *)out);
-        else
-            attention_rows_kernel<uint16_t><<<blocks, kThreads, 0, s>>>(a, (const uint16_t *)out);
-        PCCNN_LAUNCH_CHECK();
     }
     const size_t after = arena.used;
     if (d_queries != nullptr && p->m > 0) {
@@ -1174,10 +1194,18 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         if ((rc = in_workspace()) != PCCNN_OK) return rc;
         rc = attn_launch(name, kernel, a, s);
         if (rc != PCCNN_OK) return rc;
-        if (a.splits > 1) sum_parts(a.part, count, d_queries);
+        if (a.splits > 1) sum_parts(a.part, nullptr, count, d_queries, nullptr);
         PCCNN_LAUNCH_CHECK();
     }
     if (d_keys != nullptr && p->n > 0) {
+        if (d_queries == nullptr && p->m > 0) {
+            const unsigned blocks = (unsigned)pccnn_ceil_div(a.m * a.heads * 2, kThreads);
+            if (p->type == PCCNN_TYPE_F32)
+                attention_rows_kernel<float><<<blocks, kThreads, 0, s>>>(a);
+            else
+                attention_rows_kernel<uint16_t><<<blocks, kThreads, 0, s>>>(a);
+            PCCNN_LAUNCH_CHECK();
+        }
         a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
         a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
         const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(a, p->type, a.one, a.two, p->n));
@@ -1193,10 +1221,7 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         if ((rc = in_workspace()) != PCCNN_OK) return rc;
         rc = attn_launch(name, kernel, a, s);
         if (rc != PCCNN_OK) return rc;
-        if (a.splits > 1) {
-            sum_parts(a.part, count, d_keys);
-            sum_parts(a.part_v, count, d_values);
-        }
+        if (a.splits > 1) sum_parts(a.part, a.part_v, count, d_keys, d_values);
         PCCNN_LAUNCH_CHECK();
     }
     return PCCNN_OK;

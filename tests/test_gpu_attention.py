@@ -440,6 +440,18 @@ def test_attention_is_the_same_bits_on_every_run_and_stream(ops):
     assert none is None and torch.equal(dk, grads[1]) and torch.equal(dv, grads[2])
 
 
+@pytest.mark.parametrize("width", [33, 64])
+def test_attention_gradients_asked_for_alone_are_the_same_bits(ops, width):
+    # the rows' statistics come from the queries' kernel when it runs, else from a kernel of their own
+    for type in TYPES:
+        dev, plan, key_mask, out, lse, grads = _attention_check(ops, type, [90, 300], [500, 77], 4, 2, width, off=0.1, seed=24)
+        _, dk, dv = ops.cross_attention_grads(*dev[:3], *plan, out, lse, dev[3], key_mask=key_mask, grad_mask=ops.GRAD_KEYS)
+        assert torch.equal(dk, grads[1]) and torch.equal(dv, grads[2])
+        dq, _, _ = ops.cross_attention_grads(*dev[:3], *plan, out, lse, dev[3], key_mask=key_mask,
+                                             grad_mask=ops.GRAD_QUERIES)
+        assert torch.equal(dq, grads[0])
+
+
 def test_attention_past_32_bit_offsets(ops):
     # keys whose last elements lie past 2^31 elements from the first (a view with wide rows): the last cloud's result is
     # that of the same keys stored densely
