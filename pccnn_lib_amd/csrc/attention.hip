@@ -17,12 +17,13 @@
 // and the softmax are f32.  f32: three bf16 terms per value, six products (attention_tiles.h).
 //
 // Tiles go from memory to LDS without passing registers, the next while one is worked on.  What bounds the large cases is
-// the card's power: matrix pipe 45 - 60 % and vector ALU 50 - 77 % busy at 1.75 - 2.1 GHz of 2.4, and neither a wider
+// the card's power: matrix pipe 45 - 60 % and vector ALU 50 - 77 % busy at 1.65 - 2.1 GHz of 2.4, and neither a wider
 // tile, wave priorities nor interleaving the exponentials with products by hand changed their time (64 rows per wavefront:
 // 605 -> 568 us where 8 x 256 rows of 64 features walk 100000 keys, but 6.8 -> 7.4 ms at 128 features, whose registers
-// then leave one wavefront to a SIMD).  Measured: forward 34123 x 100000, 4 heads of 128, 6.8 ms = 1030 TFLOP/s; training
-// 8 x 8192 rows over 2047 keys, uneven, 8 heads of 64: forward 170 - 193, dq 203 - 227, dk / dv 324 - 367 us; one row per
-// cloud over 16 x 4096 keys 25 us = 5.4 TB/s and 4 for the join, over 10^6 keys 92 us = 5.6 TB/s and 11.
+// then leave one wavefront to a SIMD).  Measured: forward 34123 x 100000, 4 heads of 128, 6.8 - 6.9 ms = 1013 - 1030
+// TFLOP/s; training 8 x 8192 rows over 2047 keys, uneven, 8 heads of 64: forward 174 - 202, dq with the rows' statistics
+// 220 - 250, dk / dv 331 - 383 us; one row per cloud over 16 x 4096 keys 25 us = 5.4 TB/s and 4 for the join, over 10^6
+// keys 91 us = 5.6 TB/s and 10.
 #include "attention_tiles.h"
 
 #include <algorithm>

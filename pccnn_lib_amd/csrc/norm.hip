@@ -10,8 +10,8 @@
 // wavefront's registers hold (2048 values) take a workgroup each and are read again from the caches instead.
 //
 // Bound by HBM.  800000 rows of 64 bf16 values: forward 37 us = 5.5 TB/s, backward 65 us = 4.7 TB/s (three streams, the
-// column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 16
-// and 2.4 us (both passes fit the 256 MB cache).  One row: 2 us, the launch.  Two rows at a time in the backward pass and
+// column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 17
+// and 3.6 us (both passes fit the 256 MB cache).  One row: 2 us, the launch.  Two rows at a time in the backward pass and
 // half as many rows of sums took the last kernel from 6.6 to 3.9 us and left the first one as it was.
 #include "elements.h"
 
@@ -93,15 +93,16 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const T *__restrict_
     }
 }
 
-// partial: [workgroup][2][c] column sums (dgamma, dbeta), or null when nobody wants them; d_feats null likewise.  Short rows
-// are worked on two at a time, so that a lane has four loads on their way.
+// sums_gamma, sums_beta: a workgroup's column sums, sums_stride values after the last workgroup's, or null when nobody wants
+// them; d_feats null likewise.  Short rows are worked on two at a time, so that a lane has four loads on their way.
 template <typename T, int VEC, int LANES, int CHUNKS>
 __global__ __launch_bounds__(kBackThreads) void norm_bwd_kernel(const T *__restrict__ feats, int64_t stride,
                                                                const void *__restrict__ gamma, int weight_type,
                                                                const float2 *__restrict__ stats,
                                                                const T *__restrict__ grads, int64_t grads_stride,
                                                                int64_t n, int c, T *__restrict__ d_feats,
-                                                               float *__restrict__ partial)
+                                                               float *__restrict__ sums_gamma,
+                                                               float *__restrict__ sums_beta, int64_t sums_stride)
 {
     constexpr int ROWS = PCCNN_WAVE / LANES;
     constexpr int COLUMNS = LANES * CHUNKS * VEC;
@@ -171,8 +172,8 @@ __global__ __launch_bounds__(kBackThreads) void norm_bwd_kernel(const T *__restr
             }
         }
     }
-    if (partial == nullptr) return;
-    float *mine = partial + (int64_t)blockIdx.x * 2 * c;
+    if (sums_gamma == nullptr) return;
+    const int64_t mine = (int64_t)blockIdx.x * sums_stride;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(kBackThreads) void norm_bwd_kernel(const T *__restr
             float total = 0.0f;
 #pragma unroll
             for (int v = 0; v < kBackWaves; ++v) total += sums[v][col];
-            mine[which * c + col] = total;
+            (which == 0 ? sums_gamma : sums_beta)[mine + col] = total;
         }
     }
 }
@@ -358,6 +359,17 @@ unsigned norm_blocks(int64_t n, int lanes, int waves, int most)
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, pccnn_ceil_div(n, rows)));
 }
 
+// Few rows stay in one workgroup, which needs no second kernel for its sums when it can write them as they are (f32).  It may
+// pass over its rows as often as that costs less than the second launch (backward pass, two kernels -> one, f32): 32 rows of
+// 64 values 4.9 -> 2.8 us, 128 of 64 5.0 -> 3.8, 16 of 1024 7.3 -> 5.9; four passes over rows of 1024 (7.3 -> 8.4) or two over
+// rows of 1021 single values in bf16 (8.2 -> 8.8) would lose.
+unsigned norm_back_blocks(int64_t n, const NormShape &s, bool alone)
+{
+    const int64_t passes = s.chunks == 1 ? 4 : s.chunks <= 4 ? 2 : 1;
+    if (alone && n <= passes * kBackWaves * (PCCNN_WAVE / s.lanes)) return 1;
+    return norm_blocks(n, s.lanes, kBackWaves, kBackBlocks);
+}
+
 struct NormForward {
     const void *feats;
     int64_t stride;
@@ -383,13 +395,15 @@ struct NormBackward {
     const void *grads;
     int64_t grads_stride, n, c;
     void *d_feats;
-    float *partial;
+    float *sums_gamma, *sums_beta;
+    int64_t sums_stride;
+    unsigned blocks;
     hipStream_t stream;
     template <typename T, int VEC, int LANES, int CHUNKS> void launch() const
     {
-        norm_bwd_kernel<T, VEC, LANES, CHUNKS><<<norm_blocks(n, LANES, kBackWaves, kBackBlocks), kBackThreads, 0, stream>>>(
+        norm_bwd_kernel<T, VEC, LANES, CHUNKS><<<blocks, kBackThreads, 0, stream>>>(
             (const T *)feats, stride, gamma, weight_type, (const float2 *)stats, (const T *)grads, grads_stride, n, (int)c,
-            (T *)d_feats, partial);
+            (T *)d_feats, sums_gamma, sums_beta, sums_stride);
     }
 };
 template <typename T, int VEC, typename CALL> void norm_launch_shape(const NormShape &s, const CALL &call)
@@ -483,14 +497,20 @@ extern "C" int pccnn_layer_norm_backward(const void *feats, int type, int64_t ro
     }
     const hipStream_t str = (hipStream_t)stream;
     int parts = 0;
+    bool summed = false;
     if (n > 0) {
         const void *written = d_feats != nullptr ? d_feats : feats;
         const int align = norm_align(channels, type, feats, row_stride, in_grads, grads_stride, written);
         const NormShape s = norm_shape(channels, type, align);
         if (norm_in_registers(s)) {
-            parts = (int)norm_blocks(n, s.lanes, kBackWaves, kBackBlocks);
+            const bool alone = columns && weight_type == PCCNN_TYPE_F32;
+            parts = (int)norm_back_blocks(n, s, alone);
+            summed = alone && parts == 1;
+            float *sums_gamma = summed ? (float *)d_gamma : partial;
+            float *sums_beta = summed ? (float *)d_beta : partial == nullptr ? nullptr : partial + channels;
             norm_launch(s, type, NormBackward{feats, row_stride, gamma, weight_type, stats, in_grads, grads_stride, n,
-                                              channels, d_feats, partial, str});
+                                              channels, d_feats, sums_gamma, sums_beta, 2 * channels, (unsigned)parts,
+                                              str});
         } else {
             const unsigned blocks = (unsigned)std::min<int64_t>(n, 16384);
             parts = (int)std::min<int64_t>(n, std::max<int64_t>(1, kMaxBlocks / pccnn_ceil_div(channels, kThreads)));
@@ -513,7 +533,7 @@ extern "C" int pccnn_layer_norm_backward(const void *feats, int type, int64_t ro
         }
         PCCNN_LAUNCH_CHECK();
     }
-    if (columns) {
+    if (columns && !summed) {
         norm_reduce_kernel<<<(unsigned)pccnn_ceil_div(2 * channels, kReduceColumns), kReduceThreads, 0, str>>>(
             partial, parts, channels, d_gamma, d_beta, weight_type);
         PCCNN_LAUNCH_CHECK();

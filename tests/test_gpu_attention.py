@@ -77,6 +77,21 @@ def test_norm_against_the_formula(ops, type, rows, channels):
         _within(d_beta, db, uw * db.abs() + f * g.double().abs().sum(0), "dbeta")
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,channels", [(128, 64), (129, 64), (256, 64), (257, 64), (32, 256), (33, 256), (64, 256), (65, 256),
+                                           (16, 1024), (17, 1024), (8, 1021), (9, 1021)])
+def test_norm_of_as_many_rows_as_one_workgroup_takes_and_one_more(ops, type, rows, channels):
+    test_norm_against_the_formula(ops, type, rows, channels)
+    gen = _gen(rows + channels)
+    x, g = (_normal(gen, rows, channels).to(TYPES[type]).to(DEV) for _ in range(2))
+    gamma, beta = torch.full((channels,), 1.25, device=DEV), torch.zeros(channels, device=DEV)
+    _, stats = ops.layer_norm(x, gamma, beta, return_stats=True)
+    d_feats, d_gamma, d_beta = ops.layer_norm_grads(x, gamma, stats, g)
+    only, _, _ = ops.layer_norm_grads(x, gamma, stats, g, grad_mask=ops.GRAD_FEATS)
+    _, dg, db = ops.layer_norm_grads(x, gamma, stats, g, grad_mask=ops.GRAD_WEIGHTS)
+    assert torch.equal(only, d_feats) and torch.equal(dg, d_gamma) and torch.equal(db, d_beta)
+
+
 def test_norm_of_a_views_rows_and_of_unaligned_rows(ops):
     gen = _gen(5)
     for type, dtype in TYPES.items():
