@@ -27,6 +27,7 @@
 #include "attention_tiles.h"
 
 #include <algorithm>
+#include <float.h>
 #include <math.h>
 
 namespace {
@@ -324,6 +325,16 @@ __global__ __launch_bounds__(kThreads) void attention_planes_kernel(AttnStream o
 // The running maximum is only raised when a tile exceeds it by more than this many powers of two: P then stays below
 // 2^8 in f32 and bf16 (exponents to spare in both), and the accumulators are rarely scaled.
 constexpr float kSlack = 8.0f;
+// The maximum of a tile with a live key is never below this.  A maximum drops NaN, so without it a row whose scores are all
+// NaN would look like one without keys; with it a running maximum of minus infinity means that no key was live, nothing else.
+constexpr float kLowest = -FLT_MAX;
+
+// L of a row.  A row with live keys whose sum is not positive has scores that are all NaN or minus infinity: no softmax.
+__device__ __forceinline__ float log_sum(float top, float sum)
+{
+    if (top == -INFINITY) return -INFINITY;
+    return sum > 0.0f ? top * (1.0f / kLog2e) + logf(sum) : NAN;
+}
 
 template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
@@ -395,10 +406,10 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
         for (int t = 0; t < ROWS / 32; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) high = fmaxf(high, s[t][i]);
-        high = attn_max_halves(high) * c2;
+        high = fmaxf(attn_max_halves(high) * c2, kLowest);
         if (__any(high > top + kSlack)) {
             const float raised = fmaxf(top, high);
-            const float shrink = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - raised);
+            const float shrink = __builtin_amdgcn_exp2f(top - raised);
             top = raised;
             sums[0] *= shrink;
             sums[1] *= shrink;
@@ -407,7 +418,6 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
         }
-        const float shift = top == -INFINITY ? 0.0f : top;
         AttnFrag<TERMS> p;
         ahead.template run<ROWS / 16 * BLOCKS>(value_columns, [&](int i, const AttnFrag<TERMS> &f) {
             if (i % BLOCKS == 0) {                                   // the next sixteen keys' probabilities
@@ -415,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
                 const int from = 8 * (i / BLOCKS % 2);
 #pragma unroll
                 for (int j = from; j < from + 8; ++j) {
-                    x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c2, -shift));
+                    x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c2, -top));
                     sums[j % 2] += x[j];
                 }
                 p = half_of<TERMS>(x, i / BLOCKS % 2);
@@ -446,7 +456,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
     } else {
         const bool none = top == -INFINITY;                          // no live key at all: zeros
         write_column<T, DP>((T *)a.out + token * a.width, acc, none ? 0.0f : 1.0f / sum, half, a.width);
-        if (a.lse != nullptr && half == 0) a.lse[token] = none ? -INFINITY : top * (1.0f / kLog2e) + logf(sum);
+        if (a.lse != nullptr && half == 0) a.lse[token] = log_sum(top, sum);
     }
 }
 
@@ -523,7 +533,7 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(AttnArgs a, int l
         const float one[1] = {none ? 0.0f : value[i] / sum};
         if (col + i < a.width) pccnn_store<1>((T *)a.out + token * a.width + col + i, one);
     }
-    if (a.lse != nullptr && col == 0) a.lse[token] = none ? -INFINITY : top * (1.0f / kLog2e) + logf(sum);
+    if (a.lse != nullptr && col == 0) a.lse[token] = log_sum(top, sum);
 }
 
 // ------------------------------------------------------------------------------------------------- backward

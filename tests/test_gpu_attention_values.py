@@ -1,0 +1,102 @@
+"""Attention on the GPU where live features are not finite, and how exact f32 products are: against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from pccnn_lib_amd import pccnn_lib_ops
+    return pccnn_lib_ops
+
+
+def _normal(gen, *shape):
+    return torch.randn(shape, generator=gen, dtype=torch.float32)
+
+
+def _starts(*sizes):
+    return torch.tensor([sum(sizes[:i]) for i in range(len(sizes) + 1)], dtype=torch.int32, device=DEV)
+
+
+# One cloud's queries and keys: the parts that few rows are cut into by the length of the other side.
+LENGTHS = [(70, 50), (1, 90), (1, 1500), (2, 4096), (1, 200000), (1000, 40)]
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("queries,keys", LENGTHS)
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_a_query_that_is_not_finite_is_no_query_without_keys(ops, type, queries, keys, bad):
+    # row 0 of the second cloud, head 1: every score is NaN (an infinity is one in f32, whose terms of it are; with both
+    # signs of the key's features in bf16).  Its result, lse and gradient are NaN; so are, by the formula, the gradients of all
+    # that this head's keys share with it; every other row and head is what it is without.
+    gen = torch.Generator().manual_seed(queries * 7 + keys)
+    dtype, sizes, key_sizes = TYPES[type], (3, queries), (5, keys)
+    q, g = (_normal(gen, 3 + queries, 4, 32).to(dtype).to(DEV) for _ in range(2))
+    k, v = (_normal(gen, 5 + keys, 2, 32).to(dtype).to(DEV) for _ in range(2))
+    plan = (_starts(*sizes), _starts(*key_sizes), max(sizes), max(key_sizes))
+    clean, clean_lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    clean_grads = ops.cross_attention_grads(q, k, v, *plan, clean, clean_lse, g)
+    q[3, 1] = math.nan
+    if bad == "inf":
+        q[3, 1, ::2], q[3, 1, 1::2] = math.inf, -math.inf
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    grads = ops.cross_attention_grads(q, k, v, *plan, out, lse, g)
+    hit = torch.zeros(out.shape[:2], dtype=torch.bool, device=DEV)
+    hit[3, 1] = True
+    for got, want in ((out, clean), (lse, clean_lse), (grads[0], clean_grads[0])):
+        assert bool(torch.isnan(got[hit]).all())
+        assert torch.equal(got[~hit], want[~hit])
+    for got, want in zip(grads[1:], clean_grads[1:]):
+        assert bool(torch.isnan(got[5:, 0]).all())
+        assert torch.equal(got[:5], want[:5]) and torch.equal(got[5:, 1], want[5:, 1])
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("queries,keys", LENGTHS)
+@pytest.mark.parametrize("alone", [False, True])
+def test_a_live_key_that_is_nan_reaches_every_query_of_its_cloud(ops, type, queries, keys, alone):
+    # the key is one among the live ones, or the only one that is not switched off
+    gen = torch.Generator().manual_seed(queries * 5 + keys)
+    dtype = TYPES[type]
+    q, g = (_normal(gen, 3 + queries, 2, 32).to(dtype).to(DEV) for _ in range(2))
+    k, v = (_normal(gen, 5 + keys, 2, 32).to(dtype).to(DEV) for _ in range(2))
+    plan = (_starts(3, queries), _starts(5, keys), max(3, queries), max(5, keys))
+    mask = torch.ones(5 + keys, dtype=torch.bool, device=DEV)
+    if alone:
+        mask[5:] = False
+        mask[5 + keys // 2] = True
+    clean, clean_lse = ops.cross_attention(q, k, v, *plan, key_mask=mask, return_lse=True)
+    k[5 + keys // 2, 1] = math.nan
+    out, lse = ops.cross_attention(q, k, v, *plan, key_mask=mask, return_lse=True)
+    assert bool(torch.isnan(out[3:, 1]).all()) and bool(torch.isnan(lse[3:, 1]).all())
+    assert torch.equal(out[:3], clean[:3]) and torch.equal(out[3:, 0], clean[3:, 0])
+    assert torch.equal(lse[:3], clean_lse[:3]) and torch.equal(lse[3:, 0], clean_lse[3:, 0])
+    d_queries, d_keys, d_values = ops.cross_attention_grads(q, k, v, *plan, out, lse, g, key_mask=mask)
+    assert bool(torch.isnan(d_queries[3:, 1]).all()) and bool(torch.isfinite(d_queries[:3]).all())
+    assert bool(torch.isfinite(d_queries[3:, 0]).all())
+    assert bool(torch.isnan(d_keys[5:, 1][mask[5:]]).all()) and bool(torch.isnan(d_values[5:, 1][mask[5:]]).all())
+    assert float(d_keys[~mask].abs().sum()) == 0.0 and float(d_values[~mask].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("queries,keys", LENGTHS)
+def test_scores_that_are_all_minus_infinity_are_not_the_same_as_no_keys(ops, queries, keys):
+    # bf16: every key scores minus infinity, the softmax is 0 / 0; with one key that does not, that key has it all
+    gen = torch.Generator().manual_seed(3)
+    q, v = torch.ones((queries, 1, 16), device=DEV).bfloat16(), _normal(gen, keys, 1, 16).bfloat16().to(DEV)
+    k = torch.full((keys, 1, 16), -math.inf, device=DEV).bfloat16()
+    plan = (_starts(queries), _starts(keys), queries, keys)
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+    k[keys // 2] = 0.25
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    assert torch.equal(out, v[keys // 2:keys // 2 + 1].expand_as(out))
+    assert float((lse - 1.0).abs().max()) < 1e-6                       # 16 x 0.25 / sqrt(16)
+    none = torch.zeros(keys, dtype=torch.bool, device=DEV)
+    out, lse = ops.cross_attention(q, k, v, *plan, key_mask=none, return_lse=True)
+    assert float(out.abs().sum()) == 0.0 and bool((lse == -math.inf).all())
