@@ -37,9 +37,12 @@ template <int TERMS> __device__ __forceinline__ void attn_mma(pccnn_f32x16 &c, c
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], c, 0, 0, 0);
 }
 
-// Eight f32 values as terms, each rounded to nearest even from what the terms before it leave.
-template <int TERMS> __device__ __forceinline__ AttnFrag<TERMS> attn_split(const float (&x)[8])
+// Eight f32 values as terms, each rounded to nearest even from what the terms before it leave.  WHOLE: up to the largest f32
+// value, for features (a value within 2^-9 of it would round to an infinite first term; the next terms take what the largest
+// finite one leaves).
+template <int TERMS, bool WHOLE = false> __device__ __forceinline__ AttnFrag<TERMS> attn_split(const float (&x)[8])
 {
+    constexpr float most = 0x1.fep127f;                  // of bf16
     AttnFrag<TERMS> f;
     float rest[8];
 #pragma unroll
@@ -49,7 +52,11 @@ template <int TERMS> __device__ __forceinline__ AttnFrag<TERMS> attn_split(const
         pccnn_u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = pccnn_bf16_pair(rest[2 * i], rest[2 * i + 1]);
+            if (WHOLE && t == 0)
+                w[i] = pccnn_bf16_pair(__builtin_amdgcn_fmed3f(rest[2 * i], -most, most),
+                                       __builtin_amdgcn_fmed3f(rest[2 * i + 1], -most, most));
+            else
+                w[i] = pccnn_bf16_pair(rest[2 * i], rest[2 * i + 1]);
             if (t + 1 < TERMS) {
                 rest[2 * i] -= __uint_as_float(w[i] << 16);
                 rest[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
@@ -123,7 +130,7 @@ __device__ __forceinline__ AttnFrag<1> attn_frag(const AttnChunk<uint16_t> &c)
     f.t[0] = __builtin_bit_cast(pccnn_bf16x8, c.v);
     return f;
 }
-__device__ __forceinline__ AttnFrag<3> attn_frag(const AttnChunk<float> &c) { return attn_split<3>(c.v); }
+__device__ __forceinline__ AttnFrag<3> attn_frag(const AttnChunk<float> &c) { return attn_split<3, true>(c.v); }
 
 // A tile of ROWS rows in LDS, bf16, one plane per term, rows of DP features without padding.  The 16-byte units of a row
 // are exchanged among themselves by a rule on the row, chosen so that the two reads below touch every group of four banks

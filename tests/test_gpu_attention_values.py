@@ -100,3 +100,26 @@ def test_scores_that_are_all_minus_infinity_are_not_the_same_as_no_keys(ops, que
     none = torch.zeros(keys, dtype=torch.bool, device=DEV)
     out, lse = ops.cross_attention(q, k, v, *plan, key_mask=none, return_lse=True)
     assert float(out.abs().sum()) == 0.0 and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("queries,keys", [(1, 1), (3, 700), (1000, 40), (1, 20000)])
+def test_f32_features_near_the_largest_value(ops, queries, keys):
+    # values from 3.3962e38 on, whose nearest bf16 value is infinite: the key with all the weight hands them on
+    row = torch.tensor([3.4e38, -3.4e38, 3.397e38, -3.3965e38, 3.39e38, 1.0, 0.0, -2.0] * 2, device=DEV)
+    q, k, v = (torch.zeros((n, 1, 16), device=DEV) for n in (queries, keys, keys))
+    q += 1.0
+    k[keys // 2] = 8.0                                                  # a score of 32 among zeros
+    v[keys // 2, 0] = row
+    plan = (_starts(queries), _starts(keys), queries, keys)
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    want = row.double()
+    # three terms hold 24 bits, then the products, sums and the division by the sum: a few 2^-24 of the value (the other keys
+    # weigh 2^-46 each)
+    assert bool(torch.isfinite(out).all())
+    assert float(((out[:, 0].double() - want).abs() - 2.0 ** -21 * want.abs()).max()) <= 0.0
+    # and as the one output gradient that is not zero: the value's gradient is P times it, P from an lse of 32 in f32 (2^-19)
+    g = torch.zeros_like(q)
+    g[0, 0] = row
+    _, _, d_values = ops.cross_attention_grads(q, k, torch.zeros_like(v), *plan, torch.zeros_like(q), lse, g)
+    assert bool(torch.isfinite(d_values).all())
+    assert float(((d_values[keys // 2, 0].double() - want).abs() - 2.0 ** -16 * want.abs()).max()) <= 0.0
