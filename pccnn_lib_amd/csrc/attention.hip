@@ -143,8 +143,9 @@ __device__ __forceinline__ uint64_t live_keys(const AttnArgs &a, const AttnBlock
 }
 
 // Brings tile after tile of a stream into LDS.  GROUPED: a stream row is a row of the problem (query * group + head in
-// group), else a key.
-template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
+// group), else a key.  REPEAT: what lies past the last row is that row again instead of zeros (for queries: a zero times an
+// infinite key would be NaN, where the row's own score is as good as any other for a probability that is zero anyway).
+template <typename T, int DP, bool DIRECT, bool GROUPED, bool REPEAT = false> struct Feeder {
     static constexpr int TERMS = AttnTerms<T>::value;
     static constexpr int ROWS = attn_tile_rows<T, DP>();
     typedef AttnTile<TERMS, ROWS, DP> Tile;
@@ -187,11 +188,12 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
                                           bool masked, int width, const Tile &tile)
     {
         if constexpr (DIRECT) {
-            if (!regular(group)) {                       // the tile's first row may lie inside a group
+            const bool past = REPEAT && limit - row < ROWS;
+            if (!regular(group) || past) {               // the tile's first row may lie inside a group
                 base = (const char *)s.p + 2 * (at + row / group * s.n);
 #pragma unroll
                 for (int j = 0; j < COUNT; ++j) {
-                    const int r = row_of(j), unit = Tile::unit_at(r, unit_of(j));
+                    const int unit = Tile::unit_at(row_of(j), unit_of(j)), r = REPEAT ? min(row_of(j), limit - row - 1) : row_of(j);
                     const int query = (row + r) / group, head = row + r - query * group;
                     if (unit < s.units) off[j] = 2 * (uint32_t)((query - row / group) * s.n + head * s.h + 8 * unit);
                 }
@@ -202,7 +204,7 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
                 for (int j = 0; j < COUNT; ++j) at_unit[j] = (live >> row_of(j)) & 1 ? off[j] : kAttnNowhere;
             } else {
 #pragma unroll
-                for (int j = 0; j < COUNT; ++j) at_unit[j] = row_of(j) < limit - row ? off[j] : kAttnNowhere;
+                for (int j = 0; j < COUNT; ++j) at_unit[j] = REPEAT || row_of(j) < limit - row ? off[j] : kAttnNowhere;
             }
             const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
@@ -217,9 +219,8 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
 #pragma unroll
             for (int j = 0; j < COUNT; ++j) {
                 attn_clear(held[j]);
-                if (row + row_of(j) < limit)
-                    attn_load(held[j], (const T *)s.p + at + offset(s, group, row + row_of(j)), 8 * unit_of(j), width,
-                              s.wide);
+                const int r = REPEAT ? min(row + row_of(j), limit - 1) : row + row_of(j);
+                if (r < limit) attn_load(held[j], (const T *)s.p + at + offset(s, group, r), 8 * unit_of(j), width, s.wide);
             }
         }
     }
@@ -230,7 +231,7 @@ template <typename T, int DP, bool DIRECT, bool GROUPED> struct Feeder {
 #pragma unroll
             for (int j = 0; j < COUNT; ++j) {
                 AttnChunk<T> chunk = held[j];
-                if (!((live >> row_of(j)) & 1)) attn_clear(chunk);
+                if (!REPEAT && !((live >> row_of(j)) & 1)) attn_clear(chunk);
                 tile.put(row_of(j), unit_of(j), attn_frag(chunk));
             }
         }
@@ -715,7 +716,8 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
 
     int row = (int)min((int64_t)b.split * a.per_split * ROWS, (int64_t)b.rows);
     const int end = (int)min((int64_t)b.rows, row + (int64_t)a.per_split * ROWS);
-    Feed q, g;
+    Feeder<T, DP, DIRECT, true, true> q;
+    Feed g;
     q.start(a.one, q_at, a.group, row);
     g.start(a.two, g_at, a.group, row);
     // shifts and deltas of the tile's rows, one wavefront each; they pass through a register, since LDS that the compiler

@@ -123,3 +123,24 @@ def test_f32_features_near_the_largest_value(ops, queries, keys):
     _, _, d_values = ops.cross_attention_grads(q, k, torch.zeros_like(v), *plan, torch.zeros_like(q), lse, g)
     assert bool(torch.isfinite(d_values).all())
     assert float(((d_values[keys // 2, 0].double() - want).abs() - 2.0 ** -16 * want.abs()).max()) <= 0.0
+
+
+@pytest.mark.parametrize("queries,keys,heads,key_heads,width", [
+    (64, 30, 2, 2, 32), (70, 30, 2, 2, 32), (1, 30, 2, 2, 64), (33, 300, 6, 2, 32), (5, 200, 4, 1, 128), (9001, 40, 2, 2, 32),
+    (70, 30, 2, 2, 33)])
+def test_a_key_that_scores_minus_infinity_has_no_gradient(ops, queries, keys, heads, key_heads, width):
+    # bf16, queries all positive, one live key of minus infinities: probability zero, so its gradients are zero however many
+    # rows the last tile of queries has, and every other key's are what they are with that key switched off
+    gen = torch.Generator().manual_seed(queries + width)
+    normal = lambda n, h: _normal(gen, n, h, width).bfloat16().to(DEV)
+    q, g, k, v = normal(queries, heads).abs() + 0.01, normal(queries, heads), normal(keys, key_heads), normal(keys, key_heads)
+    k[7] = -math.inf
+    mask = torch.ones(keys, dtype=torch.bool, device=DEV)
+    mask[7] = False
+    plan = (_starts(queries), _starts(keys), queries, keys)
+    want, want_lse = ops.cross_attention(q, k, v, *plan, key_mask=mask, return_lse=True)
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    got = ops.cross_attention_grads(q, k, v, *plan, out, lse, g, grad_mask=ops.GRAD_KEYS)[1:]
+    for a, b in zip(got, ops.cross_attention_grads(q, k, v, *plan, out, lse, g, key_mask=mask, grad_mask=ops.GRAD_KEYS)[1:]):
+        assert torch.equal(a, b) and float(a[7].abs().max()) == 0.0
