@@ -566,7 +566,7 @@ int pccnn_rotary_points_backward(const void *feats, int type, int64_t stride_n, 
  * a multiple of key_heads: query head h reads key head h / (heads / key_heads)).  Cloud c has the queries
  * query_starts[c] .. query_starts[c+1] and the keys key_starts[c] .. key_starts[c+1]: i32[clouds+1], ascending, from 0 to
  * m and n, either side of any length, zero included; max_queries / max_keys are the largest of these lengths (rows past
- * them are not computed).  key_mask (nullable) u8[n]: a zero switches the key off for all queries; what its rows hold
+ * them, and all of a call with clouds 0, are not computed and not written).  key_mask (nullable) u8[n]: a zero switches the key off for all queries; what its rows hold
  * (infinities and NaN included) then has no effect, and its gradients are zero.  A query without any key gets zeros and
  * lse -inf.  scale: positive, finite.
  * forward: out [m,heads,width]; lse_out (nullable) f32[m,heads] = log of the sum of exp(scale q.k), for the backward call.

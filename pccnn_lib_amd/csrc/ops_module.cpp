@@ -950,6 +950,8 @@ pccnn_attention attention_args(const char *op, const Tensor &queries, const Tens
     TORCH_CHECK(query_starts.size(0) == key_starts.size(0) && query_starts.size(0) >= 1 && query_starts.size(0) <= INT32_MAX,
                 op, ": query_starts ", query_starts.sizes(), " and key_starts ", key_starts.sizes(),
                 ": expected [clouds + 1] both");
+    TORCH_CHECK(query_starts.size(0) > 1 || (queries.size(0) == 0 && keys.size(0) == 0), op, ": ", queries.size(0),
+                " queries and ", keys.size(0), " keys, but query_starts and key_starts of no clouds");
     if (key_mask.has_value()) {
         chk(*key_mask, name + ": key_mask", at::kBool, 1, &queries);
         TORCH_CHECK(key_mask->size(0) == keys.size(0), op, ": key_mask of ", key_mask->size(0), " values for ", keys.size(0),

@@ -1574,6 +1574,8 @@ def _attention_args(name, queries, keys, values, query_starts, key_starts, max_q
     if query_starts.shape != key_starts.shape or query_starts.shape[0] < 1:
         raise RuntimeError("%s: query_starts %s and key_starts %s: expected [clouds + 1] both"
                            % (name, tuple(query_starts.shape), tuple(key_starts.shape)))
+    if query_starts.shape[0] == 1 and (m > 0 or n > 0):
+        raise RuntimeError("%s: %d queries and %d keys, but query_starts and key_starts of no clouds" % (name, m, n))
     if key_mask is not None:
         _chk(key_mask, name + ": key_mask", torch.bool, 1, dev)
         if key_mask.shape[0] != n:

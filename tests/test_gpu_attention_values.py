@@ -24,6 +24,21 @@ def _starts(*sizes):
     return torch.tensor([sum(sizes[:i]) for i in range(len(sizes) + 1)], dtype=torch.int32, device=DEV)
 
 
+@pytest.mark.parametrize("binding", ["compiled", "ctypes"])
+def test_rows_without_a_cloud_are_refused(ops, binding):
+    # nothing would write their results
+    forward, backward = (ops.BINDINGS[binding][name] for name in ("cross_attention", "cross_attention_grads"))
+    q, none, zero = torch.zeros((4, 2, 16), device=DEV), torch.zeros((0, 2, 16), device=DEV), _starts()
+    lse = torch.zeros((4, 2), device=DEV)
+    for queries, keys in ((q, q), (q, none), (none, q)):
+        plan = (zero, zero, queries.shape[0], keys.shape[0])
+        with pytest.raises(RuntimeError, match="no clouds"):
+            forward(queries, keys, keys, *plan)
+        with pytest.raises(RuntimeError, match="no clouds"):
+            backward(queries, keys, keys, *plan, queries, lse[:queries.shape[0]], queries)
+    assert forward(none, none, none, zero, zero, 0, 0).shape == (0, 2, 16)
+
+
 # One cloud's queries and keys: the parts that few rows are cut into by the length of the other side.
 LENGTHS = [(70, 50), (1, 90), (1, 1500), (2, 4096), (1, 200000), (1000, 40)]
 
