@@ -72,6 +72,10 @@ class CrossAttention(torch.nn.Module):
             clouds = max(p_pc_in.batch_size_host(), p_pc_out.batch_size_host())
             p_ranges = (CloudRanges(p_pc_in, clouds), CloudRanges(p_pc_out, clouds))
         asked, asking = p_ranges
+        for ranges, pc, feats, which in ((asked, p_pc_in, p_in_features, "in"), (asking, p_pc_out, p_out_features, "out")):
+            if not ranges.num_points_ == pc.pts_.shape[0] == feats.shape[0]:
+                raise RuntimeError("CrossAttention: ranges of %d points, p_pc_%s of %d, p_%s_features of %d rows"
+                                   % (ranges.num_points_, which, pc.pts_.shape[0], which, feats.shape[0]))
         queries = self.proj_q_(self.norm_out_(asking.in_order(p_out_features)))
         queries = self.rotary_(queries.reshape(-1, self.num_heads_, self.head_width_), asking.in_order(p_pc_out.pts_))
         both = self.proj_kv_(self.norm_in_(asked.in_order(p_in_features)))

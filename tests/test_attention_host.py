@@ -154,3 +154,20 @@ def test_rotary_layer_deals_its_pairs_to_the_axes():
         lib.pc.layers.RotaryPositions(3, 32, p_pairs=17)
     with pytest.raises(RuntimeError, match="key heads"):
         lib.pc.layers.CrossAttention(3, 8, 8, 4, p_num_key_heads=3)
+
+
+def test_attention_layer_refuses_ranges_of_other_clouds():
+    # before anything is computed, so no GPU is asked: ranges in the wrong order, of another batch, features of another level
+    import pccnn_lib_amd as lib
+    ids = lambda *counts: torch.cat([torch.full((n,), i, dtype=torch.int32) for i, n in enumerate(counts)])
+    coarse, fine = (lib.pc.Pointcloud(torch.rand(sum(c), 3), ids(*c)) for c in ((3, 4), (9, 8)))
+    layer = lib.pc.layers.CrossAttention(3, 8, 8, 2)
+    ranges = (lib.pc.CloudRanges(coarse), lib.pc.CloudRanges(fine))
+    y, x = torch.zeros(7, 8), torch.zeros(17, 8)
+    for args, message in (((coarse, fine, y, x, None, ranges[::-1]), "ranges of 17 points, p_pc_in of 7"),
+                          ((coarse, fine, y, x, None, (ranges[0], ranges[0])), "ranges of 7 points, p_pc_out of 17"),
+                          ((coarse, fine, x, x, None, ranges), "p_in_features of 17 rows"),
+                          ((coarse, fine, y, y, None, ranges), "p_out_features of 7 rows"),
+                          ((coarse, fine, x, y), "p_in_features of 17 rows")):
+        with pytest.raises(RuntimeError, match=message):
+            layer(*args)
