@@ -14,20 +14,20 @@ class CloudRanges(object):
         if clouds < p_pc.batch_size_host():
             raise RuntimeError("CloudRanges: %d clouds, but the batch ids go up to %d"
                                % (clouds, p_pc.batch_size_host() - 1))
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():      # kept by programs that serve first and train later
             counts = torch.bincount(ids.to(torch.int64), minlength=clouds)
             starts = torch.zeros((clouds + 1,), dtype=torch.int64, device=ids.device)
             torch.cumsum(counts, 0, out=starts[1:])
             self.starts_ = starts.to(torch.int32)
             out_of_order = (ids[1:] < ids[:-1]).sum()
             longest, out_of_order = torch.stack([counts.max(), out_of_order]).tolist()
-        self.longest_ = int(longest)
-        self.num_points_ = ids.shape[0]
-        self.order_ = self.inverse_ = None
-        if out_of_order:
-            self.order_ = torch.argsort(ids, stable=True)
-            self.inverse_ = torch.empty_like(self.order_)
-            self.inverse_[self.order_] = torch.arange(ids.shape[0], device=ids.device)
+            self.longest_ = int(longest)
+            self.num_points_ = ids.shape[0]
+            self.order_ = self.inverse_ = None
+            if out_of_order:
+                self.order_ = torch.argsort(ids, stable=True)
+                self.inverse_ = torch.empty_like(self.order_)
+                self.inverse_[self.order_] = torch.arange(ids.shape[0], device=ids.device)
 
     def in_order(self, p_rows):
         """Per-point rows in cloud order (the tensor itself when the batch is stored that way)."""

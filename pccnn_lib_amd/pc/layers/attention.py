@@ -30,9 +30,18 @@ class RotaryPositions(torch.nn.Module):
 
     def plan(self, p_device):
         if p_device not in self.plans_:
-            self.plans_[p_device] = (torch.tensor(self.freqs_host_, dtype=torch.float32, device=p_device),
-                                     torch.tensor(self.axes_host_, dtype=torch.int32, device=p_device))
+            # whoever asks first: the plan outlives a call under inference_mode, whose tensors no training step may save
+            with torch.inference_mode(False):
+                self.plans_[p_device] = (torch.tensor(self.freqs_host_, dtype=torch.float32, device=p_device),
+                                         torch.tensor(self.axes_host_, dtype=torch.int32, device=p_device))
         return self.plans_[p_device]
+
+    def _apply(self, fn, *args, **kwargs):
+        """Moving the module makes the plan of its new place, so that a first call within a graph's capture copies nothing
+        from the host."""
+        super(RotaryPositions, self)._apply(fn, *args, **kwargs)
+        self.plan(fn(torch.empty(0)).device)
+        return self
 
     def forward(self, p_feats, p_pts):
         """p_feats [N, heads, head width], p_pts float32 [N, dims]."""

@@ -171,3 +171,27 @@ def test_attention_layer_refuses_ranges_of_other_clouds():
                           ((coarse, fine, x, y), "p_in_features of 17 rows")):
         with pytest.raises(RuntimeError, match=message):
             layer(*args)
+
+
+def test_what_a_layer_keeps_from_serving_can_be_trained_with():
+    import pccnn_lib_amd as lib
+    pc = lib.pc.Pointcloud(torch.rand(5, 3), torch.tensor([1, 0, 0, 1, 2], dtype=torch.int32))
+    with torch.inference_mode():
+        layer = lib.pc.layers.RotaryPositions(3, 32)
+        kept = list(layer.plan(torch.device("cpu")))
+        ranges = lib.pc.CloudRanges(pc)
+        kept += [ranges.starts_, ranges.order_, ranges.inverse_]
+    assert not any(t.is_inference() for t in kept)
+    rows = torch.rand(5, 4, requires_grad=True)
+    ranges.back(ranges.in_order(rows)).sum().backward()               # (saves order_ and inverse_)
+    assert torch.equal(rows.grad, torch.ones(5, 4))
+
+
+def test_moving_a_rotary_layer_makes_its_plan_there():
+    import pccnn_lib_amd as lib
+    layer = torch.nn.Sequential(lib.pc.layers.RotaryPositions(3, 32))
+    layer.to("meta")
+    freqs, axes = layer[0].plans_[torch.device("meta")]
+    assert freqs.dtype == torch.float32 and axes.dtype == torch.int32 and freqs.shape == axes.shape == (16,)
+    layer.to(torch.bfloat16)
+    assert all(plan[0].dtype == torch.float32 for plan in layer[0].plans_.values()) and not layer.state_dict()

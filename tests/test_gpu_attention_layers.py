@@ -174,3 +174,34 @@ def test_one_token_per_cloud_as_it_is_served(lib):
         pair = layer(points, twice, y, x.repeat_interleave(2, 0))
     assert float((pair[::2] - alone).abs().max()) < 1e-5 * float(alone.abs().max())
     assert float((pair[1::2] - alone).abs().max()) < 1e-5 * float(alone.abs().max())
+
+
+def test_serving_first_and_training_afterwards(lib):
+    torch.manual_seed(4)
+    pc_in, pc_out = _clouds(lib, [50, 20], 8, True), _clouds(lib, [9, 30], 9, True)
+    served, trained = (lib.pc.layers.CrossAttention(3, 12, 16, 2).to(DEV) for _ in range(2))
+    trained.load_state_dict(served.state_dict())
+    y, x = torch.randn((70, 12), device=DEV), torch.randn((39, 16), device=DEV)
+    with torch.inference_mode():
+        ranges = (lib.pc.CloudRanges(pc_in), lib.pc.CloudRanges(pc_out))
+        first = served(pc_in, pc_out, y, x, p_ranges=ranges)
+    for layer, kept in ((served, ranges), (trained, None)):
+        layer(pc_in, pc_out, y, x, p_ranges=kept).square().sum().backward()
+    assert torch.equal(first, trained(pc_in, pc_out, y, x))
+    for a, b in zip(served.parameters(), trained.parameters()):
+        assert torch.equal(a.grad, b.grad)
+
+
+def test_a_rotary_layers_first_call_in_a_graph(lib):
+    layer = lib.pc.layers.RotaryPositions(3, 32).to(DEV)
+    feats, pts = torch.randn((40, 2, 32), device=DEV), torch.rand((40, 3), device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(feats, pts)
+    for _ in range(3):
+        feats.copy_(torch.randn((40, 2, 32), device=DEV))
+        want = layer(feats, pts)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
