@@ -852,7 +852,8 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(const float *__
 
 // ------------------------------------------------------------------------------------------------- host side
 
-int attn_check(const char *name, const pccnn_attention *p)
+// Everything but the pointers, which a caller who asks for the workspace's size need not have yet.
+int attn_check_sizes(const char *name, const pccnn_attention *p)
 {
     PCCNN_REQUIRE(p != nullptr, PCCNN_ERR_INVALID, "%s: null pointer", name);
     PCCNN_REQUIRE(pccnn_type_ok(p->type), PCCNN_ERR_UNSUPPORTED, "%s: element type %d (f32 and bf16 only)", name, p->type);
@@ -875,6 +876,12 @@ int attn_check(const char *name, const pccnn_attention *p)
     const int64_t strides[] = {p->q_stride_n, p->q_stride_h, p->k_stride_n, p->k_stride_h, p->v_stride_n, p->v_stride_h};
     for (int64_t s : strides)
         PCCNN_REQUIRE(s >= 0, PCCNN_ERR_INVALID, "%s: a stride of %lld elements", name, (long long)s);
+    return PCCNN_OK;
+}
+int attn_check(const char *name, const pccnn_attention *p)
+{
+    const int rc = attn_check_sizes(name, p);
+    if (rc != PCCNN_OK) return rc;
     PCCNN_REQUIRE(p->m == 0 || p->clouds == 0 || (p->queries && p->query_starts && p->key_starts), PCCNN_ERR_INVALID,
                   "%s: null pointer", name);
     PCCNN_REQUIRE(p->n == 0 || p->clouds == 0 || (p->keys && p->values && p->query_starts && p->key_starts),
@@ -1088,9 +1095,7 @@ size_t forward_bytes(const AttnArgs &a)
 
 extern "C" size_t pccnn_attention_workspace_bytes(const pccnn_attention *p, int backward)
 {
-    if (p == nullptr || !pccnn_type_ok(p->type) || p->heads < 1 || p->key_heads < 1 || p->clouds < 1 || p->m < 0 || p->n < 0 ||
-        p->width < 1 || p->width > kMaxWidth)
-        return 256;
+    if (attn_check_sizes("attention_workspace_bytes", p) != PCCNN_OK || p->clouds < 1) return 256;   // (the call will refuse)
     AttnArgs a = attn_args(p);
     AttnKernel kernel = attn_plan_rows(a, p, !backward);
     size_t rows = planes_bytes(a, p->type, kernel, p->n, a.key_heads);

@@ -195,3 +195,21 @@ def test_moving_a_rotary_layer_makes_its_plan_there():
     assert freqs.dtype == torch.float32 and axes.dtype == torch.int32 and freqs.shape == axes.shape == (16,)
     layer.to(torch.bfloat16)
     assert all(plan[0].dtype == torch.float32 for plan in layer[0].plans_.values()) and not layer.state_dict()
+
+
+def test_a_problem_that_is_refused_asks_for_no_workspace(lib):
+    # the size is asked for before the call: a wrong length must end in the call's message, not in an allocation that fails
+    from pccnn_lib_amd import _lib
+    p = _lib.Attention()
+    p.m, p.n, p.max_queries, p.max_keys = 10, 20, 10, 20
+    p.type, p.clouds, p.heads, p.key_heads, p.width, p.scale = 0, 1, 4, 2, 16, 0.25
+    good = [lib.pccnn_attention_workspace_bytes(ctypes.byref(p), backward) for backward in (0, 1)]
+    assert good[0] >= 256 and good[1] >= 2 * 10 * 4 * 4
+    for name, value in (("max_keys", 21), ("max_keys", 1 << 62), ("max_queries", 1 << 62), ("max_queries", -1), ("m", 1 << 40),
+                        ("heads", 3), ("width", 129), ("scale", -1.0), ("k_stride_n", -1)):
+        before = getattr(p, name)
+        setattr(p, name, value)
+        assert [lib.pccnn_attention_workspace_bytes(ctypes.byref(p), backward) for backward in (0, 1)] == [256, 256], name
+        assert lib.pccnn_attention_forward(ctypes.byref(p), 16, None, None, 0, None) != 0
+        setattr(p, name, before)
+    assert good == [lib.pccnn_attention_workspace_bytes(ctypes.byref(p), backward) for backward in (0, 1)]
