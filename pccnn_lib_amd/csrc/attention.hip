@@ -919,14 +919,21 @@ AttnArgs attn_args(const pccnn_attention *p)
     return a;
 }
 
-// Whether the walked side goes to LDS without passing registers.  bf16: where rows are whole 16-byte units with 32-bit
-// offsets within a tile.  f32: where it is worth turning into planes of terms first, that is where each cloud has several
-// own tiles (`own`: rows of all clouds) to walk it.
-bool attn_direct(const AttnArgs &a, int type, const AttnStream &one, const AttnStream &two, int64_t own)
+// Whether a tile's rows, strides apart, are within 32-bit offsets in bytes of its first one.
+bool attn_reachable(int64_t stride_n, int64_t stride_h, int group)
 {
-    if (type == PCCNN_TYPE_F32) return own >= (int64_t)kPlanesFrom * kOwn * a.clouds;
-    const int64_t reach = 64 * std::max(one.n, two.n) + std::max(64, a.group) * std::max(one.h, two.h) + kMaxWidth;
-    return one.wide == 2 && two.wide == 2 && reach < (1ll << 30);
+    return std::max(stride_n, stride_h) < (1ll << 30) &&
+           64 * stride_n + std::max<int64_t>(64, group) * stride_h + kMaxWidth < (1ll << 30);
+}
+// Whether the walked side, of `heads` heads, goes to LDS without passing registers.  bf16: where rows are whole 16-byte units
+// with 32-bit offsets within a tile.  f32: where it is worth turning into planes of terms first, that is where each cloud has
+// several own tiles (`own`: rows of all clouds) to walk it, and the planes' tiles have such offsets.
+bool attn_direct(const AttnArgs &a, int type, const AttnStream &one, const AttnStream &two, int heads, int64_t own)
+{
+    const int64_t padded = (a.width + 31) / 32 * 32;
+    if (type == PCCNN_TYPE_F32)
+        return own >= (int64_t)kPlanesFrom * kOwn * a.clouds && attn_reachable(heads * padded, padded, a.group);
+    return one.wide == 2 && two.wide == 2 && attn_reachable(std::max(one.n, two.n), std::max(one.h, two.h), a.group);
 }
 
 // Calls f(type, padded width) for the instantiation that serves this type and head width.
@@ -1033,7 +1040,7 @@ AttnKernel attn_plan_rows(AttnArgs &a, const pccnn_attention *p, bool forward)
 {
     a.one = {a.k, a.k_n, a.k_h, 0, a.wide_k, a.width / 8};
     a.two = {a.v, a.v_n, a.v_h, 0, a.wide_v, a.width / 8};
-    const bool direct = attn_direct(a, p->type, a.one, a.two, p->m * a.group);
+    const bool direct = attn_direct(a, p->type, a.one, a.two, a.key_heads, p->m * a.group);
     const AttnKernel kernel = forward ? attn_kernel_of<ATTN_FORWARD>(p->type, a.width, direct)
                                       : attn_kernel_of<ATTN_QUERIES>(p->type, a.width, direct);
     attn_plan(a, kernel, p->type, forward ? 2 : 3, p->max_queries * a.group, p->m * a.group, p->max_keys, p->n);
@@ -1226,7 +1233,7 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
         }
         a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
         a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};
-        const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(a, p->type, a.one, a.two, p->n));
+        const AttnKernel kernel = attn_plan_keys(a, p, attn_direct(a, p->type, a.one, a.two, a.heads, p->n));
         const int64_t count = a.n * a.key_heads * a.width;
         a.d_k = d_keys;
         a.d_v = d_values;

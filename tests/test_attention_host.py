@@ -213,3 +213,22 @@ def test_a_problem_that_is_refused_asks_for_no_workspace(lib):
         assert lib.pccnn_attention_forward(ctypes.byref(p), 16, None, None, 0, None) != 0
         setattr(p, name, before)
     assert good == [lib.pccnn_attention_workspace_bytes(ctypes.byref(p), backward) for backward in (0, 1)]
+
+
+def test_planes_are_made_only_where_a_tiles_rows_are_within_32_bit_offsets(lib):
+    # f32 queries enough for planes of the keys: 6 bytes per padded feature of both tensors, unless a tile of 64 keys spans 2^31
+    # bytes of a plane (heads x padded width x 2 bytes a key)
+    from pccnn_lib_amd import _lib
+
+    def forward_bytes(heads, width, m=4000, n=64):
+        p = _lib.Attention()
+        p.m, p.n, p.max_queries, p.max_keys = m, n, m, n
+        p.type, p.clouds, p.heads, p.key_heads, p.width, p.scale = 0, 1, heads, heads, width, 0.25
+        return lib.pccnn_attention_workspace_bytes(ctypes.byref(p), 0)
+    for width, padded in ((1, 32), (40, 64), (96, 96), (128, 128)):
+        planes = lambda heads: 2 * 6 * 64 * heads * padded
+        fits = (1 << 30) // (64 * padded) - 64
+        assert planes(8) <= forward_bytes(8, width) < planes(8) + 1024
+        assert planes(fits) <= forward_bytes(fits, width) < planes(fits) + 1024
+        for heads in ((1 << 30) // (64 * padded), 1 << 19, 1 << 20):
+            assert forward_bytes(heads, width) < 1024
