@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+from tests import attention_f32
+
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda:0"
@@ -159,3 +161,30 @@ def test_a_key_that_scores_minus_infinity_has_no_gradient(ops, queries, keys, he
     got = ops.cross_attention_grads(q, k, v, *plan, out, lse, g, grad_mask=ops.GRAD_KEYS)[1:]
     for a, b in zip(got, ops.cross_attention_grads(q, k, v, *plan, out, lse, g, key_mask=mask, grad_mask=ops.GRAD_KEYS)[1:]):
         assert torch.equal(a, b) and float(a[7].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("queries,keys,width,spread", attention_f32.CASES)
+def test_f32_products_keep_f32_accuracy(ops, queries, keys, width, spread):
+    # two heads of the second of two clouds, each against 64 bits; what the bounds tell apart: test_attention_f32.py
+    heads = [attention_f32.inputs(queries, keys, width, spread, seed) for seed in range(2)]
+    small = attention_f32.inputs(3, 5, width, spread)
+    q, k, v, g = (torch.stack([torch.cat([small[i], head[i]]) for head in heads], 1).to(DEV) for i in range(4))
+    plan = (_starts(3, queries), _starts(5, keys), max(3, queries), max(5, keys))
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    results = [out, lse] + list(ops.cross_attention_grads(q, k, v, *plan, out, lse, g))
+    for h, head in enumerate(heads):
+        got = [t[5 if t.shape[0] == 5 + keys and i > 2 else 3:, h] for i, t in enumerate(results)]
+        for name, error in attention_f32.off(got, attention_f32.exact(*head)).items():
+            assert error < attention_f32.MOST[name], (name, h, error)
+
+
+@pytest.mark.parametrize("queries,keys", [(16, 20000), (40, 9000)])
+def test_f32_products_keep_f32_accuracy_in_many_parts(ops, queries, keys):
+    # few queries over many keys are split and joined; the sums are longer, of parts of at most some hundred keys
+    q, k, v, g = (t.unsqueeze(1).to(DEV) for t in attention_f32.inputs(queries, keys, 64, 4.0))
+    plan = (_starts(queries), _starts(keys), queries, keys)
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    results = [out, lse] + list(ops.cross_attention_grads(q, k, v, *plan, out, lse, g))
+    want = attention_f32.exact(*(t[:, 0].cpu() for t in (q, k, v, g)))
+    for name, error in attention_f32.off([t[:, 0] for t in results], want).items():
+        assert error < attention_f32.MOST[name], (name, error)
