@@ -7,7 +7,8 @@
 // squares are taken of centred values and a row is read once.  A lane keeps the same columns for every row it works on:
 // gamma, beta and the two column sums of the backward pass stay in registers over the whole loop, and one small second
 // kernel adds the workgroups' sums in a fixed order (no atomics: the same bits from run to run).  Rows longer than a
-// wavefront's registers hold (2048 values) take a workgroup each and are read again from the caches instead.
+// wavefront's registers hold (2048 values, or 1024 where rows only allow loads of single values: f32 rows that are not 16-byte
+// aligned, odd channel counts) take a workgroup each and are read again from the caches instead.
 //
 // Bound by HBM.  800000 rows of 64 bf16 values: forward 37 us = 5.5 TB/s, backward 65 us = 4.7 TB/s (three streams, the
 // column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 17
@@ -25,6 +26,7 @@ constexpr int kMaxBlocks = 1024;             // workgroups of the persistent ker
 // The backward pass has as many wavefronts in half as many workgroups: every one leaves a row of column sums.
 constexpr int kBackThreads = 512, kBackWaves = kBackThreads / PCCNN_WAVE, kBackBlocks = 512;
 constexpr int kRegisterColumns = 2048;       // the longest row that one wavefront holds (32 values per lane)
+constexpr int kMostLoads = 16;               // in at most so many loads per lane: single values reach 1024
 
 // ------------------------------------------------------------------------------------ rows in registers
 
@@ -351,7 +353,7 @@ int norm_align(int64_t c, int type, const void *a, int64_t a_stride, const void 
     return 1;
 }
 // Rows that fit a wavefront's registers at their load width.
-bool norm_in_registers(const NormShape &s) { return s.vec * s.chunks <= kRegisterColumns / PCCNN_WAVE && s.chunks <= 16; }
+bool norm_in_registers(const NormShape &s) { return s.vec * s.chunks <= kRegisterColumns / PCCNN_WAVE && s.chunks <= kMostLoads; }
 
 unsigned norm_blocks(int64_t n, int lanes, int waves, int most)
 {

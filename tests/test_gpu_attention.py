@@ -110,6 +110,27 @@ def test_norm_of_a_views_rows_and_of_unaligned_rows(ops):
                 assert torch.allclose(a.float(), b.float(), rtol=u, atol=u * float(b.float().abs().max()))
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [1000, 1024, 1026, 1536, 2048])
+def test_norm_of_long_rows_by_every_load_width(ops, type, channels):
+    # column slices: 16-byte loads, pairs of bf16 values, single values (which take the workgroup per row from 1025 on)
+    dtype, gen = TYPES[type], _gen(channels)
+    wide = [(_normal(gen, 33, channels + 8) * 1.5 + 0.7).to(dtype).to(DEV) for _ in range(2)]
+    gamma, beta = 1.0 + 0.3 * _normal(gen, channels), 0.2 * _normal(gen, channels)
+    for lo in (0, 2, 3):
+        x, g = (t[:, lo:lo + channels] for t in wide)
+        out, stats = ops.layer_norm(x, gamma.to(DEV), beta.to(DEV), 1e-5, return_stats=True)
+        d_feats, d_gamma, d_beta = ops.layer_norm_grads(x, gamma.to(DEV), stats, g)
+        y, dx, dg, db, xhat, rstd = _norm_exact(x.cpu(), gamma, beta, 1e-5, g.cpu())
+        u, f, s = UNIT[dtype], UNIT[torch.float32], (g.cpu().double() * gamma.double()).abs()
+        size = 1.0 + x.cpu().double().abs().amax(1, keepdim=True) * rstd
+        _within(out, y, u * y.abs() + f * ((xhat * gamma.double()).abs() + beta.double().abs() + size * gamma.double().abs()), "out")
+        _within(d_feats, dx, u * dx.abs() + f * rstd * size * (s + s.mean(1, keepdim=True)
+                                                               + (xhat.abs() * (s * xhat.abs()).mean(1, keepdim=True))), "dx")
+        _within(d_gamma, dg, f * dg.abs() + f * (g.cpu().double().abs() * (xhat.abs() + size)).sum(0), "dgamma")
+        _within(d_beta, db, f * db.abs() + f * g.cpu().double().abs().sum(0), "dbeta")
+
+
 def test_norm_statistics_survive_a_large_mean_and_constant_rows(ops):
     # the squares are taken of centred values: a mean of 10^4 leaves the variance of 1 intact
     gen = _gen(6)
