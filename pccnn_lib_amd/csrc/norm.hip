@@ -372,6 +372,17 @@ unsigned norm_back_blocks(int64_t n, const NormShape &s, bool alone)
     return norm_blocks(n, s.lanes, kBackWaves, kBackBlocks);
 }
 
+// Rows of column sums that a backward pass leaves: of long rows, and at most (long rows that do not fit registers only for
+// their loads' width, from 1025 values on, leave 204 or fewer).
+int64_t norm_wide_parts(int64_t n, int64_t c)
+{
+    return std::min(n, std::max<int64_t>(1, kMaxBlocks / pccnn_ceil_div(c, kThreads)));
+}
+int64_t norm_most_parts(int64_t n, int64_t c)
+{
+    return c <= kRegisterColumns ? std::min<int64_t>(n, kBackBlocks) : norm_wide_parts(n, c);
+}
+
 struct NormForward {
     const void *feats;
     int64_t stride;
@@ -446,7 +457,7 @@ int norm_check(const char *name, int type, int weight_type, int64_t n, int64_t c
 extern "C" size_t pccnn_layer_norm_workspace_bytes(int64_t n, int64_t channels)
 {
     if (n <= 0 || channels <= 0) return 256;
-    return pccnn_align((size_t)std::min<int64_t>(kMaxBlocks, n) * 2 * (size_t)channels * sizeof(float));
+    return pccnn_align((size_t)norm_most_parts(n, channels) * 2 * (size_t)channels * sizeof(float));
 }
 
 extern "C" int pccnn_layer_norm_forward(const void *feats, int type, int64_t row_stride, const void *gamma,
@@ -493,7 +504,7 @@ extern "C" int pccnn_layer_norm_backward(const void *feats, int type, int64_t ro
     float *partial = nullptr;
     if (columns && n > 0) {
         PccnnArena arena(workspace, workspace_bytes);
-        partial = arena.take<float>((size_t)std::min<int64_t>(kMaxBlocks, n) * 2 * (size_t)channels);
+        partial = arena.take<float>((size_t)norm_most_parts(n, channels) * 2 * (size_t)channels);
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "layer_norm_grads: workspace of %zu bytes is too small",
                       workspace_bytes);
     }
@@ -515,7 +526,7 @@ extern "C" int pccnn_layer_norm_backward(const void *feats, int type, int64_t ro
                                               str});
         } else {
             const unsigned blocks = (unsigned)std::min<int64_t>(n, 16384);
-            parts = (int)std::min<int64_t>(n, std::max<int64_t>(1, kMaxBlocks / pccnn_ceil_div(channels, kThreads)));
+            parts = (int)norm_wide_parts(n, channels);
             const dim3 grid((unsigned)pccnn_ceil_div(channels, kThreads), (unsigned)parts);
             auto wide = [&](auto zero) {
                 using T = decltype(zero);

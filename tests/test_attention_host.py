@@ -232,3 +232,11 @@ def test_planes_are_made_only_where_a_tiles_rows_are_within_32_bit_offsets(lib):
         assert planes(fits) <= forward_bytes(fits, width) < planes(fits) + 1024
         for heads in ((1 << 30) // (64 * padded), 1 << 19, 1 << 20):
             assert forward_bytes(heads, width) < 1024
+
+
+def test_layer_norm_asks_for_the_sums_that_it_leaves(lib):
+    # 1024 rows of 10^6 channels: few rows of sums, not as many as workgroups could leave of short ones (8 GB)
+    size = lib.pccnn_layer_norm_workspace_bytes
+    assert size(1 << 20, 1 << 20) <= 1 * 2 * (1 << 20) * 4 + 256
+    assert 8 * 5000 * 51 <= size(100000, 5000) <= 8 * 5000 * 64
+    assert 8 * 64 * 512 <= size(100000, 64) <= 8 * 64 * 1024 and size(3, 64) >= 8 * 64 * 3
