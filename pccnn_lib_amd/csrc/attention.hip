@@ -13,8 +13,8 @@
 // (attention_tiles.h).  dq and dk / dv are two kernels that each recompute S: 7 products instead of 5, no atomics, the
 // same bits from run to run.
 //
-// bf16: P and dS are rounded to bf16 as operands, D is formed from the rounded output, results are rounded once; all sums
-// and the softmax are f32.  f32: three bf16 terms per value, six products (attention_tiles.h).
+// bf16: P and dS are rounded to bf16 as operands (but P of few rows, see attention_fwd_kernel), D is formed from the rounded
+// output, results are rounded once; all sums and the softmax are f32.  f32: three bf16 terms per value, six products (attention_tiles.h).
 //
 // Tiles go from memory to LDS without passing registers, the next while one is worked on.  What bounds the large cases is
 // the card's power: matrix pipe 45 - 60 % and vector ALU 50 - 77 % busy at 1.65 - 2.1 GHz of 2.4, and neither a wider
@@ -337,7 +337,12 @@ __device__ __forceinline__ float log_sum(float top, float sum)
     return sum > 0.0f ? top * (1.0f / kLog2e) + logf(sum) : NAN;
 }
 
-template <typename T, int DP, bool DIRECT>
+// PTERMS: the terms that probabilities are carried in, as many as the values' in f32.  In bf16 one, since a second costs what
+// the large cases have least of (34123 x 100000 keys 6.8 -> 9.2 ms, 8 x 256 x 100000 555 -> 740 us); but two where a cloud has at
+// most 32 rows (ATTN_FEW), one wavefront's, which wait for memory: one row over 16 x 4096 keys 32.5 -> 33.5 us, over 10^6 keys
+// 110 and 110, 8 x 32 rows over 20000 keys 49 -> 51, 200 x 20 over 500 28 -> 30.  The result then has its own rounding alone
+// (0.0017 of it in the 2-norm), else the probabilities' too (0.0023).
+template <typename T, int DP, bool DIRECT, int PTERMS>
 __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
 {
     constexpr int TERMS = AttnTerms<T>::value;
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
         auto key_rows = [&](int i) { return tile_k.rows(32 * (i / STEPS) + (lane & 31), 2 * (i % STEPS) + half); };
         ahead.template prime<ROWS / 32 * STEPS>(key_rows);
         ahead.template run<ROWS / 32 * STEPS>(key_rows, [&](int i, const AttnFrag<TERMS> &f) {
-            attn_mma<TERMS>(s[i / STEPS], f, q[i % STEPS]);
+            attn_mma(s[i / STEPS], f, q[i % STEPS]);
         });
         auto value_columns = [&](int i) { return tile_v.columns(16 * (i / BLOCKS), 32 * (i % BLOCKS), lane); };
         ahead.template prime<ROWS / 16 * BLOCKS>(value_columns);
@@ -419,7 +424,7 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[dt][i] *= shrink;
         }
-        AttnFrag<TERMS> p;
+        AttnFrag<PTERMS> p;
         ahead.template run<ROWS / 16 * BLOCKS>(value_columns, [&](int i, const AttnFrag<TERMS> &f) {
             if (i % BLOCKS == 0) {                                   // the next sixteen keys' probabilities
                 pccnn_f32x16 &x = s[i / BLOCKS / 2];
@@ -429,9 +434,9 @@ __global__ __launch_bounds__(kThreads) void attention_fwd_kernel(AttnArgs a)
                     x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c2, -top));
                     sums[j % 2] += x[j];
                 }
-                p = half_of<TERMS>(x, i / BLOCKS % 2);
+                p = half_of<PTERMS>(x, i / BLOCKS % 2);
             }
-            attn_mma<TERMS>(acc[i % BLOCKS], f, p);
+            attn_mma(acc[i % BLOCKS], f, p);
         });
     };
     for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
@@ -652,9 +657,9 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
             ahead.template prime<2 * STEPS>(rows);
             ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
                 if (i < STEPS)
-                    attn_mma<TERMS>(s, f, q[i]);
+                    attn_mma(s, f, q[i]);
                 else
-                    attn_mma<TERMS>(dp, f, g[i - STEPS]);
+                    attn_mma(dp, f, g[i - STEPS]);
             });
             auto columns = [&](int i) { return tile_k.columns(32 * t + 16 * (i / BLOCKS), 32 * (i % BLOCKS), lane); };
             ahead.template prime<2 * BLOCKS>(columns);
@@ -668,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
                         s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -shift)) * (dp[j] - delta);
                     ds = half_of<TERMS>(s, i / BLOCKS);
                 }
-                attn_mma<TERMS>(acc[i % BLOCKS], f, ds);
+                attn_mma(acc[i % BLOCKS], f, ds);
             });
         }
     };
@@ -764,9 +769,9 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
             ahead.template prime<2 * STEPS>(rows);
             ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
                 if (i < STEPS)
-                    attn_mma<TERMS>(s, f, k[i]);
+                    attn_mma(s, f, k[i]);
                 else
-                    attn_mma<TERMS>(dp, f, v[i - STEPS]);
+                    attn_mma(dp, f, v[i - STEPS]);
             });
             // sixteen rows at a time: first the output gradients' columns (dv), then the queries' (dk)
             auto columns = [&](int i) {
@@ -792,9 +797,9 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_kernel(AttnArgs a)
                     ds = half_of<TERMS>(dp, h);
                 }
                 if (i / BLOCKS % 2 == 0)
-                    attn_mma<TERMS>(dv[i % BLOCKS], f, p);
+                    attn_mma(dv[i % BLOCKS], f, p);
                 else
-                    attn_mma<TERMS>(dk[i % BLOCKS], f, ds);
+                    attn_mma(dk[i % BLOCKS], f, ds);
             });
         }
     };
@@ -961,7 +966,7 @@ template <typename KERNEL> int attn_slots(KERNEL kernel, size_t lds)
     }
     return cus * per_cu;
 }
-enum AttnPass { ATTN_FORWARD, ATTN_QUERIES, ATTN_KEYS };
+enum AttnPass { ATTN_FORWARD, ATTN_FEW, ATTN_QUERIES, ATTN_KEYS };
 
 // The kernel of a pass, its LDS and the workgroups that are resident at once (asked once).
 struct AttnKernel {
@@ -973,7 +978,9 @@ struct AttnKernel {
 template <typename T, int DP, bool DIRECT, AttnPass PASS> AttnKernel attn_kernel()
 {
     AttnKernel k;
-    if constexpr (PASS == ATTN_FORWARD) k.run = attention_fwd_kernel<T, DP, DIRECT>;
+    constexpr int TERMS = AttnTerms<T>::value;
+    if constexpr (PASS == ATTN_FORWARD) k.run = attention_fwd_kernel<T, DP, DIRECT, TERMS>;
+    if constexpr (PASS == ATTN_FEW) k.run = attention_fwd_kernel<T, DP, DIRECT, TERMS == 1 ? 2 : TERMS>;
     if constexpr (PASS == ATTN_QUERIES) k.run = attention_dq_kernel<T, DP, DIRECT>;
     if constexpr (PASS == ATTN_KEYS) k.run = attention_dkv_kernel<T, DP, DIRECT>;
     k.rows = attn_tile_rows<T, DP>();
@@ -1041,8 +1048,9 @@ AttnKernel attn_plan_rows(AttnArgs &a, const pccnn_attention *p, bool forward)
     a.one = {a.k, a.k_n, a.k_h, 0, a.wide_k, a.width / 8};
     a.two = {a.v, a.v_n, a.v_h, 0, a.wide_v, a.width / 8};
     const bool direct = attn_direct(a, p->type, a.one, a.two, a.key_heads, p->m * a.group);
-    const AttnKernel kernel = forward ? attn_kernel_of<ATTN_FORWARD>(p->type, a.width, direct)
-                                      : attn_kernel_of<ATTN_QUERIES>(p->type, a.width, direct);
+    const AttnKernel kernel = !forward ? attn_kernel_of<ATTN_QUERIES>(p->type, a.width, direct)
+                              : p->max_queries * a.group <= 32 ? attn_kernel_of<ATTN_FEW>(p->type, a.width, direct)
+                                                               : attn_kernel_of<ATTN_FORWARD>(p->type, a.width, direct);
     attn_plan(a, kernel, p->type, forward ? 2 : 3, p->max_queries * a.group, p->m * a.group, p->max_keys, p->n);
     return kernel;
 }

@@ -24,16 +24,18 @@ template <int TERMS> struct AttnFrag {
     pccnn_bf16x8 t[TERMS];
 };
 
-template <int TERMS> __device__ __forceinline__ void attn_mma(pccnn_f32x16 &c, const AttnFrag<TERMS> &a,
-                                                             const AttnFrag<TERMS> &b)
+// a and b in three terms each, or a in one and b in one or two.
+template <int TERMS, int B> __device__ __forceinline__ void attn_mma(pccnn_f32x16 &c, const AttnFrag<TERMS> &a,
+                                                                    const AttnFrag<B> &b)
 {
+    static_assert(TERMS == B || (TERMS == 1 && B == 2), "");
     if constexpr (TERMS == 3) {                         // smallest products first
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[2], b.t[0], c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[1], c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[2], c, 0, 0, 0);
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], c, 0, 0, 0);
     }
+    if constexpr (B >= 2) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], c, 0, 0, 0);
 }
 

@@ -188,3 +188,25 @@ def test_f32_products_keep_f32_accuracy_in_many_parts(ops, queries, keys):
     want = attention_f32.exact(*(t[:, 0].cpu() for t in (q, k, v, g)))
     for name, error in attention_f32.off([t[:, 0] for t in results], want).items():
         assert error < attention_f32.MOST[name], (name, error)
+
+
+@pytest.mark.parametrize("clouds,queries,keys,heads,key_heads,width,off", [
+    (16, 1, 4096, 8, 8, 64, 0.0), (1, 1, 200000, 8, 2, 64, 0.0), (3, 8, 5000, 8, 2, 32, 0.2), (2, 32, 700, 16, 16, 128, 0.0),
+    (4, 3, 900, 8, 1, 33, 0.5), (40, 1, 300, 8, 4, 96, 0.0)])
+def test_a_few_bf16_queries_are_as_exact_as_their_results_type(ops, clouds, queries, keys, heads, key_heads, width, off):
+    # up to 32 rows to a cloud and key head: the only rounding to bf16 is the result's own.  Probabilities of two terms are off
+    # by 2^-17, which adds nothing to that in the 2-norm (rounded to one they would add as much again: 1.41 times)
+    gen = torch.Generator().manual_seed(keys + width)
+    normal = lambda n, h: _normal(gen, n, h, width).bfloat16()
+    q, k, v = normal(clouds * queries, heads) * 1.5, normal(clouds * keys, key_heads), normal(clouds * keys, key_heads)
+    live = torch.rand(clouds * keys, generator=gen) >= off
+    plan = (_starts(*[queries] * clouds), _starts(*[keys] * clouds), queries, keys)
+    out = ops.cross_attention(q.to(DEV), k.to(DEV), v.to(DEV), *plan, key_mask=live.to(DEV) if off else None).double().cpu()
+    shape = lambda t, n: t.double().reshape(clouds, n, -1, width).transpose(1, 2)
+    q, k, v = shape(q, queries), shape(k, keys), shape(v, keys)
+    k, v = (t.repeat_interleave(heads // key_heads, 1) for t in (k, v))
+    scores = (q @ k.transpose(2, 3)) * width ** -0.5
+    scores = scores.masked_fill(~live.reshape(clouds, 1, 1, keys), -math.inf)
+    want = (torch.softmax(scores, 3) @ v).transpose(1, 2).reshape(out.shape)
+    own = (want.bfloat16().double() - want).norm()
+    assert float((out - want).norm() / own) < 1.05
