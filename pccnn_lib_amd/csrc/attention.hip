@@ -14,7 +14,8 @@
 // same bits from run to run.
 //
 // bf16: P and dS are rounded to bf16 as operands (but P of few rows, see attention_fwd_kernel), D is formed from the rounded
-// output, results are rounded once; all sums and the softmax are f32.  f32: three bf16 terms per value, six products (attention_tiles.h).
+// output (but among few keys, see attention_dq_kernel), results are rounded once; all sums and the softmax are f32.
+// f32: three bf16 terms per value, six products (attention_tiles.h).
 //
 // Tiles go from memory to LDS without passing registers, the next while one is worked on.  What bounds the large cases is
 // the card's power: matrix pipe 45 - 60 % and vector ALU 50 - 77 % busy at 1.65 - 2.1 GHz of 2.4, and neither a wider
@@ -544,10 +545,10 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(AttnArgs a, int l
 
 // ------------------------------------------------------------------------------------------------- backward
 
-// What the kernel of dk and dv needs of a row, for a call that wants no dq (whose kernel leaves it on the way): D = dO . O,
+// What the kernel of dk and dv needs of a row, for an f32 call that wants no dq (whose kernel leaves it on the way): D = dO . O,
 // and L in units of log 2 (+inf for a row without keys: every P is zero).  Two lanes to a row, which add in the order of
 // the halves of a wavefront there: the same bits.
-template <typename T> __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a)
+__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttnArgs a)
 {
     const int64_t token = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 2;
     const bool live = token < a.m * a.heads;
@@ -556,9 +557,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void attention_rows
     float delta = 0.0f;
     if (live)
         for (int col = 8 * (threadIdx.x % 2); col < a.width; col += 16) {
-            AttnChunk<T> o, d;
-            attn_load(o, (const T *)a.o + token * a.width, col, a.width, a.wide_o);
-            attn_load(d, (const T *)a.g + query * a.g_n + head * a.g_h, col, a.width, a.wide_g);
+            AttnChunk<float> o, d;
+            attn_load(o, (const float *)a.o + token * a.width, col, a.width, a.wide_o);
+            attn_load(d, (const float *)a.g + query * a.g_n + head * a.g_h, col, a.width, a.wide_g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) delta = fmaf(attn_value(o, i), attn_value(d, i), delta);
         }
@@ -583,6 +584,9 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     if (block >= a.blocks) return;
     const AttnBlock b(a, block, a.k_starts);
     if (b.tile * kOwn >= b.rows) return;
+    const bool one_tile = TERMS == 1 && b.keys <= ROWS;              // D is formed from the probabilities (below)
+    const bool wanted = a.out != nullptr;                            // else the rows' statistics alone
+    if (!wanted && b.split != 0) return;
     const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE, half = lane >> 5;
     const int row = b.tile * kOwn + wave * 32 + (lane & 31);
     const bool working = b.tile * kOwn + wave * 32 < b.rows;
@@ -595,7 +599,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     uint8_t flag = 0;
     k.start(a.one, k_at, 1, key);
     v.start(a.two, v_at, 1, key);
-    if (key < end) {
+    if (key < end && (wanted || one_tile)) {
         flag = key_flag(a, b, key, lane);
         live = live_keys(a, b, key, flag, ROWS);
         k.fetch(a.one, k_at, 1, key, b.keys, live, a.mask != nullptr, a.width, Tile{lds});
@@ -627,11 +631,63 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     const float lse = real ? a.lse[token] : -INFINITY;
     const float shift = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys: every P is zero
     if (lse == -INFINITY) delta = 0.0f;
+    const float c2 = a.scale * kLog2e;
+    // S and dP of 32 keys of a tile
+    auto both = [&](const Tile &tile_k, const Tile &tile_v, int t, pccnn_f32x16 &s, pccnn_f32x16 &dp) {
+        clear(s);
+        clear(dp);
+        AttnAhead<TERMS> ahead;
+        auto rows = [&](int i) { return (i < STEPS ? tile_k : tile_v).rows(32 * t + (lane & 31), 2 * (i % STEPS) + half); };
+        ahead.template prime<2 * STEPS>(rows);
+        ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
+            if (i < STEPS)
+                attn_mma(s, f, q[i]);
+            else
+                attn_mma(dp, f, g[i - STEPS]);
+        });
+    };
+    // Waits for a tile that was fetched.
+    auto land = [&](uint16_t *here, const uint64_t now) {
+        if constexpr (DIRECT) {
+            attn_landed();
+        } else {
+            k.put(Tile{here}, now);
+            v.put(Tile{here + Tile::ELEMENTS}, now);
+            __syncthreads();
+        }
+    };
+    // bf16: O is rounded, and D of a rounded O is off by as much of dO . O.  Among few keys that is most of dP - D (two keys: dq and
+    // dk off by 0.0044 in the 2-norm where their own rounding is 0.0017), so where a cloud's keys are one tile D is formed as
+    // sum P dP over it, whose products are done twice then (16 x 4096 rows over 48 keys, 8 heads of 64: dq 83 -> 87 us, all
+    // gradients 118 -> 121; over 64 keys, 4 heads of 32: 27 -> 29 and 47 -> 49, keys' and values' alone 31 -> 43).
+    bool landed = false;
+    if (one_tile && key < end) {
+        land(lds, live);
+        landed = true;
+        if (working) {
+            float sum = 0.0f, dot = 0.0f;
+#pragma unroll 1
+            for (int t = 0; t < ROWS / 32; ++t) {
+                pccnn_f32x16 s, dp;
+                both(Tile{lds}, Tile{lds + Tile::ELEMENTS}, t, s, dp);
+                hide(s, (uint32_t)(live >> (32 * t)), half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -shift));
+                    sum += p;
+                    dot = fmaf(p, dp[i], dot);
+                }
+            }
+            sum = pccnn_add_row_xor32(sum);
+            dot = pccnn_add_row_xor32(dot);
+            if (sum > 0.0f) delta = dot / sum;
+        }
+    }
     if (real && half == 0 && b.split == 0) {
         a.shift[b.stat(a, row)] = shift;
         a.delta[b.stat(a, row)] = delta;
     }
-    const float c2 = a.scale * kLog2e;
+    if (!wanted) return;
     pccnn_f32x16 acc[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) clear(acc[dt]);
@@ -650,17 +706,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
 #pragma unroll
         for (int t = 0; t < ROWS / 32; ++t) {
             pccnn_f32x16 s, dp;
-            clear(s);
-            clear(dp);
+            both(tile_k, tile_v, t, s, dp);
             AttnAhead<TERMS> ahead;
-            auto rows = [&](int i) { return (i < STEPS ? tile_k : tile_v).rows(32 * t + (lane & 31), 2 * (i % STEPS) + half); };
-            ahead.template prime<2 * STEPS>(rows);
-            ahead.template run<2 * STEPS>(rows, [&](int i, const AttnFrag<TERMS> &f) {
-                if (i < STEPS)
-                    attn_mma(s, f, q[i]);
-                else
-                    attn_mma(dp, f, g[i - STEPS]);
-            });
             auto columns = [&](int i) { return tile_k.columns(32 * t + 16 * (i / BLOCKS), 32 * (i % BLOCKS), lane); };
             ahead.template prime<2 * BLOCKS>(columns);
             if (now != first_bits(ROWS, ROWS)) hide(s, (uint32_t)(now >> (32 * t)), half);
@@ -680,13 +727,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttnArgs a)
     for (int stage = 0; key < end; key += ROWS, stage ^= 1) {
         uint16_t *const here = lds + stage * 2 * Tile::ELEMENTS, *const there = lds + (stage ^ 1) * 2 * Tile::ELEMENTS;
         const uint64_t now = live;
-        if constexpr (DIRECT) {
-            attn_landed();
-        } else {
-            k.put(Tile{here}, now);
-            v.put(Tile{here + Tile::ELEMENTS}, now);
-            __syncthreads();
-        }
+        if (!landed) land(here, now);
+        landed = false;
         walk(here, there, now);
     }
     if (!real) return;
@@ -1232,12 +1274,15 @@ extern "C" int pccnn_attention_backward(const pccnn_attention *p, const void *ou
     }
     if (d_keys != nullptr && p->n > 0) {
         if (d_queries == nullptr && p->m > 0) {
-            const unsigned blocks = (unsigned)pccnn_ceil_div(a.m * a.heads * 2, kThreads);
-            if (p->type == PCCNN_TYPE_F32)
-                attention_rows_kernel<float><<<blocks, kThreads, 0, s>>>(a);
-            else
-                attention_rows_kernel<uint16_t><<<blocks, kThreads, 0, s>>>(a);
-            PCCNN_LAUNCH_CHECK();
+            if (p->type == PCCNN_TYPE_F32) {
+                attention_rows_kernel<<<(unsigned)pccnn_ceil_div(a.m * a.heads * 2, kThreads), kThreads, 0, s>>>(a);
+                PCCNN_LAUNCH_CHECK();
+            } else {                                 // (D of clouds of few keys takes their keys and values)
+                const AttnKernel kernel = attn_plan_rows(a, p, false);
+                a.out = nullptr;
+                a.splits = 1;
+                if ((rc = attn_launch(name, kernel, a, s)) != PCCNN_OK) return rc;
+            }
         }
         a.one = {a.q, a.q_n, a.q_h, 0, a.wide_q, a.width / 8};
         a.two = {a.g, a.g_n, a.g_h, 0, a.wide_g, a.width / 8};

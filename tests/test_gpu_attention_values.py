@@ -210,3 +210,47 @@ def test_a_few_bf16_queries_are_as_exact_as_their_results_type(ops, clouds, quer
     want = (torch.softmax(scores, 3) @ v).transpose(1, 2).reshape(out.shape)
     own = (want.bfloat16().double() - want).norm()
     assert float((out - want).norm() / own) < 1.05
+
+
+@pytest.mark.parametrize("clouds,queries,keys,heads,key_heads,width,off", [
+    (2, 2000, 2, 4, 4, 32, 0.0), (3, 700, 5, 8, 2, 64, 0.3), (2, 900, 17, 2, 2, 24, 0.0), (2, 1500, 33, 4, 4, 128, 0.2),
+    (1, 2000, 64, 4, 2, 33, 0.0), (8, 40, 3, 4, 1, 96, 0.0)])
+def test_bf16_gradients_of_few_keys(ops, clouds, queries, keys, heads, key_heads, width, off):
+    # up to 64 keys to a cloud.  Score gradients and results are rounded to bf16 once each: sqrt(2) times the result's own
+    # rounding in the 2-norm, 1.5 with what the sizes of few values scatter; D = dO . O of a rounded O would add up to twice
+    # that again.  dq and dk are asked for together and alone, with the same bits.
+    gen = torch.Generator().manual_seed(keys + width)
+    normal = lambda n, h: _normal(gen, n, h, width).bfloat16()
+    q, g = normal(clouds * queries, heads) * 1.5, normal(clouds * queries, heads)
+    k, v = normal(clouds * keys, key_heads), normal(clouds * keys, key_heads)
+    live = torch.rand(clouds * keys, generator=gen) >= off
+    plan = (_starts(*[queries] * clouds), _starts(*[keys] * clouds), queries, keys)
+    dev, mask = [t.to(DEV) for t in (q, k, v)], live.to(DEV) if off else None
+    out, lse = ops.cross_attention(*dev, *plan, key_mask=mask, return_lse=True)
+    grads = ops.cross_attention_grads(*dev, *plan, out, lse, g.to(DEV), key_mask=mask)
+    dq, _, _ = ops.cross_attention_grads(*dev, *plan, out, lse, g.to(DEV), key_mask=mask, grad_mask=ops.GRAD_QUERIES)
+    _, dk, dv = ops.cross_attention_grads(*dev, *plan, out, lse, g.to(DEV), key_mask=mask, grad_mask=ops.GRAD_KEYS)
+    assert all(torch.equal(a, b) for a, b in zip(grads, (dq, dk, dv)))
+    leaves = [t.double().requires_grad_(True) for t in (q, k, v)]
+    shape = lambda t, n: t.reshape(clouds, n, -1, width).transpose(1, 2)
+    x, y, z = (shape(t, n) for t, n in zip(leaves, (queries, keys, keys)))
+    y, z = (t.repeat_interleave(heads // key_heads, 1) for t in (y, z))
+    scores = (x @ y.transpose(2, 3)) * width ** -0.5
+    scores = scores.masked_fill(~live.reshape(clouds, 1, 1, keys), -math.inf)
+    probabilities = torch.softmax(scores, 3).nan_to_num(0.0)            # (a cloud without a live key)
+    want = torch.autograd.grad((probabilities @ z).transpose(1, 2).reshape(g.shape), leaves, g.double())
+    for name, a, b in zip(("d_queries", "d_keys", "d_values"), grads, want):
+        own = (b.bfloat16().double() - b).norm()
+        assert float((a.double().cpu() - b).norm() / own) < 1.5, name
+
+
+def test_bf16_gradients_of_one_key(ops):
+    # P is 1 and dP - D zero: what is left is the f32 rounding of the two
+    gen = torch.Generator().manual_seed(2)
+    q, k, v, g = (_normal(gen, n, 2, 32).bfloat16().to(DEV) for n in (500, 1, 1, 500))
+    plan = (_starts(500), _starts(1), 500, 1)
+    out, lse = ops.cross_attention(q, k, v, *plan, return_lse=True)
+    d_queries, d_keys, _ = ops.cross_attention_grads(q, k, v, *plan, out, lse, g)
+    size = (g.float().abs().amax() * v.float().abs().amax() * 32).item()
+    assert float(d_queries.float().abs().max()) < 2.0 ** -20 * size * float(k.float().abs().max())
+    assert float(d_keys.float().abs().max()) < 2.0 ** -20 * size * float(q.float().abs().sum(0).max())
