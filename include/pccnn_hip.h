@@ -529,8 +529,9 @@ int pccnn_conv_backward_bf16(const pccnn_basis *basis, const float *pts, const f
 /* ---- attention between levels --------------------------------------------
  * Three operators with no counterpart in the reference, which moves features between levels with local convolutions only:
  * layer norm of features, rotary positions over the point coordinates, and softmax attention of the points of one level
- * to those of another.  Features are f32 or bf16 (bit patterns), `type` one of PCCNN_TYPE_*; everything is computed in
- * f32 and a bf16 result is rounded once.  Strides are in elements and not negative; features of a row (of a head) lie
+ * to those of another.  Features are f32 or bf16 (bit patterns), `type` one of PCCNN_TYPE_*.  Layer norm and rotary
+ * positions compute in f32 and round a bf16 result once; attention's sums and softmax are f32 too, but its bf16 products take
+ * probabilities and score gradients in bf16 (see there).  Strides are in elements and not negative; features of a row (of a head) lie
  * one behind the other; results are dense and start at multiples of 16 bytes. */
 #define PCCNN_GRAD_QUERIES 64
 #define PCCNN_GRAD_KEYS 128 /* keys and values */
@@ -571,8 +572,12 @@ int pccnn_rotary_points_backward(const void *feats, int type, int64_t stride_n, 
  * lse -inf.  scale: positive, finite.
  * forward: out [m,heads,width]; lse_out (nullable) f32[m,heads] = log of the sum of exp(scale q.k), for the backward call.
  * backward: d_queries (nullable) [m,heads,width], d_keys and d_values (both or neither) [n,key_heads,width]; results do
- * not depend on the order of anything (no atomics).  f32 products keep f32 accuracy; infinities in f32 features that are
- * not switched off give NaN. */
+ * not depend on the order of anything (no atomics).
+ * f32 products keep f32 accuracy (2^-22 to 2^-20 in the 2-norm); infinities in f32 features that are not switched off give NaN.
+ * bf16: probabilities and score gradients are rounded to bf16 for the products they enter, results once more, and dO . O is
+ * formed from the rounded output.  In the 2-norm a result is then off by 0.0023 to 0.0028 of itself where its last rounding
+ * alone is 0.0017.  Two exceptions: up to 32 queries x heads to a cloud and key head, whose output has its last rounding alone,
+ * and up to 64 keys to a cloud, whose dO . O is formed anew.  Scores that are NaN, or all minus infinity, give NaN. */
 typedef struct pccnn_attention {
     const void *queries, *keys, *values;
     int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h;

@@ -18,13 +18,13 @@
 // f32: three bf16 terms per value, six products (attention_tiles.h).
 //
 // Tiles go from memory to LDS without passing registers, the next while one is worked on.  What bounds the large cases is
-// the card's power: matrix pipe 45 - 60 % and vector ALU 50 - 77 % busy at 1.65 - 2.1 GHz of 2.4, and neither a wider
-// tile, wave priorities nor interleaving the exponentials with products by hand changed their time (64 rows per wavefront:
-// 605 -> 568 us where 8 x 256 rows of 64 features walk 100000 keys, but 6.8 -> 7.4 ms at 128 features, whose registers
-// then leave one wavefront to a SIMD).  Measured: forward 34123 x 100000, 4 heads of 128, 6.8 - 6.9 ms = 1013 - 1030
-// TFLOP/s; training 8 x 8192 rows over 2047 keys, uneven, 8 heads of 64: forward 174 - 202, dq with the rows' statistics
-// 220 - 250, dk / dv 331 - 383 us; one row per cloud over 16 x 4096 keys 25 us = 5.4 TB/s and 4 for the join, over 10^6
-// keys 91 us = 5.6 TB/s and 10.
+// the card's power: matrix pipe 40 - 59 % and vector ALU 45 - 78 % busy at 1.65 - 2.1 GHz of 2.4, LDS 20 - 35 % without a
+// conflict.  Wave priorities and exponentials interleaved with the next products by hand changed nothing.  64 rows per
+// wavefront, which halve the reads of LDS, are faster for even clouds of 64 features (8 x 256 rows over 100000 keys 605 -> 568
+// us) and slower for uneven ones (8 x 8192 rows 216 -> 240) and at 128 features (6.8 -> 7.4 ms, one wavefront to a SIMD).
+// Measured: forward 34123 x 100000, 4 heads of 128, 6.5 - 6.9 ms = 1013 - 1075 TFLOP/s; training 8 x 8192 rows over 2047 keys,
+// uneven, 8 heads of 64: forward 169 - 202, dq with the rows' statistics 212 - 250, dk / dv 325 - 383 us; one row per cloud over
+// 16 x 4096 keys 25 us = 5.4 TB/s and 4 for the join, over 10^6 keys 92 us = 5.6 TB/s and 10.
 #include "attention_tiles.h"
 
 #include <algorithm>
@@ -38,8 +38,10 @@ constexpr int kWaves = kThreads / PCCNN_WAVE;
 constexpr int kOwn = 32 * kWaves;            // rows (forward, dq) or keys (dk, dv) of a workgroup
 constexpr int kMaxWidth = 128;
 constexpr int64_t kMostTokens = 1ll << 32;   // queries x heads, keys x key heads
-// Own tiles per cloud from which on f32 is turned into planes of terms first.  Measured with and without: 6 tiles over
-// 1201 keys 51 and 47 us, 32 over 600 keys 162 and 176, 50 tiles 603 and 755, 5 over 4096 rows (backward) 313 and 302.
+// Own tiles per cloud from which on f32 is turned into planes of terms first.  Measured with and without, 4 clouds of 4 heads
+// over 2048 keys, forward in us: 64 features, 2 tiles 36 and 34, 6 tiles 58 and 56, 7 tiles 66 and 70, 24 tiles 159 and 178; 128
+// features, 2 tiles 53 and 47, 6 tiles 106 and 116, 24 tiles 295 and 371; 32 features gain later, 7 tiles 47 and 44, 12 tiles 60
+// and 59, 24 tiles 103 and 106.  dq, dk and dv have their crossing at 4 to 8 tiles of 64 to 128 features, 8 to 12 of 32.
 constexpr int kPlanesFrom = 7;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -1077,7 +1079,10 @@ void attn_plan(AttnArgs &a, const AttnKernel &kernel, int type, int products, in
     // Workgroups that walk the same tiles on one XCD: its L2 serves them once (8 x 256 rows over 100000 keys 605 -> 560 us,
     // dk and dv 970 -> 945).  The XCDs are dealt their workgroups in turn, whatever these weigh, so where clouds differ the
     // runs are all tiles of a head and only where a cloud's heads and parts fill the eight evenly (8 uneven clouds of 8
-    // heads: 216 -> 187 us, with runs of 16 242), else single workgroups.
+    // heads: 216 -> 187 us, with runs of 16 242), else single workgroups.  Against single workgroups, runs of 8 and of all
+    // tiles for every call, over nine uneven batches of 3 to 30 clouds, 2 to 16 heads and 32 to 128 features, 23 of 27 passes
+    // are within 5 % of the best of the three; the others lose 8 to 14 % to runs of 8 or of all tiles (dk and dv of 16 clouds of
+    // 4 heads and of 12 of 2 key heads, dq and dk, dv of 6 f32 clouds of 4 heads).
     const bool uneven = other * a.clouds > other_all || own * a.clouds > own_all;
     const int64_t blocks = (int64_t)a.tiles * a.splits * a.key_heads * a.clouds;
     a.run = uneven ? (a.key_heads * a.splits % PCCNN_XCDS == 0 ? a.tiles : 1) : blocks >= 4 * kernel.slots ? 16 : 8;

@@ -1,5 +1,6 @@
 // Element types of the feature operators (layer norm, rotary positions, attention): f32, or bf16 as bit patterns.
-// Everything is computed in f32; a bf16 result is rounded once, to nearest even, when it is stored.
+// Values are f32 in registers; a bf16 result is rounded when it is stored, to nearest even (what attention's products round
+// before is said there).
 #pragma once
 #include "common.h"
 

@@ -10,10 +10,12 @@
 // wavefront's registers hold (2048 values, or 1024 where rows only allow loads of single values: f32 rows that are not 16-byte
 // aligned, odd channel counts) take a workgroup each and are read again from the caches instead.
 //
-// Bound by HBM.  800000 rows of 64 bf16 values: forward 37 us = 5.5 TB/s, backward 65 us = 4.7 TB/s (three streams, the
-// column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 17
-// and 3.6 us (both passes fit the 256 MB cache).  One row: 2 us, the launch.  Two rows at a time in the backward pass and
-// half as many rows of sums took the last kernel from 6.6 to 3.9 us and left the first one as it was.
+// Bound by HBM.  800000 rows of 64 bf16 values: forward 39 us = 5.3 TB/s, backward 64 us = 4.8 TB/s (three streams, the
+// column sums in registers cost nothing), sums 4 us; a copy of that size runs at 5.1 TB/s.  65536 rows of 128 f32: 13, 17 - 18
+// and 3.7 us (both passes fit the 256 MB cache).  One row: 2 us, the launch.  Two rows at a time in the backward pass and
+// half as many rows of sums took the last kernel from 6.6 to 3.9 us and left the first one as it was.  Single-value loads:
+// 32768 rows of 1021 f32 as fast as aligned rows of 1024 (6.2 TB/s forward, 4.8 backward), of bf16 1.9 TB/s and 3.3 where aligned
+// rows have 4.0 and 4.9.  A workgroup per row: 16384 rows of 2056 f32 3.5 TB/s and 2.2, of bf16 1.8 and 1.7.
 #include "elements.h"
 
 #include <algorithm>

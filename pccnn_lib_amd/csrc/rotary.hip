@@ -10,7 +10,10 @@
 // multiplication serves now); 2048 points of 4 heads of 32 f32 values 2.8 us.  The angle is formed in f64 and reduced to its
 // fraction of a turn there: coordinates are not small numbers, and an f32 product of a position of 10^4 and a frequency of
 // 1 would already be off by 10^-3.  Gradients of the positions come from the turned features (d angle = b' a_g - ...),
-// summed per point by one wavefront.
+// summed per point by one wavefront with a lane per pair and loads of single values: 119997 points of 8 heads of 64, all turned,
+// 71 us in bf16 (3.5 TB/s) and 115 in f32 (4.3); with 16 pairs in a head, a quarter of the lanes at work, 75 and 70.  Features
+// that are not turned are copied value by value: the same points with 16 pairs take 149 us in f32 where 32 take 90, 45 and 39 in
+// bf16.
 #include "elements.h"
 
 #include <algorithm>

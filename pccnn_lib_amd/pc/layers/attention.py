@@ -76,7 +76,8 @@ class CrossAttention(torch.nn.Module):
 
     def forward(self, p_pc_in, p_pc_out, p_in_features, p_out_features, p_key_mask=None, p_ranges=None):
         """``p_key_mask`` bool [N]: False leaves a point of ``p_pc_in`` out.  ``p_ranges``: the two ``CloudRanges`` of
-        (p_pc_in, p_pc_out) when the program keeps them (several layers of one pair of levels)."""
+        (p_pc_in, p_pc_out) when the program keeps them (several layers of one pair of levels); without them a call makes both,
+        which reads back twice and cannot be captured in a graph."""
         if p_ranges is None:
             clouds = max(p_pc_in.batch_size_host(), p_pc_out.batch_size_host())
             p_ranges = (CloudRanges(p_pc_in, clouds), CloudRanges(p_pc_out, clouds))

@@ -1431,7 +1431,8 @@ def point_conv_weight_var(basis, feats, neigh, ends):
 # ----------------------------------------------------------------------------- attention between levels
 #
 # Layer norm, rotary positions and attention: operators the reference does not have.  Features are float32 or bfloat16
-# (computed in fp32, rounded once); beside contiguous tensors they may be views whose last dimension is dense.
+# (sums in fp32; bfloat16 results of the first two are rounded once, attention's as its docstring says); beside contiguous
+# tensors they may be views whose last dimension is dense.
 
 _FEATURE_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 GRAD_QUERIES, GRAD_KEYS = 64, 128
@@ -1602,7 +1603,12 @@ def cross_attention(queries, keys, values, query_starts, key_starts, max_queries
     number of a cloud's queries and keys (rows past them are not computed).  ``key_mask`` bool [N]: False switches a key
     off, whatever its features hold; ``scale`` (positive; default W ** -0.5) multiplies the scores.  -> out [M, H, W] (zeros
     for a query without any key), and with ``return_lse`` also f32 [M, H], the log of the sum of the exponentials, which
-    ``cross_attention_grads`` takes.  Few queries over many keys (one token per cloud) are split over the keys and joined."""
+    ``cross_attention_grads`` takes.  Few queries over many keys (one token per cloud) are split over the keys and joined.
+
+    float32 keeps float32 accuracy.  bfloat16 holds sums and softmax in fp32 and rounds the probabilities for their product with
+    the values, then the result: 0.0023 of it in the 2-norm, where its own rounding is 0.0017, and no more than that for up to
+    32 queries times heads to a cloud and key head.  Scores that are not finite give NaN, never the zeros of a query
+    without keys."""
     p = _attention_args("cross_attention", queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask,
                         scale)
     dev = queries.device
@@ -1617,7 +1623,8 @@ def cross_attention_grads(queries, keys, values, query_starts, key_starts, max_q
                           key_mask=None, scale=None, grad_mask=GRAD_QUERIES | GRAD_KEYS):
     """Gradients of ``cross_attention`` from its result and ``lse`` -> (d_queries [M, H, W], d_keys [N, G, W],
     d_values [N, G, W]); None for a group that ``grad_mask`` (GRAD_QUERIES; GRAD_KEYS: keys and values) does not name.  No
-    float atomics: the same bits from run to run."""
+    float atomics: the same bits from run to run.  bfloat16 rounds probabilities and score gradients for their products: results
+    are off by 0.0023 to 0.0028 of themselves in the 2-norm."""
     name = "cross_attention_grads"
     p = _attention_args(name, queries, keys, values, query_starts, key_starts, max_queries, max_keys, key_mask, scale)
     dev = queries.device
