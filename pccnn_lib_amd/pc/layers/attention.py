@@ -29,7 +29,8 @@ class RotaryPositions(torch.nn.Module):
         self.plans_ = {}                # device -> (frequencies, axes); float32 whatever type the module is moved to
 
     def plan(self, p_device):
-        if p_device not in self.plans_:
+        kept = self.plans_.get(p_device)
+        if kept is None or kept[0].device != p_device:      # (a module that was saved elsewhere brings its tensors along)
             # whoever asks first: the plan outlives a call under inference_mode, whose tensors no training step may save
             with torch.inference_mode(False):
                 self.plans_[p_device] = (torch.tensor(self.freqs_host_, dtype=torch.float32, device=p_device),

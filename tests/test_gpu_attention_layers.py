@@ -205,3 +205,13 @@ def test_a_rotary_layers_first_call_in_a_graph(lib):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_a_layer_saved_on_the_gpu_and_loaded_on_the_host_comes_back(lib, tmp_path):
+    # (the file is this test's own; a whole module is pickled)
+    layer = lib.pc.layers.RotaryPositions(3, 32).to(DEV)
+    feats, pts = torch.randn((40, 2, 32), device=DEV), torch.rand((40, 3), device=DEV)
+    want = layer(feats, pts)
+    torch.save(layer, tmp_path / "layer.pt")
+    loaded = torch.load(tmp_path / "layer.pt", map_location="cpu", weights_only=False)
+    assert torch.equal(loaded(feats, pts), want) and torch.equal(loaded.to(DEV)(feats, pts), want)
