@@ -594,6 +594,66 @@ int pccnn_attention_backward(const pccnn_attention *problem, const void *out, co
                              int64_t grads_stride_n, int64_t grads_stride_h, void *d_queries, void *d_keys,
                              void *d_values, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- feed-forward ---------------------------------------------------------
+ * Operators of the half of a block that follows attention between levels, with no counterpart in the reference: root-mean-square
+ * norm with the addition of a residual, rows brought to 8 bits, the gated linear map act(x G') (x U'), and linear maps of 8-bit
+ * rows.  Features are f32 or bf16 as above; 8-bit values are signed integers (codes) with one f32 scale for a row, whose value
+ * is code * scale.  Strides are in elements, results are dense and start at multiples of 16 bytes.  No result depends on the
+ * order of anything (no atomics). */
+#define PCCNN_TYPE_I8 2 /* operands of pccnn_gated_forward */
+#define PCCNN_ACT_SILU 0
+#define PCCNN_ACT_GELU 1 /* x Phi(x) */
+#define PCCNN_ACT_SIGMOID 2
+#define PCCNN_ACT_RELU 3
+#define PCCNN_MAX_INNER_8BIT 131071 /* products of 8-bit values that a 32-bit sum holds whatever they are */
+
+/* s = feats (+ residual, nullable: rounded to the type and written to total_out [n,channels]); out[n,channels] =
+ * s gamma / sqrt(avg(s^2) + eps) per row.  gamma [channels] of weight_type.  rstd_out (nullable) f32[n] = 1 / sqrt(..), which the
+ * backward call takes.  pccnn_rms_norm_8bit: the same result as codes_out i8[n,channels] and scales_out f32[n]: scale = largest
+ * magnitude / 127, codes the nearest integers (ties to even; the row's factor cancels, so they are decided on s gamma, in 64 bits).
+ * A row of zeros has scale 0, a row that holds an infinity or NaN has codes 0 and scale NaN.  pccnn_quantize_rows: feats as they are.
+ * Backward, from s (feats, or total_out where there was a residual): d_feats (nullable) [n,channels] = the gradient of s along
+ * the norm plus total_grads (nullable, the gradient of total_out): of feats and of residual alike; d_gamma (nullable) [channels]
+ * of weight_type, summed in a fixed order; the workspace is only needed for it. */
+size_t pccnn_rms_norm_workspace_bytes(int64_t n, int64_t channels);
+int pccnn_rms_norm_forward(const void *feats, int type, int64_t row_stride, const void *residual, int64_t residual_stride,
+                           const void *gamma, int weight_type, float eps, int64_t n, int64_t channels, void *out,
+                           void *total_out, float *rstd_out, void *stream);
+int pccnn_rms_norm_backward(const void *total, int type, int64_t row_stride, const void *gamma, int weight_type,
+                            const float *rstd, const void *in_grads, int64_t grads_stride, const void *total_grads,
+                            int64_t total_grads_stride, int64_t n, int64_t channels, void *d_feats, void *d_gamma,
+                            void *workspace, size_t workspace_bytes, void *stream);
+int pccnn_rms_norm_8bit(const void *feats, int type, int64_t row_stride, const void *residual, int64_t residual_stride,
+                        const void *gamma, int weight_type, float eps, int64_t n, int64_t channels, int8_t *codes_out,
+                        float *scales_out, void *total_out, void *stream);
+int pccnn_quantize_rows(const void *feats, int type, int64_t row_stride, int64_t n, int64_t channels, int8_t *codes_out,
+                        float *scales_out, void *stream);
+
+/* out[n,outer] (f32 or bf16) = (sum_k codes[n,k] weights[outer,k]) scales[n] weight_scales[outer] + bias[outer] (nullable);
+ * codes and weights dense rows of `inner` <= PCCNN_MAX_INNER_8BIT.  The sums are exact. */
+size_t pccnn_linear_8bit_workspace_bytes(const int8_t *codes, const int8_t *weights, int64_t n, int64_t inner, int64_t outer);
+int pccnn_linear_8bit(const int8_t *codes, const float *scales, const int8_t *weights, const float *weight_scales,
+                      const float *bias, int64_t n, int64_t inner, int64_t outer, void *out, int out_type, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* h[n,hidden] = act(feats gate^T) * (feats up^T): feats [n,channels], gate and up [hidden,channels], `type` f32 or bf16 for all
+ * three (h likewise), or PCCNN_TYPE_I8: codes with their scales [n], [hidden], [hidden] (h f32 or bf16, out_type).  channels and
+ * hidden <= 2^20.  Backward (f32, bf16) from the inputs and in_grads [n,hidden]: d_feats (nullable) [n,channels], d_gate and d_up
+ * (both or neither) [hidden,channels].  Products of f32 keep f32 accuracy; infinities in f32 operands give NaN.  bf16: both
+ * projections stay in f32, the gradients of the projections are rounded to bf16 for the products that they enter. */
+typedef struct pccnn_gated {
+    const void *feats, *gate, *up;
+    const float *feats_scales, *gate_scales, *up_scales;
+    int64_t feats_stride, gate_stride, up_stride;
+    int64_t n, channels, hidden;
+    int type, activation;
+} pccnn_gated;
+size_t pccnn_gated_workspace_bytes(const pccnn_gated *problem, int backward);
+int pccnn_gated_forward(const pccnn_gated *problem, void *out, int out_type, void *workspace, size_t workspace_bytes,
+                        void *stream);
+int pccnn_gated_backward(const pccnn_gated *problem, const void *in_grads, int64_t grads_stride, void *d_feats, void *d_gate,
+                         void *d_up, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- per-kernel timing ---------------------------------------------------
  * Measurement hooks with no counterpart in the reference (it has no profiler hooks).  While
  * enabled, the entry points above bracket their main kernels with HIP events on the launch

@@ -37,6 +37,16 @@ class Attention(ctypes.Structure):
 
 AP = ctypes.POINTER(Attention)
 
+
+class Gated(ctypes.Structure):
+    """struct pccnn_gated of include/pccnn_hip.h."""
+    _fields_ = [("feats", P), ("gate", P), ("up", P), ("feats_scales", P), ("gate_scales", P), ("up_scales", P),
+                ("feats_stride", I64), ("gate_stride", I64), ("up_stride", I64), ("n", I64), ("channels", I64),
+                ("hidden", I64), ("type", ctypes.c_int), ("activation", ctypes.c_int)]
+
+
+GP = ctypes.POINTER(Gated)
+
 # name -> (restype, argtypes); mirrors include/pccnn_hip.h declaration by declaration.
 SIGNATURES = {
     "pccnn_last_error": (ctypes.c_char_p, []),
@@ -110,6 +120,16 @@ SIGNATURES = {
     "pccnn_attention_workspace_bytes": (SZ, [AP, I32]),
     "pccnn_attention_forward": (I32, [AP, P, P, P, SZ, P]),
     "pccnn_attention_backward": (I32, [AP, P, P, P, I64, I64, P, P, P, P, SZ, P]),
+    "pccnn_rms_norm_workspace_bytes": (SZ, [I64, I64]),
+    "pccnn_rms_norm_forward": (I32, [P, I32, I64, P, I64, P, I32, F32, I64, I64, P, P, P, P]),
+    "pccnn_rms_norm_backward": (I32, [P, I32, I64, P, I32, P, P, I64, P, I64, I64, I64, P, P, P, SZ, P]),
+    "pccnn_rms_norm_8bit": (I32, [P, I32, I64, P, I64, P, I32, F32, I64, I64, P, P, P, P]),
+    "pccnn_quantize_rows": (I32, [P, I32, I64, I64, I64, P, P, P]),
+    "pccnn_linear_8bit_workspace_bytes": (SZ, [P, P, I64, I64, I64]),
+    "pccnn_linear_8bit": (I32, [P, P, P, P, P, I64, I64, I64, P, I32, P, SZ, P]),
+    "pccnn_gated_workspace_bytes": (SZ, [GP, I32]),
+    "pccnn_gated_forward": (I32, [GP, P, I32, P, SZ, P]),
+    "pccnn_gated_backward": (I32, [GP, P, I64, P, P, P, P, SZ, P]),
     "pccnn_timing_enable": (I32, [I32]),
     "pccnn_timing_reset": (I32, []),
     "pccnn_timing_count": (I32, []),

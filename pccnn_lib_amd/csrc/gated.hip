@@ -1,0 +1,686 @@
+// Gated linear map of feature rows, forward and backward: both projections, the activation and the product in one kernel.
+//
+//   G = x Wg^T   U = x Wu^T   h = act(G) U                                     x [n, c], Wg and Wu [hidden, c]
+//   dG = dh U act'(G)   dU = dh act(G)   dx = dG Wg + dU Wu   dWg = dG^T x   dWu = dU^T x
+//
+// Nothing is kept for the backward pass but the inputs: it forms G and U anew in the kernel that turns dh into dG and dU.
+#include "product_tiles.h"
+
+#include <algorithm>
+#include <math.h>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kMostWidth = 1 << 20;      // channels and hidden channels: a tile's rows stay within 32-bit offsets
+constexpr int kFewRows = 64;
+
+// ------------------------------------------------------------------------------------------- activations
+
+// Phi(x), the normal distribution function, and its density.  bf16 results take erfc by Abramowitz and Stegun 7.1.26 (absolute
+// error 1.5e-7, far below their rounding): one exponential and one reciprocal instead of a call of 60 instructions.
+template <bool EXACT> __device__ __forceinline__ void normal_of(float x, float &phi, float &density)
+{
+    const float e = EXACT ? expf(-0.5f * x * x) : __expf(-0.5f * x * x);
+    density = 0.3989422804014327f * e;
+    if constexpr (EXACT) {
+        phi = 0.5f * erfcf(-0.7071067811865476f * x);
+    } else {
+        const float z = fabsf(x) * 0.7071067811865476f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+        float p = fmaf(1.061405429f, t, -1.453152027f);
+        p = fmaf(p, t, 1.421413741f);
+        p = fmaf(p, t, -0.284496736f);
+        p = fmaf(p, t, 0.254829592f);
+        const float tail = 0.5f * p * t * e;
+        phi = x < 0.0f ? tail : 1.0f - tail;
+        if (x != x) phi = x;
+    }
+}
+// act(g) and, if asked for, its derivative.  EXACT: to f32, else to what a bf16 result shows.
+template <bool EXACT, bool SLOPE> __device__ __forceinline__ float activate(float g, int which, float &slope)
+{
+    if (which == PCCNN_ACT_RELU) {
+        if (SLOPE) slope = g > 0.0f ? 1.0f : 0.0f;
+        return g > 0.0f ? g : g != g ? g : 0.0f;
+    }
+    if (which == PCCNN_ACT_GELU) {
+        float phi, density;
+        normal_of<EXACT>(g, phi, density);
+        if (SLOPE) slope = fmaf(g, density, phi);
+        return g * phi;
+    }
+    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    if (which == PCCNN_ACT_SIGMOID) {
+        if (SLOPE) slope = s * (1.0f - s);
+        return s;
+    }
+    if (SLOPE) slope = s * fmaf(g, 1.0f - s, 1.0f);
+    return g * s;
+}
+
+// ------------------------------------------------------------------------------------------- G and U
+
+struct GatedArgs {
+    ProductRows x, gate, up;                 // operands with whole units
+    int64_t n, hidden;
+    int units, pairs, activation;
+    const float *x_scales, *gate_scales, *up_scales;                  // 8-bit operands
+    int64_t blocks;
+    int tiles, run;                          // tiles of hidden channels to a tile of rows; workgroups that go to one XCD
+    void *out;                               // forward: h [n, hidden]
+    const void *grads;                       // backward: dh
+    int64_t grads_stride;
+    int grads_wide;
+    uint16_t *d_pre;                         // backward: (dG | dU) rows of 2 padded bf16 values, planes of terms in f32
+    int64_t padded, d_plane;
+};
+
+// E: operands; T: result (forward), type of the tensors (backward).
+template <class E, typename T, bool BACK, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
+{
+    typedef ProductNT<E, BM, BN, WM, WN, true> Product;
+    constexpr int COLS = BN / 2, HALF = Product::NT / 2;
+    constexpr bool EXACT = std::is_same<T, float>::value;
+    typedef ProductStage<T, BM, COLS, Product::THREADS> Stage;
+    extern __shared__ __align__(16) uint16_t lds[];
+    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
+    if (block >= a.blocks) return;
+    const int64_t row0 = block / a.tiles * BM, col0 = block % a.tiles * COLS;
+    Product p;
+    p.run(a.x, row0, a.gate, a.up, col0, a.units, a.pairs, lds);
+    const Stage stage = {(T *)lds}, second = {(T *)lds + BM * COLS};
+    if constexpr (BACK) {
+        stage.bring((const T *)a.grads, a.grads_stride, row0, a.n, col0, a.hidden, a.grads_wide);
+        attn_landed();
+    }
+#pragma unroll
+    for (int m = 0; m < Product::MT; ++m) {
+        const int row = p.row_of(m);
+        float x_scale = 1.0f;
+        if constexpr (std::is_same<E, ProductI8>::value) x_scale = a.x_scales[min(row0 + row, a.n - 1)];
+#pragma unroll
+        for (int n = 0; n < HALF; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = p.col_of(n) + 8 * q + 4 * p.half;
+                float v[4], w[4];
+                if constexpr (BACK) stage.get(row, col, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float g = p.acc[m][n][4 * q + i], u = p.acc[m][n + HALF][4 * q + i], slope;
+                    if constexpr (std::is_same<E, ProductI8>::value) {
+                        const int64_t channel = min(col0 + col + i, a.hidden - 1);
+                        g *= x_scale * a.gate_scales[channel];
+                        u *= x_scale * a.up_scales[channel];
+                    }
+                    const float act = activate<EXACT, BACK>(g, a.activation, slope);
+                    if constexpr (BACK) {
+                        w[i] = v[i] * act;
+                        v[i] *= u * slope;
+                    } else {
+                        v[i] = act * u;
+                    }
+                }
+                if constexpr (BACK) {                                 // channels that only fill up a unit
+                    if (col0 + col + 4 > a.hidden)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (col0 + col + i >= a.hidden) v[i] = w[i] = 0.0f;
+                }
+                stage.put(row, col, v);
+                if constexpr (BACK) second.put(row, col, w);
+            }
+    }
+    __syncthreads();
+    if constexpr (!BACK) {
+        stage.out((T *)a.out, a.hidden, row0, a.n, col0, a.hidden);
+    } else if constexpr (!EXACT) {
+        stage.out(a.d_pre, 2 * a.padded, row0, a.n, col0, a.padded);
+        second.out(a.d_pre + a.padded, 2 * a.padded, row0, a.n, col0, a.padded);
+    } else {
+        for (int i = threadIdx.x; i < 2 * BM * COLS / 8; i += Product::THREADS) {
+            const int which = i / (BM * COLS / 8), r = i % (BM * COLS / 8) / (COLS / 8), col = i % (COLS / 8) * 8;
+            if (row0 + r >= a.n || col0 + col >= a.padded) continue;
+            const Stage &from = which ? second : stage;
+            float x[8], y[4];
+            from.get(r, col, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = y[e];
+            from.get(r, col + 4, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 + e] = y[e];
+            const AttnFrag<3> f = attn_split<3, true>(x);
+            uint16_t *to = a.d_pre + (row0 + r) * 2 * a.padded + which * a.padded + col0 + col;
+#pragma unroll
+            for (int t = 0; t < 3; ++t) *(pccnn_u32x4 *)(to + t * a.d_plane) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
+        }
+    }
+}
+
+struct GatedFew {
+    FewRows x, w[2];
+    int64_t n, hidden, channels;
+    const float *x_scales, *gate_scales, *up_scales;
+    int activation;
+    void *out;
+};
+template <typename T, typename OUT, int RT, int WAVES>
+__global__ __launch_bounds__(WAVES *PCCNN_WAVE) void gated_few_kernel(GatedFew a)
+{
+    __shared__ pccnn_u32x4 lds[WAVES - 1][RT * 2][PCCNN_WAVE];
+    const int64_t col0 = (int64_t)blockIdx.x * 16;
+    FewProduct<T, 2, RT, WAVES> p;
+    if (!p.run(a.x, a.n, a.w, col0, a.hidden, a.channels, lds)) return;
+    const int lane = threadIdx.x % PCCNN_WAVE;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int64_t row = 16 * r + (lane & 15);
+        if (row >= a.n) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t channel = col0 + 4 * (lane >> 4) + i;
+            if (channel >= a.hidden) continue;
+            float g = p.acc[r][0][i], u = p.acc[r][1][i], slope;
+            if constexpr (std::is_same<T, int8_t>::value) {
+                g *= a.x_scales[row] * a.gate_scales[channel];
+                u *= a.x_scales[row] * a.up_scales[channel];
+            }
+            const float h[1] = {activate<std::is_same<OUT, float>::value, false>(g, a.activation, slope) * u};
+            pccnn_store<1>((OUT *)a.out + row * a.hidden + channel, h);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- backward products
+
+// Both weights one below the other and turned: row c of the result is (Wg[:, c] | Wu[:, c]), each padded to whole units with
+// zeros.  f32: three planes of terms.
+template <typename T> struct TurnArgs {
+    const T *gate, *up;
+    int64_t gate_stride, up_stride, hidden, channels, padded;
+    uint16_t *to;
+};
+template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_kernel(TurnArgs<T> a)
+{
+    __shared__ float tile[64][65];
+    const int64_t c0 = (int64_t)blockIdx.x * 64, h0 = (int64_t)blockIdx.y * 64;
+    const T *from = blockIdx.z ? a.up : a.gate;
+    const int64_t stride = blockIdx.z ? a.up_stride : a.gate_stride;
+    for (int i = threadIdx.x; i < 64 * 64; i += kThreads) {
+        const int64_t h = h0 + i / 64, c = c0 + i % 64;
+        float v[1] = {0.0f};
+        if (h < a.hidden && c < a.channels) pccnn_load<1>(from + h * stride + c, v);
+        tile[i / 64][i % 64] = v[0];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
+        const int64_t c = c0 + i / 8, h = h0 + i % 8 * 8;
+        if (c >= a.channels || h >= a.padded) continue;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = tile[i % 8 * 8 + e][i / 8];
+        constexpr int TERMS = AttnTerms<T>::value;
+        const AttnFrag<TERMS> f = attn_split<TERMS, TERMS == 3>(x);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+            *(pccnn_u32x4 *)(a.to + (t * a.channels + c) * 2 * a.padded + blockIdx.z * a.padded + h) =
+                __builtin_bit_cast(pccnn_u32x4, f.t[t]);
+    }
+}
+
+// dx: rows of (dG | dU) times the turned weights.
+struct BackArgs {
+    ProductRows x, w;
+    int64_t n, cols;
+    int units, pairs;
+    int64_t blocks;
+    int tiles, run;
+    void *out;
+};
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a)
+{
+    typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
+    typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
+    extern __shared__ __align__(16) uint16_t lds[];
+    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
+    if (block >= a.blocks) return;
+    const int64_t row0 = block / a.tiles * BM, col0 = block % a.tiles * BN;
+    Product p;
+    p.run(a.x, row0, a.w, a.w, col0, a.units, a.pairs, lds);
+    const Stage stage = {(T *)lds};
+#pragma unroll
+    for (int m = 0; m < Product::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < Product::NT; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = p.acc[m][n][4 * q + i];
+                stage.put(p.row_of(m), p.col_of(n) + 8 * q + 4 * p.half, v);
+            }
+    __syncthreads();
+    stage.out((T *)a.out, a.cols, row0, a.n, col0, a.cols);
+}
+
+// dWg and dWu: columns of (dG | dU) times columns of x, the inner dimension over the rows, which are cut into parts whose sums
+// are added afterwards in their order.
+struct WeightsArgs {
+    ProductRows x, d;                        // rows with whole units; stride in bytes
+    int64_t n, cols_x, cols_d;               // columns that exist, in whole units
+    int pairs;
+    int tiles_x, tiles_d, splits;
+    int64_t per_split;                       // rows of a part, a multiple of 64
+    float *part;                             // [split][cols_d][channels]
+    int64_t channels;
+};
+constexpr int kTurnRows = 64, kTurnCols = 128;
+
+struct ColumnsFeeder {
+    typedef AttnTile<1, kTurnRows, kTurnCols> Tile;
+    static constexpr int COUNT = kTurnRows * Tile::UNITS / kThreads;
+    static_assert(kThreads / Tile::UNITS % 16 == 0, "the same unit in every round");
+    const char *base;
+    int64_t stride;
+    int unit, row;
+    bool live;
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t col0, int64_t cols)
+    {
+        row = (int)threadIdx.x / Tile::UNITS;
+        unit = Tile::unit_at(row, (int)threadIdx.x % Tile::UNITS);
+        base = (const char *)s.p + 2 * col0;
+        stride = s.stride;
+        live = col0 + 8 * unit < cols;
+    }
+    __device__ __forceinline__ void fetch(int64_t at_row, int64_t plane, int64_t rows, uint16_t *tile) const
+    {
+        const __amdgpu_buffer_rsrc_t window = attn_window(base + at_row * stride + plane);
+        const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            const int r = row + j * (kThreads / Tile::UNITS);
+            attn_bring(window, live && at_row + r < rows ? (uint32_t)(r * stride + 16 * unit) : kAttnNowhere,
+                       tile + 8 * (j * kThreads + wave_unit));
+        }
+    }
+};
+__global__ __launch_bounds__(kThreads) void gated_weights_kernel(WeightsArgs a)
+{
+    typedef ColumnsFeeder::Tile Tile;
+    extern __shared__ __align__(16) uint16_t lds[];
+    const int lane = threadIdx.x % PCCNN_WAVE, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE), wd = wave % 2, wx = wave / 2;
+    int64_t block = blockIdx.x;
+    const int64_t x0 = block % a.tiles_x * kTurnCols;
+    block /= a.tiles_x;
+    const int64_t d0 = block % a.tiles_d * kTurnCols;
+    const int64_t split = block / a.tiles_d;
+    const int64_t first = split * a.per_split, last = min(a.n, first + a.per_split);
+    ColumnsFeeder fx, fd;
+    fx.start(a.x, x0, a.cols_x);
+    fd.start(a.d, d0, a.cols_d);
+    pccnn_f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    const int64_t steps = (last - first + kTurnRows - 1) / kTurnRows, total = steps * a.pairs;
+    int64_t k = 0;
+    int pair = a.pairs == 1 ? PRODUCT_PAIRS - 1 : 0;
+    constexpr int STAGE = 2 * Tile::ELEMENTS;
+    auto fetch = [&](uint16_t *to) {
+        fx.fetch(first + k * kTurnRows, product_term_a(pair) * a.x.plane, last, to);
+        fd.fetch(first + k * kTurnRows, product_term_b(pair) * a.d.plane, last, to + Tile::ELEMENTS);
+        if (++k == steps) k = 0, ++pair;
+    };
+    if (total > 0) fetch(lds);
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+        if (more) fetch(there);
+        const Tile tx = {here}, td = {here + Tile::ELEMENTS};
+#pragma unroll
+        for (int kk = 0; kk < kTurnRows / 16; ++kk) {
+            AttnFrag<1> fa[2], fb[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fa[i] = tx.columns(16 * kk, 64 * wx + 32 * i, lane);
+                fb[i] = td.columns(16 * kk, 64 * wd + 32 * i, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) attn_mma(acc[i][j], fa[i], fb[j]);
+        }
+    };
+    for (int64_t step = 0; step < total; ++step) {
+        attn_landed();
+        walk(lds + (step & 1) * STAGE, lds + ((step & 1) ^ 1) * STAGE, step + 1 < total);
+    }
+    float *part = a.part + split * a.cols_d * a.channels;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t d = d0 + 64 * wd + 32 * j + (lane & 31);
+        if (d >= a.cols_d) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t c = x0 + 64 * wx + 32 * i + 8 * q + 4 * half;
+                if (a.channels % 4 == 0) {
+                    if (c < a.channels)
+                        *(float4 *)(part + d * a.channels + c) =
+                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < a.channels) part[d * a.channels + c + e] = acc[i][j][4 * q + e];
+                }
+            }
+    }
+}
+// Sum of the parts, in their order, into the two gradients.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void gated_weights_sum_kernel(const float *__restrict__ part, int splits, int64_t hidden,
+                                                                    int64_t padded, int64_t channels, T *__restrict__ d_gate,
+                                                                    T *__restrict__ d_up)
+{
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= hidden * channels) return;
+    const float *from = part + (blockIdx.y ? padded * channels : 0) + i;
+    const int64_t step = 2 * padded * channels;
+    float sum = 0.0f;
+    for (int s = 0; s < splits; ++s) sum += from[s * step];
+    const float v[1] = {sum};
+    pccnn_store<1>((blockIdx.y ? d_up : d_gate) + i, v);
+}
+
+// ------------------------------------------------------------------------------------------- host
+
+int64_t unit_of(int type) { return type == PCCNN_TYPE_I8 ? 16 : 8; }
+int wide_of(const void *p, int64_t stride, int64_t width, int type)
+{
+    const int bytes = type == PCCNN_TYPE_I8 ? 1 : pccnn_type_bytes(type);
+    const bool whole = (uintptr_t)p % 16 == 0 && stride * bytes % 16 == 0;
+    if (type == PCCNN_TYPE_I8) return whole && width % 16 == 0 ? 2 : 0;
+    if (type == PCCNN_TYPE_F32) return whole && width % 4 == 0 ? 2 : 0;
+    if (whole && width % 8 == 0) return 2;
+    return (uintptr_t)p % 8 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
+}
+// Whether rows are operands as they are.
+bool as_they_are(const void *p, int64_t stride, int64_t width, int type)
+{
+    return type != PCCNN_TYPE_F32 && wide_of(p, stride, width, type) == 2 && stride <= kMostWidth;
+}
+
+struct GatedPlan {
+    int64_t units;                           // 16-byte units of an operand row
+    int planes;
+    bool few;
+    bool stage[3];                           // x, gate, up are laid out anew
+    size_t bytes[3];
+    int64_t rows[3];
+    const void *p[3];
+    int64_t stride[3];
+    int64_t padded;                          // hidden channels in whole units
+    int tiles_x, tiles_d, splits;            // weights' gradients
+    int64_t per_split;
+};
+int gated_check(const char *name, const pccnn_gated *p)
+{
+    PCCNN_REQUIRE(p != nullptr, PCCNN_ERR_INVALID, "%s: null pointer", name);
+    PCCNN_REQUIRE(pccnn_type_ok(p->type) || p->type == PCCNN_TYPE_I8, PCCNN_ERR_UNSUPPORTED,
+                  "%s: element type %d (f32, bf16 and 8-bit integers only)", name, p->type);
+    PCCNN_REQUIRE(p->activation >= PCCNN_ACT_SILU && p->activation <= PCCNN_ACT_RELU, PCCNN_ERR_UNSUPPORTED, "%s: activation %d",
+                  name, p->activation);
+    PCCNN_REQUIRE(p->n >= 0 && p->channels >= 1 && p->hidden >= 1 && p->feats_stride >= 0 && p->gate_stride >= 0 &&
+                      p->up_stride >= 0,
+                  PCCNN_ERR_INVALID, "%s: n=%lld, channels=%lld, hidden=%lld, row strides %lld, %lld, %lld", name,
+                  (long long)p->n, (long long)p->channels, (long long)p->hidden, (long long)p->feats_stride,
+                  (long long)p->gate_stride, (long long)p->up_stride);
+    PCCNN_REQUIRE(p->n <= INT32_MAX && p->channels <= kMostWidth && p->hidden <= kMostWidth, PCCNN_ERR_UNSUPPORTED,
+                  "%s: %lld rows of %lld channels, %lld hidden (2^31 - 1 rows, 2^20 channels at most)", name, (long long)p->n,
+                  (long long)p->channels, (long long)p->hidden);
+    PCCNN_REQUIRE(p->type != PCCNN_TYPE_I8 || p->channels <= PCCNN_MAX_INNER_8BIT, PCCNN_ERR_UNSUPPORTED,
+                  "%s: sums over %lld 8-bit products (%d at most)", name, (long long)p->channels, PCCNN_MAX_INNER_8BIT);
+    return PCCNN_OK;
+}
+GatedPlan gated_plan(const pccnn_gated *p, bool backward)
+{
+    GatedPlan plan = {};
+    const int64_t unit = unit_of(p->type);
+    plan.units = pccnn_ceil_div(p->channels, unit);
+    plan.planes = p->type == PCCNN_TYPE_F32 ? 3 : 1;
+    plan.few = !backward && p->n <= kFewRows;
+    plan.p[0] = p->feats, plan.p[1] = p->gate, plan.p[2] = p->up;
+    plan.stride[0] = p->feats_stride, plan.stride[1] = p->gate_stride, plan.stride[2] = p->up_stride;
+    plan.rows[0] = p->n, plan.rows[1] = plan.rows[2] = p->hidden;
+    for (int i = 0; i < 3; ++i) {
+        plan.stage[i] = !plan.few && !as_they_are(plan.p[i], plan.stride[i], p->channels, p->type);
+        plan.bytes[i] = plan.stage[i] ? (size_t)plan.planes * plan.rows[i] * plan.units * 16 : 0;
+    }
+    plan.padded = pccnn_ceil_div(p->hidden, 8) * 8;
+    // parts enough to fill the chip twice over, of at least four steps
+    plan.tiles_x = (int)pccnn_ceil_div(p->channels, kTurnCols);
+    plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, kTurnCols);
+    const int64_t want = std::max<int64_t>(1, 512 / ((int64_t)plan.tiles_x * plan.tiles_d));
+    const int64_t steps = std::max<int64_t>(1, pccnn_ceil_div(p->n, kTurnRows));
+    const int64_t per = std::max<int64_t>(std::min<int64_t>(4, steps), pccnn_ceil_div(steps, want));
+    plan.per_split = per * kTurnRows;
+    plan.splits = (int)pccnn_ceil_div(steps, per);
+    return plan;
+}
+// Operands of the products: the tensors themselves, or their rows laid out anew in the workspace.
+int gated_operands(const char *name, const pccnn_gated *p, const GatedPlan &plan, PccnnArena &arena, ProductRows (&r)[3],
+                   hipStream_t s)
+{
+    StageArgs a = {};
+    a.width = p->channels;
+    a.units = (int)plan.units;
+    int count = 0;
+    int64_t most = 0;
+    const int bytes = p->type == PCCNN_TYPE_I8 ? 1 : pccnn_type_bytes(p->type);
+    for (int i = 0; i < 3; ++i) {
+        if (!plan.stage[i]) {
+            r[i] = {plan.p[i], plan.stride[i] * bytes, plan.rows[i], 0};
+            continue;
+        }
+        void *to = arena.take<char>(plan.bytes[i]);
+        PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, arena.size);
+        r[i] = {to, plan.units * 16, plan.rows[i], plan.rows[i] * plan.units * 16};
+        a.s[count++] = {plan.p[i], plan.stride[i], plan.rows[i], wide_of(plan.p[i], plan.stride[i], p->channels, p->type), to};
+        most = std::max(most, plan.rows[i] * plan.units);
+    }
+    if (count == 0) return PCCNN_OK;
+    const dim3 grid((unsigned)std::min<int64_t>(pccnn_ceil_div(most, 256), 8192), (unsigned)count);
+    if (p->type == PCCNN_TYPE_F32)
+        product_stage_kernel<float><<<grid, 256, 0, s>>>(a);
+    else if (p->type == PCCNN_TYPE_BF16)
+        product_stage_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
+    else
+        product_stage_kernel<int8_t><<<grid, 256, 0, s>>>(a);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)
+{
+    constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
+    typedef ProductNT<E, BM, BN, WM, WN, true> Product;
+    const size_t lds = std::max(Product::LDS, (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
+    return product_launch(name, gated_kernel<E, T, BACK, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
+                          pccnn_ceil_div(a.hidden, BN / 2), s);
+}
+template <typename T, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+{
+    constexpr int BM = 128;
+    typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
+    const size_t lds = std::max(Product::LDS, (size_t)BM * BN * sizeof(T));
+    return product_launch(name, gated_dx_kernel<T, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
+                          pccnn_ceil_div(a.cols, BN), s);
+}
+
+template <typename T, typename OUT> int few_launch(GatedFew &a, hipStream_t s)
+{
+    constexpr int WAVES = 8;
+    const unsigned blocks = (unsigned)pccnn_ceil_div(a.hidden, 16);
+    if (a.n <= 16)
+        gated_few_kernel<T, OUT, 1, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
+    else if (a.n <= 32)
+        gated_few_kernel<T, OUT, 2, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
+    else
+        gated_few_kernel<T, OUT, 4, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+
+struct BackBytes {
+    size_t d_pre, turned, part;
+    size_t all() const { return pccnn_align(d_pre) + pccnn_align(turned) + pccnn_align(part); }
+};
+BackBytes back_bytes(const pccnn_gated *p, const GatedPlan &plan)
+{
+    BackBytes b;
+    b.d_pre = (size_t)plan.planes * p->n * 2 * plan.padded * 2;
+    b.turned = (size_t)plan.planes * p->channels * 2 * plan.padded * 2;
+    b.part = (size_t)plan.splits * 2 * plan.padded * p->channels * sizeof(float);
+    return b;
+}
+
+} // namespace
+
+extern "C" size_t pccnn_gated_workspace_bytes(const pccnn_gated *p, int backward)
+{
+    if (gated_check("gated_workspace_bytes", p) != PCCNN_OK) return 256;
+    const GatedPlan plan = gated_plan(p, backward != 0);
+    size_t total = 256;
+    for (size_t bytes : plan.bytes) total += pccnn_align(bytes);
+    if (backward && p->type != PCCNN_TYPE_I8) total += back_bytes(p, plan).all();
+    return total;
+}
+
+extern "C" int pccnn_gated_forward(const pccnn_gated *p, void *out, int out_type, void *workspace, size_t workspace_bytes,
+                                   void *stream)
+{
+    const char *name = "gated_linear";
+    int rc = gated_check(name, p);
+    if (rc != PCCNN_OK) return rc;
+    PCCNN_REQUIRE(pccnn_type_ok(out_type) && (p->type == PCCNN_TYPE_I8 || out_type == p->type), PCCNN_ERR_UNSUPPORTED,
+                  "%s: result type %d of operands of type %d", name, out_type, p->type);
+    if (p->n == 0) return PCCNN_OK;
+    PCCNN_REQUIRE(p->feats && p->gate && p->up && out, PCCNN_ERR_INVALID, "%s: null pointer", name);
+    PCCNN_REQUIRE(p->type != PCCNN_TYPE_I8 || (p->feats_scales && p->gate_scales && p->up_scales), PCCNN_ERR_INVALID,
+                  "%s: 8-bit operands without their scales", name);
+    PCCNN_REQUIRE((uintptr_t)out % 16 == 0, PCCNN_ERR_INVALID, "%s: a result that is not 16-byte aligned", name);
+    const hipStream_t s = (hipStream_t)stream;
+    const GatedPlan plan = gated_plan(p, false);
+    if (plan.few) {
+        GatedFew a = {{p->feats, p->feats_stride, wide_of(p->feats, p->feats_stride, p->channels, p->type)},
+                      {{p->gate, p->gate_stride, wide_of(p->gate, p->gate_stride, p->channels, p->type)},
+                       {p->up, p->up_stride, wide_of(p->up, p->up_stride, p->channels, p->type)}},
+                      p->n, p->hidden, p->channels, p->feats_scales, p->gate_scales, p->up_scales, p->activation, out};
+        if (p->type == PCCNN_TYPE_F32) return few_launch<float, float>(a, s);
+        if (p->type == PCCNN_TYPE_BF16) return few_launch<uint16_t, uint16_t>(a, s);
+        return out_type == PCCNN_TYPE_F32 ? few_launch<int8_t, float>(a, s) : few_launch<int8_t, uint16_t>(a, s);
+    }
+    PccnnArena arena(workspace, workspace_bytes);
+    ProductRows r[3];
+    rc = gated_operands(name, p, plan, arena, r, s);
+    if (rc != PCCNN_OK) return rc;
+    GatedArgs a = {};
+    a.x = r[0], a.gate = r[1], a.up = r[2];
+    a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation;
+    a.pairs = plan.planes == 3 ? PRODUCT_PAIRS : 1;
+    a.x_scales = p->feats_scales, a.gate_scales = p->gate_scales, a.up_scales = p->up_scales;
+    a.out = out;
+    if (p->type == PCCNN_TYPE_F32) return gated_launch<ProductBf16, float, false>(name, a, s);
+    if (p->type == PCCNN_TYPE_BF16) return gated_launch<ProductBf16, uint16_t, false>(name, a, s);
+    return out_type == PCCNN_TYPE_F32 ? gated_launch<ProductI8, float, false>(name, a, s)
+                                      : gated_launch<ProductI8, uint16_t, false>(name, a, s);
+}
+
+extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, int64_t grads_stride, void *d_feats, void *d_gate,
+                                    void *d_up, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *name = "gated_linear_grads";
+    int rc = gated_check(name, p);
+    if (rc != PCCNN_OK) return rc;
+    PCCNN_REQUIRE(p->type != PCCNN_TYPE_I8, PCCNN_ERR_UNSUPPORTED, "%s: 8-bit operands have no gradients", name);
+    PCCNN_REQUIRE(grads_stride >= 0 && grads_stride <= (1 << 21), PCCNN_ERR_INVALID, "%s: gradient rows %lld apart", name,
+                  (long long)grads_stride);
+    PCCNN_REQUIRE((d_gate != nullptr) == (d_up != nullptr), PCCNN_ERR_INVALID, "%s: the gradients of both weights come together",
+                  name);
+    if (d_gate == nullptr && (d_feats == nullptr || p->n == 0)) return PCCNN_OK;
+    PCCNN_REQUIRE(p->gate && p->up && (p->n == 0 || (p->feats && in_grads)), PCCNN_ERR_INVALID, "%s: null pointer", name);
+    PCCNN_REQUIRE(((uintptr_t)d_feats | (uintptr_t)d_gate | (uintptr_t)d_up) % 16 == 0, PCCNN_ERR_INVALID,
+                  "%s: a result that is not 16-byte aligned", name);
+    const hipStream_t s = (hipStream_t)stream;
+    const GatedPlan plan = gated_plan(p, true);
+    const BackBytes bytes = back_bytes(p, plan);
+    PccnnArena arena(workspace, workspace_bytes);
+    ProductRows r[3];
+    const bool f32 = p->type == PCCNN_TYPE_F32;
+    const int pairs = f32 ? PRODUCT_PAIRS : 1;
+    const ProductRows d = {arena.take<char>(bytes.d_pre), 4 * plan.padded, p->n, p->n * 4 * plan.padded};
+    uint16_t *turned = arena.take<uint16_t>(bytes.turned / 2);
+    float *part = arena.take<float>(bytes.part / sizeof(float));
+    PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
+    if (p->n > 0) {
+        rc = gated_operands(name, p, plan, arena, r, s);
+        if (rc != PCCNN_OK) return rc;
+        GatedArgs a = {};
+        a.x = r[0], a.gate = r[1], a.up = r[2];
+        a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation, a.pairs = pairs;
+        a.grads = in_grads, a.grads_stride = grads_stride;
+        a.grads_wide = wide_of(in_grads, grads_stride, p->hidden, p->type);
+        a.d_pre = (uint16_t *)d.p, a.padded = plan.padded, a.d_plane = d.plane / 2;
+        rc = f32 ? gated_launch<ProductBf16, float, true>(name, a, s) : gated_launch<ProductBf16, uint16_t, true>(name, a, s);
+        if (rc != PCCNN_OK) return rc;
+    }
+    if (d_feats != nullptr && p->n > 0) {
+        auto turn = [&](auto zero) {
+            using T = decltype(zero);
+            const TurnArgs<T> t = {(const T *)p->gate, (const T *)p->up, p->gate_stride, p->up_stride, p->hidden, p->channels,
+                                   plan.padded, turned};
+            const dim3 grid((unsigned)pccnn_ceil_div(p->channels, 64), (unsigned)pccnn_ceil_div(plan.padded, 64), 2);
+            gated_turn_kernel<T><<<grid, kThreads, 0, s>>>(t);
+        };
+        if (f32)
+            turn(0.0f);
+        else
+            turn((uint16_t)0);
+        PCCNN_LAUNCH_CHECK();
+        BackArgs a = {};
+        a.x = d;
+        a.w = {turned, 4 * plan.padded, p->channels, p->channels * 4 * plan.padded};
+        a.n = p->n, a.cols = p->channels, a.units = (int)(2 * plan.padded / 8), a.pairs = pairs, a.out = d_feats;
+        if (p->channels <= 64)
+            rc = f32 ? dx_launch<float, 64, 4, 1>(name, a, s) : dx_launch<uint16_t, 64, 4, 1>(name, a, s);
+        else
+            rc = f32 ? dx_launch<float, 128, 2, 2>(name, a, s) : dx_launch<uint16_t, 128, 2, 2>(name, a, s);
+        if (rc != PCCNN_OK) return rc;
+    }
+    if (d_gate != nullptr) {
+        int splits = 0;
+        if (p->n > 0) {
+            WeightsArgs a = {};
+            a.x = r[0], a.d = d, a.n = p->n, a.cols_x = plan.units * 8, a.cols_d = 2 * plan.padded, a.pairs = pairs;
+            a.tiles_x = plan.tiles_x, a.tiles_d = plan.tiles_d, a.splits = splits = plan.splits, a.per_split = plan.per_split;
+            a.part = part, a.channels = p->channels;
+            const int64_t blocks = (int64_t)a.tiles_x * a.tiles_d * a.splits;
+            PCCNN_REQUIRE(blocks <= INT32_MAX, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
+            gated_weights_kernel<<<(unsigned)blocks, kThreads, 4 * ColumnsFeeder::Tile::ELEMENTS * sizeof(uint16_t), s>>>(a);
+            PCCNN_LAUNCH_CHECK();
+        }
+        const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads), 2);
+        if (f32)
+            gated_weights_sum_kernel<float><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
+                                                                     (float *)d_gate, (float *)d_up);
+        else
+            gated_weights_sum_kernel<uint16_t><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
+                                                                        (uint16_t *)d_gate, (uint16_t *)d_up);
+        PCCNN_LAUNCH_CHECK();
+    }
+    return PCCNN_OK;
+}

@@ -1026,6 +1026,222 @@ py::tuple cross_attention_grads(const Tensor &queries, const Tensor &keys, const
     return py::make_tuple(opt(d_queries), opt(d_keys), opt(d_values));
 }
 
+// ------------------------------------------------------------------ feed-forward
+//
+// Operators the reference does not have: root-mean-square norm with the residual's addition, rows in 8 bits, the gated linear
+// map, linear maps of 8-bit rows.
+
+int activation_of(const char *op, const std::string &activation)
+{
+    if (activation == "silu") return PCCNN_ACT_SILU;
+    if (activation == "gelu") return PCCNN_ACT_GELU;
+    if (activation == "sigmoid") return PCCNN_ACT_SIGMOID;
+    TORCH_CHECK(activation == "relu", op, ": activation '", activation, "' (silu, gelu, sigmoid, relu)");
+    return PCCNN_ACT_RELU;
+}
+// The result's type: bfloat16 unless the caller says.
+at::ScalarType result_dtype(const char *op, const c10::optional<at::ScalarType> &asked)
+{
+    const at::ScalarType dtype = asked.value_or(at::kBFloat16);
+    TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16, op,
+                ": expected dtype torch.float32 or torch.bfloat16 for the result, got ", dtype);
+    return dtype;
+}
+
+// The features' checks; with a residual also its sum's tensor.
+OptTensor rms_args(const char *op, const Tensor &feats, const Tensor &gamma, const OptTensor &residual)
+{
+    chk_features(feats, op, "features", 2);
+    norm_weight(op, "gamma", gamma, feats);
+    OptTensor total;
+    if (residual.has_value()) {
+        chk_features(*residual, op, "residual", 2, &feats);
+        TORCH_CHECK(residual->sizes() == feats.sizes(), op, ": residual ", residual->sizes(), " for features ", feats.sizes());
+        total = feature_result(feats);
+    }
+    return total;
+}
+
+py::object rms_norm(const Tensor &feats, const Tensor &gamma, const OptTensor &residual, double eps, bool return_stats)
+{
+    const OptTensor total = rms_args("rms_norm", feats, gamma, residual);
+    Tensor out = feature_result(feats);
+    OptTensor rstd;
+    if (return_stats) rstd = at::empty({feats.size(0)}, feats.options().dtype(at::kFloat));
+    rc_check(pccnn_rms_norm_forward(feats.data_ptr(), feature_type(feats), feats.stride(0), optr(residual),
+                                    residual.has_value() ? residual->stride(0) : 0, gamma.data_ptr(), feature_type(gamma),
+                                    (float)eps, feats.size(0), feats.size(1), out.data_ptr(), optr(total), ofptr(rstd),
+                                    cur_stream()),
+             "pccnn_rms_norm_forward");
+    if (total.has_value() && return_stats) return py::make_tuple(out, *total, *rstd);
+    if (total.has_value()) return py::make_tuple(out, *total);
+    if (return_stats) return py::make_tuple(out, *rstd);
+    return py::cast(out);
+}
+
+py::tuple rms_norm_grads(const Tensor &total, const Tensor &gamma, const Tensor &rstd, const Tensor &in_grads,
+                         const OptTensor &total_grads, int64_t grad_mask)
+{
+    const char *op = "rms_norm_grads";
+    chk_features(total, op, "features", 2);
+    norm_weight(op, "gamma", gamma, total);
+    chk(rstd, "rms_norm_grads: rstd", at::kFloat, 1, &total);
+    chk_features(in_grads, op, "in_grads", 2, &total);
+    if (total_grads.has_value()) chk_features(*total_grads, op, "total_grads", 2, &total);
+    const int64_t n = total.size(0), c = total.size(1);
+    TORCH_CHECK(rstd.size(0) == n && in_grads.sizes() == total.sizes() &&
+                    (!total_grads.has_value() || total_grads->sizes() == total.sizes()),
+                op, ": inconsistent shapes");
+    OptTensor d_feats, d_gamma, ws;
+    if (grad_mask & PCCNN_GRAD_FEATS) d_feats = feature_result(total);
+    if (grad_mask & PCCNN_GRAD_WEIGHTS) {
+        d_gamma = at::empty({c}, gamma.options());
+        ws = workspace(pccnn_rms_norm_workspace_bytes(n, c), total);
+    }
+    rc_check(pccnn_rms_norm_backward(total.data_ptr(), feature_type(total), total.stride(0), gamma.data_ptr(),
+                                     feature_type(gamma), fptr(rstd), in_grads.data_ptr(), in_grads.stride(0),
+                                     optr(total_grads), total_grads.has_value() ? total_grads->stride(0) : 0, n, c,
+                                     optr(d_feats), optr(d_gamma), optr(ws),
+                                     ws.has_value() ? (size_t)ws->numel() : 0, cur_stream()),
+             "pccnn_rms_norm_backward");
+    return py::make_tuple(opt(d_feats), opt(d_gamma));
+}
+
+py::tuple rms_norm_8bit(const Tensor &feats, const Tensor &gamma, const OptTensor &residual, double eps)
+{
+    const OptTensor total = rms_args("rms_norm_8bit", feats, gamma, residual);
+    const int64_t n = feats.size(0), c = feats.size(1);
+    Tensor codes = at::empty({n, c}, feats.options().dtype(at::kChar));
+    Tensor scales = at::empty({n}, feats.options().dtype(at::kFloat));
+    rc_check(pccnn_rms_norm_8bit(feats.data_ptr(), feature_type(feats), feats.stride(0), optr(residual),
+                                 residual.has_value() ? residual->stride(0) : 0, gamma.data_ptr(), feature_type(gamma),
+                                 (float)eps, n, c, codes.data_ptr<int8_t>(), scales.data_ptr<float>(), optr(total),
+                                 cur_stream()),
+             "pccnn_rms_norm_8bit");
+    return total.has_value() ? py::make_tuple(codes, scales, *total) : py::make_tuple(codes, scales);
+}
+
+py::tuple quantize_rows(const Tensor &feats)
+{
+    const char *op = "quantize_rows";
+    chk_features(feats, op, "features", 2);
+    TORCH_CHECK(feats.size(1) >= 1, op, ": features without channels");
+    const int64_t n = feats.size(0), c = feats.size(1);
+    Tensor codes = at::empty({n, c}, feats.options().dtype(at::kChar));
+    Tensor scales = at::empty({n}, feats.options().dtype(at::kFloat));
+    rc_check(pccnn_quantize_rows(feats.data_ptr(), feature_type(feats), feats.stride(0), n, c, codes.data_ptr<int8_t>(),
+                                 scales.data_ptr<float>(), cur_stream()),
+             "pccnn_quantize_rows");
+    return py::make_tuple(codes, scales);
+}
+
+void codes_args(const char *op, const char *what, const Tensor &codes, const Tensor &scales, const Tensor *first = nullptr)
+{
+    const std::string name = std::string(op) + ": ";
+    chk(codes, name + what, at::kChar, 2, first);
+    chk(scales, name + "scales of " + what, at::kFloat, 1, &codes);
+    TORCH_CHECK(scales.size(0) == codes.size(0), op, ": ", scales.size(0), " scales for ", codes.size(0), " rows of ", what);
+}
+
+Tensor linear_8bit(const Tensor &codes, const Tensor &scales, const Tensor &weight_codes, const Tensor &weight_scales,
+                   const OptTensor &bias, const c10::optional<at::ScalarType> &dtype)
+{
+    const char *op = "linear_8bit";
+    codes_args(op, "codes", codes, scales);
+    codes_args(op, "weight_codes", weight_codes, weight_scales, &codes);
+    const int64_t n = codes.size(0), c = codes.size(1), o = weight_codes.size(0);
+    TORCH_CHECK(weight_codes.size(1) == c && c >= 1 && o >= 1, op, ": codes ", codes.sizes(), ", weight_codes ",
+                weight_codes.sizes(), ": expected [N, C], [O, C]");
+    if (bias.has_value()) {
+        chk(*bias, "linear_8bit: bias", at::kFloat, 1, &codes);
+        TORCH_CHECK(bias->size(0) == o, op, ": bias of ", bias->size(0), " values for ", o, " channels");
+    }
+    Tensor out = at::empty({n, o}, codes.options().dtype(result_dtype(op, dtype)));
+    const int8_t *x = codes.data_ptr<int8_t>(), *w = weight_codes.data_ptr<int8_t>();
+    Tensor ws = workspace(pccnn_linear_8bit_workspace_bytes(x, w, n, c, o), codes);
+    rc_check(pccnn_linear_8bit(x, fptr(scales), w, fptr(weight_scales), ofptr(bias), n, c, o, out.data_ptr(), feature_type(out),
+                               ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
+             "pccnn_linear_8bit");
+    return out;
+}
+
+pccnn_gated gated_problem(const char *op, const Tensor &feats, const Tensor &gate, const Tensor &up, int type,
+                          const std::string &activation)
+{
+    TORCH_CHECK(gate.sizes() == up.sizes() && gate.size(1) == feats.size(1) && gate.size(0) >= 1 && gate.size(1) >= 1, op,
+                ": features ", feats.sizes(), ", gate ", gate.sizes(), ", up ", up.sizes(), ": expected [N, C], [H, C], [H, C]");
+    pccnn_gated p = {};
+    p.feats = feats.data_ptr();
+    p.gate = gate.data_ptr();
+    p.up = up.data_ptr();
+    p.feats_stride = feats.stride(0);
+    p.gate_stride = gate.stride(0);
+    p.up_stride = up.stride(0);
+    p.n = feats.size(0);
+    p.channels = feats.size(1);
+    p.hidden = gate.size(0);
+    p.type = type;
+    p.activation = activation_of(op, activation);
+    return p;
+}
+pccnn_gated gated_args(const char *op, const Tensor &feats, const Tensor &gate, const Tensor &up,
+                       const std::string &activation)
+{
+    chk_features(feats, op, "features", 2);
+    chk_features(gate, op, "gate", 2, &feats);
+    chk_features(up, op, "up", 2, &feats);
+    return gated_problem(op, feats, gate, up, feature_type(feats), activation);
+}
+Tensor gated_forward(const pccnn_gated &p, const Tensor &like, at::ScalarType dtype)
+{
+    Tensor out = at::empty({p.n, p.hidden}, like.options().dtype(dtype));
+    Tensor ws = workspace(pccnn_gated_workspace_bytes(&p, 0), like);
+    rc_check(pccnn_gated_forward(&p, out.data_ptr(), feature_type(out), ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
+             "pccnn_gated_forward");
+    return out;
+}
+
+Tensor gated_linear(const Tensor &feats, const Tensor &gate, const Tensor &up, const std::string &activation)
+{
+    return gated_forward(gated_args("gated_linear", feats, gate, up, activation), feats, feats.scalar_type());
+}
+
+py::tuple gated_linear_grads(const Tensor &feats, const Tensor &gate, const Tensor &up, const Tensor &in_grads,
+                             const std::string &activation, int64_t grad_mask)
+{
+    const char *op = "gated_linear_grads";
+    const pccnn_gated p = gated_args(op, feats, gate, up, activation);
+    chk_features(in_grads, op, "in_grads", 2, &feats);
+    TORCH_CHECK(in_grads.size(0) == p.n && in_grads.size(1) == p.hidden, op, ": in_grads ", in_grads.sizes(), ": expected [",
+                p.n, ", ", p.hidden, "]");
+    OptTensor d_feats, d_gate, d_up;
+    if (grad_mask & PCCNN_GRAD_FEATS) d_feats = feature_result(feats);
+    if (grad_mask & PCCNN_GRAD_WEIGHTS) {
+        d_gate = feature_result(gate);
+        d_up = feature_result(up);
+    }
+    Tensor ws = workspace(pccnn_gated_workspace_bytes(&p, 1), feats);
+    rc_check(pccnn_gated_backward(&p, in_grads.data_ptr(), in_grads.stride(0), optr(d_feats), optr(d_gate), optr(d_up),
+                                  ws.data_ptr(), (size_t)ws.numel(), cur_stream()),
+             "pccnn_gated_backward");
+    return py::make_tuple(opt(d_feats), opt(d_gate), opt(d_up));
+}
+
+Tensor gated_linear_8bit(const Tensor &codes, const Tensor &scales, const Tensor &gate_codes, const Tensor &gate_scales,
+                         const Tensor &up_codes, const Tensor &up_scales, const std::string &activation,
+                         const c10::optional<at::ScalarType> &dtype)
+{
+    const char *op = "gated_linear_8bit";
+    codes_args(op, "codes", codes, scales);
+    codes_args(op, "gate_codes", gate_codes, gate_scales, &codes);
+    codes_args(op, "up_codes", up_codes, up_scales, &codes);
+    pccnn_gated p = gated_problem(op, codes, gate_codes, up_codes, PCCNN_TYPE_I8, activation);
+    p.feats_scales = fptr(scales);
+    p.gate_scales = fptr(gate_scales);
+    p.up_scales = fptr(up_scales);
+    return gated_forward(p, codes, result_dtype(op, dtype));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(pccnn_lib_ops, mod)
@@ -1167,6 +1383,22 @@ PYBIND11_MODULE(pccnn_lib_ops, mod)
             "scale"_a = by_width, "grad_mask"_a = (int)(PCCNN_GRAD_QUERIES | PCCNN_GRAD_KEYS));
     mod.attr("ADDED_NAMES") = py::make_tuple("layer_norm", "layer_norm_grads", "rotary", "rotary_grads", "cross_attention",
                                              "cross_attention_grads");
+    // feed-forward (no counterpart in the reference)
+    const c10::optional<at::ScalarType> none_type;
+    mod.def("rms_norm", &rms_norm, "feats"_a, "gamma"_a, "residual"_a = none, "eps"_a = 1e-6, "return_stats"_a = false);
+    mod.def("rms_norm_grads", &rms_norm_grads, "total"_a, "gamma"_a, "rstd"_a, "in_grads"_a, "total_grads"_a = none,
+            "grad_mask"_a = all);
+    mod.def("rms_norm_8bit", &rms_norm_8bit, "feats"_a, "gamma"_a, "residual"_a = none, "eps"_a = 1e-6);
+    mod.def("quantize_rows", &quantize_rows, "feats"_a);
+    mod.def("linear_8bit", &linear_8bit, "codes"_a, "scales"_a, "weight_codes"_a, "weight_scales"_a, "bias"_a = none,
+            "dtype"_a = none_type);
+    mod.def("gated_linear", &gated_linear, "feats"_a, "gate"_a, "up"_a, "activation"_a = "silu");
+    mod.def("gated_linear_grads", &gated_linear_grads, "feats"_a, "gate"_a, "up"_a, "in_grads"_a, "activation"_a = "silu",
+            "grad_mask"_a = all);
+    mod.def("gated_linear_8bit", &gated_linear_8bit, "codes"_a, "scales"_a, "gate_codes"_a, "gate_scales"_a, "up_codes"_a,
+            "up_scales"_a, "activation"_a = "silu", "dtype"_a = none_type);
+    mod.attr("FEED_FORWARD_NAMES") = py::make_tuple("rms_norm", "rms_norm_grads", "rms_norm_8bit", "quantize_rows", "linear_8bit",
+                                                    "gated_linear", "gated_linear_grads", "gated_linear_8bit");
 
     mod.attr("GRAD_WEIGHTS") = PCCNN_GRAD_WEIGHTS;
     mod.attr("GRAD_FEATS") = PCCNN_GRAD_FEATS;

@@ -1,0 +1,394 @@
+// Products of the feed-forward operators (gated.hip, eight_bit.hip): tiles of rows in LDS, 32 x 32 blocks of results in
+// registers.  The layouts are those of attention_tiles.h: a product C = A B has C's column in the lane and C's rows in the
+// registers, an operand is sixteen bytes of one row.  Here the lane's side are points (rows of the result), the registers' side
+// output channels, so a lane holds runs of four neighboring channels of one point.
+//
+// Operands are bf16 or 8-bit integers whose rows start at multiples of 16 bytes and have whole 16-byte units (zeros behind the
+// last element); whatever is not like that is laid out so first (product_stage_kernel), f32 as three planes of bf16 terms.  A
+// product of f32 operands is then the sum of the six products of planes whose indices add up to at most 2, one after the other
+// over the same accumulators, smallest first.
+#pragma once
+#include "attention_tiles.h"
+
+#include <type_traits>
+
+#ifdef __HIPCC__
+typedef int pccnn_i32x4 __attribute__((ext_vector_type(4)));
+typedef int pccnn_i32x16 __attribute__((ext_vector_type(16)));
+typedef float pccnn_f32x4 __attribute__((ext_vector_type(4)));
+#endif
+
+// One operand: rows of 16-byte units, and the distance of the planes of terms (f32; else one plane).
+struct ProductRows {
+    const void *p;
+    int64_t stride, rows, plane;             // in bytes, rows, bytes
+};
+
+enum { PRODUCT_PAIRS = 6 };                  // f32: products of planes
+// Terms of the pair-th product: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0).
+static inline constexpr int product_term_a(int pair) { return pair == 0 ? 2 : pair == 1 || pair == 3 ? 1 : 0; }
+static inline constexpr int product_term_b(int pair) { return pair == 2 ? 2 : pair == 1 || pair == 4 ? 1 : 0; }
+
+#ifdef __HIPCC__
+// What a lane's operand of 16 bytes is multiplied as.
+struct ProductBf16 {
+    typedef pccnn_f32x16 Acc;
+    typedef float Sum;
+    static constexpr int UNIT = 8;           // elements of a 16-byte unit
+    static __device__ __forceinline__ void mma(Acc &c, pccnn_u32x4 a, pccnn_u32x4 b)
+    {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a), __builtin_bit_cast(pccnn_bf16x8, b),
+                                                    c, 0, 0, 0);
+    }
+};
+struct ProductI8 {
+    typedef pccnn_i32x16 Acc;
+    typedef int Sum;
+    static constexpr int UNIT = 16;
+    static __device__ __forceinline__ void mma(Acc &c, pccnn_u32x4 a, pccnn_u32x4 b)
+    {
+        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(pccnn_i32x4, a), __builtin_bit_cast(pccnn_i32x4, b), c, 0,
+                                                  0, 0);
+    }
+};
+
+// Brings tile after tile of ROWS operand rows, 128 bytes of each, into LDS: the inner dimension lies along the rows.
+template <int ROWS, int THREADS> struct RowsFeeder {
+    typedef AttnTile<1, ROWS, 64> Tile;
+    static constexpr int COUNT = ROWS * 8 / THREADS;
+    static_assert(COUNT >= 1 && COUNT * THREADS == ROWS * 8 && THREADS / 8 % 16 == 0, "whole units, the same one in every round");
+    const char *base;                        // the tile's first row (the same in all lanes)
+    uint32_t off[COUNT];                     // the lane's units from there, in bytes
+    int unit;                                // which of a row's eight units the lane brings
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t row)
+    {
+        base = (const char *)s.p + row * s.stride;
+        unit = Tile::unit_at((int)threadIdx.x / 8, (int)threadIdx.x % 8);
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            const int r = (int)threadIdx.x / 8 + j * (THREADS / 8);
+            off[j] = row + r < s.rows ? (uint32_t)(r * s.stride + 16 * unit) : kAttnNowhere;
+        }
+    }
+    // The 128 bytes from `at` (the same in all lanes) of every row; `units`: how many of these eight units exist.
+    __device__ __forceinline__ void fetch(int64_t at, int units, uint16_t *tile) const
+    {
+        const __amdgpu_buffer_rsrc_t window = attn_window(base + at);
+        const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j)
+            attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + 8 * (j * THREADS + wave_unit));
+    }
+};
+
+// The product of BM rows of the lane's side with BN rows of the registers' side, both with the inner dimension along the rows.
+// WM x WN wavefronts, each with MT x NT blocks of 32 x 32.  PAIR: the registers' side is BN / 2 rows of one operand and as many
+// of another (gate and up), and the first half of a wavefront's NT blocks is of the first, the second half of the second, of the
+// same channels.  Two tiles of 128 bytes of every row are in LDS, one worked on while the next is brought.
+template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
+    static constexpr int THREADS = WM * WN * PCCNN_WAVE, MT = BM / WM / 32, NT = BN / WN / 32;
+    static constexpr int STAGE = (BM + BN) * 64;                      // uint16_t
+    static constexpr size_t LDS = 2 * STAGE * sizeof(uint16_t);
+    static constexpr int PART = PAIR ? BN / 2 : BN;                   // rows of one operand of the registers' side
+    typedef RowsFeeder<BM, THREADS> FeedM;
+    typedef RowsFeeder<PART, THREADS> FeedN;
+    typename E::Acc acc[MT][NT];
+    int lane, half, wm, wn;
+    __device__ __forceinline__ ProductNT()
+    {
+        lane = threadIdx.x % PCCNN_WAVE;
+        half = lane >> 5;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE);
+        wm = wave % WM;
+        wn = wave / WM;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
+    }
+    // Tile row of the lane's side of block m; first tile row of the registers' side of block n.
+    __device__ __forceinline__ int row_of(int m) const { return wm * (32 * MT) + 32 * m + (lane & 31); }
+    __device__ __forceinline__ int col_of(int n) const
+    {
+        if constexpr (PAIR) return n / (NT / 2) * PART + wn * (16 * NT) + 32 * (n % (NT / 2));
+        return wn * (32 * NT) + 32 * n;
+    }
+    __device__ __forceinline__ void multiply(const uint16_t *tile)
+    {
+        typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
+        uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + BM * 64;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            pccnn_u32x4 a[NT], b[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                b[m] = __builtin_bit_cast(pccnn_u32x4, Tile{tm}.rows(row_of(m), 2 * kk + half).t[0]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                a[n] = __builtin_bit_cast(pccnn_u32x4, Tile{tn}.rows(col_of(n) + (lane & 31), 2 * kk + half).t[0]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[n], b[m]);
+        }
+    }
+    // Rows from `row` of `x`, rows from `col` of `one` (and `two`); `units`: 16-byte units of every row; `pairs`: 1, or
+    // PRODUCT_PAIRS for planes of terms.
+    __device__ __forceinline__ void run(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two,
+                                        int64_t col, int units, int pairs, uint16_t *lds)
+    {
+        FeedM fm;
+        FeedN f1, f2;
+        fm.start(x, row);
+        f1.start(one, col);
+        if constexpr (PAIR) f2.start(two, col);
+        const int steps = (units + 7) / 8, total = steps * pairs;
+        int k = 0, pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0;        // of the tile that is brought next
+        auto fetch = [&](uint16_t *to) {
+            const int left = units - 8 * k;
+            const int64_t at_x = product_term_b(pair) * x.plane + 128 * (int64_t)k, at = 128 * (int64_t)k;
+            fm.fetch(at_x, left, to);
+            f1.fetch(product_term_a(pair) * one.plane + at, left, to + BM * 64);
+            if constexpr (PAIR) f2.fetch(product_term_a(pair) * two.plane + at, left, to + (BM + PART) * 64);
+            if (++k == steps) k = 0, ++pair;
+        };
+        if (total > 0) fetch(lds);
+        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+            if (more) fetch(there);
+            multiply(here);
+        };
+        for (int step = 0; step < total; ++step) {
+            attn_landed();
+            walk(lds + (step & 1) * STAGE, lds + ((step & 1) ^ 1) * STAGE, step + 1 < total);
+        }
+        __syncthreads();                                              // LDS is free for the results
+    }
+};
+
+// A tile of BM rows of COLS results in LDS, on its way between the lanes that computed it and whole lines of memory.  The 16-byte
+// units of a row are exchanged among themselves by the row, since 32 lanes write the same columns of 32 rows.
+template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
+    static constexpr int PER = 16 / sizeof(T), UNITS = COLS / PER;
+    static constexpr size_t BYTES = (size_t)BM * COLS * sizeof(T);
+    T *base;
+    static __device__ __forceinline__ int place(int row, int unit) { return unit ^ (row & (UNITS < 8 ? UNITS - 1 : 7)); }
+    __device__ __forceinline__ T *at(int row, int col) const
+    {
+        return base + row * COLS + PER * place(row, col / PER) + col % PER;
+    }
+    // Columns col .. col + 3 (col a multiple of four) of a row.
+    __device__ __forceinline__ void put(int row, int col, const float (&v)[4]) const { pccnn_store<4>(at(row, col), v); }
+    __device__ __forceinline__ void get(int row, int col, float (&v)[4]) const { pccnn_load<4>(at(row, col), v); }
+    // Rows row0 .. of `from`, columns col0 .. , zeros past `rows` and `width`.  Needs a barrier behind it; `wide` as attn_load has
+    // it.  Rows that are whole 16-byte units land by attn_landed().
+    __device__ __forceinline__ void bring(const T *from, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width,
+                                          int wide) const
+    {
+        constexpr int COUNT = BM * UNITS / THREADS;
+        static_assert(COUNT * THREADS == BM * UNITS && THREADS % (8 * UNITS) == 0, "the same unit in every round");
+        const int r0 = (int)threadIdx.x / UNITS;
+        if (wide == 2) {
+            const int unit = place(r0, (int)threadIdx.x % UNITS);
+            const int64_t col = col0 + unit * PER;
+            const __amdgpu_buffer_rsrc_t window = attn_window(from + row0 * stride + col0);
+            const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j) {
+                const int r = r0 + j * (THREADS / UNITS);
+                attn_bring(window, row0 + r < rows && col < width ? (uint32_t)((r * stride + unit * PER) * sizeof(T)) : kAttnNowhere,
+                           base + PER * (j * THREADS + wave_unit));
+            }
+        } else {
+            for (int j = 0; j < COUNT; ++j) {
+                const int r = r0 + j * (THREADS / UNITS), unit = (int)threadIdx.x % UNITS;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int64_t col = col0 + unit * PER + i;
+                    base[r * COLS + PER * place(r, unit) + i] =
+                        row0 + r < rows && col < width ? from[(row0 + r) * stride + col] : (T)0;
+                }
+            }
+        }
+    }
+    // Writes the tile to rows of `stride` elements, columns below `width`, as whole units where every row allows it.
+    __device__ __forceinline__ void out(T *to, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
+    {
+        const bool whole = stride % PER == 0 && width % PER == 0;
+        for (int i = threadIdx.x; i < BM * UNITS; i += THREADS) {
+            const int r = i / UNITS, unit = i % UNITS;
+            const int64_t col = col0 + unit * PER;
+            if (row0 + r >= rows || col >= width) continue;
+            const T *from = base + r * COLS + PER * place(r, unit);
+            T *at = to + (row0 + r) * stride + col;
+            if (whole) {
+                *(pccnn_u32x4 *)at = *(const pccnn_u32x4 *)from;
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    if (col + e < width) at[e] = from[e];
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- few rows
+//
+// Up to 64 rows: no tile is shared by enough of them to be worth LDS.  A workgroup has sixteen output channels (of one or two
+// operands); its wavefronts deal the inner dimension among themselves in steps of 64 bytes, take weights and rows from memory
+// straight into operands of 16 x 16 products, and add their sums in LDS in a fixed order.
+template <typename T> struct FewStep;                                // elements of a lane's operand, of a step of four lanes
+template <> struct FewStep<uint16_t> { static constexpr int UNIT = 8, TERMS = 1; typedef pccnn_f32x4 Acc; typedef float Sum; };
+template <> struct FewStep<float> { static constexpr int UNIT = 8, TERMS = 3; typedef pccnn_f32x4 Acc; typedef float Sum; };
+template <> struct FewStep<int8_t> { static constexpr int UNIT = 16, TERMS = 1; typedef pccnn_i32x4 Acc; typedef int Sum; };
+
+template <int TERMS> struct FewFrag { pccnn_u32x4 t[TERMS]; };
+
+template <typename T> __device__ __forceinline__ FewFrag<FewStep<T>::TERMS> few_load(const T *row, int64_t col, int64_t width, int wide)
+{
+    FewFrag<FewStep<T>::TERMS> f;
+    if constexpr (std::is_same<T, int8_t>::value) {
+        f.t[0] = (pccnn_u32x4){0u, 0u, 0u, 0u};
+        if (col < width) {
+            if (wide == 2) {
+                f.t[0] = *(const pccnn_u32x4 *)(row + col);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (col + i < width) f.t[0][i / 4] |= (uint32_t)(uint8_t)row[col + i] << (8 * (i % 4));
+            }
+        }
+    } else {
+        AttnChunk<T> c;
+        attn_load(c, row, (int)col, (int)width, wide);
+        const auto g = attn_frag(c);
+#pragma unroll
+        for (int t = 0; t < FewStep<T>::TERMS; ++t) f.t[t] = __builtin_bit_cast(pccnn_u32x4, g.t[t]);
+    }
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ void few_mma(typename FewStep<T>::Acc &c, const FewFrag<FewStep<T>::TERMS> &a,
+                                        const FewFrag<FewStep<T>::TERMS> &b)
+{
+    if constexpr (std::is_same<T, int8_t>::value) {
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(pccnn_i32x4, a.t[0]), __builtin_bit_cast(pccnn_i32x4, b.t[0]),
+                                                  c, 0, 0, 0);
+    } else {
+        auto one = [&](int i, int j) {
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pccnn_bf16x8, a.t[i]),
+                                                        __builtin_bit_cast(pccnn_bf16x8, b.t[j]), c, 0, 0, 0);
+        };
+        if constexpr (FewStep<T>::TERMS == 3) {
+            one(2, 0); one(1, 1); one(0, 2); one(1, 0); one(0, 1);
+        }
+        one(0, 0);
+    }
+}
+
+struct FewRows {
+    const void *p;
+    int64_t stride;                          // elements
+    int wide;
+};
+// Sums of sixteen output channels from `col` of OUTS operands with RT x 16 rows, in the first wavefront's registers: lane & 15 is
+// the row, 4 (lane / 16) + i the channel.  False in the other wavefronts.
+template <typename T, int OUTS, int RT, int WAVES> struct FewProduct {
+    typedef FewStep<T> S;
+    typename S::Acc acc[RT][OUTS];
+    __device__ __forceinline__ bool run(const FewRows &x, int64_t rows, const FewRows (&w)[OUTS], int64_t col, int64_t cols,
+                                        int64_t inner, pccnn_u32x4 (*lds)[RT * OUTS][PCCNN_WAVE])
+    {
+        const int lane = threadIdx.x % PCCNN_WAVE, wave = threadIdx.x / PCCNN_WAVE;
+        const int line = lane & 15, quarter = lane >> 4;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int o = 0; o < OUTS; ++o) acc[r][o] = (typename S::Acc){0, 0, 0, 0};
+        const T *xr[RT], *wr[OUTS];
+        // rows and channels that do not exist take the last one's values, and nobody reads their sums
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int64_t row = 16 * r + line;
+            xr[r] = (const T *)x.p + (row < rows ? row : rows - 1) * x.stride;
+        }
+#pragma unroll
+        for (int o = 0; o < OUTS; ++o) wr[o] = (const T *)w[o].p + (col + line < cols ? col + line : cols - 1) * w[o].stride;
+        for (int64_t k = (int64_t)wave * 4 * S::UNIT; k < inner; k += WAVES * 4 * S::UNIT) {
+            const int64_t at = k + quarter * S::UNIT;
+            FewFrag<S::TERMS> a[OUTS], b[RT];
+#pragma unroll
+            for (int o = 0; o < OUTS; ++o) a[o] = few_load<T>(wr[o], at, inner, w[o].wide);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) b[r] = few_load<T>(xr[r], at, inner, x.wide);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int o = 0; o < OUTS; ++o) few_mma<T>(acc[r][o], a[o], b[r]);
+        }
+        if (wave > 0)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int o = 0; o < OUTS; ++o) lds[wave - 1][r * OUTS + o][lane] = __builtin_bit_cast(pccnn_u32x4, acc[r][o]);
+        __syncthreads();
+        if (wave > 0) return false;
+        for (int v = 0; v < WAVES - 1; ++v)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int o = 0; o < OUTS; ++o)
+                    acc[r][o] += __builtin_bit_cast(typename S::Acc, lds[v][r * OUTS + o][lane]);
+        return true;
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- operands laid out
+//
+// Rows of `width` elements, `stride` apart, as rows of whole 16-byte units with zeros behind the last element; f32 as three planes
+// of bf16 terms, `plane` elements apart.  Up to three tensors in one launch (blockIdx.y), a unit per thread.
+struct StageSource {
+    const void *p;
+    int64_t stride, rows;
+    int wide;
+    void *to;
+};
+struct StageArgs {
+    StageSource s[3];
+    int64_t width;
+    int units;
+};
+template <typename T> static __global__ __launch_bounds__(256) void product_stage_kernel(StageArgs a)
+{
+    constexpr int UNIT = FewStep<T>::UNIT, TERMS = FewStep<T>::TERMS;
+    const StageSource s = blockIdx.y == 0 ? a.s[0] : blockIdx.y == 1 ? a.s[1] : a.s[2];
+    const int64_t count = s.rows * a.units;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / a.units;
+        const FewFrag<TERMS> f = few_load<T>((const T *)s.p + row * s.stride, (i - row * a.units) * UNIT, a.width, s.wide);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) ((pccnn_u32x4 *)s.to)[t * count + i] = f.t[t];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- launches
+//
+// Tiles of output channels follow each other within a tile of rows; those of a run go to one XCD, whose L2 then serves the rows.
+static inline int product_run(int tiles) { return tiles <= 64 ? tiles : 32; }
+
+template <typename KERNEL, typename ARGS>
+static int product_launch(const char *name, KERNEL kernel, size_t lds, int threads, ARGS &a, int64_t tiles_m, int64_t tiles_n, hipStream_t s)
+{
+    a.blocks = tiles_m * tiles_n;
+    a.tiles = (int)tiles_n;
+    a.run = product_run(a.tiles);
+    PCCNN_REQUIRE(a.blocks <= INT32_MAX - PCCNN_XCDS * (int64_t)a.run, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name,
+                  (long long)a.blocks);
+    if (lds > 65536)
+        PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    kernel<<<pccnn_xcd_grid(a.blocks, a.run), threads, lds, s>>>(a);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+#endif

@@ -1645,6 +1645,205 @@ def cross_attention_grads(queries, keys, values, query_starts, key_starts, max_q
     return d_queries, d_keys, d_values
 
 
+# ----------------------------------------------------------------------------- feed-forward
+#
+# The half of a block that follows attention between levels: root-mean-square norm with the residual's addition, rows in 8
+# bits, the gated linear map and linear maps of 8-bit rows.  Features as above; 8-bit rows are int8 codes with one float32
+# scale for a row, whose value is code * scale.
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2, "relu": 3}
+_TYPE_I8 = 2
+
+
+def _activation(name, activation):
+    if activation not in ACTIVATIONS:
+        raise RuntimeError("%s: activation %r (%s)" % (name, activation, ", ".join(ACTIVATIONS)))
+    return ACTIVATIONS[activation]
+
+
+def _result_dtype(name, dtype):
+    if dtype is not None and dtype not in _FEATURE_TYPES:
+        raise RuntimeError("%s: expected dtype torch.float32 or torch.bfloat16 for the result, got %s" % (name, dtype))
+    return torch.bfloat16 if dtype is None else dtype
+
+
+def _rms_args(name, feats, gamma, residual):
+    _norm_args(name, feats, (("gamma", gamma),))
+    if residual is not None:
+        _chk_features(residual, name + ": residual", 2, feats.dtype, feats.device)
+        if residual.shape != feats.shape:
+            raise RuntimeError("%s: residual %s for features %s" % (name, tuple(residual.shape), tuple(feats.shape)))
+    n, c = feats.shape
+    total = None if residual is None else torch.empty((n, c), dtype=feats.dtype, device=feats.device)
+    return n, c, total, 0 if residual is None else residual.stride(0)
+
+
+def rms_norm(feats, gamma, residual=None, eps=1e-6, return_stats=False):
+    """Root-mean-square norm of every row, of s = feats (+ residual): s / sqrt(avg(s^2) + eps) * gamma.  feats, residual [N, C]
+    float32 or bfloat16 (rows may be a view's); gamma [C], float32 or of the features' dtype.  -> out [N, C]; with a residual
+    also s [N, C] in the features' dtype (the norm is of the rounded s); with ``return_stats`` also f32 [N] = 1 / sqrt(...),
+    which ``rms_norm_grads`` takes."""
+    name = "rms_norm"
+    n, c, total, residual_stride = _rms_args(name, feats, gamma, residual)
+    out = torch.empty((n, c), dtype=feats.dtype, device=feats.device)
+    rstd = torch.empty((n,), dtype=torch.float32, device=feats.device) if return_stats else None
+    _lib.call("pccnn_rms_norm_forward", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), _optr(residual),
+              residual_stride, _ptr(gamma), _FEATURE_TYPES[gamma.dtype], float(eps), n, c, _ptr(out), _optr(total),
+              _optr(rstd), _stream())
+    results = [t for t in (out, total, rstd) if t is not None]
+    return results[0] if len(results) == 1 else tuple(results)
+
+
+def rms_norm_grads(total, gamma, rstd, in_grads, total_grads=None, grad_mask=GRAD_ALL):
+    """Gradients of ``rms_norm`` -> (d_feats [N, C], d_gamma [C]), the second in gamma's dtype and summed over the rows in a
+    fixed order; None for a group that ``grad_mask`` (GRAD_FEATS, GRAD_WEIGHTS) does not name.  ``total``: s, which is feats
+    where there was no residual; ``total_grads``: the gradient of s as a result, added to d_feats.  d_feats is the gradient of
+    feats and of residual alike."""
+    name = "rms_norm_grads"
+    _norm_args(name, total, (("gamma", gamma),))
+    n, c = total.shape
+    _chk(rstd, name + ": rstd", torch.float32, 1, total.device)
+    _chk_features(in_grads, name + ": in_grads", 2, total.dtype, total.device)
+    if total_grads is not None:
+        _chk_features(total_grads, name + ": total_grads", 2, total.dtype, total.device)
+    if rstd.shape[0] != n or in_grads.shape != total.shape or (total_grads is not None and total_grads.shape != total.shape):
+        raise RuntimeError(name + ": inconsistent shapes")
+    d_feats = torch.empty((n, c), dtype=total.dtype, device=total.device) if grad_mask & GRAD_FEATS else None
+    d_gamma = ws = None
+    if grad_mask & GRAD_WEIGHTS:
+        d_gamma = torch.empty_like(gamma)
+        ws = _workspace(_lib.load().pccnn_rms_norm_workspace_bytes(n, c), total.device)
+    _lib.call("pccnn_rms_norm_backward", _ptr(total), _FEATURE_TYPES[total.dtype], total.stride(0), _ptr(gamma),
+              _FEATURE_TYPES[gamma.dtype], _ptr(rstd), _ptr(in_grads), in_grads.stride(0), _optr(total_grads),
+              0 if total_grads is None else total_grads.stride(0), n, c, _optr(d_feats), _optr(d_gamma), _optr(ws),
+              0 if ws is None else ws.numel(), _stream())
+    return d_feats, d_gamma
+
+
+def _codes_for(n, c, device):
+    return (torch.empty((n, c), dtype=torch.int8, device=device), torch.empty((n,), dtype=torch.float32, device=device))
+
+
+def rms_norm_8bit(feats, gamma, residual=None, eps=1e-6):
+    """``rms_norm`` with its result in 8 bits -> (codes int8 [N, C], scales f32 [N]), with a residual also s [N, C].  A row's
+    scale is its largest magnitude / 127, its codes are the nearest integers of value / scale (ties to even, decided in 64
+    bits).  A row of zeros has scale 0; one that holds an infinity or NaN has codes 0 and scale NaN."""
+    name = "rms_norm_8bit"
+    n, c, total, residual_stride = _rms_args(name, feats, gamma, residual)
+    codes, scales = _codes_for(n, c, feats.device)
+    _lib.call("pccnn_rms_norm_8bit", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), _optr(residual),
+              residual_stride, _ptr(gamma), _FEATURE_TYPES[gamma.dtype], float(eps), n, c, _ptr(codes), _ptr(scales),
+              _optr(total), _stream())
+    return (codes, scales) if total is None else (codes, scales, total)
+
+
+def quantize_rows(feats):
+    """Rows in 8 bits as they are, by ``rms_norm_8bit``'s rule -> (codes int8 [N, C], scales f32 [N]).  Lays out weights
+    [out, in] for ``linear_8bit`` and ``gated_linear_8bit`` (a scale for every output channel) as well as features."""
+    name = "quantize_rows"
+    _chk_features(feats, name + ": features", 2)
+    if feats.shape[1] < 1:
+        raise RuntimeError(name + ": features without channels")
+    n, c = feats.shape
+    codes, scales = _codes_for(n, c, feats.device)
+    _lib.call("pccnn_quantize_rows", _ptr(feats), _FEATURE_TYPES[feats.dtype], feats.stride(0), n, c, _ptr(codes),
+              _ptr(scales), _stream())
+    return codes, scales
+
+
+def _codes_args(name, label, codes, scales, device=None):
+    _chk(codes, "%s: %s" % (name, label), torch.int8, 2, device)
+    _chk(scales, "%s: scales of %s" % (name, label), torch.float32, 1, codes.device)
+    if scales.shape[0] != codes.shape[0]:
+        raise RuntimeError("%s: %d scales for %d rows of %s" % (name, scales.shape[0], codes.shape[0], label))
+
+
+def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None, dtype=None):
+    """Linear map of 8-bit rows: (codes weight_codes^T) * scales[:, None] * weight_scales (+ bias).  codes int8 [N, C], scales
+    f32 [N], weight_codes int8 [O, C], weight_scales f32 [O], bias f32 [O] -> [N, O], bfloat16 or what ``dtype`` says (float32).
+    The sums are exact (C <= 131071)."""
+    name = "linear_8bit"
+    _codes_args(name, "codes", codes, scales)
+    _codes_args(name, "weight_codes", weight_codes, weight_scales, codes.device)
+    (n, c), o = codes.shape, weight_codes.shape[0]
+    if weight_codes.shape[1] != c or c < 1 or o < 1:
+        raise RuntimeError("%s: codes %s, weight_codes %s: expected [N, C], [O, C]" % (name, tuple(codes.shape),
+                                                                                    tuple(weight_codes.shape)))
+    if bias is not None:
+        _chk(bias, name + ": bias", torch.float32, 1, codes.device)
+        if bias.shape[0] != o:
+            raise RuntimeError("%s: bias of %d values for %d channels" % (name, bias.shape[0], o))
+    out = torch.empty((n, o), dtype=_result_dtype(name, dtype), device=codes.device)
+    ws = _workspace(_lib.load().pccnn_linear_8bit_workspace_bytes(_ptr(codes), _ptr(weight_codes), n, c, o), codes.device)
+    _lib.call("pccnn_linear_8bit", _ptr(codes), _ptr(scales), _ptr(weight_codes), _ptr(weight_scales), _optr(bias), n, c, o,
+              _ptr(out), _FEATURE_TYPES[out.dtype], _ptr(ws), ws.numel(), _stream())
+    return out
+
+
+def _gated_problem(name, feats, gate, up, type, activation):
+    (n, c), h = feats.shape, gate.shape[0]
+    if gate.shape != up.shape or gate.shape[1] != c or c < 1 or h < 1:
+        raise RuntimeError("%s: features %s, gate %s, up %s: expected [N, C], [H, C], [H, C]"
+                           % (name, tuple(feats.shape), tuple(gate.shape), tuple(up.shape)))
+    p = _lib.Gated()
+    p.feats, p.gate, p.up = feats.data_ptr(), gate.data_ptr(), up.data_ptr()
+    p.feats_stride, p.gate_stride, p.up_stride = feats.stride(0), gate.stride(0), up.stride(0)
+    p.n, p.channels, p.hidden, p.type, p.activation = n, c, h, type, _activation(name, activation)
+    return p
+
+
+def _gated_args(name, feats, gate, up, activation):
+    _chk_features(feats, name + ": features", 2)
+    _chk_features(gate, name + ": gate", 2, feats.dtype, feats.device)
+    _chk_features(up, name + ": up", 2, feats.dtype, feats.device)
+    return _gated_problem(name, feats, gate, up, _FEATURE_TYPES[feats.dtype], activation)
+
+
+def _gated_forward(p, out):
+    ws = _workspace(_lib.load().pccnn_gated_workspace_bytes(ctypes.byref(p), 0), out.device)
+    _lib.call("pccnn_gated_forward", ctypes.byref(p), _ptr(out), _FEATURE_TYPES[out.dtype], _ptr(ws), ws.numel(), _stream())
+    return out
+
+
+def gated_linear(feats, gate, up, activation="silu"):
+    """act(feats gate^T) * (feats up^T), element by element: both projections, the activation and their product in one kernel.
+    feats [N, C], gate and up [H, C] (the weights of linear maps; rows may be a view's), all float32 or all bfloat16;
+    ``activation``: "silu", "gelu" (x Phi(x)), "sigmoid" or "relu".  -> [N, H].  float32 keeps float32 accuracy (infinities give
+    NaN); bfloat16 keeps both projections in fp32 and rounds the result once."""
+    p = _gated_args("gated_linear", feats, gate, up, activation)
+    return _gated_forward(p, torch.empty((p.n, p.hidden), dtype=feats.dtype, device=feats.device))
+
+
+def gated_linear_grads(feats, gate, up, in_grads, activation="silu", grad_mask=GRAD_ALL):
+    """Gradients of ``gated_linear`` from its inputs (the projections are formed anew) -> (d_feats [N, C], d_gate [H, C],
+    d_up [H, C]); None for a group that ``grad_mask`` (GRAD_FEATS; GRAD_WEIGHTS: gate and up) does not name.  bfloat16 rounds the
+    gradients of the projections for the products that they enter.  No float atomics: the same bits from run to run."""
+    name = "gated_linear_grads"
+    p = _gated_args(name, feats, gate, up, activation)
+    _chk_features(in_grads, name + ": in_grads", 2, feats.dtype, feats.device)
+    if tuple(in_grads.shape) != (p.n, p.hidden):
+        raise RuntimeError("%s: in_grads %s: expected [%d, %d]" % (name, tuple(in_grads.shape), p.n, p.hidden))
+    new = lambda like: torch.empty(like.shape, dtype=like.dtype, device=like.device)  # noqa: E731
+    d_feats = new(feats) if grad_mask & GRAD_FEATS else None
+    d_gate, d_up = (new(gate), new(up)) if grad_mask & GRAD_WEIGHTS else (None, None)
+    ws = _workspace(_lib.load().pccnn_gated_workspace_bytes(ctypes.byref(p), 1), feats.device)
+    _lib.call("pccnn_gated_backward", ctypes.byref(p), _ptr(in_grads), in_grads.stride(0), _optr(d_feats), _optr(d_gate),
+              _optr(d_up), _ptr(ws), ws.numel(), _stream())
+    return d_feats, d_gate, d_up
+
+
+def gated_linear_8bit(codes, scales, gate_codes, gate_scales, up_codes, up_scales, activation="silu", dtype=None):
+    """``gated_linear`` of 8-bit rows and weights: codes int8 [N, C] with scales f32 [N], gate_codes and up_codes int8 [H, C] with
+    scales f32 [H] -> [N, H], bfloat16 or what ``dtype`` says (float32).  The sums are exact (C <= 131071)."""
+    name = "gated_linear_8bit"
+    _codes_args(name, "codes", codes, scales)
+    _codes_args(name, "gate_codes", gate_codes, gate_scales, codes.device)
+    _codes_args(name, "up_codes", up_codes, up_scales, codes.device)
+    p = _gated_problem(name, codes, gate_codes, up_codes, _TYPE_I8, activation)
+    p.feats_scales, p.gate_scales, p.up_scales = scales.data_ptr(), gate_scales.data_ptr(), up_scales.data_ptr()
+    return _gated_forward(p, torch.empty((p.n, p.hidden), dtype=_result_dtype(name, dtype), device=codes.device))
+
+
 REFERENCE_NAMES = (
     "build_grid_ds", "compute_keys", "find_neighbors", "compute_pdf", "compute_pdf_grads", "poisson_disk_sampling",
     "mc_conv", "mc_conv_grads", "mc_conv_weight_var", "point_conv_basis", "point_conv_basis_grads", "point_conv",
@@ -1654,6 +1853,8 @@ REFERENCE_NAMES = (
 # Operators the reference does not have that the compiled module serves too (a Python call through ctypes costs about
 # ten microseconds, more than the smallest of them run).
 ADDED_NAMES = ("layer_norm", "layer_norm_grads", "rotary", "rotary_grads", "cross_attention", "cross_attention_grads")
+FEED_FORWARD_NAMES = ("rms_norm", "rms_norm_grads", "rms_norm_8bit", "quantize_rows", "linear_8bit", "gated_linear",
+                      "gated_linear_grads", "gated_linear_8bit")
 
 
 # ----------------------------------------------------------------------------- bindings
@@ -1661,10 +1862,11 @@ ADDED_NAMES = ("layer_norm", "layer_norm_grads", "rotary", "rotary_grads", "cros
 # Two bindings of the same C ABI serve the 26 reference names: the compiled extension module ``pccnn_lib_ops`` (what
 # the reference builds from setup.py:7-31; csrc/ops_module.cpp here: pybind11, TORCH_CHECK contracts, at::empty
 # outputs, torch's current HIP stream) and the ctypes functions above, which need no compiler.  The compiled one is
-# used when it has been built; ``use_binding`` switches.  Both also serve ``ADDED_NAMES``; other functions beyond the 26
-# names exist only in this module.
+# used when it has been built; ``use_binding`` switches.  Both also serve ``ADDED_NAMES`` and ``FEED_FORWARD_NAMES``; other
+# functions beyond the 26 names exist only in this module.
 
-BINDINGS = {"ctypes": {name: globals()[name] for name in REFERENCE_NAMES + ADDED_NAMES}}
+_BOUND_NAMES = REFERENCE_NAMES + ADDED_NAMES + FEED_FORWARD_NAMES
+BINDINGS = {"ctypes": {name: globals()[name] for name in _BOUND_NAMES}}
 binding = "ctypes"
 
 
@@ -1688,8 +1890,8 @@ def _load_compiled():
 
 
 def use_binding(which):
-    """Route the 26 reference names and ``ADDED_NAMES`` through the "compiled" extension or through "ctypes"; returns the name of the
-    binding in use before the call.  Raises if the compiled module has not been built."""
+    """Route the 26 reference names, ``ADDED_NAMES`` and ``FEED_FORWARD_NAMES`` through the "compiled" extension or through
+    "ctypes"; returns the name of the binding in use before the call.  Raises if the compiled module has not been built."""
     global binding
     if which not in BINDINGS:
         if which != "compiled":
@@ -1698,11 +1900,11 @@ def use_binding(which):
         if mod is None:
             raise RuntimeError("use_binding: the compiled pccnn_lib_ops extension has not been built "
                                "(python -m pccnn_lib_amd.build)")
-        missing = [name for name in ADDED_NAMES if not hasattr(mod, name)]
+        missing = [name for name in ADDED_NAMES + FEED_FORWARD_NAMES if not hasattr(mod, name)]
         if missing:
             raise RuntimeError("use_binding: the compiled pccnn_lib_ops extension was built from older sources (it has no "
                                "%s); rebuild it with `python -m pccnn_lib_amd.build`" % missing[0])
-        BINDINGS["compiled"] = {name: getattr(mod, name) for name in REFERENCE_NAMES + ADDED_NAMES}
+        BINDINGS["compiled"] = {name: getattr(mod, name) for name in _BOUND_NAMES}
     before, binding = binding, which
     globals().update(BINDINGS[which])
     return before
