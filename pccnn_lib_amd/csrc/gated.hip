@@ -607,8 +607,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
     int rc = gated_check(name, p);
     if (rc != PCCNN_OK) return rc;
     PCCNN_REQUIRE(p->type != PCCNN_TYPE_I8, PCCNN_ERR_UNSUPPORTED, "%s: 8-bit operands have no gradients", name);
-    PCCNN_REQUIRE(grads_stride >= 0 && grads_stride <= (1 << 21), PCCNN_ERR_INVALID, "%s: gradient rows %lld apart", name,
-                  (long long)grads_stride);
+    PCCNN_REQUIRE(grads_stride >= 0, PCCNN_ERR_INVALID, "%s: gradient rows %lld apart", name, (long long)grads_stride);
     PCCNN_REQUIRE((d_gate != nullptr) == (d_up != nullptr), PCCNN_ERR_INVALID, "%s: the gradients of both weights come together",
                   name);
     if (d_gate == nullptr && (d_feats == nullptr || p->n == 0)) return PCCNN_OK;
@@ -633,7 +632,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         a.x = r[0], a.gate = r[1], a.up = r[2];
         a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation, a.pairs = pairs;
         a.grads = in_grads, a.grads_stride = grads_stride;
-        a.grads_wide = wide_of(in_grads, grads_stride, p->hidden, p->type);
+        a.grads_wide = grads_stride <= kMostWidth ? wide_of(in_grads, grads_stride, p->hidden, p->type) : 0;
         a.d_pre = (uint16_t *)d.p, a.padded = plan.padded, a.d_plane = d.plane / 2;
         rc = f32 ? gated_launch<ProductBf16, float, true>(name, a, s) : gated_launch<ProductBf16, uint16_t, true>(name, a, s);
         if (rc != PCCNN_OK) return rc;

@@ -7,9 +7,11 @@ from .convolutions import (ComputeKPConv, ComputeKPConvWeightVar, ComputeMCConv,
                            ComputeKPConvNWeightVar, ComputeSPHConv, ComputeSPHConvWeightVar, ComputePCCNN,
                            ComputePCCNNWeightVar)
 from .attention import ComputeCrossAttention, ComputeLayerNorm, ComputeRotary
+from .feed_forward import ComputeGatedLinear, ComputeRMSNorm
 
 __all__ = ["BuildGridDS", "ComputeKeys", "FindNeighbors", "PoissonDiskSamlping", "ComputePDF",
            "ComputeKPConv", "ComputeKPConvWeightVar", "ComputeMCConv", "ComputeMCConvWeightVar",
            "ComputePointConvBasis", "ComputePointConv", "ComputePointConvWeightVar",
            "ComputeKPConvN", "ComputeKPConvNWeightVar", "ComputeSPHConv", "ComputeSPHConvWeightVar",
-           "ComputePCCNN", "ComputePCCNNWeightVar", "ComputeLayerNorm", "ComputeRotary", "ComputeCrossAttention"]
+           "ComputePCCNN", "ComputePCCNNWeightVar", "ComputeLayerNorm", "ComputeRotary", "ComputeCrossAttention",
+           "ComputeRMSNorm", "ComputeGatedLinear"]

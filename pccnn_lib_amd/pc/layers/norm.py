@@ -1,6 +1,6 @@
 import torch
 
-from ...op_wrappers import ComputeLayerNorm
+from ...op_wrappers import ComputeLayerNorm, ComputeRMSNorm
 
 
 class Bias(torch.nn.Module):
@@ -57,3 +57,17 @@ class LayerNormalization(torch.nn.Module):
 
     def forward(self, p_feats):
         return ComputeLayerNorm.apply(p_feats, self.gamma_.reshape(-1), self.betas_.reshape(-1), self.eps_)
+
+
+class RMSNormalization(torch.nn.Module):
+    """Root-mean-square norm of every point's features, parameter ``gamma_`` [1, F] (no counterpart in the reference).  Features
+    float32, or bfloat16 under a parameter of either type.  With ``p_residual`` (the update that the features get first) the sum
+    comes back too: (norm of the sum, the sum)."""
+
+    def __init__(self, p_num_features, p_eps=1e-6):
+        super(RMSNormalization, self).__init__()
+        self.num_features_, self.eps_ = p_num_features, p_eps
+        self.gamma_ = torch.nn.Parameter(torch.ones(1, p_num_features))
+
+    def forward(self, p_feats, p_residual=None):
+        return ComputeRMSNorm.apply(p_feats, self.gamma_.reshape(-1), p_residual, self.eps_)
