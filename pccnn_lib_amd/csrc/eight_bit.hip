@@ -82,12 +82,17 @@ template <typename OUT, int RT, int WAVES> __global__ __launch_bounds__(WAVES *P
     }
 }
 
-template <typename T, int BN, int WM, int WN> int linear_launch(LinearArgs &a, hipStream_t s)
+template <typename T, int BM, int BN, int WM, int WN> int linear_launch(LinearArgs &a, hipStream_t s)
 {
-    constexpr int BM = 128;
     typedef ProductNT<ProductI8, BM, BN, WM, WN, false> Product;
-    return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>, std::max(Product::LDS, (size_t)BM * BN * sizeof(T)),
+    return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>, std::max(Product::lds_bytes(a.units, 1), (size_t)BM * BN * sizeof(T)),
                           Product::THREADS, a, pccnn_ceil_div(a.n, BM), pccnn_ceil_div(a.outer, BN), s);
+}
+template <typename T> int linear_tiles(LinearArgs &a, hipStream_t s)
+{
+    if constexpr (!std::is_same<T, float>::value)
+        if (product_large(a.n, a.outer, a.units, 1)) return linear_launch<T, 256, 256, 2, 4>(a, s);
+    return a.outer <= 64 ? linear_launch<T, 128, 64, 4, 1>(a, s) : linear_launch<T, 128, 128, 2, 2>(a, s);
 }
 template <typename OUT> int linear_few(const LinearFew &a, hipStream_t s)
 {
@@ -164,7 +169,5 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
         product_stage_kernel<int8_t><<<grid, 256, 0, s>>>(stage);
         PCCNN_LAUNCH_CHECK();
     }
-    if (outer <= 64)
-        return out_type == PCCNN_TYPE_F32 ? linear_launch<float, 64, 4, 1>(a, s) : linear_launch<uint16_t, 64, 4, 1>(a, s);
-    return out_type == PCCNN_TYPE_F32 ? linear_launch<float, 128, 2, 2>(a, s) : linear_launch<uint16_t, 128, 2, 2>(a, s);
+    return out_type == PCCNN_TYPE_F32 ? linear_tiles<float>(a, s) : linear_tiles<uint16_t>(a, s);
 }

@@ -271,17 +271,19 @@ struct WeightsArgs {
     ProductRows x, d;                        // rows with whole units; stride in bytes
     int64_t n, cols_x, cols_d;               // columns that exist, in whole units
     int pairs;
-    int tiles_x, tiles_d, splits;
+    int tiles_x, tiles_d, splits, run;
+    int64_t blocks;
     int64_t per_split;                       // rows of a part, a multiple of 64
     float *part;                             // [split][cols_d][channels]
     int64_t channels;
 };
-constexpr int kTurnRows = 64, kTurnCols = 128;
+constexpr int kTurnRows = 64;                // rows of a step
 
-struct ColumnsFeeder {
-    typedef AttnTile<1, kTurnRows, kTurnCols> Tile;
-    static constexpr int COUNT = kTurnRows * Tile::UNITS / kThreads;
-    static_assert(kThreads / Tile::UNITS % 16 == 0, "the same unit in every round");
+// Brings kTurnRows rows of up to 128 columns each into LDS, where the transposing reads take their columns.
+template <int COLS, int THREADS> struct ColumnsFeeder {
+    typedef AttnTile<1, kTurnRows, COLS> Tile;
+    static constexpr int COUNT = kTurnRows * Tile::UNITS / THREADS;
+    static_assert(COUNT >= 1 && THREADS / Tile::UNITS % 16 == 0, "whole units, the same one in every round");
     const char *base;
     int64_t stride;
     int unit, row;
@@ -300,69 +302,103 @@ struct ColumnsFeeder {
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
-            const int r = row + j * (kThreads / Tile::UNITS);
+            const int r = row + j * (THREADS / Tile::UNITS);
             attn_bring(window, live && at_row + r < rows ? (uint32_t)(r * stride + 16 * unit) : kAttnNowhere,
-                       tile + 8 * (j * kThreads + wave_unit));
+                       tile + 8 * (j * THREADS + wave_unit));
         }
     }
 };
-__global__ __launch_bounds__(kThreads) void gated_weights_kernel(WeightsArgs a)
+// DP x 128 columns of (dG | dU) times XP x XT columns of x; a wavefront has 32 MT x 64 of them.
+constexpr int weights_threads(int dp, int xp, int xt, int mt) { return dp * 128 / (32 * mt) * (xp * xt / 64) * PCCNN_WAVE; }
+template <int DP, int XP, int XT, int MT> struct WeightsShape {
+    static constexpr int COLS_D = DP * 128, COLS_X = XP * XT, WAVES_X = COLS_X / 64, WAVES_D = COLS_D / (32 * MT);
+    static constexpr int THREADS = WAVES_X * WAVES_D * PCCNN_WAVE;
+    static_assert(THREADS == weights_threads(DP, XP, XT, MT), "");
+    static constexpr int STAGE = kTurnRows * (COLS_D + COLS_X);       // uint16_t
+    static constexpr size_t LDS = 2 * STAGE * sizeof(uint16_t);
+};
+template <int DP, int XP, int XT, int MT>
+__global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights_kernel(WeightsArgs a)
 {
-    typedef ColumnsFeeder::Tile Tile;
+    typedef WeightsShape<DP, XP, XT, MT> Shape;
+    constexpr int WAVES_X = Shape::WAVES_X, STAGE = Shape::STAGE;
+    typedef ColumnsFeeder<128, Shape::THREADS> FeedD;
+    typedef ColumnsFeeder<XT, Shape::THREADS> FeedX;
+    typedef typename FeedD::Tile TileD;
+    typedef typename FeedX::Tile TileX;
     extern __shared__ __align__(16) uint16_t lds[];
     const int lane = threadIdx.x % PCCNN_WAVE, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE), wd = wave % 2, wx = wave / 2;
-    int64_t block = blockIdx.x;
-    const int64_t x0 = block % a.tiles_x * kTurnCols;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE), wx = wave % WAVES_X, wd = wave / WAVES_X;
+    int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
+    if (block >= a.blocks) return;
+    const int64_t x0 = block % a.tiles_x * Shape::COLS_X;
     block /= a.tiles_x;
-    const int64_t d0 = block % a.tiles_d * kTurnCols;
+    const int64_t d0 = block % a.tiles_d * Shape::COLS_D;
     const int64_t split = block / a.tiles_d;
     const int64_t first = split * a.per_split, last = min(a.n, first + a.per_split);
-    ColumnsFeeder fx, fd;
-    fx.start(a.x, x0, a.cols_x);
-    fd.start(a.d, d0, a.cols_d);
-    pccnn_f32x16 acc[2][2];
+    FeedX fx[XP];
+    FeedD fd[DP];
+#pragma unroll
+    for (int i = 0; i < XP; ++i) fx[i].start(a.x, x0 + i * XT, a.cols_x);
+#pragma unroll
+    for (int i = 0; i < DP; ++i) fd[i].start(a.d, d0 + i * 128, a.cols_d);
+    pccnn_f32x16 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     const int64_t steps = (last - first + kTurnRows - 1) / kTurnRows, total = steps * a.pairs;
     int64_t k = 0;
     int pair = a.pairs == 1 ? PRODUCT_PAIRS - 1 : 0;
-    constexpr int STAGE = 2 * Tile::ELEMENTS;
     auto fetch = [&](uint16_t *to) {
-        fx.fetch(first + k * kTurnRows, product_term_a(pair) * a.x.plane, last, to);
-        fd.fetch(first + k * kTurnRows, product_term_b(pair) * a.d.plane, last, to + Tile::ELEMENTS);
+        const int64_t at = first + k * kTurnRows;
+#pragma unroll
+        for (int i = 0; i < DP; ++i) fd[i].fetch(at, product_term_b(pair) * a.d.plane, last, to + i * TileD::ELEMENTS);
+#pragma unroll
+        for (int i = 0; i < XP; ++i)
+            fx[i].fetch(at, product_term_a(pair) * a.x.plane, last, to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
         if (++k == steps) k = 0, ++pair;
     };
-    if (total > 0) fetch(lds);
-    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool work, bool more) {
         if (more) fetch(there);
-        const Tile tx = {here}, td = {here + Tile::ELEMENTS};
-#pragma unroll
-        for (int kk = 0; kk < kTurnRows / 16; ++kk) {
-            AttnFrag<1> fa[2], fb[2];
+        if (!work) return;                   // (the first round only asks)
+        AttnFrag<1> fa[2][2], fb[2][MT];
+        auto read = [&](int kk) {            // a step of products ahead of their use
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                fa[i] = tx.columns(16 * kk, 64 * wx + 32 * i, lane);
-                fb[i] = td.columns(16 * kk, 64 * wd + 32 * i, lane);
+                const int col = 64 * wx + 32 * i;
+                fa[kk & 1][i] = TileX{here + DP * TileD::ELEMENTS + col / XT * TileX::ELEMENTS}.columns(16 * kk, col % XT, lane);
             }
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int col = 32 * (MT * wd + j);
+                fb[kk & 1][j] = TileD{here + col / 128 * TileD::ELEMENTS}.columns(16 * kk, col % 128, lane);
+            }
+        };
+        constexpr int COUNT = kTurnRows / 16;
+        read(0);
+#pragma unroll
+        for (int kk = 0; kk < COUNT; ++kk) {
+            if (kk + 1 < COUNT) read(kk + 1);
+            __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) attn_mma(acc[i][j], fa[i], fb[j]);
+                for (int j = 0; j < MT; ++j) attn_mma(acc[i][j], fa[kk & 1][i], fb[kk & 1][j]);
+            __builtin_amdgcn_sched_barrier(0x6);
         }
     };
-    for (int64_t step = 0; step < total; ++step) {
-        attn_landed();
-        walk(lds + (step & 1) * STAGE, lds + ((step & 1) ^ 1) * STAGE, step + 1 < total);
+    for (int64_t step = -1; step < total; ++step) {
+        product_landed();
+        const int stage = (int)step & 1;
+        walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step >= 0, step + 1 < total);
     }
     float *part = a.part + split * a.cols_d * a.channels;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t d = d0 + 64 * wd + 32 * j + (lane & 31);
+    for (int j = 0; j < MT; ++j) {
+        const int64_t d = d0 + 32 * (MT * wd + j) + (lane & 31);
         if (d >= a.cols_d) continue;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -463,9 +499,9 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     }
     plan.padded = pccnn_ceil_div(p->hidden, 8) * 8;
     // parts enough to fill the chip twice over, of at least four steps
-    plan.tiles_x = (int)pccnn_ceil_div(p->channels, kTurnCols);
-    plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, kTurnCols);
-    const int64_t want = std::max<int64_t>(1, 512 / ((int64_t)plan.tiles_x * plan.tiles_d));
+    plan.tiles_x = (int)pccnn_ceil_div(p->channels, p->channels <= 64 ? 64 : p->channels <= 128 ? 128 : 256);
+    plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, 256);
+    const int64_t want = std::max<int64_t>(1, 256 / ((int64_t)plan.tiles_x * plan.tiles_d));
     const int64_t steps = std::max<int64_t>(1, pccnn_ceil_div(p->n, kTurnRows));
     const int64_t per = std::max<int64_t>(std::min<int64_t>(4, steps), pccnn_ceil_div(steps, want));
     plan.per_split = per * kTurnRows;
@@ -504,21 +540,47 @@ int gated_operands(const char *name, const pccnn_gated *p, const GatedPlan &plan
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
 }
-template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)
+template <class E, typename T, bool BACK, int BM, int BN, int WM, int WN>
+int gated_launch_tile(const char *name, GatedArgs &a, hipStream_t s)
 {
-    constexpr int BM = 128, BN = 128, WM = 2, WN = 2;
     typedef ProductNT<E, BM, BN, WM, WN, true> Product;
-    const size_t lds = std::max(Product::LDS, (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
+    const size_t lds = std::max(Product::lds_bytes(a.units, a.pairs), (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
     return product_launch(name, gated_kernel<E, T, BACK, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
                           pccnn_ceil_div(a.hidden, BN / 2), s);
 }
-template <typename T, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)
 {
-    constexpr int BM = 128;
+    if constexpr (!(BACK && std::is_same<T, float>::value))
+        if (product_large(a.n, 2 * a.hidden, a.units, a.pairs)) return gated_launch_tile<E, T, BACK, 256, 256, 2, 4>(name, a, s);
+    return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
+}
+template <typename T, int BM, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+{
     typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
-    const size_t lds = std::max(Product::LDS, (size_t)BM * BN * sizeof(T));
+    const size_t lds = std::max(Product::lds_bytes(a.units, a.pairs), (size_t)BM * BN * sizeof(T));
     return product_launch(name, gated_dx_kernel<T, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
                           pccnn_ceil_div(a.cols, BN), s);
+}
+template <typename T> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+{
+    if constexpr (!std::is_same<T, float>::value)
+        if (product_large(a.n, a.cols, a.units, a.pairs)) return dx_launch<T, 256, 256, 2, 4>(name, a, s);
+    return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 1>(name, a, s) : dx_launch<T, 128, 128, 2, 2>(name, a, s);
+}
+
+// A part's tiles go to one XCD as far as they may: they read the same rows, and its L2 serves them once.
+template <int DP, int XP, int XT, int MT> int weights_launch(const char *name, WeightsArgs &a, hipStream_t s)
+{
+    typedef WeightsShape<DP, XP, XT, MT> Shape;
+    a.blocks = (int64_t)a.tiles_x * a.tiles_d * a.splits;
+    PCCNN_REQUIRE(a.blocks <= INT32_MAX / 2, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)a.blocks);
+    a.run = (int)pccnn_ceil_div(a.blocks, PCCNN_XCDS);
+    const auto kernel = gated_weights_kernel<DP, XP, XT, MT>;
+    if (Shape::LDS > 65536)
+        PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::LDS));
+    kernel<<<pccnn_xcd_grid(a.blocks, a.run), Shape::THREADS, Shape::LDS, s>>>(a);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
 }
 
 template <typename T, typename OUT> int few_launch(GatedFew &a, hipStream_t s)
@@ -654,10 +716,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         a.x = d;
         a.w = {turned, 4 * plan.padded, p->channels, p->channels * 4 * plan.padded};
         a.n = p->n, a.cols = p->channels, a.units = (int)(2 * plan.padded / 8), a.pairs = pairs, a.out = d_feats;
-        if (p->channels <= 64)
-            rc = f32 ? dx_launch<float, 64, 4, 1>(name, a, s) : dx_launch<uint16_t, 64, 4, 1>(name, a, s);
-        else
-            rc = f32 ? dx_launch<float, 128, 2, 2>(name, a, s) : dx_launch<uint16_t, 128, 2, 2>(name, a, s);
+        rc = f32 ? dx_launch<float>(name, a, s) : dx_launch<uint16_t>(name, a, s);
         if (rc != PCCNN_OK) return rc;
     }
     if (d_gate != nullptr) {
@@ -667,10 +726,10 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
             a.x = r[0], a.d = d, a.n = p->n, a.cols_x = plan.units * 8, a.cols_d = 2 * plan.padded, a.pairs = pairs;
             a.tiles_x = plan.tiles_x, a.tiles_d = plan.tiles_d, a.splits = splits = plan.splits, a.per_split = plan.per_split;
             a.part = part, a.channels = p->channels;
-            const int64_t blocks = (int64_t)a.tiles_x * a.tiles_d * a.splits;
-            PCCNN_REQUIRE(blocks <= INT32_MAX, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
-            gated_weights_kernel<<<(unsigned)blocks, kThreads, 4 * ColumnsFeeder::Tile::ELEMENTS * sizeof(uint16_t), s>>>(a);
-            PCCNN_LAUNCH_CHECK();
+            rc = p->channels <= 64    ? weights_launch<2, 1, 64, 2>(name, a, s)
+                 : p->channels <= 128 ? weights_launch<2, 1, 128, 2>(name, a, s)
+                                      : weights_launch<2, 2, 128, 4>(name, a, s);
+            if (rc != PCCNN_OK) return rc;
         }
         const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads), 2);
         if (f32)

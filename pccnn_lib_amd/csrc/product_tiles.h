@@ -52,7 +52,8 @@ struct ProductI8 {
     }
 };
 
-// Brings tile after tile of ROWS operand rows, 128 bytes of each, into LDS: the inner dimension lies along the rows.
+// Brings tile after tile of ROWS operand rows, 128 bytes of each (a whole line of L2), into LDS: the inner dimension lies along
+// the rows.
 template <int ROWS, int THREADS> struct RowsFeeder {
     typedef AttnTile<1, ROWS, 64> Tile;
     static constexpr int COUNT = ROWS * 8 / THREADS;
@@ -81,6 +82,15 @@ template <int ROWS, int THREADS> struct RowsFeeder {
     }
 };
 
+// What this wavefront asked for has landed and its reads of LDS are done; behind the barrier, those of the workgroup.
+__device__ __forceinline__ void product_landed()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);                               // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // The product of BM rows of the lane's side with BN rows of the registers' side, both with the inner dimension along the rows.
 // WM x WN wavefronts, each with MT x NT blocks of 32 x 32.  PAIR: the registers' side is BN / 2 rows of one operand and as many
 // of another (gate and up), and the first half of a wavefront's NT blocks is of the first, the second half of the second, of the
@@ -88,7 +98,10 @@ template <int ROWS, int THREADS> struct RowsFeeder {
 template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     static constexpr int THREADS = WM * WN * PCCNN_WAVE, MT = BM / WM / 32, NT = BN / WN / 32;
     static constexpr int STAGE = (BM + BN) * 64;                      // uint16_t
-    static constexpr size_t LDS = 2 * STAGE * sizeof(uint16_t);
+    static constexpr size_t lds_bytes(int units, int pairs)           // (one tile will do where there is one step)
+    {
+        return (units <= 8 && pairs == 1 ? 1 : 2) * STAGE * sizeof(uint16_t);
+    }
     static constexpr int PART = PAIR ? BN / 2 : BN;                   // rows of one operand of the registers' side
     typedef RowsFeeder<BM, THREADS> FeedM;
     typedef RowsFeeder<PART, THREADS> FeedN;
@@ -119,19 +132,26 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     {
         typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
         uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + BM * 64;
+        // operands are read a step of products ahead of their use: the compiler, left alone, reads them just before
+        pccnn_u32x4 a[2][NT], b[2][MT];
+        auto read = [&](int kk) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            pccnn_u32x4 a[NT], b[MT];
+            for (int n = 0; n < NT; ++n)
+                a[kk & 1][n] = __builtin_bit_cast(pccnn_u32x4, Tile{tn}.rows(col_of(n) + (lane & 31), 2 * kk + half).t[0]);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                b[m] = __builtin_bit_cast(pccnn_u32x4, Tile{tm}.rows(row_of(m), 2 * kk + half).t[0]);
+                b[kk & 1][m] = __builtin_bit_cast(pccnn_u32x4, Tile{tm}.rows(row_of(m), 2 * kk + half).t[0]);
+        };
+        read(0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (kk < 3) read(kk + 1);
+            __builtin_amdgcn_sched_barrier(0x6);                      // VALU and SALU may cross
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                a[n] = __builtin_bit_cast(pccnn_u32x4, Tile{tn}.rows(col_of(n) + (lane & 31), 2 * kk + half).t[0]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[n], b[m]);
+                for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[kk & 1][n], b[kk & 1][m]);
+            __builtin_amdgcn_sched_barrier(0x6);
         }
     }
     // Rows from `row` of `x`, rows from `col` of `one` (and `two`); `units`: 16-byte units of every row; `pairs`: 1, or
@@ -145,25 +165,27 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         f1.start(one, col);
         if constexpr (PAIR) f2.start(two, col);
         const int steps = (units + 7) / 8, total = steps * pairs;
-        int k = 0, pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0;        // of the tile that is brought next
+        int k = 0, pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0;        // of the tile that is asked for next
         auto fetch = [&](uint16_t *to) {
             const int left = units - 8 * k;
-            const int64_t at_x = product_term_b(pair) * x.plane + 128 * (int64_t)k, at = 128 * (int64_t)k;
-            fm.fetch(at_x, left, to);
+            const int64_t at = 128 * (int64_t)k;
+            fm.fetch(product_term_b(pair) * x.plane + at, left, to);
             f1.fetch(product_term_a(pair) * one.plane + at, left, to + BM * 64);
             if constexpr (PAIR) f2.fetch(product_term_a(pair) * two.plane + at, left, to + (BM + PART) * 64);
             if (++k == steps) k = 0, ++pair;
         };
-        if (total > 0) fetch(lds);
-        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+        // `here` holds what is worked on, `there` is where the next tile goes.  That the two do not overlap is what lets the reads go
+        // on while the tile is on its way; the first round only asks, by the same code.
+        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool work, bool more) {
             if (more) fetch(there);
-            multiply(here);
+            if (work) multiply(here);
         };
-        for (int step = 0; step < total; ++step) {
-            attn_landed();
-            walk(lds + (step & 1) * STAGE, lds + ((step & 1) ^ 1) * STAGE, step + 1 < total);
+        for (int step = -1; step < total; ++step) {
+            product_landed();
+            const int stage = step & 1;
+            walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step >= 0, step + 1 < total);
         }
-        __syncthreads();                                              // LDS is free for the results
+        product_landed();                                             // LDS is free for the results
     }
 };
 
@@ -375,6 +397,11 @@ template <typename T> static __global__ __launch_bounds__(256) void product_stag
 // ---------------------------------------------------------------------------------------------- launches
 //
 // Tiles of output channels follow each other within a tile of rows; those of a run go to one XCD, whose L2 then serves the rows.
+// Whether a product takes tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128.
+static inline bool product_large(int64_t rows, int64_t cols, int units, int pairs)
+{
+    return cols >= 256 && units * pairs >= 32 && pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256) >= 256;
+}
 static inline int product_run(int tiles) { return tiles <= 64 ? tiles : 32; }
 
 template <typename KERNEL, typename ARGS>
