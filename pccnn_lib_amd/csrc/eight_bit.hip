@@ -28,7 +28,8 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
     extern __shared__ __align__(16) uint16_t lds[];
     const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
     if (block >= a.blocks) return;
-    const int64_t row0 = block / a.tiles * BM, col0 = block % a.tiles * BN;
+    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
+    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * BN, row0 = (int64_t)tile * BM;
     Product p;
     p.run(a.x, row0, a.w, a.w, col0, a.units, 1, lds);
     const Stage stage = {(T *)lds};

@@ -86,7 +86,8 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
     extern __shared__ __align__(16) uint16_t lds[];
     const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
     if (block >= a.blocks) return;
-    const int64_t row0 = block / a.tiles * BM, col0 = block % a.tiles * COLS;
+    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
+    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * COLS, row0 = (int64_t)tile * BM;
     Product p;
     p.run(a.x, row0, a.gate, a.up, col0, a.units, a.pairs, lds);
     const Stage stage = {(T *)lds}, second = {(T *)lds + BM * COLS};
@@ -246,7 +247,8 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a
     extern __shared__ __align__(16) uint16_t lds[];
     const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
     if (block >= a.blocks) return;
-    const int64_t row0 = block / a.tiles * BM, col0 = block % a.tiles * BN;
+    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
+    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * BN, row0 = (int64_t)tile * BM;
     Product p;
     p.run(a.x, row0, a.w, a.w, col0, a.units, a.pairs, lds);
     const Stage stage = {(T *)lds};
@@ -284,31 +286,34 @@ template <int COLS, int THREADS> struct ColumnsFeeder {
     typedef AttnTile<1, kTurnRows, COLS> Tile;
     static constexpr int COUNT = kTurnRows * Tile::UNITS / THREADS;
     static_assert(COUNT >= 1 && THREADS / Tile::UNITS % 16 == 0, "whole units, the same one in every round");
-    const char *base;
-    int64_t stride;
-    int unit, row;
-    bool live;
-    __device__ __forceinline__ void start(const ProductRows &s, int64_t col0, int64_t cols)
+    const char *base, *at;                   // the first row's columns, and the rows that are asked for next (the same in all lanes)
+    int64_t step, plane;
+    uint32_t off[COUNT];                     // the lane's units, in bytes
+    int row;
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t first, int64_t col0, int64_t cols, int term)
     {
         row = (int)threadIdx.x / Tile::UNITS;
-        unit = Tile::unit_at(row, (int)threadIdx.x % Tile::UNITS);
-        base = (const char *)s.p + 2 * col0;
-        stride = s.stride;
-        live = col0 + 8 * unit < cols;
+        const int unit = Tile::unit_at(row, (int)threadIdx.x % Tile::UNITS);
+        base = (const char *)s.p + first * s.stride + 2 * col0;
+        plane = s.plane;
+        step = kTurnRows * s.stride;
+        at = base + term * plane;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j)
+            off[j] = col0 + 8 * unit < cols ? (uint32_t)((row + j * (THREADS / Tile::UNITS)) * s.stride + 16 * unit) : kAttnNowhere;
     }
-    __device__ __forceinline__ void fetch(int64_t at_row, int64_t plane, int64_t rows, uint16_t *tile) const
+    // The next rows, in four parts; `rows`: how many of them exist.
+    __device__ __forceinline__ void fetch(int part, int rows, uint16_t *tile) const
     {
-        const __amdgpu_buffer_rsrc_t window = attn_window(base + at_row * stride + plane);
+        const __amdgpu_buffer_rsrc_t window = product_window(at);
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const int r = row + j * (THREADS / Tile::UNITS);
-            attn_bring(window, live && at_row + r < rows ? (uint32_t)(r * stride + 16 * unit) : kAttnNowhere,
+        for (int j = part * COUNT / 4; j < (part + 1) * COUNT / 4; ++j)
+            attn_bring(window, row + j * (THREADS / Tile::UNITS) < rows ? off[j] : kAttnNowhere,
                        tile + 8 * (j * THREADS + wave_unit));
-        }
     }
+    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + step; }
 };
-// DP x 128 columns of (dG | dU) times XP x XT columns of x; a wavefront has 32 MT x 64 of them.
 constexpr int weights_threads(int dp, int xp, int xt, int mt) { return dp * 128 / (32 * mt) * (xp * xt / 64) * PCCNN_WAVE; }
 template <int DP, int XP, int XT, int MT> struct WeightsShape {
     static constexpr int COLS_D = DP * 128, COLS_X = XP * XT, WAVES_X = COLS_X / 64, WAVES_D = COLS_D / (32 * MT);
@@ -329,19 +334,20 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
     extern __shared__ __align__(16) uint16_t lds[];
     const int lane = threadIdx.x % PCCNN_WAVE, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE), wx = wave % WAVES_X, wd = wave / WAVES_X;
-    int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
+    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
     if (block >= a.blocks) return;
-    const int64_t x0 = block % a.tiles_x * Shape::COLS_X;
-    block /= a.tiles_x;
-    const int64_t d0 = block % a.tiles_d * Shape::COLS_D;
-    const int64_t split = block / a.tiles_d;
-    const int64_t first = split * a.per_split, last = min(a.n, first + a.per_split);
+    uint32_t split = __builtin_amdgcn_readfirstlane((uint32_t)block);
+    const int64_t x0 = (int64_t)product_split(split, a.tiles_x) * Shape::COLS_X;
+    const int64_t d0 = (int64_t)product_split(split, a.tiles_d) * Shape::COLS_D;
+    const int64_t first = split * a.per_split;
+    const int rows = (int)min(a.n - first, a.per_split);
+    int pair = a.pairs == 1 ? PRODUCT_PAIRS - 1 : 0, left = rows;     // of the tile that is asked for next
     FeedX fx[XP];
     FeedD fd[DP];
 #pragma unroll
-    for (int i = 0; i < XP; ++i) fx[i].start(a.x, x0 + i * XT, a.cols_x);
+    for (int i = 0; i < XP; ++i) fx[i].start(a.x, first, x0 + i * XT, a.cols_x, product_term_a(pair));
 #pragma unroll
-    for (int i = 0; i < DP; ++i) fd[i].start(a.d, d0 + i * 128, a.cols_d);
+    for (int i = 0; i < DP; ++i) fd[i].start(a.d, first, d0 + i * 128, a.cols_d, product_term_b(pair));
     pccnn_f32x16 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -349,21 +355,24 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
         for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    const int64_t steps = (last - first + kTurnRows - 1) / kTurnRows, total = steps * a.pairs;
-    int64_t k = 0;
-    int pair = a.pairs == 1 ? PRODUCT_PAIRS - 1 : 0;
-    auto fetch = [&](uint16_t *to) {
-        const int64_t at = first + k * kTurnRows;
+    const int total = (rows + kTurnRows - 1) / kTurnRows * a.pairs;
+    auto fetch = [&](int part, uint16_t *to) {
 #pragma unroll
-        for (int i = 0; i < DP; ++i) fd[i].fetch(at, product_term_b(pair) * a.d.plane, last, to + i * TileD::ELEMENTS);
+        for (int i = 0; i < DP; ++i) fd[i].fetch(part, left, to + i * TileD::ELEMENTS);
 #pragma unroll
-        for (int i = 0; i < XP; ++i)
-            fx[i].fetch(at, product_term_a(pair) * a.x.plane, last, to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
-        if (++k == steps) k = 0, ++pair;
+        for (int i = 0; i < XP; ++i) fx[i].fetch(part, left, to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
+        if (part < 3) return;
+        left -= kTurnRows;
+        const bool wrap = left <= 0;
+        if (wrap) left = rows, ++pair;
+#pragma unroll
+        for (int i = 0; i < DP; ++i) fd[i].next(wrap, product_term_b(pair));
+#pragma unroll
+        for (int i = 0; i < XP; ++i) fx[i].next(wrap, product_term_a(pair));
     };
-    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool work, bool more) {
-        if (more) fetch(there);
-        if (!work) return;                   // (the first round only asks)
+#pragma unroll
+    for (int part = 0; part < 4; ++part) fetch(part, lds);
+    auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
         AttnFrag<1> fa[2][2], fb[2][MT];
         auto read = [&](int kk) {            // a step of products ahead of their use
 #pragma unroll
@@ -378,22 +387,29 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
             }
         };
         constexpr int COUNT = kTurnRows / 16;
+        static_assert(COUNT == 4, "four parts of the next tile are asked for in between");
         read(0);
 #pragma unroll
         for (int kk = 0; kk < COUNT; ++kk) {
             if (kk + 1 < COUNT) read(kk + 1);
             __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < MT; ++j) attn_mma(acc[i][j], fa[kk & 1][i], fb[kk & 1][j]);
+                if (i == 0) {
+                    __builtin_amdgcn_sched_barrier(0x6);
+                    if (more) fetch(kk, there);
+                    __builtin_amdgcn_sched_barrier(0x6);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0x6);
         }
     };
-    for (int64_t step = -1; step < total; ++step) {
+    for (int step = 0; step < total; ++step) {
         product_landed();
-        const int stage = (int)step & 1;
-        walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step >= 0, step + 1 < total);
+        const int stage = step & 1;
+        walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
     }
     float *part = a.part + split * a.cols_d * a.channels;
 #pragma unroll

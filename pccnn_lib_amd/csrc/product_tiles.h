@@ -52,18 +52,37 @@ struct ProductI8 {
     }
 };
 
+// A window whose base the compiler takes as the same in all lanes, which it cannot always see.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t product_window(const void *base)
+{
+    const uint64_t bits = (uint64_t)base;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)bits), hi = __builtin_amdgcn_readfirstlane((uint32_t)(bits >> 32));
+    return attn_window((const void *)((uint64_t)hi << 32 | lo));
+}
+
+// quotient and rest of a workgroup's number, in scalar registers (the division itself runs in vector ones).
+__device__ __forceinline__ uint32_t product_split(uint32_t &block, uint32_t by)
+{
+    const uint32_t quotient = __builtin_amdgcn_readfirstlane(block / by), rest = block - quotient * by;
+    block = quotient;
+    return rest;
+}
+
 // Brings tile after tile of ROWS operand rows, 128 bytes of each (a whole line of L2), into LDS: the inner dimension lies along
 // the rows.
 template <int ROWS, int THREADS> struct RowsFeeder {
     typedef AttnTile<1, ROWS, 64> Tile;
     static constexpr int COUNT = ROWS * 8 / THREADS;
     static_assert(COUNT >= 1 && COUNT * THREADS == ROWS * 8 && THREADS / 8 % 16 == 0, "whole units, the same one in every round");
-    const char *base;                        // the tile's first row (the same in all lanes)
+    const char *base, *at;                   // the tile's first row, and of it what is asked for next (the same in all lanes)
+    int64_t plane;
     uint32_t off[COUNT];                     // the lane's units from there, in bytes
     int unit;                                // which of a row's eight units the lane brings
-    __device__ __forceinline__ void start(const ProductRows &s, int64_t row)
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t row, int term)
     {
         base = (const char *)s.p + row * s.stride;
+        plane = s.plane;
+        at = base + term * plane;
         unit = Tile::unit_at((int)threadIdx.x / 8, (int)threadIdx.x % 8);
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
@@ -71,15 +90,16 @@ template <int ROWS, int THREADS> struct RowsFeeder {
             off[j] = row + r < s.rows ? (uint32_t)(r * s.stride + 16 * unit) : kAttnNowhere;
         }
     }
-    // The 128 bytes from `at` (the same in all lanes) of every row; `units`: how many of these eight units exist.
-    __device__ __forceinline__ void fetch(int64_t at, int units, uint16_t *tile) const
+    // The next 128 bytes of every row, in four parts; `units`: how many of these eight units exist.
+    __device__ __forceinline__ void fetch(int part, int units, uint16_t *tile) const
     {
-        const __amdgpu_buffer_rsrc_t window = attn_window(base + at);
+        const __amdgpu_buffer_rsrc_t window = product_window(at);
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
+        for (int j = part * COUNT / 4; j < (part + 1) * COUNT / 4; ++j)
             attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + 8 * (j * THREADS + wave_unit));
     }
+    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + 128; }
 };
 
 // What this wavefront asked for has landed and its reads of LDS are done; behind the barrier, those of the workgroup.
@@ -128,7 +148,9 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         if constexpr (PAIR) return n / (NT / 2) * PART + wn * (16 * NT) + 32 * (n % (NT / 2));
         return wn * (32 * NT) + 32 * n;
     }
-    __device__ __forceinline__ void multiply(const uint16_t *tile)
+    // One tile's products, and in between, in four parts, what `ask` asks memory for: a compute unit takes a request of a
+    // wavefront every sixteen cycles, so eight wavefronts that asked for a whole tile at once would wait for each other.
+    template <typename ASK> __device__ __forceinline__ void multiply(const uint16_t *tile, ASK ask)
     {
         typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
         uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + BM * 64;
@@ -148,9 +170,15 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             if (kk < 3) read(kk + 1);
             __builtin_amdgcn_sched_barrier(0x6);                      // VALU and SALU may cross
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[kk & 1][n], b[kk & 1][m]);
+                if (n == 0) {
+                    __builtin_amdgcn_sched_barrier(0x6);
+                    ask(kk);
+                    __builtin_amdgcn_sched_barrier(0x6);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0x6);
         }
     }
@@ -161,29 +189,36 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     {
         FeedM fm;
         FeedN f1, f2;
-        fm.start(x, row);
-        f1.start(one, col);
-        if constexpr (PAIR) f2.start(two, col);
-        const int steps = (units + 7) / 8, total = steps * pairs;
-        int k = 0, pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0;        // of the tile that is asked for next
-        auto fetch = [&](uint16_t *to) {
-            const int left = units - 8 * k;
-            const int64_t at = 128 * (int64_t)k;
-            fm.fetch(product_term_b(pair) * x.plane + at, left, to);
-            f1.fetch(product_term_a(pair) * one.plane + at, left, to + BM * 64);
-            if constexpr (PAIR) f2.fetch(product_term_a(pair) * two.plane + at, left, to + (BM + PART) * 64);
-            if (++k == steps) k = 0, ++pair;
+        int pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0, left = units;  // of the tile that is asked for next
+        fm.start(x, row, product_term_b(pair));
+        f1.start(one, col, product_term_a(pair));
+        if constexpr (PAIR) f2.start(two, col, product_term_a(pair));
+        const int total = (units + 7) / 8 * pairs;
+        auto fetch = [&](int part, uint16_t *to) {
+            fm.fetch(part, left, to);
+            f1.fetch(part, left, to + BM * 64);
+            if constexpr (PAIR) f2.fetch(part, left, to + (BM + PART) * 64);
+            if (part < 3) return;
+            left -= 8;
+            const bool wrap = left <= 0;
+            if (wrap) left = units, ++pair;
+            fm.next(wrap, product_term_b(pair));
+            f1.next(wrap, product_term_a(pair));
+            if constexpr (PAIR) f2.next(wrap, product_term_a(pair));
         };
+#pragma unroll
+        for (int part = 0; part < 4; ++part) fetch(part, lds);
         // `here` holds what is worked on, `there` is where the next tile goes.  That the two do not overlap is what lets the reads go
-        // on while the tile is on its way; the first round only asks, by the same code.
-        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool work, bool more) {
-            if (more) fetch(there);
-            if (work) multiply(here);
+        // on while the tile is on its way.
+        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+            multiply(here, [&](int part) {
+                if (more) fetch(part, there);
+            });
         };
-        for (int step = -1; step < total; ++step) {
+        for (int step = 0; step < total; ++step) {
             product_landed();
             const int stage = step & 1;
-            walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step >= 0, step + 1 < total);
+            walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
         }
         product_landed();                                             // LDS is free for the results
     }
@@ -214,7 +249,7 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
         if (wide == 2) {
             const int unit = place(r0, (int)threadIdx.x % UNITS);
             const int64_t col = col0 + unit * PER;
-            const __amdgpu_buffer_rsrc_t window = attn_window(from + row0 * stride + col0);
+            const __amdgpu_buffer_rsrc_t window = product_window(from + row0 * stride + col0);
             const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
             for (int j = 0; j < COUNT; ++j) {
