@@ -52,7 +52,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
             }
     }
     __syncthreads();
-    stage.out((T *)a.out, a.outer, row0, a.n, col0, a.outer);
+    stage.out(DenseRow<T>{(T *)a.out, a.outer}, row0, a.n, col0, a.outer);
 }
 
 struct LinearFew {

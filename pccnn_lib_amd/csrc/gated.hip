@@ -71,8 +71,8 @@ struct GatedArgs {
     const void *grads;                       // backward: dh
     int64_t grads_stride;
     int grads_wide;
-    uint16_t *d_pre;                         // backward: (dG | dU) rows of 2 padded bf16 values, planes of terms in f32
-    int64_t padded, d_plane;
+    uint16_t *d_pre;                         // backward: rows (dG | dU) of 2 padded bf16 values, in pieces of 64 columns that lie one
+    int64_t padded, d_plane;                 // behind the other; planes of terms in f32
 };
 
 // E: operands; T: result (forward), type of the tensors (backward).
@@ -135,10 +135,10 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
     }
     __syncthreads();
     if constexpr (!BACK) {
-        stage.out((T *)a.out, a.hidden, row0, a.n, col0, a.hidden);
+        stage.out(DenseRow<T>{(T *)a.out, a.hidden}, row0, a.n, col0, a.hidden);
     } else if constexpr (!EXACT) {
-        stage.out(a.d_pre, 2 * a.padded, row0, a.n, col0, a.padded);
-        second.out(a.d_pre + a.padded, 2 * a.padded, row0, a.n, col0, a.padded);
+        stage.out(PieceRow<T>{a.d_pre, a.n, 0}, row0, a.n, col0, a.padded);
+        second.out(PieceRow<T>{a.d_pre, a.n, a.padded}, row0, a.n, col0, a.padded);
     } else {
         for (int i = threadIdx.x; i < 2 * BM * COLS / 8; i += Product::THREADS) {
             const int which = i / (BM * COLS / 8), r = i % (BM * COLS / 8) / (COLS / 8), col = i % (COLS / 8) * 8;
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 + e] = y[e];
             const AttnFrag<3> f = attn_split<3, true>(x);
-            uint16_t *to = a.d_pre + (row0 + r) * 2 * a.padded + which * a.padded + col0 + col;
+            uint16_t *to = PieceRow<uint16_t>{a.d_pre, a.n, which * a.padded}.at(row0 + r, col0 + col);
 #pragma unroll
             for (int t = 0; t < 3; ++t) *(pccnn_u32x4 *)(to + t * a.d_plane) = __builtin_bit_cast(pccnn_u32x4, f.t[t]);
         }
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a
                 stage.put(p.row_of(m), p.col_of(n) + 8 * q + 4 * p.half, v);
             }
     __syncthreads();
-    stage.out((T *)a.out, a.cols, row0, a.n, col0, a.cols);
+    stage.out(DenseRow<T>{(T *)a.out, a.cols}, row0, a.n, col0, a.cols);
 }
 
 // dWg and dWu: columns of (dG | dU) times columns of x, the inner dimension over the rows, which are cut into parts whose sums
@@ -290,11 +290,12 @@ template <int COLS, int THREADS> struct ColumnsFeeder {
     int64_t step, plane;
     uint32_t off[COUNT];                     // the lane's units, in bytes
     int row;
+    // (columns of 64 a piece where the rows do not lie in one)
     __device__ __forceinline__ void start(const ProductRows &s, int64_t first, int64_t col0, int64_t cols, int term)
     {
         row = (int)threadIdx.x / Tile::UNITS;
         const int unit = Tile::unit_at(row, (int)threadIdx.x % Tile::UNITS);
-        base = (const char *)s.p + first * s.stride + 2 * col0;
+        base = (const char *)s.p + first * s.stride + col0 / 64 * s.step;
         plane = s.plane;
         step = kTurnRows * s.stride;
         at = base + term * plane;
@@ -302,21 +303,22 @@ template <int COLS, int THREADS> struct ColumnsFeeder {
         for (int j = 0; j < COUNT; ++j)
             off[j] = col0 + 8 * unit < cols ? (uint32_t)((row + j * (THREADS / Tile::UNITS)) * s.stride + 16 * unit) : kAttnNowhere;
     }
-    // The next rows, in four parts; `rows`: how many of them exist.
-    __device__ __forceinline__ void fetch(int part, int rows, uint16_t *tile) const
+    // The next rows; `rows`: how many of them exist.  Parts as RowsFeeder has them.
+    template <int ALL> __device__ __forceinline__ void fetch(int first, int part, int rows, uint16_t *tile) const
     {
         const __amdgpu_buffer_rsrc_t window = product_window(at);
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = part * COUNT / 4; j < (part + 1) * COUNT / 4; ++j)
-            attn_bring(window, row + j * (THREADS / Tile::UNITS) < rows ? off[j] : kAttnNowhere,
-                       tile + 8 * (j * THREADS + wave_unit));
+        for (int j = 0; j < COUNT; ++j)
+            if ((first + j) * 2 / ALL == part)
+                attn_bring(window, row + j * (THREADS / Tile::UNITS) < rows ? off[j] : kAttnNowhere,
+                           tile + 8 * (j * THREADS + wave_unit));
     }
     __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + step; }
 };
-constexpr int weights_threads(int dp, int xp, int xt, int mt) { return dp * 128 / (32 * mt) * (xp * xt / 64) * PCCNN_WAVE; }
+constexpr int weights_threads(int dp, int xp, int xt, int mt) { return dp * 64 / (32 * mt) * (xp * xt / 64) * PCCNN_WAVE; }
 template <int DP, int XP, int XT, int MT> struct WeightsShape {
-    static constexpr int COLS_D = DP * 128, COLS_X = XP * XT, WAVES_X = COLS_X / 64, WAVES_D = COLS_D / (32 * MT);
+    static constexpr int COLS_D = DP * 64, COLS_X = XP * XT, WAVES_X = COLS_X / 64, WAVES_D = COLS_D / (32 * MT);
     static constexpr int THREADS = WAVES_X * WAVES_D * PCCNN_WAVE;
     static_assert(THREADS == weights_threads(DP, XP, XT, MT), "");
     static constexpr int STAGE = kTurnRows * (COLS_D + COLS_X);       // uint16_t
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 {
     typedef WeightsShape<DP, XP, XT, MT> Shape;
     constexpr int WAVES_X = Shape::WAVES_X, STAGE = Shape::STAGE;
-    typedef ColumnsFeeder<128, Shape::THREADS> FeedD;
+    typedef ColumnsFeeder<64, Shape::THREADS> FeedD;
     typedef ColumnsFeeder<XT, Shape::THREADS> FeedX;
     typedef typename FeedD::Tile TileD;
     typedef typename FeedX::Tile TileX;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
     for (int i = 0; i < XP; ++i) fx[i].start(a.x, first, x0 + i * XT, a.cols_x, product_term_a(pair));
 #pragma unroll
-    for (int i = 0; i < DP; ++i) fd[i].start(a.d, first, d0 + i * 128, a.cols_d, product_term_b(pair));
+    for (int i = 0; i < DP; ++i) fd[i].start(a.d, first, d0 + i * 64, a.cols_d, product_term_b(pair));
     pccnn_f32x16 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -356,12 +358,15 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     const int total = (rows + kTurnRows - 1) / kTurnRows * a.pairs;
+    constexpr int ALL = DP * FeedD::COUNT + XP * FeedX::COUNT;
     auto fetch = [&](int part, uint16_t *to) {
 #pragma unroll
-        for (int i = 0; i < DP; ++i) fd[i].fetch(part, left, to + i * TileD::ELEMENTS);
+        for (int i = 0; i < DP; ++i) fd[i].template fetch<ALL>(i * FeedD::COUNT, part, left, to + i * TileD::ELEMENTS);
 #pragma unroll
-        for (int i = 0; i < XP; ++i) fx[i].fetch(part, left, to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
-        if (part < 3) return;
+        for (int i = 0; i < XP; ++i)
+            fx[i].template fetch<ALL>(DP * FeedD::COUNT + i * FeedX::COUNT, part, left,
+                                      to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
+        if (part == 0) return;
         left -= kTurnRows;
         const bool wrap = left <= 0;
         if (wrap) left = rows, ++pair;
@@ -370,8 +375,8 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
         for (int i = 0; i < XP; ++i) fx[i].next(wrap, product_term_a(pair));
     };
-#pragma unroll
-    for (int part = 0; part < 4; ++part) fetch(part, lds);
+    fetch(0, lds);
+    fetch(1, lds);
     auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
         AttnFrag<1> fa[2][2], fb[2][MT];
         auto read = [&](int kk) {            // a step of products ahead of their use
@@ -383,11 +388,11 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
                 const int col = 32 * (MT * wd + j);
-                fb[kk & 1][j] = TileD{here + col / 128 * TileD::ELEMENTS}.columns(16 * kk, col % 128, lane);
+                fb[kk & 1][j] = TileD{here + col / 64 * TileD::ELEMENTS}.columns(16 * kk, col % 64, lane);
             }
         };
         constexpr int COUNT = kTurnRows / 16;
-        static_assert(COUNT == 4, "four parts of the next tile are asked for in between");
+        static_assert(COUNT >= 2, "two parts of the next tile are asked for in between");
         read(0);
 #pragma unroll
         for (int kk = 0; kk < COUNT; ++kk) {
@@ -397,7 +402,7 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < MT; ++j) attn_mma(acc[i][j], fa[kk & 1][i], fb[kk & 1][j]);
-                if (i == 0) {
+                if (i == 0 && kk < 2) {
                     __builtin_amdgcn_sched_barrier(0x6);
                     if (more) fetch(kk, there);
                     __builtin_amdgcn_sched_barrier(0x6);
@@ -476,7 +481,7 @@ struct GatedPlan {
     int64_t rows[3];
     const void *p[3];
     int64_t stride[3];
-    int64_t padded;                          // hidden channels in whole units
+    int64_t padded, pieces;                  // hidden channels in whole units; 64 columns of (dG | dU) each
     int tiles_x, tiles_d, splits;            // weights' gradients
     int64_t per_split;
 };
@@ -514,6 +519,7 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
         plan.bytes[i] = plan.stage[i] ? (size_t)plan.planes * plan.rows[i] * plan.units * 16 : 0;
     }
     plan.padded = pccnn_ceil_div(p->hidden, 8) * 8;
+    plan.pieces = pccnn_ceil_div(2 * plan.padded, 64);
     // parts enough to fill the chip twice over, of at least four steps
     plan.tiles_x = (int)pccnn_ceil_div(p->channels, p->channels <= 64 ? 64 : p->channels <= 128 ? 128 : 256);
     plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, 256);
@@ -567,7 +573,7 @@ int gated_launch_tile(const char *name, GatedArgs &a, hipStream_t s)
 template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)
 {
     if constexpr (!(BACK && std::is_same<T, float>::value))
-        if (product_large(a.n, 2 * a.hidden, a.units, a.pairs)) return gated_launch_tile<E, T, BACK, 256, 256, 2, 4>(name, a, s);
+        if (product_large(a.n, 2 * a.hidden, a.units, a.pairs)) return gated_launch_tile<E, T, BACK, 256, 256, 4, 2>(name, a, s);
     return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
 }
 template <typename T, int BM, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
@@ -580,7 +586,7 @@ template <typename T, int BM, int BN, int WM, int WN> int dx_launch(const char *
 template <typename T> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
 {
     if constexpr (!std::is_same<T, float>::value)
-        if (product_large(a.n, a.cols, a.units, a.pairs)) return dx_launch<T, 256, 256, 2, 4>(name, a, s);
+        if (product_large(a.n, a.cols, a.units, a.pairs)) return dx_launch<T, 256, 256, 4, 2>(name, a, s);
     return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 1>(name, a, s) : dx_launch<T, 128, 128, 2, 2>(name, a, s);
 }
 
@@ -620,7 +626,7 @@ struct BackBytes {
 BackBytes back_bytes(const pccnn_gated *p, const GatedPlan &plan)
 {
     BackBytes b;
-    b.d_pre = (size_t)plan.planes * p->n * 2 * plan.padded * 2;
+    b.d_pre = (size_t)plan.planes * p->n * plan.pieces * 128;
     b.turned = (size_t)plan.planes * p->channels * 2 * plan.padded * 2;
     b.part = (size_t)plan.splits * 2 * plan.padded * p->channels * sizeof(float);
     return b;
@@ -699,7 +705,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
     ProductRows r[3];
     const bool f32 = p->type == PCCNN_TYPE_F32;
     const int pairs = f32 ? PRODUCT_PAIRS : 1;
-    const ProductRows d = {arena.take<char>(bytes.d_pre), 4 * plan.padded, p->n, p->n * 4 * plan.padded};
+    const ProductRows d = {arena.take<char>(bytes.d_pre), 128, p->n, p->n * plan.pieces * 128, p->n * 128};
     uint16_t *turned = arena.take<uint16_t>(bytes.turned / 2);
     float *part = arena.take<float>(bytes.part / sizeof(float));
     PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
@@ -742,9 +748,9 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
             a.x = r[0], a.d = d, a.n = p->n, a.cols_x = plan.units * 8, a.cols_d = 2 * plan.padded, a.pairs = pairs;
             a.tiles_x = plan.tiles_x, a.tiles_d = plan.tiles_d, a.splits = splits = plan.splits, a.per_split = plan.per_split;
             a.part = part, a.channels = p->channels;
-            rc = p->channels <= 64    ? weights_launch<2, 1, 64, 2>(name, a, s)
-                 : p->channels <= 128 ? weights_launch<2, 1, 128, 2>(name, a, s)
-                                      : weights_launch<2, 2, 128, 4>(name, a, s);
+            rc = p->channels <= 64    ? weights_launch<4, 1, 64, 2>(name, a, s)
+                 : p->channels <= 128 ? weights_launch<4, 1, 128, 2>(name, a, s)
+                                      : weights_launch<4, 2, 128, 4>(name, a, s);
             if (rc != PCCNN_OK) return rc;
         }
         const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads), 2);

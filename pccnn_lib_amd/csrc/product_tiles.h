@@ -18,10 +18,11 @@ typedef int pccnn_i32x16 __attribute__((ext_vector_type(16)));
 typedef float pccnn_f32x4 __attribute__((ext_vector_type(4)));
 #endif
 
-// One operand: rows of 16-byte units, and the distance of the planes of terms (f32; else one plane).
+// One operand: rows of 16-byte units.  In bytes: the distance of rows, of the next 128 bytes of a row (128 where the row lies in
+// one piece), of the planes of terms (f32; else there is one).
 struct ProductRows {
     const void *p;
-    int64_t stride, rows, plane;             // in bytes, rows, bytes
+    int64_t stride, rows, plane, step = 128;
 };
 
 enum { PRODUCT_PAIRS = 6 };                  // f32: products of planes
@@ -75,13 +76,14 @@ template <int ROWS, int THREADS> struct RowsFeeder {
     static constexpr int COUNT = ROWS * 8 / THREADS;
     static_assert(COUNT >= 1 && COUNT * THREADS == ROWS * 8 && THREADS / 8 % 16 == 0, "whole units, the same one in every round");
     const char *base, *at;                   // the tile's first row, and of it what is asked for next (the same in all lanes)
-    int64_t plane;
+    int64_t plane, step;
     uint32_t off[COUNT];                     // the lane's units from there, in bytes
     int unit;                                // which of a row's eight units the lane brings
     __device__ __forceinline__ void start(const ProductRows &s, int64_t row, int term)
     {
         base = (const char *)s.p + row * s.stride;
         plane = s.plane;
+        step = s.step;
         at = base + term * plane;
         unit = Tile::unit_at((int)threadIdx.x / 8, (int)threadIdx.x % 8);
 #pragma unroll
@@ -90,16 +92,18 @@ template <int ROWS, int THREADS> struct RowsFeeder {
             off[j] = row + r < s.rows ? (uint32_t)(r * s.stride + 16 * unit) : kAttnNowhere;
         }
     }
-    // The next 128 bytes of every row, in four parts; `units`: how many of these eight units exist.
-    __device__ __forceinline__ void fetch(int part, int units, uint16_t *tile) const
+    // The next 128 bytes of every row; `units`: how many of these eight units exist.  A tile comes in ALL requests of a wavefront,
+    // of which this operand's are those from FIRST on; `part`: which half of them.
+    template <int FIRST, int ALL> __device__ __forceinline__ void fetch(int part, int units, uint16_t *tile) const
     {
         const __amdgpu_buffer_rsrc_t window = product_window(at);
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = part * COUNT / 4; j < (part + 1) * COUNT / 4; ++j)
-            attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + 8 * (j * THREADS + wave_unit));
+        for (int j = 0; j < COUNT; ++j)
+            if ((FIRST + j) * 2 / ALL == part)
+                attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + 8 * (j * THREADS + wave_unit));
     }
-    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + 128; }
+    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + step; }
 };
 
 // What this wavefront asked for has landed and its reads of LDS are done; behind the barrier, those of the workgroup.
@@ -148,8 +152,10 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         if constexpr (PAIR) return n / (NT / 2) * PART + wn * (16 * NT) + 32 * (n % (NT / 2));
         return wn * (32 * NT) + 32 * n;
     }
-    // One tile's products, and in between, in four parts, what `ask` asks memory for: a compute unit takes a request of a
-    // wavefront every sixteen cycles, so eight wavefronts that asked for a whole tile at once would wait for each other.
+    // One tile's products, and among their first half, in two parts, what `ask` asks memory for.  A compute unit takes a request
+    // of a wavefront every sixteen cycles, so eight wavefronts that ask for a whole tile at once wait for each other; what is
+    // asked for in the second half is late for the next tile.  65536 x 2816 x 512: at once 196 us, four parts over the whole 205,
+    // two parts over the first half 197; 65536 x 512 x 512 40.1, 40.6 and 39.3, 65536 x 1408 x 512 83.7, 85.0 and 81.2.
     template <typename ASK> __device__ __forceinline__ void multiply(const uint16_t *tile, ASK ask)
     {
         typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
@@ -173,7 +179,7 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[kk & 1][n], b[kk & 1][m]);
-                if (n == 0) {
+                if (n == 0 && kk < 2) {
                     __builtin_amdgcn_sched_barrier(0x6);
                     ask(kk);
                     __builtin_amdgcn_sched_barrier(0x6);
@@ -194,11 +200,12 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         f1.start(one, col, product_term_a(pair));
         if constexpr (PAIR) f2.start(two, col, product_term_a(pair));
         const int total = (units + 7) / 8 * pairs;
+        constexpr int ALL = FeedM::COUNT + (PAIR ? 2 : 1) * FeedN::COUNT;
         auto fetch = [&](int part, uint16_t *to) {
-            fm.fetch(part, left, to);
-            f1.fetch(part, left, to + BM * 64);
-            if constexpr (PAIR) f2.fetch(part, left, to + (BM + PART) * 64);
-            if (part < 3) return;
+            fm.template fetch<0, ALL>(part, left, to);
+            f1.template fetch<FeedM::COUNT, ALL>(part, left, to + BM * 64);
+            if constexpr (PAIR) f2.template fetch<FeedM::COUNT + FeedN::COUNT, ALL>(part, left, to + (BM + PART) * 64);
+            if (part == 0) return;
             left -= 8;
             const bool wrap = left <= 0;
             if (wrap) left = units, ++pair;
@@ -206,8 +213,8 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             f1.next(wrap, product_term_a(pair));
             if constexpr (PAIR) f2.next(wrap, product_term_a(pair));
         };
-#pragma unroll
-        for (int part = 0; part < 4; ++part) fetch(part, lds);
+        fetch(0, lds);
+        fetch(1, lds);
         // `here` holds what is worked on, `there` is where the next tile goes.  That the two do not overlap is what lets the reads go
         // on while the tile is on its way.
         auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
@@ -269,16 +276,16 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
             }
         }
     }
-    // Writes the tile to rows of `stride` elements, columns below `width`, as whole units where every row allows it.
-    __device__ __forceinline__ void out(T *to, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
+    // Writes the tile to `to`'s rows, columns below `width`, as whole units where every row allows it.
+    template <typename ROW> __device__ __forceinline__ void out(const ROW &to, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
     {
-        const bool whole = stride % PER == 0 && width % PER == 0;
+        const bool whole = to.whole() && width % PER == 0;
         for (int i = threadIdx.x; i < BM * UNITS; i += THREADS) {
             const int r = i / UNITS, unit = i % UNITS;
             const int64_t col = col0 + unit * PER;
             if (row0 + r >= rows || col >= width) continue;
             const T *from = base + r * COLS + PER * place(r, unit);
-            T *at = to + (row0 + r) * stride + col;
+            T *at = to.at(row0 + r, col);
             if (whole) {
                 *(pccnn_u32x4 *)at = *(const pccnn_u32x4 *)from;
             } else {
@@ -287,6 +294,23 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
                     if (col + e < width) at[e] = from[e];
             }
         }
+    }
+};
+// Where a unit of a result lies: rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what
+// a tile of rows takes of one piece lies together (65536 x 2816 x 512 with its rows in one piece: XXX us).
+template <typename T> struct DenseRow {
+    T *p;
+    int64_t stride;
+    __device__ __forceinline__ bool whole() const { return stride * (int)sizeof(T) % 16 == 0; }
+    __device__ __forceinline__ T *at(int64_t row, int64_t col) const { return p + row * stride + col; }
+};
+template <typename T> struct PieceRow {
+    T *p;
+    int64_t rows, from;                      // `from`: the column of all pieces that column 0 is
+    __device__ __forceinline__ bool whole() const { return true; }
+    __device__ __forceinline__ T *at(int64_t row, int64_t col) const
+    {
+        return p + ((from + col) / 64 * rows + row) * 64 + (from + col) % 64;
     }
 };
 
