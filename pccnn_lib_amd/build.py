@@ -20,11 +20,11 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument", "-Wno-ignored-optimization-argument",
 ]
 
-# Flags of single sources.  attention.hip, gated.hip, eight_bit.hip: matrix results in ordinary registers, where the softmax
+# Flags of single sources.  attention.hip, gated.hip: matrix results in ordinary registers, where the softmax
 # and the activations work on them; the compiler's own choice puts them into accumulation registers and moves every value out
 # and in again.
 _MFMA_IN_VGPRS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-EXTRA_FLAGS = {"attention.hip": _MFMA_IN_VGPRS, "gated.hip": _MFMA_IN_VGPRS, "eight_bit.hip": _MFMA_IN_VGPRS}
+EXTRA_FLAGS = {"attention.hip": _MFMA_IN_VGPRS, "gated.hip": _MFMA_IN_VGPRS}
 
 
 def sources():

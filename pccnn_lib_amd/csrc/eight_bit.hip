@@ -18,6 +18,7 @@ struct LinearArgs {
     const float *scales, *weight_scales, *bias;
     int64_t blocks;
     int tiles, run;
+    size_t lds;
     void *out;
 };
 template <typename T, int BM, int BN, int WM, int WN>
@@ -31,22 +32,28 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
     uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
     const int64_t col0 = (int64_t)product_split(tile, a.tiles) * BN, row0 = (int64_t)tile * BM;
     Product p;
+    float x_scale[Product::MT];
+    const ProductChannels<2, BN, Product::THREADS> channels = {(float *)((char *)lds + a.lds)};
+    channels.start(0, a.weight_scales, col0, a.outer);
+    channels.start(1, a.bias, col0, a.outer);
+#pragma unroll
+    for (int m = 0; m < Product::MT; ++m) x_scale[m] = a.scales[min(row0 + p.row_of(m), a.n - 1)];
     p.run(a.x, row0, a.w, a.w, col0, a.units, 1, lds);
     const Stage stage = {(T *)lds};
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m) {
-        const float scale = a.scales[min(row0 + p.row_of(m), a.n - 1)];
 #pragma unroll
         for (int n = 0; n < Product::NT; ++n)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int col = p.col_of(n) + 8 * q + 4 * p.half;
-                float v[4];
+                float v[4], weight_scales[4], bias[4];
+                channels.get(0, col, weight_scales);
+                channels.get(1, col, bias);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int64_t o = min(col0 + col + i, a.outer - 1);
-                    v[i] = (float)p.acc[m][n][4 * q + i] * (scale * a.weight_scales[o]);
-                    if (a.bias != nullptr) v[i] += a.bias[o];
+                    const float scaled = (float)p.acc[m][n][4 * q + i] * (x_scale[m] * weight_scales[i]);
+                    v[i] = a.bias != nullptr ? scaled + bias[i] : scaled;
                 }
                 stage.put(p.row_of(m), col, v);
             }
@@ -86,8 +93,9 @@ template <typename OUT, int RT, int WAVES> __global__ __launch_bounds__(WAVES *P
 template <typename T, int BM, int BN, int WM, int WN> int linear_launch(LinearArgs &a, hipStream_t s)
 {
     typedef ProductNT<ProductI8, BM, BN, WM, WN, false> Product;
-    return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>, std::max(Product::lds_bytes(a.units, 1), (size_t)BM * BN * sizeof(T)),
-                          Product::THREADS, a, pccnn_ceil_div(a.n, BM), pccnn_ceil_div(a.outer, BN), s);
+    a.lds = std::max(Product::lds_bytes(a.units, 1), (size_t)BM * BN * sizeof(T));
+    return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>,
+                          a.lds + ProductChannels<2, BN, Product::THREADS>::BYTES, Product::THREADS, a, pccnn_ceil_div(a.n, BM), pccnn_ceil_div(a.outer, BN), s);
 }
 template <typename T> int linear_tiles(LinearArgs &a, hipStream_t s)
 {
@@ -150,7 +158,7 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
     }
     const int units = (int)pccnn_ceil_div(inner, 16);
     PccnnArena arena(workspace, workspace_bytes);
-    LinearArgs a = {{codes, inner, n, 0}, {weights, inner, outer, 0}, n, outer, units, scales, weight_scales, bias, 0, 0, 0, out};
+    LinearArgs a = {{codes, inner, n, 0}, {weights, inner, outer, 0}, n, outer, units, scales, weight_scales, bias, 0, 0, 0, 0, out};
     StageArgs stage = {};
     stage.width = inner;
     stage.units = units;

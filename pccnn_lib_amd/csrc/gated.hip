@@ -17,24 +17,25 @@ constexpr int kFewRows = 64;
 
 // ------------------------------------------------------------------------------------------- activations
 
-// Phi(x), the normal distribution function, and its density.  bf16 results take erfc by Abramowitz and Stegun 7.1.26 (absolute
-// error 1.5e-7, far below their rounding): one exponential and one reciprocal instead of a call of 60 instructions.
-template <bool EXACT> __device__ __forceinline__ void normal_of(float x, float &phi, float &density)
+// Phi(x), the normal distribution function, and its density, to f32.
+__device__ __forceinline__ void normal_of(float x, float &phi, float &density)
 {
-    const float e = EXACT ? expf(-0.5f * x * x) : __expf(-0.5f * x * x);
-    density = 0.3989422804014327f * e;
-    if constexpr (EXACT) {
-        phi = 0.5f * erfcf(-0.7071067811865476f * x);
-    } else {
-        const float z = fabsf(x) * 0.7071067811865476f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-        float p = fmaf(1.061405429f, t, -1.453152027f);
-        p = fmaf(p, t, 1.421413741f);
-        p = fmaf(p, t, -0.284496736f);
-        p = fmaf(p, t, 0.254829592f);
-        const float tail = 0.5f * p * t * e;
-        phi = x < 0.0f ? tail : 1.0f - tail;
-        if (x != x) phi = x;
-    }
+    density = 0.3989422804014327f * expf(-0.5f * x * x);
+    phi = 0.5f * erfcf(-0.7071067811865476f * x);
+}
+// To what a bf16 result shows: Phi(-|x|) = t (a1 + .. + a5 t^4) exp(-x^2 / 2) / 2, t = 1 / (1 + k |x|), Abramowitz and Stegun 7.1.26
+// (absolute error 8e-8).  `shrunk` = t exp(-x^2 / 2), the polynomial halved: one exponential, one reciprocal and a dozen other
+// instructions, where a call of erfcf is some sixty and 205 million results (800000 x 256) took 250 us with it.
+__device__ __forceinline__ float normal_tail(float x, float &shrunk, float &bell)
+{
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.7071067811865476f, fabsf(x), 1.0f));
+    bell = __builtin_amdgcn_exp2f(x * x * -0.7213475204444817f);
+    float p = fmaf(0.5307027145f, t, -0.7265760135f);
+    p = fmaf(p, t, 0.7107068705f);
+    p = fmaf(p, t, -0.142248368f);
+    p = fmaf(p, t, 0.127414796f);
+    shrunk = t * bell;
+    return p;
 }
 // act(g) and, if asked for, its derivative.  EXACT: to f32, else to what a bf16 result shows.
 template <bool EXACT, bool SLOPE> __device__ __forceinline__ float activate(float g, int which, float &slope)
@@ -44,12 +45,22 @@ template <bool EXACT, bool SLOPE> __device__ __forceinline__ float activate(floa
         return g > 0.0f ? g : g != g ? g : 0.0f;
     }
     if (which == PCCNN_ACT_GELU) {
-        float phi, density;
-        normal_of<EXACT>(g, phi, density);
-        if (SLOPE) slope = fmaf(g, density, phi);
-        return g * phi;
+        if constexpr (EXACT) {
+            float phi, density;
+            normal_of(g, phi, density);
+            if (SLOPE) slope = fmaf(g, density, phi);
+            return g * phi;
+        }
+        float shrunk, bell;
+        const float p = normal_tail(g, shrunk, bell);
+        if (SLOPE) {
+            const float tail = p * shrunk;
+            slope = fmaf(g * 0.3989422804014327f, bell, g < 0.0f ? tail : 1.0f - tail);
+        }
+        // max(g, 0) - |g| Phi(-|g|); `shrunk` is zero from 64 on, but not times infinity (a NaN is in it)
+        return fmaf(-__builtin_amdgcn_fmed3f(fabsf(g), 0.0f, 64.0f) * shrunk, p, fmaxf(g, 0.0f));
     }
-    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
     if (which == PCCNN_ACT_SIGMOID) {
         if (SLOPE) slope = s * (1.0f - s);
         return s;
@@ -67,6 +78,7 @@ struct GatedArgs {
     const float *x_scales, *gate_scales, *up_scales;                  // 8-bit operands
     int64_t blocks;
     int tiles, run;                          // tiles of hidden channels to a tile of rows; workgroups that go to one XCD
+    size_t lds;                              // bytes of the products' tiles and of the results
     void *out;                               // forward: h [n, hidden]
     const void *grads;                       // backward: dh
     int64_t grads_stride;
@@ -89,6 +101,14 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
     uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
     const int64_t col0 = (int64_t)product_split(tile, a.tiles) * COLS, row0 = (int64_t)tile * BM;
     Product p;
+    float x_scale[Product::MT];
+    const ProductChannels<2, COLS, Product::THREADS> channels = {(float *)((char *)lds + a.lds)};
+    if constexpr (std::is_same<E, ProductI8>::value) {
+        channels.start(0, a.gate_scales, col0, a.hidden);
+        channels.start(1, a.up_scales, col0, a.hidden);
+#pragma unroll
+        for (int m = 0; m < Product::MT; ++m) x_scale[m] = a.x_scales[min(row0 + p.row_of(m), a.n - 1)];
+    }
     p.run(a.x, row0, a.gate, a.up, col0, a.units, a.pairs, lds);
     const Stage stage = {(T *)lds}, second = {(T *)lds + BM * COLS};
     if constexpr (BACK) {
@@ -98,22 +118,23 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m) {
         const int row = p.row_of(m);
-        float x_scale = 1.0f;
-        if constexpr (std::is_same<E, ProductI8>::value) x_scale = a.x_scales[min(row0 + row, a.n - 1)];
 #pragma unroll
         for (int n = 0; n < HALF; ++n)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int col = p.col_of(n) + 8 * q + 4 * p.half;
-                float v[4], w[4];
+                float v[4], w[4], gate_scales[4], up_scales[4];
                 if constexpr (BACK) stage.get(row, col, v);
+                if constexpr (std::is_same<E, ProductI8>::value) {
+                    channels.get(0, col, gate_scales);
+                    channels.get(1, col, up_scales);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float g = p.acc[m][n][4 * q + i], u = p.acc[m][n + HALF][4 * q + i], slope;
                     if constexpr (std::is_same<E, ProductI8>::value) {
-                        const int64_t channel = min(col0 + col + i, a.hidden - 1);
-                        g *= x_scale * a.gate_scales[channel];
-                        u *= x_scale * a.up_scales[channel];
+                        g *= x_scale[m] * gate_scales[i];
+                        u *= x_scale[m] * up_scales[i];
                     }
                     const float act = activate<EXACT, BACK>(g, a.activation, slope);
                     if constexpr (BACK) {
@@ -566,8 +587,9 @@ template <class E, typename T, bool BACK, int BM, int BN, int WM, int WN>
 int gated_launch_tile(const char *name, GatedArgs &a, hipStream_t s)
 {
     typedef ProductNT<E, BM, BN, WM, WN, true> Product;
-    const size_t lds = std::max(Product::lds_bytes(a.units, a.pairs), (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
-    return product_launch(name, gated_kernel<E, T, BACK, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
+    a.lds = std::max(Product::lds_bytes(a.units, a.pairs), (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
+    const size_t channels = std::is_same<E, ProductI8>::value ? ProductChannels<2, BN / 2, Product::THREADS>::BYTES : 0;
+    return product_launch(name, gated_kernel<E, T, BACK, BM, BN, WM, WN>, a.lds + channels, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
                           pccnn_ceil_div(a.hidden, BN / 2), s);
 }
 template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)

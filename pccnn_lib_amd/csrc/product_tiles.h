@@ -276,42 +276,64 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
             }
         }
     }
-    // Writes the tile to `to`'s rows, columns below `width`, as whole units where every row allows it.
+    // Writes the tile to `to`'s rows, columns below `width`, as whole units where every row allows it.  A thread has the same unit of
+    // every THREADS / UNITS-th row.
     template <typename ROW> __device__ __forceinline__ void out(const ROW &to, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
     {
-        const bool whole = to.whole() && width % PER == 0;
-        for (int i = threadIdx.x; i < BM * UNITS; i += THREADS) {
-            const int r = i / UNITS, unit = i % UNITS;
-            const int64_t col = col0 + unit * PER;
-            if (row0 + r >= rows || col >= width) continue;
-            const T *from = base + r * COLS + PER * place(r, unit);
-            T *at = to.at(row0 + r, col);
-            if (whole) {
-                *(pccnn_u32x4 *)at = *(const pccnn_u32x4 *)from;
-            } else {
+        constexpr int COUNT = BM * UNITS / THREADS, EVERY = THREADS / UNITS;
+        static_assert(COUNT * THREADS == BM * UNITS && EVERY % 8 == 0, "the same unit in every round");
+        const int r0 = (int)threadIdx.x / UNITS, unit = (int)threadIdx.x % UNITS;
+        const int64_t col = col0 + unit * PER;
+        const int left = (int)min(rows - row0, (int64_t)BM);
+        if (col >= width) return;
+        const T *from = base + r0 * COLS + PER * place(r0, unit);
+        T *at = to.at(row0 + r0, col);
+        const int64_t step = EVERY * to.row_step();
+        if (to.whole() && width % PER == 0) {
 #pragma unroll
-                for (int e = 0; e < PER; ++e)
-                    if (col + e < width) at[e] = from[e];
-            }
+            for (int j = 0; j < COUNT; ++j, at += step)
+                if (r0 + j * EVERY < left) *(pccnn_u32x4 *)at = *(const pccnn_u32x4 *)(from + j * EVERY * COLS);
+        } else {
+            for (int j = 0; j < COUNT; ++j, at += step)
+                if (r0 + j * EVERY < left)
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (col + e < width) at[e] = from[j * EVERY * COLS + e];
         }
     }
 };
 // Where a unit of a result lies: rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what
-// a tile of rows takes of one piece lies together (65536 x 2816 x 512 with its rows in one piece: XXX us).
+// a tile of rows takes of one piece lies together (65536 x 2816 x 512: 167 us, with rows in one piece 196; 65536 x 512 under 2816
+// columns, the inner dimension over the rows, 191 and 219).
 template <typename T> struct DenseRow {
     T *p;
     int64_t stride;
     __device__ __forceinline__ bool whole() const { return stride * (int)sizeof(T) % 16 == 0; }
+    __device__ __forceinline__ int64_t row_step() const { return stride; }
     __device__ __forceinline__ T *at(int64_t row, int64_t col) const { return p + row * stride + col; }
 };
 template <typename T> struct PieceRow {
     T *p;
     int64_t rows, from;                      // `from`: the column of all pieces that column 0 is
     __device__ __forceinline__ bool whole() const { return true; }
+    __device__ __forceinline__ int64_t row_step() const { return 64; }
     __device__ __forceinline__ T *at(int64_t row, int64_t col) const
     {
         return p + ((from + col) / 64 * rows + row) * 64 + (from + col) % 64;
     }
+};
+
+// What belongs to the tile's output channels (scales, a bias), in LDS before the products begin: COUNT arrays of COLS values, those
+// of channels that do not exist zero.  There by the first barrier.
+template <int COUNT, int COLS, int THREADS> struct ProductChannels {
+    static constexpr size_t BYTES = COUNT * COLS * sizeof(float);
+    float *base;
+    __device__ __forceinline__ void start(int which, const float *from, int64_t col0, int64_t cols) const
+    {
+        for (int i = threadIdx.x; i < COLS; i += THREADS)
+            base[which * COLS + i] = from != nullptr && col0 + i < cols ? from[col0 + i] : 0.0f;
+    }
+    __device__ __forceinline__ void get(int which, int col, float (&v)[4]) const { pccnn_load<4>(base + which * COLS + col, v); }
 };
 
 // ---------------------------------------------------------------------------------------------- few rows
