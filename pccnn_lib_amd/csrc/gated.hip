@@ -38,13 +38,13 @@ __device__ __forceinline__ float normal_tail(float x, float &shrunk, float &bell
     return p;
 }
 // act(g) and, if asked for, its derivative.  EXACT: to f32, else to what a bf16 result shows.
-template <bool EXACT, bool SLOPE> __device__ __forceinline__ float activate(float g, int which, float &slope)
+template <bool EXACT, bool SLOPE, int which> __device__ __forceinline__ float activate(float g, float &slope)
 {
-    if (which == PCCNN_ACT_RELU) {
+    if constexpr (which == PCCNN_ACT_RELU) {
         if (SLOPE) slope = g > 0.0f ? 1.0f : 0.0f;
         return g > 0.0f ? g : g != g ? g : 0.0f;
     }
-    if (which == PCCNN_ACT_GELU) {
+    if constexpr (which == PCCNN_ACT_GELU) {
         if constexpr (EXACT) {
             float phi, density;
             normal_of(g, phi, density);
@@ -61,12 +61,24 @@ template <bool EXACT, bool SLOPE> __device__ __forceinline__ float activate(floa
         return fmaf(-__builtin_amdgcn_fmed3f(fabsf(g), 0.0f, 64.0f) * shrunk, p, fmaxf(g, 0.0f));
     }
     const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
-    if (which == PCCNN_ACT_SIGMOID) {
+    if constexpr (which == PCCNN_ACT_SIGMOID) {
         if (SLOPE) slope = s * (1.0f - s);
         return s;
     }
     if (SLOPE) slope = s * fmaf(g, 1.0f - s, 1.0f);
     return g * s;
+}
+// `call` with the activation as a constant: one branch for a tile, not one for a value.
+template <typename CALL> __device__ __forceinline__ void by_activation(int which, CALL call)
+{
+    if (which == PCCNN_ACT_SILU)
+        call(std::integral_constant<int, PCCNN_ACT_SILU>());
+    else if (which == PCCNN_ACT_GELU)
+        call(std::integral_constant<int, PCCNN_ACT_GELU>());
+    else if (which == PCCNN_ACT_SIGMOID)
+        call(std::integral_constant<int, PCCNN_ACT_SIGMOID>());
+    else
+        call(std::integral_constant<int, PCCNN_ACT_RELU>());
 }
 
 // ------------------------------------------------------------------------------------------- G and U
@@ -115,6 +127,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
         stage.bring((const T *)a.grads, a.grads_stride, row0, a.n, col0, a.hidden, a.grads_wide);
         attn_landed();
     }
+    by_activation(a.activation, [&](auto which) {
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m) {
         const int row = p.row_of(m);
@@ -136,7 +149,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
                         g *= x_scale[m] * gate_scales[i];
                         u *= x_scale[m] * up_scales[i];
                     }
-                    const float act = activate<EXACT, BACK>(g, a.activation, slope);
+                    const float act = activate<EXACT, BACK, decltype(which)::value>(g, slope);
                     if constexpr (BACK) {
                         w[i] = v[i] * act;
                         v[i] *= u * slope;
@@ -154,6 +167,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
                 if constexpr (BACK) second.put(row, col, w);
             }
     }
+    });
     __syncthreads();
     if constexpr (!BACK) {
         stage.out(DenseRow<T>{(T *)a.out, a.hidden}, row0, a.n, col0, a.hidden);
@@ -195,6 +209,7 @@ __global__ __launch_bounds__(WAVES *PCCNN_WAVE) void gated_few_kernel(GatedFew a
     FewProduct<T, 2, RT, WAVES> p;
     if (!p.run(a.x, a.n, a.w, col0, a.hidden, a.channels, lds)) return;
     const int lane = threadIdx.x % PCCNN_WAVE;
+    by_activation(a.activation, [&](auto which) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int64_t row = 16 * r + (lane & 15);
@@ -208,10 +223,11 @@ __global__ __launch_bounds__(WAVES *PCCNN_WAVE) void gated_few_kernel(GatedFew a
                 g *= a.x_scales[row] * a.gate_scales[channel];
                 u *= a.x_scales[row] * a.up_scales[channel];
             }
-            const float h[1] = {activate<std::is_same<OUT, float>::value, false>(g, a.activation, slope) * u};
+            const float h[1] = {activate<std::is_same<OUT, float>::value, false, decltype(which)::value>(g, slope) * u};
             pccnn_store<1>((OUT *)a.out + row * a.hidden + channel, h);
         }
     }
+    });
 }
 
 // ------------------------------------------------------------------------------------------- backward products
