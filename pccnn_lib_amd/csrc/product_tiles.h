@@ -36,20 +36,20 @@ struct ProductBf16 {
     typedef pccnn_f32x16 Acc;
     typedef float Sum;
     static constexpr int UNIT = 8;           // elements of a 16-byte unit
-    static __device__ __forceinline__ void mma(Acc &c, pccnn_u32x4 a, pccnn_u32x4 b)
+    static __device__ __forceinline__ Acc mma(pccnn_u32x4 a, pccnn_u32x4 b, Acc c)
     {
-        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a), __builtin_bit_cast(pccnn_bf16x8, b),
-                                                    c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a), __builtin_bit_cast(pccnn_bf16x8, b),
+                                                       c, 0, 0, 0);
     }
 };
 struct ProductI8 {
     typedef pccnn_i32x16 Acc;
     typedef int Sum;
     static constexpr int UNIT = 16;
-    static __device__ __forceinline__ void mma(Acc &c, pccnn_u32x4 a, pccnn_u32x4 b)
+    static __device__ __forceinline__ Acc mma(pccnn_u32x4 a, pccnn_u32x4 b, Acc c)
     {
-        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(pccnn_i32x4, a), __builtin_bit_cast(pccnn_i32x4, b), c, 0,
-                                                  0, 0);
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(pccnn_i32x4, a), __builtin_bit_cast(pccnn_i32x4, b), c,
+                                                     0, 0, 0);
     }
 };
 
@@ -138,12 +138,6 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PCCNN_WAVE);
         wm = wave % WM;
         wn = wave / WM;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
     }
     // Tile row of the lane's side of block m; first tile row of the registers' side of block n.
     __device__ __forceinline__ int row_of(int m) const { return wm * (32 * MT) + 32 * m + (lane & 31); }
@@ -156,8 +150,11 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     // of a wavefront every sixteen cycles, so eight wavefronts that ask for a whole tile at once wait for each other; what is
     // asked for in the second half is late for the next tile.  65536 x 2816 x 512: at once 196 us, four parts over the whole 205,
     // two parts over the first half 197; 65536 x 512 x 512 40.1, 40.6 and 39.3, 65536 x 1408 x 512 83.7, 85.0 and 81.2.
-    template <typename ASK> __device__ __forceinline__ void multiply(const uint16_t *tile, ASK ask)
+    // BEGIN: the first tile, whose first products begin the sums (clearing the registers would cost two instructions a result,
+    // a tenth of what a gelu takes).
+    template <bool BEGIN, typename ASK> __device__ __forceinline__ void multiply(const uint16_t *tile, ASK ask)
     {
+        const typename E::Acc zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
         uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + BM * 64;
         // operands are read a step of products ahead of their use: the compiler, left alone, reads them just before
@@ -178,7 +175,7 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) E::mma(acc[m][n], a[kk & 1][n], b[kk & 1][m]);
+                for (int m = 0; m < MT; ++m) acc[m][n] = E::mma(a[kk & 1][n], b[kk & 1][m], BEGIN && kk == 0 ? zero : acc[m][n]);
                 if (n == 0 && kk < 2) {
                     __builtin_amdgcn_sched_barrier(0x6);
                     ask(kk);
@@ -217,15 +214,17 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         fetch(1, lds);
         // `here` holds what is worked on, `there` is where the next tile goes.  That the two do not overlap is what lets the reads go
         // on while the tile is on its way.
-        auto walk = [&](const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
-            multiply(here, [&](int part) {
+        auto walk = [&](auto begin, const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+            multiply<decltype(begin)::value>(here, [&](int part) {
                 if (more) fetch(part, there);
             });
         };
-        for (int step = 0; step < total; ++step) {
+        product_landed();
+        walk(std::true_type(), lds, lds + STAGE, total > 1);
+        for (int step = 1; step < total; ++step) {
             product_landed();
             const int stage = step & 1;
-            walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
+            walk(std::false_type(), lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
         }
         product_landed();                                             // LDS is free for the results
     }
