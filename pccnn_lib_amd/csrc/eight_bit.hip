@@ -16,8 +16,7 @@ struct LinearArgs {
     int64_t n, outer;
     int units;
     const float *scales, *weight_scales, *bias;
-    int64_t blocks;
-    int tiles, run;
+    ProductGrid grid;
     size_t lds;
     void *out;
 };
@@ -27,10 +26,9 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
     typedef ProductNT<ProductI8, BM, BN, WM, WN, false> Product;
     typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
-    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
-    if (block >= a.blocks) return;
-    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
-    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * BN, row0 = (int64_t)tile * BM;
+    uint32_t row_tile, col_tile;
+    if (!product_tile(a.grid, row_tile, col_tile)) return;
+    const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
     float x_scale[Product::MT];
     const ProductChannels<2, BN, Product::THREADS> channels = {(float *)((char *)lds + a.lds)};
@@ -158,7 +156,7 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
     }
     const int units = (int)pccnn_ceil_div(inner, 16);
     PccnnArena arena(workspace, workspace_bytes);
-    LinearArgs a = {{codes, inner, n, 0}, {weights, inner, outer, 0}, n, outer, units, scales, weight_scales, bias, 0, 0, 0, 0, out};
+    LinearArgs a = {{codes, inner, n, 0}, {weights, inner, outer, 0}, n, outer, units, scales, weight_scales, bias, {}, 0, out};
     StageArgs stage = {};
     stage.width = inner;
     stage.units = units;

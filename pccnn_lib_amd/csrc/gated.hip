@@ -58,7 +58,7 @@ template <bool EXACT, bool SLOPE, int which> __device__ __forceinline__ float ac
             slope = fmaf(g * 0.3989422804014327f, bell, g < 0.0f ? tail : 1.0f - tail);
         }
         // max(g, 0) - |g| Phi(-|g|); `shrunk` is zero from 64 on, but not times infinity (a NaN is in it)
-        return fmaf(-__builtin_amdgcn_fmed3f(fabsf(g), 0.0f, 64.0f) * shrunk, p, fmaxf(g, 0.0f));
+        return fmaf(-__builtin_amdgcn_fmed3f(fabsf(g), 0.0f, 64.0f) * shrunk, p, __int_as_float(max(__float_as_int(g), 0)));
     }
     const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
     if constexpr (which == PCCNN_ACT_SIGMOID) {
@@ -88,8 +88,7 @@ struct GatedArgs {
     int64_t n, hidden;
     int units, pairs, activation;
     const float *x_scales, *gate_scales, *up_scales;                  // 8-bit operands
-    int64_t blocks;
-    int tiles, run;                          // tiles of hidden channels to a tile of rows; workgroups that go to one XCD
+    ProductGrid grid;
     size_t lds;                              // bytes of the products' tiles and of the results
     void *out;                               // forward: h [n, hidden]
     const void *grads;                       // backward: dh
@@ -108,10 +107,9 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
     constexpr bool EXACT = std::is_same<T, float>::value;
     typedef ProductStage<T, BM, COLS, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
-    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
-    if (block >= a.blocks) return;
-    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
-    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * COLS, row0 = (int64_t)tile * BM;
+    uint32_t row_tile, col_tile;
+    if (!product_tile(a.grid, row_tile, col_tile)) return;
+    const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * COLS;
     Product p;
     float x_scale[Product::MT];
     const ProductChannels<2, COLS, Product::THREADS> channels = {(float *)((char *)lds + a.lds)};
@@ -272,8 +270,7 @@ struct BackArgs {
     ProductRows x, w;
     int64_t n, cols;
     int units, pairs;
-    int64_t blocks;
-    int tiles, run;
+    ProductGrid grid;
     void *out;
 };
 template <typename T, int BM, int BN, int WM, int WN>
@@ -282,10 +279,9 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a
     typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
     typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
-    const int64_t block = pccnn_xcd_block(blockIdx.x, gridDim.x, a.run);
-    if (block >= a.blocks) return;
-    uint32_t tile = __builtin_amdgcn_readfirstlane((uint32_t)block);
-    const int64_t col0 = (int64_t)product_split(tile, a.tiles) * BN, row0 = (int64_t)tile * BM;
+    uint32_t row_tile, col_tile;
+    if (!product_tile(a.grid, row_tile, col_tile)) return;
+    const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
     p.run(a.x, row0, a.w, a.w, col0, a.units, a.pairs, lds);
     const Stage stage = {(T *)lds};

@@ -30,7 +30,40 @@ enum { PRODUCT_PAIRS = 6 };                  // f32: products of planes
 static inline constexpr int product_term_a(int pair) { return pair == 0 ? 2 : pair == 1 || pair == 3 ? 1 : 0; }
 static inline constexpr int product_term_b(int pair) { return pair == 2 ? 2 : pair == 1 || pair == 4 ? 1 : 0; }
 
+// The tiles of a product in the order of their workgroups: those of a tile of rows one behind the other, runs of 2^run_log2 of them
+// on one XCD, whose L2 then serves the rows.  Numbers come apart by shifts and a multiplication with 2^shift / tiles rounded up
+// (exact below 2^31): the divisions themselves were a hundred instructions, as much as six results of a gelu.
+struct ProductGrid {
+    uint32_t blocks, tiles, magic;
+    int shift, run_log2;
+};
+static inline ProductGrid product_grid(int64_t tiles_m, int64_t tiles_n)
+{
+    ProductGrid g = {(uint32_t)(tiles_m * tiles_n), (uint32_t)tiles_n, 0, 31, 0};
+    while (((int64_t)1 << (g.shift - 31)) < tiles_n) ++g.shift;
+    g.magic = (uint32_t)((((uint64_t)1 << g.shift) + tiles_n - 1) / tiles_n);
+    // as many as a tile of rows has, 64 at most, and no more than leave every XCD one
+    while (((int64_t)1 << g.run_log2) < tiles_n && g.run_log2 < 6 && ((uint64_t)PCCNN_XCDS << (g.run_log2 + 1)) <= g.blocks) ++g.run_log2;
+    return g;
+}
+static inline uint32_t product_workgroups(const ProductGrid &g)
+{
+    const uint32_t super = (uint32_t)PCCNN_XCDS << g.run_log2;
+    return (g.blocks + super - 1) / super * super;
+}
+
 #ifdef __HIPCC__
+// The tile of the workgroup, in scalar registers; false: it has none.
+__device__ __forceinline__ bool product_tile(const ProductGrid &g, uint32_t &row_tile, uint32_t &col_tile)
+{
+    const uint32_t within = blockIdx.x & ((PCCNN_XCDS << g.run_log2) - 1);
+    const uint32_t block = blockIdx.x - within + ((within % PCCNN_XCDS) << g.run_log2) + within / PCCNN_XCDS;
+    if (block >= g.blocks) return false;
+    row_tile = (uint32_t)(((uint64_t)block * g.magic) >> g.shift);
+    col_tile = block - row_tile * g.tiles;
+    return true;
+}
+
 // What a lane's operand of 16 bytes is multiplied as.
 struct ProductBf16 {
     typedef pccnn_f32x16 Acc;
@@ -85,12 +118,12 @@ template <int ROWS, int THREADS> struct RowsFeeder {
         plane = s.plane;
         step = s.step;
         at = base + term * plane;
-        unit = Tile::unit_at((int)threadIdx.x / 8, (int)threadIdx.x % 8);
+        const int r = (int)threadIdx.x / 8, stride = (int)s.stride, left = (int)min(s.rows - row, (int64_t)ROWS);
+        unit = Tile::unit_at(r, (int)threadIdx.x % 8);
+        const uint32_t first = r * stride + 16 * unit;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const int r = (int)threadIdx.x / 8 + j * (THREADS / 8);
-            off[j] = row + r < s.rows ? (uint32_t)(r * s.stride + 16 * unit) : kAttnNowhere;
-        }
+        for (int j = 0; j < COUNT; ++j)
+            off[j] = r + j * (THREADS / 8) < left ? first + j * (THREADS / 8 * stride) : kAttnNowhere;
     }
     // The next 128 bytes of every row; `units`: how many of these eight units exist.  A tile comes in ALL requests of a wavefront,
     // of which this operand's are those from FIRST on; `part`: which half of them.
@@ -476,25 +509,20 @@ template <typename T> static __global__ __launch_bounds__(256) void product_stag
 
 // ---------------------------------------------------------------------------------------------- launches
 //
-// Tiles of output channels follow each other within a tile of rows; those of a run go to one XCD, whose L2 then serves the rows.
 // Whether a product takes tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128.
 static inline bool product_large(int64_t rows, int64_t cols, int units, int pairs)
 {
     return cols >= 256 && units * pairs >= 32 && pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256) >= 256;
 }
-static inline int product_run(int tiles) { return tiles <= 64 ? tiles : 32; }
-
 template <typename KERNEL, typename ARGS>
 static int product_launch(const char *name, KERNEL kernel, size_t lds, int threads, ARGS &a, int64_t tiles_m, int64_t tiles_n, hipStream_t s)
 {
-    a.blocks = tiles_m * tiles_n;
-    a.tiles = (int)tiles_n;
-    a.run = product_run(a.tiles);
-    PCCNN_REQUIRE(a.blocks <= INT32_MAX - PCCNN_XCDS * (int64_t)a.run, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name,
-                  (long long)a.blocks);
+    PCCNN_REQUIRE(tiles_m * tiles_n <= INT32_MAX - 1024, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name,
+                  (long long)(tiles_m * tiles_n));
+    a.grid = product_grid(tiles_m, tiles_n);
     if (lds > 65536)
         PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    kernel<<<pccnn_xcd_grid(a.blocks, a.run), threads, lds, s>>>(a);
+    kernel<<<product_workgroups(a.grid), threads, lds, s>>>(a);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
 }
