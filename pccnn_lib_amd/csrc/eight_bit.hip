@@ -36,7 +36,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
     channels.start(1, a.bias, col0, a.outer);
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m) x_scale[m] = a.scales[min(row0 + p.row_of(m), a.n - 1)];
-    p.run(a.x, row0, a.w, a.w, col0, a.units, 1, lds);
+    p.run(a.x, row0, a.w, a.w, col0, a.units, lds);
     const Stage stage = {(T *)lds};
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m) {
@@ -91,14 +91,15 @@ template <typename OUT, int RT, int WAVES> __global__ __launch_bounds__(WAVES *P
 template <typename T, int BM, int BN, int WM, int WN> int linear_launch(LinearArgs &a, hipStream_t s)
 {
     typedef ProductNT<ProductI8, BM, BN, WM, WN, false> Product;
-    a.lds = std::max(Product::lds_bytes(a.units, 1), (size_t)BM * BN * sizeof(T));
+    a.lds = std::max(Product::lds_bytes(a.units), (size_t)BM * BN * sizeof(T));
     return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>,
                           a.lds + ProductChannels<2, BN, Product::THREADS>::BYTES, Product::THREADS, a, pccnn_ceil_div(a.n, BM), pccnn_ceil_div(a.outer, BN), s);
 }
 template <typename T> int linear_tiles(LinearArgs &a, hipStream_t s)
 {
     if constexpr (!std::is_same<T, float>::value)
-        if (product_large(a.n, a.outer, a.units, 1)) return linear_launch<T, 256, 256, 2, 4>(a, s);
+        if (product_large(a.n, a.outer, a.units)) return linear_launch<T, 256, 256, 2, 4>(a, s);
+    if (product_small(a.n, a.outer)) return linear_launch<T, 64, 64, 2, 2>(a, s);
     return a.outer <= 64 ? linear_launch<T, 128, 64, 4, 1>(a, s) : linear_launch<T, 128, 128, 2, 2>(a, s);
 }
 template <typename OUT> int linear_few(const LinearFew &a, hipStream_t s)

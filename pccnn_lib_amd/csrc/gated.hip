@@ -86,7 +86,7 @@ template <typename CALL> __device__ __forceinline__ void by_activation(int which
 struct GatedArgs {
     ProductRows x, gate, up;                 // operands with whole units
     int64_t n, hidden;
-    int units, pairs, activation;
+    int units, activation;
     const float *x_scales, *gate_scales, *up_scales;                  // 8-bit operands
     ProductGrid grid;
     size_t lds;                              // bytes of the products' tiles and of the results
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
 #pragma unroll
         for (int m = 0; m < Product::MT; ++m) x_scale[m] = a.x_scales[min(row0 + p.row_of(m), a.n - 1)];
     }
-    p.run(a.x, row0, a.gate, a.up, col0, a.units, a.pairs, lds);
+    p.run(a.x, row0, a.gate, a.up, col0, a.units, lds);
     const Stage stage = {(T *)lds}, second = {(T *)lds + BM * COLS};
     if constexpr (BACK) {
         stage.bring((const T *)a.grads, a.grads_stride, row0, a.n, col0, a.hidden, a.grads_wide);
@@ -243,7 +243,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_ker
     const int64_t c0 = (int64_t)blockIdx.x * 64, h0 = (int64_t)blockIdx.y * 64;
     const T *from = blockIdx.z ? a.up : a.gate;
     const int64_t stride = blockIdx.z ? a.up_stride : a.gate_stride;
-    for (int i = threadIdx.x; i < 64 * 64; i += kThreads) {
+#pragma unroll
+    for (int j = 0; j < 64 * 64 / kThreads; ++j) {
+        const int i = threadIdx.x + j * kThreads;
         const int64_t h = h0 + i / 64, c = c0 + i % 64;
         float v[1] = {0.0f};
         if (h < a.hidden && c < a.channels) pccnn_load<1>(from + h * stride + c, v);
@@ -265,25 +267,28 @@ template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_ker
     }
 }
 
+template <typename T> struct ProductOf { typedef ProductBf16 type; };
+template <> struct ProductOf<float> { typedef ProductF32 type; };
+
 // dx: rows of (dG | dU) times the turned weights.
 struct BackArgs {
     ProductRows x, w;
     int64_t n, cols;
-    int units, pairs;
+    int units;
     ProductGrid grid;
     void *out;
 };
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a)
 {
-    typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
+    typedef ProductNT<typename ProductOf<T>::type, BM, BN, WM, WN, false> Product;
     typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
     uint32_t row_tile, col_tile;
     if (!product_tile(a.grid, row_tile, col_tile)) return;
     const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
-    p.run(a.x, row0, a.w, a.w, col0, a.units, a.pairs, lds);
+    p.run(a.x, row0, a.w, a.w, col0, a.units, lds);
     const Stage stage = {(T *)lds};
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m)
@@ -305,65 +310,72 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a
 struct WeightsArgs {
     ProductRows x, d;                        // rows with whole units; stride in bytes
     int64_t n, cols_x, cols_d;               // columns that exist, in whole units
-    int pairs;
     int tiles_x, tiles_d, splits, run;
     int64_t blocks;
     int64_t per_split;                       // rows of a part, a multiple of 64
     float *part;                             // [split][cols_d][channels]
     int64_t channels;
 };
-constexpr int kTurnRows = 64;                // rows of a step
 
-// Brings kTurnRows rows of up to 128 columns each into LDS, where the transposing reads take their columns.
-template <int COLS, int THREADS> struct ColumnsFeeder {
-    typedef AttnTile<1, kTurnRows, COLS> Tile;
-    static constexpr int COUNT = kTurnRows * Tile::UNITS / THREADS;
-    static_assert(COUNT >= 1 && THREADS / Tile::UNITS % 16 == 0, "whole units, the same one in every round");
-    const char *base, *at;                   // the first row's columns, and the rows that are asked for next (the same in all lanes)
+// Brings ROWS rows of up to 128 columns each into LDS, where the transposing reads take their columns; TERMS planes.
+template <int ROWS, int COLS, int THREADS, int TERMS> struct ColumnsFeeder {
+    typedef AttnTile<1, ROWS, COLS> Tile;
+    static constexpr int ROUNDS = (ROWS * Tile::UNITS + THREADS - 1) / THREADS, COUNT = ROUNDS * TERMS;
+    static constexpr int ELEMENTS = TERMS * Tile::PLANE;
+    static_assert(THREADS / Tile::UNITS % 16 == 0 && (ROUNDS == 1 || ROUNDS * THREADS == ROWS * Tile::UNITS),
+                  "whole wavefronts, the same unit in every round");
+    const char *at;                          // the rows that are asked for next (the same in all lanes)
     int64_t step, plane;
-    uint32_t off[COUNT];                     // the lane's units, in bytes
+    uint32_t off[ROUNDS];                    // the lane's units, in bytes
     int row;
+    bool mine;
     // (columns of 64 a piece where the rows do not lie in one)
-    __device__ __forceinline__ void start(const ProductRows &s, int64_t first, int64_t col0, int64_t cols, int term)
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t first, int64_t col0, int64_t cols)
     {
         row = (int)threadIdx.x / Tile::UNITS;
-        const int unit = Tile::unit_at(row, (int)threadIdx.x % Tile::UNITS);
-        base = (const char *)s.p + first * s.stride + col0 / 64 * s.step;
+        const int unit = Tile::unit_at(row % ROWS, (int)threadIdx.x % Tile::UNITS);
+        mine = ROWS * Tile::UNITS >= THREADS || __builtin_amdgcn_readfirstlane(threadIdx.x) < ROWS * Tile::UNITS;
+        at = (const char *)s.p + first * s.stride + col0 / 64 * s.step;
         plane = s.plane;
-        step = kTurnRows * s.stride;
-        at = base + term * plane;
+        step = ROWS * s.stride;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
-            off[j] = col0 + 8 * unit < cols ? (uint32_t)((row + j * (THREADS / Tile::UNITS)) * s.stride + 16 * unit) : kAttnNowhere;
+        for (int j = 0; j < ROUNDS; ++j)
+            off[j] = col0 + 8 * unit < cols ? (uint32_t)((row + j * (THREADS / Tile::UNITS)) * (int)s.stride + 16 * unit) : kAttnNowhere;
     }
     // The next rows; `rows`: how many of them exist.  Parts as RowsFeeder has them.
     template <int ALL> __device__ __forceinline__ void fetch(int first, int part, int rows, uint16_t *tile) const
     {
-        const __amdgpu_buffer_rsrc_t window = product_window(at);
+        if (!mine) return;
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
-            if ((first + j) * 2 / ALL == part)
-                attn_bring(window, row + j * (THREADS / Tile::UNITS) < rows ? off[j] : kAttnNowhere,
-                           tile + 8 * (j * THREADS + wave_unit));
+        for (int t = 0; t < TERMS; ++t) {
+            const __amdgpu_buffer_rsrc_t window = product_window(at + t * plane);
+#pragma unroll
+            for (int j = 0; j < ROUNDS; ++j)
+                if ((first + t * ROUNDS + j) * 2 / ALL == part)
+                    attn_bring(window, row + j * (THREADS / Tile::UNITS) < rows ? off[j] : kAttnNowhere,
+                               tile + t * Tile::PLANE + 8 * (j * THREADS + wave_unit));
+        }
     }
-    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + step; }
+    __device__ __forceinline__ void next() { at += step; }
 };
+// DP x 64 columns of (dG | dU) times XP x XT columns of x; a wavefront has 32 MT x 64 of them.  64 rows a step, 32 of three planes.
 constexpr int weights_threads(int dp, int xp, int xt, int mt) { return dp * 64 / (32 * mt) * (xp * xt / 64) * PCCNN_WAVE; }
-template <int DP, int XP, int XT, int MT> struct WeightsShape {
+constexpr int weights_rows(int terms) { return terms == 3 ? 32 : 64; }
+template <class E, int DP, int XP, int XT, int MT> struct WeightsShape {
     static constexpr int COLS_D = DP * 64, COLS_X = XP * XT, WAVES_X = COLS_X / 64, WAVES_D = COLS_D / (32 * MT);
-    static constexpr int THREADS = WAVES_X * WAVES_D * PCCNN_WAVE;
+    static constexpr int THREADS = WAVES_X * WAVES_D * PCCNN_WAVE, TERMS = E::TERMS, ROWS = weights_rows(TERMS);
     static_assert(THREADS == weights_threads(DP, XP, XT, MT), "");
-    static constexpr int STAGE = kTurnRows * (COLS_D + COLS_X);       // uint16_t
+    static constexpr int STAGE = TERMS * ROWS * (COLS_D + COLS_X);    // uint16_t
     static constexpr size_t LDS = 2 * STAGE * sizeof(uint16_t);
 };
-template <int DP, int XP, int XT, int MT>
+template <class E, int DP, int XP, int XT, int MT>
 __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights_kernel(WeightsArgs a)
 {
-    typedef WeightsShape<DP, XP, XT, MT> Shape;
-    constexpr int WAVES_X = Shape::WAVES_X, STAGE = Shape::STAGE;
-    typedef ColumnsFeeder<64, Shape::THREADS> FeedD;
-    typedef ColumnsFeeder<XT, Shape::THREADS> FeedX;
+    typedef WeightsShape<E, DP, XP, XT, MT> Shape;
+    constexpr int WAVES_X = Shape::WAVES_X, STAGE = Shape::STAGE, TERMS = Shape::TERMS, ROWS = Shape::ROWS;
+    typedef ColumnsFeeder<ROWS, 64, Shape::THREADS, TERMS> FeedD;
+    typedef ColumnsFeeder<ROWS, XT, Shape::THREADS, TERMS> FeedX;
     typedef typename FeedD::Tile TileD;
     typedef typename FeedX::Tile TileX;
     extern __shared__ __align__(16) uint16_t lds[];
@@ -376,13 +388,13 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
     const int64_t d0 = (int64_t)product_split(split, a.tiles_d) * Shape::COLS_D;
     const int64_t first = split * a.per_split;
     const int rows = (int)min(a.n - first, a.per_split);
-    int pair = a.pairs == 1 ? PRODUCT_PAIRS - 1 : 0, left = rows;     // of the tile that is asked for next
+    int left = rows;                         // of the tile that is asked for next
     FeedX fx[XP];
     FeedD fd[DP];
 #pragma unroll
-    for (int i = 0; i < XP; ++i) fx[i].start(a.x, first, x0 + i * XT, a.cols_x, product_term_a(pair));
+    for (int i = 0; i < XP; ++i) fx[i].start(a.x, first, x0 + i * XT, a.cols_x);
 #pragma unroll
-    for (int i = 0; i < DP; ++i) fd[i].start(a.d, first, d0 + i * 64, a.cols_d, product_term_b(pair));
+    for (int i = 0; i < DP; ++i) fd[i].start(a.d, first, d0 + i * 64, a.cols_d);
     pccnn_f32x16 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -390,41 +402,46 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
         for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    const int total = (rows + kTurnRows - 1) / kTurnRows * a.pairs;
+    const int total = (rows + ROWS - 1) / ROWS;
     constexpr int ALL = DP * FeedD::COUNT + XP * FeedX::COUNT;
     auto fetch = [&](int part, uint16_t *to) {
 #pragma unroll
-        for (int i = 0; i < DP; ++i) fd[i].template fetch<ALL>(i * FeedD::COUNT, part, left, to + i * TileD::ELEMENTS);
+        for (int i = 0; i < DP; ++i) fd[i].template fetch<ALL>(i * FeedD::COUNT, part, left, to + i * FeedD::ELEMENTS);
 #pragma unroll
         for (int i = 0; i < XP; ++i)
             fx[i].template fetch<ALL>(DP * FeedD::COUNT + i * FeedX::COUNT, part, left,
-                                      to + DP * TileD::ELEMENTS + i * TileX::ELEMENTS);
+                                      to + DP * FeedD::ELEMENTS + i * FeedX::ELEMENTS);
         if (part == 0) return;
-        left -= kTurnRows;
-        const bool wrap = left <= 0;
-        if (wrap) left = rows, ++pair;
+        left -= ROWS;
 #pragma unroll
-        for (int i = 0; i < DP; ++i) fd[i].next(wrap, product_term_b(pair));
+        for (int i = 0; i < DP; ++i) fd[i].next();
 #pragma unroll
-        for (int i = 0; i < XP; ++i) fx[i].next(wrap, product_term_a(pair));
+        for (int i = 0; i < XP; ++i) fx[i].next();
     };
     fetch(0, lds);
     fetch(1, lds);
     auto walk = [&](uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
-        AttnFrag<1> fa[2][2], fb[2][MT];
+        pccnn_u32x4 fa[2][2][TERMS], fb[2][MT][TERMS];
         auto read = [&](int kk) {            // a step of products ahead of their use
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int col = 64 * wx + 32 * i;
-                fa[kk & 1][i] = TileX{here + DP * TileD::ELEMENTS + col / XT * TileX::ELEMENTS}.columns(16 * kk, col % XT, lane);
-            }
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                const int col = 32 * (MT * wd + j);
-                fb[kk & 1][j] = TileD{here + col / 64 * TileD::ELEMENTS}.columns(16 * kk, col % 64, lane);
-            }
+                for (int t = 0; t < TERMS; ++t) {
+                    const int col = 64 * wx + 32 * i;
+                    fa[kk & 1][i][t] = __builtin_bit_cast(
+                        pccnn_u32x4, TileX{here + DP * FeedD::ELEMENTS + col / XT * FeedX::ELEMENTS + t * TileX::PLANE}
+                                         .columns(16 * kk, col % XT, lane).t[0]);
+                }
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) {
+                    const int col = 32 * (MT * wd + j);
+                    fb[kk & 1][j][t] = __builtin_bit_cast(
+                        pccnn_u32x4, TileD{here + col / 64 * FeedD::ELEMENTS + t * TileD::PLANE}.columns(16 * kk, col % 64, lane).t[0]);
+                }
         };
-        constexpr int COUNT = kTurnRows / 16;
+        constexpr int COUNT = ROWS / 16;
         static_assert(COUNT >= 2, "two parts of the next tile are asked for in between");
         read(0);
 #pragma unroll
@@ -434,7 +451,7 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int j = 0; j < MT; ++j) attn_mma(acc[i][j], fa[kk & 1][i], fb[kk & 1][j]);
+                for (int j = 0; j < MT; ++j) acc[i][j] = E::mma(fa[kk & 1][i], fb[kk & 1][j], acc[i][j]);
                 if (i == 0 && kk < 2) {
                     __builtin_amdgcn_sched_barrier(0x6);
                     if (more) fetch(kk, there);
@@ -482,6 +499,7 @@ __global__ __launch_bounds__(kThreads) void gated_weights_sum_kernel(const float
     const float *from = part + (blockIdx.y ? padded * channels : 0) + i;
     const int64_t step = 2 * padded * channels;
     float sum = 0.0f;
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) sum += from[s * step];
     const float v[1] = {sum};
     pccnn_store<1>((blockIdx.y ? d_up : d_gate) + i, v);
@@ -553,13 +571,15 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     }
     plan.padded = pccnn_ceil_div(p->hidden, 8) * 8;
     plan.pieces = pccnn_ceil_div(2 * plan.padded, 64);
-    // parts enough to fill the chip twice over, of at least four steps
-    plan.tiles_x = (int)pccnn_ceil_div(p->channels, p->channels <= 64 ? 64 : p->channels <= 128 ? 128 : 256);
-    plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, 256);
+    // parts enough to fill the chip, of at least four steps
+    const bool f32 = p->type == PCCNN_TYPE_F32;
+    const int rows = weights_rows(plan.planes);
+    plan.tiles_x = (int)pccnn_ceil_div(p->channels, p->channels <= 64 ? 64 : f32 || p->channels <= 128 ? 128 : 256);
+    plan.tiles_d = (int)pccnn_ceil_div(2 * plan.padded, f32 ? 128 : 256);
     const int64_t want = std::max<int64_t>(1, 256 / ((int64_t)plan.tiles_x * plan.tiles_d));
-    const int64_t steps = std::max<int64_t>(1, pccnn_ceil_div(p->n, kTurnRows));
+    const int64_t steps = std::max<int64_t>(1, pccnn_ceil_div(p->n, rows));
     const int64_t per = std::max<int64_t>(std::min<int64_t>(4, steps), pccnn_ceil_div(steps, want));
-    plan.per_split = per * kTurnRows;
+    plan.per_split = per * rows;
     plan.splits = (int)pccnn_ceil_div(steps, per);
     return plan;
 }
@@ -599,39 +619,47 @@ template <class E, typename T, bool BACK, int BM, int BN, int WM, int WN>
 int gated_launch_tile(const char *name, GatedArgs &a, hipStream_t s)
 {
     typedef ProductNT<E, BM, BN, WM, WN, true> Product;
-    a.lds = std::max(Product::lds_bytes(a.units, a.pairs), (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
+    a.lds = std::max(Product::lds_bytes(a.units), (BACK ? 2 : 1) * (size_t)BM * BN / 2 * sizeof(T));
     const size_t channels = std::is_same<E, ProductI8>::value ? ProductChannels<2, BN / 2, Product::THREADS>::BYTES : 0;
     return product_launch(name, gated_kernel<E, T, BACK, BM, BN, WM, WN>, a.lds + channels, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
                           pccnn_ceil_div(a.hidden, BN / 2), s);
 }
 template <class E, typename T, bool BACK> int gated_launch(const char *name, GatedArgs &a, hipStream_t s)
 {
-    if constexpr (!(BACK && std::is_same<T, float>::value))
-        if (product_large(a.n, 2 * a.hidden, a.units, a.pairs)) return gated_launch_tile<E, T, BACK, 256, 256, 4, 2>(name, a, s);
-    return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
+    if (product_small(a.n, 2 * a.hidden)) return gated_launch_tile<E, T, BACK, 64, 64, 2, 1>(name, a, s);
+    if constexpr (std::is_same<E, ProductF32>::value) {
+        return gated_launch_tile<E, T, BACK, 128, 128, 4, 2>(name, a, s);
+    } else {
+        if (product_large(a.n, 2 * a.hidden, a.units)) return gated_launch_tile<E, T, BACK, 256, 256, 4, 2>(name, a, s);
+        return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
+    }
 }
 template <typename T, int BM, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
 {
-    typedef ProductNT<ProductBf16, BM, BN, WM, WN, false> Product;
-    const size_t lds = std::max(Product::lds_bytes(a.units, a.pairs), (size_t)BM * BN * sizeof(T));
+    typedef ProductNT<typename ProductOf<T>::type, BM, BN, WM, WN, false> Product;
+    const size_t lds = std::max(Product::lds_bytes(a.units), (size_t)BM * BN * sizeof(T));
     return product_launch(name, gated_dx_kernel<T, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
                           pccnn_ceil_div(a.cols, BN), s);
 }
 template <typename T> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
 {
-    if constexpr (!std::is_same<T, float>::value)
-        if (product_large(a.n, a.cols, a.units, a.pairs)) return dx_launch<T, 256, 256, 4, 2>(name, a, s);
-    return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 1>(name, a, s) : dx_launch<T, 128, 128, 2, 2>(name, a, s);
+    if (product_small(a.n, a.cols)) return dx_launch<T, 64, 64, 2, 2>(name, a, s);
+    if constexpr (std::is_same<T, float>::value) {
+        return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 2>(name, a, s) : dx_launch<T, 128, 128, 4, 2>(name, a, s);
+    } else {
+        if (product_large(a.n, a.cols, a.units)) return dx_launch<T, 256, 256, 4, 2>(name, a, s);
+        return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 1>(name, a, s) : dx_launch<T, 128, 128, 2, 2>(name, a, s);
+    }
 }
 
 // A part's tiles go to one XCD as far as they may: they read the same rows, and its L2 serves them once.
-template <int DP, int XP, int XT, int MT> int weights_launch(const char *name, WeightsArgs &a, hipStream_t s)
+template <class E, int DP, int XP, int XT, int MT> int weights_launch(const char *name, WeightsArgs &a, hipStream_t s)
 {
-    typedef WeightsShape<DP, XP, XT, MT> Shape;
+    typedef WeightsShape<E, DP, XP, XT, MT> Shape;
     a.blocks = (int64_t)a.tiles_x * a.tiles_d * a.splits;
     PCCNN_REQUIRE(a.blocks <= INT32_MAX / 2, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)a.blocks);
     a.run = (int)pccnn_ceil_div(a.blocks, PCCNN_XCDS);
-    const auto kernel = gated_weights_kernel<DP, XP, XT, MT>;
+    const auto kernel = gated_weights_kernel<E, DP, XP, XT, MT>;
     if (Shape::LDS > 65536)
         PCCNN_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::LDS));
     kernel<<<pccnn_xcd_grid(a.blocks, a.run), Shape::THREADS, Shape::LDS, s>>>(a);
@@ -709,10 +737,9 @@ extern "C" int pccnn_gated_forward(const pccnn_gated *p, void *out, int out_type
     GatedArgs a = {};
     a.x = r[0], a.gate = r[1], a.up = r[2];
     a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation;
-    a.pairs = plan.planes == 3 ? PRODUCT_PAIRS : 1;
     a.x_scales = p->feats_scales, a.gate_scales = p->gate_scales, a.up_scales = p->up_scales;
     a.out = out;
-    if (p->type == PCCNN_TYPE_F32) return gated_launch<ProductBf16, float, false>(name, a, s);
+    if (p->type == PCCNN_TYPE_F32) return gated_launch<ProductF32, float, false>(name, a, s);
     if (p->type == PCCNN_TYPE_BF16) return gated_launch<ProductBf16, uint16_t, false>(name, a, s);
     return out_type == PCCNN_TYPE_F32 ? gated_launch<ProductI8, float, false>(name, a, s)
                                       : gated_launch<ProductI8, uint16_t, false>(name, a, s);
@@ -738,7 +765,6 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
     PccnnArena arena(workspace, workspace_bytes);
     ProductRows r[3];
     const bool f32 = p->type == PCCNN_TYPE_F32;
-    const int pairs = f32 ? PRODUCT_PAIRS : 1;
     const ProductRows d = {arena.take<char>(bytes.d_pre), 128, p->n, p->n * plan.pieces * 128, p->n * 128};
     uint16_t *turned = arena.take<uint16_t>(bytes.turned / 2);
     float *part = arena.take<float>(bytes.part / sizeof(float));
@@ -748,11 +774,11 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         if (rc != PCCNN_OK) return rc;
         GatedArgs a = {};
         a.x = r[0], a.gate = r[1], a.up = r[2];
-        a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation, a.pairs = pairs;
+        a.n = p->n, a.hidden = p->hidden, a.units = (int)plan.units, a.activation = p->activation;
         a.grads = in_grads, a.grads_stride = grads_stride;
         a.grads_wide = grads_stride <= kMostWidth ? wide_of(in_grads, grads_stride, p->hidden, p->type) : 0;
         a.d_pre = (uint16_t *)d.p, a.padded = plan.padded, a.d_plane = d.plane / 2;
-        rc = f32 ? gated_launch<ProductBf16, float, true>(name, a, s) : gated_launch<ProductBf16, uint16_t, true>(name, a, s);
+        rc = f32 ? gated_launch<ProductF32, float, true>(name, a, s) : gated_launch<ProductBf16, uint16_t, true>(name, a, s);
         if (rc != PCCNN_OK) return rc;
     }
     if (d_feats != nullptr && p->n > 0) {
@@ -771,7 +797,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         BackArgs a = {};
         a.x = d;
         a.w = {turned, 4 * plan.padded, p->channels, p->channels * 4 * plan.padded};
-        a.n = p->n, a.cols = p->channels, a.units = (int)(2 * plan.padded / 8), a.pairs = pairs, a.out = d_feats;
+        a.n = p->n, a.cols = p->channels, a.units = (int)(2 * plan.padded / 8), a.out = d_feats;
         rc = f32 ? dx_launch<float>(name, a, s) : dx_launch<uint16_t>(name, a, s);
         if (rc != PCCNN_OK) return rc;
     }
@@ -779,12 +805,16 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         int splits = 0;
         if (p->n > 0) {
             WeightsArgs a = {};
-            a.x = r[0], a.d = d, a.n = p->n, a.cols_x = plan.units * 8, a.cols_d = 2 * plan.padded, a.pairs = pairs;
+            a.x = r[0], a.d = d, a.n = p->n, a.cols_x = plan.units * 8, a.cols_d = 2 * plan.padded;
             a.tiles_x = plan.tiles_x, a.tiles_d = plan.tiles_d, a.splits = splits = plan.splits, a.per_split = plan.per_split;
             a.part = part, a.channels = p->channels;
-            rc = p->channels <= 64    ? weights_launch<4, 1, 64, 2>(name, a, s)
-                 : p->channels <= 128 ? weights_launch<4, 1, 128, 2>(name, a, s)
-                                      : weights_launch<4, 2, 128, 4>(name, a, s);
+            if (f32)
+                rc = p->channels <= 64 ? weights_launch<ProductF32, 2, 1, 64, 1>(name, a, s)
+                                       : weights_launch<ProductF32, 2, 1, 128, 1>(name, a, s);
+            else
+                rc = p->channels <= 64    ? weights_launch<ProductBf16, 4, 1, 64, 2>(name, a, s)
+                     : p->channels <= 128 ? weights_launch<ProductBf16, 4, 1, 128, 2>(name, a, s)
+                                          : weights_launch<ProductBf16, 4, 2, 128, 4>(name, a, s);
             if (rc != PCCNN_OK) return rc;
         }
         const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads), 2);

@@ -4,9 +4,9 @@
 // output channels, so a lane holds runs of four neighboring channels of one point.
 //
 // Operands are bf16 or 8-bit integers whose rows start at multiples of 16 bytes and have whole 16-byte units (zeros behind the
-// last element); whatever is not like that is laid out so first (product_stage_kernel), f32 as three planes of bf16 terms.  A
-// product of f32 operands is then the sum of the six products of planes whose indices add up to at most 2, one after the other
-// over the same accumulators, smallest first.
+// last element); whatever is not like that is laid out so first (product_stage_kernel), f32 as three planes of bf16 terms, whose
+// tiles lie in LDS together: a product of f32 operands is the sum of the six products of planes whose indices add up to at most 2,
+// smallest first.
 #pragma once
 #include "attention_tiles.h"
 
@@ -25,10 +25,6 @@ struct ProductRows {
     int64_t stride, rows, plane, step = 128;
 };
 
-enum { PRODUCT_PAIRS = 6 };                  // f32: products of planes
-// Terms of the pair-th product: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0).
-static inline constexpr int product_term_a(int pair) { return pair == 0 ? 2 : pair == 1 || pair == 3 ? 1 : 0; }
-static inline constexpr int product_term_b(int pair) { return pair == 2 ? 2 : pair == 1 || pair == 4 ? 1 : 0; }
 
 // The tiles of a product in the order of their workgroups: those of a tile of rows one behind the other, runs of 2^run_log2 of them
 // on one XCD, whose L2 then serves the rows.  Numbers come apart by shifts and a multiplication with 2^shift / tiles rounded up
@@ -64,25 +60,37 @@ __device__ __forceinline__ bool product_tile(const ProductGrid &g, uint32_t &row
     return true;
 }
 
-// What a lane's operand of 16 bytes is multiplied as.
+// What operands are multiplied as: TERMS planes, UNIT elements to 16 bytes, UNITS units of a row in LDS at a time.  One plane takes
+// whole lines of L2 (128 bytes); three planes, with six products to a unit, half of them.
 struct ProductBf16 {
     typedef pccnn_f32x16 Acc;
-    typedef float Sum;
-    static constexpr int UNIT = 8;           // elements of a 16-byte unit
-    static __device__ __forceinline__ Acc mma(pccnn_u32x4 a, pccnn_u32x4 b, Acc c)
+    static constexpr int TERMS = 1, UNIT = 8, UNITS = 8;
+    static __device__ __forceinline__ Acc mma(const pccnn_u32x4 (&a)[1], const pccnn_u32x4 (&b)[1], Acc c)
     {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a), __builtin_bit_cast(pccnn_bf16x8, b),
-                                                       c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a[0]),
+                                                       __builtin_bit_cast(pccnn_bf16x8, b[0]), c, 0, 0, 0);
+    }
+};
+struct ProductF32 {
+    typedef pccnn_f32x16 Acc;
+    static constexpr int TERMS = 3, UNIT = 8, UNITS = 4;
+    static __device__ __forceinline__ Acc mma(const pccnn_u32x4 (&a)[3], const pccnn_u32x4 (&b)[3], Acc c)
+    {
+        auto one = [&](int i, int j) {
+            c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pccnn_bf16x8, a[i]),
+                                                        __builtin_bit_cast(pccnn_bf16x8, b[j]), c, 0, 0, 0);
+        };
+        one(2, 0); one(1, 1); one(0, 2); one(1, 0); one(0, 1); one(0, 0);
+        return c;
     }
 };
 struct ProductI8 {
     typedef pccnn_i32x16 Acc;
-    typedef int Sum;
-    static constexpr int UNIT = 16;
-    static __device__ __forceinline__ Acc mma(pccnn_u32x4 a, pccnn_u32x4 b, Acc c)
+    static constexpr int TERMS = 1, UNIT = 16, UNITS = 8;
+    static __device__ __forceinline__ Acc mma(const pccnn_u32x4 (&a)[1], const pccnn_u32x4 (&b)[1], Acc c)
     {
-        return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(pccnn_i32x4, a), __builtin_bit_cast(pccnn_i32x4, b), c,
-                                                     0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(pccnn_i32x4, a[0]), __builtin_bit_cast(pccnn_i32x4, b[0]),
+                                                     c, 0, 0, 0);
     }
 };
 
@@ -102,41 +110,57 @@ __device__ __forceinline__ uint32_t product_split(uint32_t &block, uint32_t by)
     return rest;
 }
 
-// Brings tile after tile of ROWS operand rows, 128 bytes of each (a whole line of L2), into LDS: the inner dimension lies along
-// the rows.
-template <int ROWS, int THREADS> struct RowsFeeder {
-    typedef AttnTile<1, ROWS, 64> Tile;
-    static constexpr int COUNT = ROWS * 8 / THREADS;
-    static_assert(COUNT >= 1 && COUNT * THREADS == ROWS * 8 && THREADS / 8 % 16 == 0, "whole units, the same one in every round");
+// Brings tile after tile of ROWS operand rows, UNITS units of 16 bytes of each, into LDS: the inner dimension lies along the rows.
+// TERMS tiles, one of each plane, one behind the other.
+template <int ROWS, int THREADS, int UNITS, int TERMS> struct RowsFeeder {
+    typedef AttnTile<1, ROWS, 8 * UNITS> Tile;
+    static constexpr int ROUNDS = (ROWS * UNITS + THREADS - 1) / THREADS, COUNT = ROUNDS * TERMS;     // requests of a wavefront
+    static constexpr int ELEMENTS = TERMS * Tile::PLANE;
+    static_assert(THREADS / UNITS % 16 == 0 && ROWS * UNITS % PCCNN_WAVE == 0 && (ROUNDS == 1 || ROUNDS * THREADS == ROWS * UNITS),
+                  "whole wavefronts, the same unit in every round");
     const char *base, *at;                   // the tile's first row, and of it what is asked for next (the same in all lanes)
     int64_t plane, step;
-    uint32_t off[COUNT];                     // the lane's units from there, in bytes
-    int unit;                                // which of a row's eight units the lane brings
-    __device__ __forceinline__ void start(const ProductRows &s, int64_t row, int term)
+    uint32_t off[ROUNDS];                    // the lane's units from there, in bytes
+    int unit;                                // which of a row's units the lane brings
+    bool mine, second;                       // this wavefront brings any (tiles of few rows); UNITS 4: the second half is next
+    __device__ __forceinline__ void start(const ProductRows &s, int64_t row)
     {
-        base = (const char *)s.p + row * s.stride;
+        at = (const char *)s.p + row * s.stride;
         plane = s.plane;
         step = s.step;
-        at = base + term * plane;
-        const int r = (int)threadIdx.x / 8, stride = (int)s.stride, left = (int)min(s.rows - row, (int64_t)ROWS);
-        unit = Tile::unit_at(r, (int)threadIdx.x % 8);
+        second = false;
+        const int r = (int)threadIdx.x / UNITS, stride = (int)s.stride, left = (int)min(s.rows - row, (int64_t)ROWS);
+        unit = Tile::unit_at(r % ROWS, (int)threadIdx.x % UNITS);
+        mine = ROWS * UNITS >= THREADS || __builtin_amdgcn_readfirstlane(threadIdx.x) < ROWS * UNITS;
         const uint32_t first = r * stride + 16 * unit;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
-            off[j] = r + j * (THREADS / 8) < left ? first + j * (THREADS / 8 * stride) : kAttnNowhere;
+        for (int j = 0; j < ROUNDS; ++j)
+            off[j] = r + j * (THREADS / UNITS) < left ? first + j * (THREADS / UNITS * stride) : kAttnNowhere;
     }
-    // The next 128 bytes of every row; `units`: how many of these eight units exist.  A tile comes in ALL requests of a wavefront,
-    // of which this operand's are those from FIRST on; `part`: which half of them.
+    // The next units of every row; `units`: how many of them exist.  A tile comes in ALL requests of a wavefront, of which this
+    // operand's are those from FIRST on; `part`: which half of them.
     template <int FIRST, int ALL> __device__ __forceinline__ void fetch(int part, int units, uint16_t *tile) const
     {
-        const __amdgpu_buffer_rsrc_t window = product_window(at);
+        if (!mine) return;
         const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j)
-            if ((FIRST + j) * 2 / ALL == part)
-                attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + 8 * (j * THREADS + wave_unit));
+        for (int t = 0; t < TERMS; ++t) {
+            const __amdgpu_buffer_rsrc_t window = product_window(at + t * plane);
+#pragma unroll
+            for (int j = 0; j < ROUNDS; ++j)
+                if ((FIRST + t * ROUNDS + j) * 2 / ALL == part)
+                    attn_bring(window, unit < units ? off[j] : kAttnNowhere, tile + t * Tile::PLANE + 8 * (j * THREADS + wave_unit));
+        }
     }
-    __device__ __forceinline__ void next(bool wrap, int term) { at = wrap ? base + term * plane : at + step; }
+    __device__ __forceinline__ void next()
+    {
+        if constexpr (UNITS == 8) {
+            at += step;
+        } else {                             // the other half of 128 bytes, then on
+            at += second ? step - 64 : 64;
+            second = !second;
+        }
+    }
 };
 
 // What this wavefront asked for has landed and its reads of LDS are done; behind the barrier, those of the workgroup.
@@ -151,17 +175,18 @@ __device__ __forceinline__ void product_landed()
 // The product of BM rows of the lane's side with BN rows of the registers' side, both with the inner dimension along the rows.
 // WM x WN wavefronts, each with MT x NT blocks of 32 x 32.  PAIR: the registers' side is BN / 2 rows of one operand and as many
 // of another (gate and up), and the first half of a wavefront's NT blocks is of the first, the second half of the second, of the
-// same channels.  Two tiles of 128 bytes of every row are in LDS, one worked on while the next is brought.
+// same channels.  Two tiles are in LDS, one worked on while the next is brought.
 template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     static constexpr int THREADS = WM * WN * PCCNN_WAVE, MT = BM / WM / 32, NT = BN / WN / 32;
-    static constexpr int STAGE = (BM + BN) * 64;                      // uint16_t
-    static constexpr size_t lds_bytes(int units, int pairs)           // (one tile will do where there is one step)
-    {
-        return (units <= 8 && pairs == 1 ? 1 : 2) * STAGE * sizeof(uint16_t);
-    }
+    static constexpr int TERMS = E::TERMS, UNITS = E::UNITS, STEPS = UNITS / 2;       // products of sixteen bf16 to a tile
     static constexpr int PART = PAIR ? BN / 2 : BN;                   // rows of one operand of the registers' side
-    typedef RowsFeeder<BM, THREADS> FeedM;
-    typedef RowsFeeder<PART, THREADS> FeedN;
+    typedef RowsFeeder<BM, THREADS, UNITS, TERMS> FeedM;
+    typedef RowsFeeder<PART, THREADS, UNITS, TERMS> FeedN;
+    static constexpr int STAGE = FeedM::ELEMENTS + (PAIR ? 2 : 1) * FeedN::ELEMENTS;  // uint16_t
+    static constexpr size_t lds_bytes(int units)                      // (one tile will do where there is one step)
+    {
+        return (units <= UNITS ? 1 : 2) * STAGE * sizeof(uint16_t);
+    }
     typename E::Acc acc[MT][NT];
     int lane, half, wm, wn;
     __device__ __forceinline__ ProductNT()
@@ -188,22 +213,31 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
     template <bool BEGIN, typename ASK> __device__ __forceinline__ void multiply(const uint16_t *tile, ASK ask)
     {
         const typename E::Acc zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        typedef AttnTile<1, BM, 64> Tile;                             // (only the place of a unit in its row, whatever the rows)
-        uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + BM * 64;
+        typedef typename FeedM::Tile TileM;
+        typedef typename FeedN::Tile TileN;
+        uint16_t *const tm = const_cast<uint16_t *>(tile), *const tn = tm + FeedM::ELEMENTS;
         // operands are read a step of products ahead of their use: the compiler, left alone, reads them just before
-        pccnn_u32x4 a[2][NT], b[2][MT];
+        pccnn_u32x4 a[2][NT][TERMS], b[2][MT][TERMS];
         auto read = [&](int kk) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                a[kk & 1][n] = __builtin_bit_cast(pccnn_u32x4, Tile{tn}.rows(col_of(n) + (lane & 31), 2 * kk + half).t[0]);
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) {
+                    const int col = col_of(n), which = col / PART;    // gate or up: one behind the other, each with its planes
+                    a[kk & 1][n][t] = __builtin_bit_cast(
+                        pccnn_u32x4, TileN{tn + (which * TERMS + t) * TileN::PLANE}.rows(col % PART + (lane & 31), 2 * kk + half).t[0]);
+                }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                b[kk & 1][m] = __builtin_bit_cast(pccnn_u32x4, Tile{tm}.rows(row_of(m), 2 * kk + half).t[0]);
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t)
+                    b[kk & 1][m][t] =
+                        __builtin_bit_cast(pccnn_u32x4, TileM{tm + t * TileM::PLANE}.rows(row_of(m), 2 * kk + half).t[0]);
         };
         read(0);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            if (kk < 3) read(kk + 1);
+        for (int kk = 0; kk < STEPS; ++kk) {
+            if (kk + 1 < STEPS) read(kk + 1);
             __builtin_amdgcn_sched_barrier(0x6);                      // VALU and SALU may cross
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -218,30 +252,28 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             __builtin_amdgcn_sched_barrier(0x6);
         }
     }
-    // Rows from `row` of `x`, rows from `col` of `one` (and `two`); `units`: 16-byte units of every row; `pairs`: 1, or
-    // PRODUCT_PAIRS for planes of terms.
+    // Rows from `row` of `x`, rows from `col` of `one` (and `two`); `units`: 16-byte units of every row, at least one.
     __device__ __forceinline__ void run(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two,
-                                        int64_t col, int units, int pairs, uint16_t *lds)
+                                        int64_t col, int units, uint16_t *lds)
     {
         FeedM fm;
         FeedN f1, f2;
-        int pair = pairs == 1 ? PRODUCT_PAIRS - 1 : 0, left = units;  // of the tile that is asked for next
-        fm.start(x, row, product_term_b(pair));
-        f1.start(one, col, product_term_a(pair));
-        if constexpr (PAIR) f2.start(two, col, product_term_a(pair));
-        const int total = (units + 7) / 8 * pairs;
+        fm.start(x, row);
+        f1.start(one, col);
+        if constexpr (PAIR) f2.start(two, col);
+        int left = units;                                             // of the tile that is asked for next
+        const int total = (units + UNITS - 1) / UNITS;
         constexpr int ALL = FeedM::COUNT + (PAIR ? 2 : 1) * FeedN::COUNT;
         auto fetch = [&](int part, uint16_t *to) {
             fm.template fetch<0, ALL>(part, left, to);
-            f1.template fetch<FeedM::COUNT, ALL>(part, left, to + BM * 64);
-            if constexpr (PAIR) f2.template fetch<FeedM::COUNT + FeedN::COUNT, ALL>(part, left, to + (BM + PART) * 64);
+            f1.template fetch<FeedM::COUNT, ALL>(part, left, to + FeedM::ELEMENTS);
+            if constexpr (PAIR)
+                f2.template fetch<FeedM::COUNT + FeedN::COUNT, ALL>(part, left, to + FeedM::ELEMENTS + FeedN::ELEMENTS);
             if (part == 0) return;
-            left -= 8;
-            const bool wrap = left <= 0;
-            if (wrap) left = units, ++pair;
-            fm.next(wrap, product_term_b(pair));
-            f1.next(wrap, product_term_a(pair));
-            if constexpr (PAIR) f2.next(wrap, product_term_a(pair));
+            left -= UNITS;
+            fm.next();
+            f1.next();
+            if constexpr (PAIR) f2.next();
         };
         fetch(0, lds);
         fetch(1, lds);
@@ -509,11 +541,13 @@ template <typename T> static __global__ __launch_bounds__(256) void product_stag
 
 // ---------------------------------------------------------------------------------------------- launches
 //
-// Whether a product takes tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128.
-static inline bool product_large(int64_t rows, int64_t cols, int units, int pairs)
+// Whether a product takes tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128, and 64 x 64 ones
+// where those leave compute units without work.
+static inline bool product_large(int64_t rows, int64_t cols, int units)
 {
-    return cols >= 256 && units * pairs >= 32 && pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256) >= 256;
+    return cols >= 256 && units >= 32 && pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256) >= 256;
 }
+static inline bool product_small(int64_t rows, int64_t cols) { return pccnn_ceil_div(rows, 128) * pccnn_ceil_div(cols, 128) < 256; }
 template <typename KERNEL, typename ARGS>
 static int product_launch(const char *name, KERNEL kernel, size_t lds, int threads, ARGS &a, int64_t tiles_m, int64_t tiles_n, hipStream_t s)
 {
