@@ -353,7 +353,12 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
         const T *from = base + r0 * COLS + PER * place(r0, unit);
         T *at = to.at(row0 + r0, col);
         const int64_t step = EVERY * to.row_step();
-        if (to.whole() && width % PER == 0) {
+        if (to.lines()) {                    // whole lines that no kernel of the call reads again: past the caches (see below)
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j, at += step)
+                if (r0 + j * EVERY < left)
+                    __builtin_nontemporal_store(*(const pccnn_u32x4 *)(from + j * EVERY * COLS), (pccnn_u32x4 *)at);
+        } else if (to.whole() && width % PER == 0) {
 #pragma unroll
             for (int j = 0; j < COUNT; ++j, at += step)
                 if (r0 + j * EVERY < left) *(pccnn_u32x4 *)at = *(const pccnn_u32x4 *)(from + j * EVERY * COLS);
@@ -366,13 +371,16 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
         }
     }
 };
-// Where a unit of a result lies: rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what
+// Where a unit of a result lies, and whether it goes past the caches.  Results whose rows are whole lines do (800000 x 64 -> 256
+// 159 -> 144 us, 34123 x 512 -> 1408 in 8 bits 86 -> 79); partial lines do not (34123 x 1000 f32 49 -> 54), nor does what the next
+// kernels read (training 8192 x 512 -> 1408 174 -> 182, 400000 x 64 -> 176 341 -> 368; 65536 x 512 -> 1408 832 -> 823).  Rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what
 // a tile of rows takes of one piece lies together (65536 x 2816 x 512: 167 us, with rows in one piece 196; 65536 x 512 under 2816
 // columns, the inner dimension over the rows, 191 and 219).
 template <typename T> struct DenseRow {
     T *p;
     int64_t stride;
     __device__ __forceinline__ bool whole() const { return stride * (int)sizeof(T) % 16 == 0; }
+    __device__ __forceinline__ bool lines() const { return stride * (int)sizeof(T) % 128 == 0; }
     __device__ __forceinline__ int64_t row_step() const { return stride; }
     __device__ __forceinline__ T *at(int64_t row, int64_t col) const { return p + row * stride + col; }
 };
@@ -380,6 +388,7 @@ template <typename T> struct PieceRow {
     T *p;
     int64_t rows, from;                      // `from`: the column of all pieces that column 0 is
     __device__ __forceinline__ bool whole() const { return true; }
+    __device__ __forceinline__ bool lines() const { return false; }  // (the next kernels read it)
     __device__ __forceinline__ int64_t row_step() const { return 64; }
     __device__ __forceinline__ T *at(int64_t row, int64_t col) const
     {
