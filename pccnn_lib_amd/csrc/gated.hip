@@ -247,9 +247,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_ker
     for (int j = 0; j < 64 * 64 / kThreads; ++j) {
         const int i = threadIdx.x + j * kThreads;
         const int64_t h = h0 + i / 64, c = c0 + i % 64;
-        float v[1] = {0.0f};
-        if (h < a.hidden && c < a.channels) pccnn_load<1>(from + h * stride + c, v);
-        tile[i / 64][i % 64] = v[0];
+        float v[1];                          // (loaded unasked, so that all loads are on their way at once)
+        pccnn_load<1>(from + min(h, a.hidden - 1) * stride + min(c, a.channels - 1), v);
+        tile[i / 64][i % 64] = h < a.hidden && c < a.channels ? v[0] : 0.0f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 8; i += kThreads) {
@@ -488,21 +488,25 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
             }
     }
 }
-// Sum of the parts, in their order, into the two gradients.
-template <typename T>
+// Sum of the parts, in their order, into the two gradients, VEC values to a thread.
+template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void gated_weights_sum_kernel(const float *__restrict__ part, int splits, int64_t hidden,
                                                                     int64_t padded, int64_t channels, T *__restrict__ d_gate,
                                                                     T *__restrict__ d_up)
 {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (i >= hidden * channels) return;
     const float *from = part + (blockIdx.y ? padded * channels : 0) + i;
     const int64_t step = 2 * padded * channels;
-    float sum = 0.0f;
+    float sum[VEC] = {};
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) sum += from[s * step];
-    const float v[1] = {sum};
-    pccnn_store<1>((blockIdx.y ? d_up : d_gate) + i, v);
+    for (int s = 0; s < splits; ++s) {
+        float v[VEC];
+        pccnn_load<VEC>(from + s * step, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += v[e];
+    }
+    pccnn_store<VEC>((blockIdx.y ? d_up : d_gate) + i, sum);
 }
 
 // ------------------------------------------------------------------------------------------- host
@@ -817,13 +821,18 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
                                           : weights_launch<ProductBf16, 4, 2, 128, 4>(name, a, s);
             if (rc != PCCNN_OK) return rc;
         }
-        const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads), 2);
+        auto sum = [&](auto zero, auto vec) {
+            using T = decltype(zero);
+            constexpr int VEC = decltype(vec)::value;
+            const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads * VEC), 2);
+            gated_weights_sum_kernel<T, VEC><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
+                                                                      (T *)d_gate, (T *)d_up);
+        };
+        const bool wide = p->channels % 4 == 0;
         if (f32)
-            gated_weights_sum_kernel<float><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
-                                                                     (float *)d_gate, (float *)d_up);
+            wide ? sum(0.0f, std::integral_constant<int, 4>()) : sum(0.0f, std::integral_constant<int, 1>());
         else
-            gated_weights_sum_kernel<uint16_t><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
-                                                                        (uint16_t *)d_gate, (uint16_t *)d_up);
+            wide ? sum((uint16_t)0, std::integral_constant<int, 4>()) : sum((uint16_t)0, std::integral_constant<int, 1>());
         PCCNN_LAUNCH_CHECK();
     }
     return PCCNN_OK;

@@ -373,9 +373,10 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
 };
 // Where a unit of a result lies, and whether it goes past the caches.  Results whose rows are whole lines do (800000 x 64 -> 256
 // 159 -> 144 us, 34123 x 512 -> 1408 in 8 bits 86 -> 79); partial lines do not (34123 x 1000 f32 49 -> 54), nor does what the next
-// kernels read (training 8192 x 512 -> 1408 174 -> 182, 400000 x 64 -> 176 341 -> 368; 65536 x 512 -> 1408 832 -> 823).  Rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what
-// a tile of rows takes of one piece lies together (65536 x 2816 x 512: 167 us, with rows in one piece 196; 65536 x 512 under 2816
-// columns, the inner dimension over the rows, 191 and 219).
+// kernels read (training 8192 x 512 -> 1408 174 -> 182, 400000 x 64 -> 176 341 -> 368; 65536 x 512 -> 1408 832 -> 823).
+// Rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what a tile of rows takes of one
+// piece lies together (65536 x 2816 x 512: 167 us, with rows in one piece 196; 65536 x 512 under 2816 columns, the inner
+// dimension over the rows, 191 and 219).
 template <typename T> struct DenseRow {
     T *p;
     int64_t stride;
