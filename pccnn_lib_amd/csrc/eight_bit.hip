@@ -8,7 +8,7 @@
 
 namespace {
 
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;                 // rows that need no tiles (1408 x 512: 17, 32, 33 and 64 rows 5.2, 5.8, 6.8 and 8.6 us, in tiles 6.2)
 constexpr int64_t kMostWidth = 1 << 20;
 
 struct LinearArgs {
@@ -108,14 +108,17 @@ template <typename OUT> int linear_few(const LinearFew &a, hipStream_t s)
     const unsigned blocks = (unsigned)pccnn_ceil_div(a.outer, 16);
     if (a.n <= 16)
         linear_i8_few_kernel<OUT, 1, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
-    else if (a.n <= 32)
-        linear_i8_few_kernel<OUT, 2, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
     else
-        linear_i8_few_kernel<OUT, 4, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
+        linear_i8_few_kernel<OUT, 2, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
 }
 
+// How wide rows of 8-bit values can be loaded (few_load).
+int linear_wide(const void *p, int64_t inner)
+{
+    return inner % 16 == 0 && (uintptr_t)p % 16 == 0 ? 2 : inner % 4 == 0 && (uintptr_t)p % 4 == 0 ? 1 : 0;
+}
 // Whether a call lays its rows (which = 0) or weights (1) out anew: rows that are not whole 16-byte units.
 bool linear_staged(const void *p, int64_t n, int64_t inner) { return n > kFewRows && (inner % 16 != 0 || (uintptr_t)p % 16 != 0); }
 bool linear_sizes_ok(int64_t n, int64_t inner, int64_t outer)
@@ -150,9 +153,7 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
     PCCNN_REQUIRE((uintptr_t)out % 16 == 0, PCCNN_ERR_INVALID, "%s: a result that is not 16-byte aligned", name);
     const hipStream_t s = (hipStream_t)stream;
     if (n <= kFewRows) {
-        const int wide_x = inner % 16 == 0 && (uintptr_t)codes % 16 == 0 ? 2 : 0;
-        const int wide_w = inner % 16 == 0 && (uintptr_t)weights % 16 == 0 ? 2 : 0;
-        const LinearFew a = {{codes, inner, wide_x}, {{weights, inner, wide_w}}, n, outer, inner, scales, weight_scales, bias, out};
+        const LinearFew a = {{codes, inner, linear_wide(codes, inner)}, {{weights, inner, linear_wide(weights, inner)}}, n, outer, inner, scales, weight_scales, bias, out};
         return out_type == PCCNN_TYPE_F32 ? linear_few<float>(a, s) : linear_few<uint16_t>(a, s);
     }
     const int units = (int)pccnn_ceil_div(inner, 16);
@@ -167,7 +168,7 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
         if (!linear_staged(r->p, n, inner)) continue;
         void *to = arena.take<char>((size_t)r->rows * units * 16);
         PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
-        stage.s[count++] = {r->p, inner, r->rows, 0, to};
+        stage.s[count++] = {r->p, inner, r->rows, linear_wide(r->p, inner), to};
         most = std::max(most, r->rows * units);
         r->p = to;
         r->stride = (int64_t)units * 16;

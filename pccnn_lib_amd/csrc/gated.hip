@@ -13,7 +13,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMostWidth = 1 << 20;      // channels and hidden channels: a tile's rows stay within 32-bit offsets
-constexpr int kFewRows = 64;
+// Rows that need no tiles: up to 32 (512 -> 1408 in bf16, 17, 32, 33 and 64 rows 5.3, 5.5, 6.9 and 7.5 us, in tiles 5.6; in 8 bits 5.2,
+// 5.5, 6.8 and 8.0 against 5.0), up to 64 of f32, whose operands are laid out for tiles (8.5 to 12.4 against 22).
+constexpr int few_rows(int type) { return type == PCCNN_TYPE_F32 ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------------- activations
 
@@ -516,7 +518,7 @@ int wide_of(const void *p, int64_t stride, int64_t width, int type)
 {
     const int bytes = type == PCCNN_TYPE_I8 ? 1 : pccnn_type_bytes(type);
     const bool whole = (uintptr_t)p % 16 == 0 && stride * bytes % 16 == 0;
-    if (type == PCCNN_TYPE_I8) return whole && width % 16 == 0 ? 2 : 0;
+    if (type == PCCNN_TYPE_I8) return whole && width % 16 == 0 ? 2 : (uintptr_t)p % 4 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
     if (type == PCCNN_TYPE_F32) return whole && width % 4 == 0 ? 2 : 0;
     if (whole && width % 8 == 0) return 2;
     return (uintptr_t)p % 8 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
@@ -565,7 +567,7 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     const int64_t unit = unit_of(p->type);
     plan.units = pccnn_ceil_div(p->channels, unit);
     plan.planes = p->type == PCCNN_TYPE_F32 ? 3 : 1;
-    plan.few = !backward && p->n <= kFewRows;
+    plan.few = !backward && p->n <= few_rows(p->type);
     plan.p[0] = p->feats, plan.p[1] = p->gate, plan.p[2] = p->up;
     plan.stride[0] = p->feats_stride, plan.stride[1] = p->gate_stride, plan.stride[2] = p->up_stride;
     plan.rows[0] = p->n, plan.rows[1] = plan.rows[2] = p->hidden;
@@ -679,7 +681,7 @@ template <typename T, typename OUT> int few_launch(GatedFew &a, hipStream_t s)
         gated_few_kernel<T, OUT, 1, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
     else if (a.n <= 32)
         gated_few_kernel<T, OUT, 2, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
-    else
+    else if constexpr (std::is_same<T, float>::value)
         gated_few_kernel<T, OUT, 4, WAVES><<<blocks, WAVES * PCCNN_WAVE, 0, s>>>(a);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;

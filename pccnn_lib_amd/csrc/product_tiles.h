@@ -412,7 +412,7 @@ template <int COUNT, int COLS, int THREADS> struct ProductChannels {
 
 // ---------------------------------------------------------------------------------------------- few rows
 //
-// Up to 64 rows: no tile is shared by enough of them to be worth LDS.  A workgroup has sixteen output channels (of one or two
+// Few rows (32 or 64 at most): no tile is shared by enough of them to be worth LDS.  A workgroup has sixteen output channels (of one or two
 // operands); its wavefronts deal the inner dimension among themselves in steps of 64 bytes, take weights and rows from memory
 // straight into operands of 16 x 16 products, and add their sums in LDS in a fixed order.
 template <typename T> struct FewStep;                                // elements of a lane's operand, of a step of four lanes
@@ -430,6 +430,10 @@ template <typename T> __device__ __forceinline__ FewFrag<FewStep<T>::TERMS> few_
         if (col < width) {
             if (wide == 2) {
                 f.t[0] = *(const pccnn_u32x4 *)(row + col);
+            } else if (wide == 1) {          // (rows of whole four bytes)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + 4 * i < width) f.t[0][i] = *(const uint32_t *)(row + col + 4 * i);
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)

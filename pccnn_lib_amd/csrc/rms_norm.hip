@@ -17,7 +17,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
-constexpr int kMaxBlocks = 2048;
+constexpr int kMaxBlocks = 1536;             // six workgroups to a compute unit: all at once, whatever the registers (800000 x 128 in 8 bits
+                                             // 171 -> 153 us, 65536 x 512 51 -> 46; eight to a unit, of which seven fit, wait for the last)
 constexpr int kBackBlocks = 512;
 constexpr int kMostValues = 32, kMostLoads = 16;       // of a lane: values of a row, loads they take
 
