@@ -8,7 +8,8 @@
 
 namespace {
 
-constexpr int kFewRows = 32;                 // rows that need no tiles (1408 x 512: 17, 32, 33 and 64 rows 5.2, 5.8, 6.8 and 8.6 us, in tiles 6.2)
+// Rows that need no tiles (1408 x 512: 17, 32, 33 and 64 rows 5.2, 5.8, 6.8 and 8.6 us, in tiles 6.2).
+constexpr int kFewRows = 32;
 constexpr int64_t kMostWidth = 1 << 20;
 
 struct LinearArgs {
@@ -93,12 +94,13 @@ template <typename T, int BM, int BN, int WM, int WN> int linear_launch(LinearAr
     typedef ProductNT<ProductI8, BM, BN, WM, WN, false> Product;
     a.lds = std::max(Product::lds_bytes(a.units), (size_t)BM * BN * sizeof(T));
     return product_launch("linear_8bit", linear_i8_kernel<T, BM, BN, WM, WN>,
-                          a.lds + ProductChannels<2, BN, Product::THREADS>::BYTES, Product::THREADS, a, pccnn_ceil_div(a.n, BM), pccnn_ceil_div(a.outer, BN), s);
+                          a.lds + ProductChannels<2, BN, Product::THREADS>::BYTES, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
+                          pccnn_ceil_div(a.outer, BN), s);
 }
 template <typename T> int linear_tiles(LinearArgs &a, hipStream_t s)
 {
     if constexpr (!std::is_same<T, float>::value)
-        if (product_large(a.n, a.outer, a.units)) return linear_launch<T, 256, 256, 2, 4>(a, s);
+        if (product_large(a.n, a.outer, (int64_t)a.units * 16)) return linear_launch<T, 256, 256, 2, 4>(a, s);
     if (product_small(a.n, a.outer)) return linear_launch<T, 64, 64, 2, 2>(a, s);
     return a.outer <= 64 ? linear_launch<T, 128, 64, 4, 1>(a, s) : linear_launch<T, 128, 128, 2, 2>(a, s);
 }
@@ -153,7 +155,8 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
     PCCNN_REQUIRE((uintptr_t)out % 16 == 0, PCCNN_ERR_INVALID, "%s: a result that is not 16-byte aligned", name);
     const hipStream_t s = (hipStream_t)stream;
     if (n <= kFewRows) {
-        const LinearFew a = {{codes, inner, linear_wide(codes, inner)}, {{weights, inner, linear_wide(weights, inner)}}, n, outer, inner, scales, weight_scales, bias, out};
+        const LinearFew a = {{codes, inner, linear_wide(codes, inner)}, {{weights, inner, linear_wide(weights, inner)}}, n,
+                             outer, inner, scales, weight_scales, bias, out};
         return out_type == PCCNN_TYPE_F32 ? linear_few<float>(a, s) : linear_few<uint16_t>(a, s);
     }
     const int units = (int)pccnn_ceil_div(inner, 16);

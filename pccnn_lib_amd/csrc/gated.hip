@@ -13,8 +13,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMostWidth = 1 << 20;      // channels and hidden channels: a tile's rows stay within 32-bit offsets
-// Rows that need no tiles: up to 32 (512 -> 1408 in bf16, 17, 32, 33 and 64 rows 5.3, 5.5, 6.9 and 7.5 us, in tiles 5.6; in 8 bits 5.2,
-// 5.5, 6.8 and 8.0 against 5.0), up to 64 of f32, whose operands are laid out for tiles (8.5 to 12.4 against 22).
+// Rows that need no tiles: up to 32 (512 -> 1408 in bf16, 17, 32, 33 and 64 rows 5.3, 5.5, 6.9 and 7.5 us, in tiles 5.6; in 8 bits
+// 5.2, 5.5, 6.8 and 8.0 against 5.0), up to 64 of f32, whose operands are laid out for tiles (8.5 to 12.4 against 22).
 constexpr int few_rows(int type) { return type == PCCNN_TYPE_F32 ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------------- activations
@@ -518,7 +518,8 @@ int wide_of(const void *p, int64_t stride, int64_t width, int type)
 {
     const int bytes = type == PCCNN_TYPE_I8 ? 1 : pccnn_type_bytes(type);
     const bool whole = (uintptr_t)p % 16 == 0 && stride * bytes % 16 == 0;
-    if (type == PCCNN_TYPE_I8) return whole && width % 16 == 0 ? 2 : (uintptr_t)p % 4 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
+    if (type == PCCNN_TYPE_I8)
+        return whole && width % 16 == 0 ? 2 : (uintptr_t)p % 4 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
     if (type == PCCNN_TYPE_F32) return whole && width % 4 == 0 ? 2 : 0;
     if (whole && width % 8 == 0) return 2;
     return (uintptr_t)p % 8 == 0 && stride % 4 == 0 && width % 4 == 0 ? 1 : 0;
@@ -636,7 +637,8 @@ template <class E, typename T, bool BACK> int gated_launch(const char *name, Gat
     if constexpr (std::is_same<E, ProductF32>::value) {
         return gated_launch_tile<E, T, BACK, 128, 128, 4, 2>(name, a, s);
     } else {
-        if (product_large(a.n, 2 * a.hidden, a.units)) return gated_launch_tile<E, T, BACK, 256, 256, 4, 2>(name, a, s);
+        if (product_large(a.n, 2 * a.hidden, (int64_t)a.units * E::UNIT))
+            return gated_launch_tile<E, T, BACK, 256, 256, 4, 2>(name, a, s);
         return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
     }
 }
@@ -653,17 +655,16 @@ template <typename T> int dx_launch(const char *name, BackArgs &a, hipStream_t s
     if constexpr (std::is_same<T, float>::value) {
         return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 2>(name, a, s) : dx_launch<T, 128, 128, 4, 2>(name, a, s);
     } else {
-        if (product_large(a.n, a.cols, a.units)) return dx_launch<T, 256, 256, 4, 2>(name, a, s);
+        if (product_large(a.n, a.cols, (int64_t)a.units * 8)) return dx_launch<T, 256, 256, 4, 2>(name, a, s);
         return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 1>(name, a, s) : dx_launch<T, 128, 128, 2, 2>(name, a, s);
     }
 }
 
 // A part's tiles go to one XCD as far as they may: they read the same rows, and its L2 serves them once.
-template <class E, int DP, int XP, int XT, int MT> int weights_launch(const char *name, WeightsArgs &a, hipStream_t s)
+template <class E, int DP, int XP, int XT, int MT> int weights_launch(WeightsArgs &a, hipStream_t s)
 {
     typedef WeightsShape<E, DP, XP, XT, MT> Shape;
     a.blocks = (int64_t)a.tiles_x * a.tiles_d * a.splits;
-    PCCNN_REQUIRE(a.blocks <= INT32_MAX / 2, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)a.blocks);
     a.run = (int)pccnn_ceil_div(a.blocks, PCCNN_XCDS);
     const auto kernel = gated_weights_kernel<E, DP, XP, XT, MT>;
     if (Shape::LDS > 65536)
@@ -759,6 +760,8 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
     if (rc != PCCNN_OK) return rc;
     PCCNN_REQUIRE(p->type != PCCNN_TYPE_I8, PCCNN_ERR_UNSUPPORTED, "%s: 8-bit operands have no gradients", name);
     PCCNN_REQUIRE(grads_stride >= 0, PCCNN_ERR_INVALID, "%s: gradient rows %lld apart", name, (long long)grads_stride);
+    PCCNN_REQUIRE(p->hidden * p->channels <= INT32_MAX, PCCNN_ERR_UNSUPPORTED, "%s: weights of %lld x %lld (2^31 - 1 values at most)",
+                  name, (long long)p->hidden, (long long)p->channels);
     PCCNN_REQUIRE((d_gate != nullptr) == (d_up != nullptr), PCCNN_ERR_INVALID, "%s: the gradients of both weights come together",
                   name);
     if (d_gate == nullptr && (d_feats == nullptr || p->n == 0)) return PCCNN_OK;
@@ -815,12 +818,12 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
             a.tiles_x = plan.tiles_x, a.tiles_d = plan.tiles_d, a.splits = splits = plan.splits, a.per_split = plan.per_split;
             a.part = part, a.channels = p->channels;
             if (f32)
-                rc = p->channels <= 64 ? weights_launch<ProductF32, 2, 1, 64, 1>(name, a, s)
-                                       : weights_launch<ProductF32, 2, 1, 128, 1>(name, a, s);
+                rc = p->channels <= 64 ? weights_launch<ProductF32, 2, 1, 64, 1>(a, s)
+                                       : weights_launch<ProductF32, 2, 1, 128, 1>(a, s);
             else
-                rc = p->channels <= 64    ? weights_launch<ProductBf16, 4, 1, 64, 2>(name, a, s)
-                     : p->channels <= 128 ? weights_launch<ProductBf16, 4, 1, 128, 2>(name, a, s)
-                                          : weights_launch<ProductBf16, 4, 2, 128, 4>(name, a, s);
+                rc = p->channels <= 64    ? weights_launch<ProductBf16, 4, 1, 64, 2>(a, s)
+                     : p->channels <= 128 ? weights_launch<ProductBf16, 4, 1, 128, 2>(a, s)
+                                          : weights_launch<ProductBf16, 4, 2, 128, 4>(a, s);
             if (rc != PCCNN_OK) return rc;
         }
         auto sum = [&](auto zero, auto vec) {

@@ -25,7 +25,6 @@ struct ProductRows {
     int64_t stride, rows, plane, step = 128;
 };
 
-
 // The tiles of a product in the order of their workgroups: those of a tile of rows one behind the other, runs of 2^run_log2 of them
 // on one XCD, whose L2 then serves the rows.  Numbers come apart by shifts and a multiplication with 2^shift / tiles rounded up
 // (exact below 2^31): the divisions themselves were a hundred instructions, as much as six results of a gelu.
@@ -412,8 +411,8 @@ template <int COUNT, int COLS, int THREADS> struct ProductChannels {
 
 // ---------------------------------------------------------------------------------------------- few rows
 //
-// Few rows (32 or 64 at most): no tile is shared by enough of them to be worth LDS.  A workgroup has sixteen output channels (of one or two
-// operands); its wavefronts deal the inner dimension among themselves in steps of 64 bytes, take weights and rows from memory
+// Few rows (32 or 64 at most): no tile is shared by enough of them to be worth LDS.  A workgroup has sixteen output channels (of one
+// or two operands); its wavefronts deal the inner dimension among themselves in steps of 64 bytes, take weights and rows from memory
 // straight into operands of 16 x 16 products, and add their sums in LDS in a fixed order.
 template <typename T> struct FewStep;                                // elements of a lane's operand, of a step of four lanes
 template <> struct FewStep<uint16_t> { static constexpr int UNIT = 8, TERMS = 1; typedef pccnn_f32x4 Acc; typedef float Sum; };
@@ -555,17 +554,25 @@ template <typename T> static __global__ __launch_bounds__(256) void product_stag
 
 // ---------------------------------------------------------------------------------------------- launches
 //
-// Whether a product takes tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128, and 64 x 64 ones
-// where those leave compute units without work.
-static inline bool product_large(int64_t rows, int64_t cols, int units)
+// Tiles of 256 x 256 (one workgroup of eight wavefronts to a CU) rather than 128 x 128: for sums of 512 terms and more where the
+// last round of workgroups leaves no more than 15 % of all rounds idle.  Gated maps in us, 256 x 256 against 128 x 128:
+// 32000 x 512 -> 1408 bf16 102 : 108, in 8 bits 79 : 82; 8000 x 1024 -> 2800 (0.92 of the rounds filled) 99 : 111, 8 bits 68 : 72;
+// not for 8000 x 512 -> 1408 (0.69 of them) 34 : 30, 8 bits 27 : 22, nor for 256 terms, 32000 x 256 -> 704 36 : 34.
+static inline bool product_large(int64_t rows, int64_t cols, int64_t depth)
 {
-    return cols >= 256 && units >= 32 && pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256) >= 256;
+    const int64_t tiles = pccnn_ceil_div(rows, 256) * pccnn_ceil_div(cols, 256);
+    return depth >= 512 && cols >= 256 && tiles * 20 >= pccnn_ceil_div(tiles, 256) * 256 * 17;
 }
-static inline bool product_small(int64_t rows, int64_t cols) { return pccnn_ceil_div(rows, 128) * pccnn_ceil_div(cols, 128) < 256; }
+// Tiles of 64 x 64 rather than 128 x 128 where those leave compute units without work.  In us, 64 x 64 against 128 x 128: 88 tiles
+// of 128 (1000 x 256 -> 704) bf16 5.1 : 5.6, 8 bits 5.0 : 5.7, f32 18.2 : 20.3; 176 of them (1000 x 512 -> 1408) 9.1 : 8.1,
+// 6.8 : 6.9, 51 : 36; 192 (4000 x 128 -> 344) 5.2 : 5.2, 5.1 : 5.5, 15.5 : 15.1.
+static inline bool product_small(int64_t rows, int64_t cols) { return pccnn_ceil_div(rows, 128) * pccnn_ceil_div(cols, 128) < 160; }
 template <typename KERNEL, typename ARGS>
-static int product_launch(const char *name, KERNEL kernel, size_t lds, int threads, ARGS &a, int64_t tiles_m, int64_t tiles_n, hipStream_t s)
+static int product_launch(const char *name, KERNEL kernel, size_t lds, int threads, ARGS &a, int64_t tiles_m, int64_t tiles_n,
+                          hipStream_t s)
 {
-    PCCNN_REQUIRE(tiles_m * tiles_n <= INT32_MAX - 1024, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name,
+    // (a launch has less than 2^32 threads)
+    PCCNN_REQUIRE(tiles_m * tiles_n <= (int64_t)UINT32_MAX / threads - 1024, PCCNN_ERR_UNSUPPORTED, "%s: %lld workgroups", name,
                   (long long)(tiles_m * tiles_n));
     a.grid = product_grid(tiles_m, tiles_n);
     if (lds > 65536)

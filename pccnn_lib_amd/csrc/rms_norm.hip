@@ -17,8 +17,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / PCCNN_WAVE;
-constexpr int kMaxBlocks = 1536;             // six workgroups to a compute unit: all at once, whatever the registers (800000 x 128 in 8 bits
-                                             // 171 -> 153 us, 65536 x 512 51 -> 46; eight to a unit, of which seven fit, wait for the last)
+// Six workgroups to a compute unit are there all at once, whatever the registers; of 2048, seven to a unit fit and the rest wait
+// (800000 x 128 in 8 bits 153 us, with 2048 171; 65536 x 512 46 and 51).
+constexpr int kMaxBlocks = 1536;
 constexpr int kBackBlocks = 512;
 constexpr int kMostValues = 32, kMostLoads = 16;       // of a lane: values of a row, loads they take
 
@@ -63,7 +64,7 @@ template <typename AGAIN> __device__ __forceinline__ float rstd_of(float squares
 {
     if (__any(!(squares <= FLT_MAX))) {
         const float scaled = again();
-        if (!(squares <= FLT_MAX)) return scaled == scaled && scaled <= FLT_MAX ? kShrink / sqrtf(scaled * inv_c) : scaled != scaled ? scaled : 0.0f;
+        if (!(squares <= FLT_MAX)) return scaled <= FLT_MAX ? kShrink / sqrtf(scaled * inv_c) : scaled != scaled ? scaled : 0.0f;
     }
     return 1.0f / sqrtf(squares * inv_c + eps);
 }

@@ -105,6 +105,20 @@ def test_gated_entry_points_refuse_bad_arguments(lib):
     assert backward() == -3 and backward(dx=None, dg=None, du=None) == 0 and backward(n=0, dg=None, du=None) == 0
 
 
+def test_gated_gradients_refuse_weights_of_more_values_than_a_launch_has(lib):
+    def backward(channels, hidden):
+        p = _problem(channels=channels, hidden=hidden, feats_stride=channels, gate_stride=channels, up_stride=channels)
+        return lib.pccnn_gated_backward(ctypes.byref(p), 16, hidden, 16, 16, 16, None, 0, None)
+    assert backward(1 << 16, 1 << 15) == -2 and b"65536 (2^31 - 1" in lib.pccnn_last_error()
+    assert backward((1 << 16) - 1, 1 << 15) == -3
+
+
+def test_products_refuse_more_workgroups_than_a_launch_has(lib):
+    # 2^24 tiles of 128 rows, 256 threads each
+    out = lib.pccnn_linear_8bit(SOME, SOME, SOME, SOME, None, (1 << 31) - 1, 16, 16, SOME, 0, None, 0, None)
+    assert out == -2 and b"16777216 workgroups" in lib.pccnn_last_error()
+
+
 def test_gated_workspace_covers_what_is_laid_out(lib):
     size = lambda backward=0, **changes: lib.pccnn_gated_workspace_bytes(ctypes.byref(_problem(**changes)), backward)  # noqa: E731
     assert size() == 256 and size(n=5, type=0) == 256
