@@ -177,8 +177,7 @@ extern "C" int pccnn_linear_8bit(const int8_t *codes, const float *scales, const
         r->stride = (int64_t)units * 16;
     }
     if (count > 0) {
-        const dim3 grid((unsigned)std::min<int64_t>(pccnn_ceil_div(most, 256), 8192), (unsigned)count);
-        product_stage_kernel<int8_t><<<grid, 256, 0, s>>>(stage);
+        product_stage_kernel<int8_t><<<dim3(product_stage_blocks(most), (unsigned)count), 256, 0, s>>>(stage);
         PCCNN_LAUNCH_CHECK();
     }
     return out_type == PCCNN_TYPE_F32 ? linear_tiles<float>(a, s) : linear_tiles<uint16_t>(a, s);

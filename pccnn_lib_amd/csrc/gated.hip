@@ -233,18 +233,30 @@ __global__ __launch_bounds__(WAVES *PCCNN_WAVE) void gated_few_kernel(GatedFew a
 // ------------------------------------------------------------------------------------------- backward products
 
 // Both weights one below the other and turned: row c of the result is (Wg[:, c] | Wu[:, c]), each padded to whole units with
-// zeros.  f32: three planes of terms.
-template <typename T> struct TurnArgs {
-    const T *gate, *up;
+// zeros.  f32: three planes of terms.  In one launch with the operands that are laid out anew (f32 training 3885 x 96 -> 256 57
+// us, in two launches 62).
+struct TurnArgs {
+    const void *gate, *up;
     int64_t gate_stride, up_stride, hidden, channels, padded;
     uint16_t *to;
+    uint32_t tiles_c, blocks;                // tiles of 64 channels; workgroups that turn (both weights'), the first of the launch
+    uint32_t stage_blocks;                   // and those behind them for each operand
 };
-template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_kernel(TurnArgs<T> a)
+template <typename T> __global__ __launch_bounds__(kThreads) void gated_prepare_kernel(TurnArgs a, StageArgs stage)
 {
     __shared__ float tile[64][65];
-    const int64_t c0 = (int64_t)blockIdx.x * 64, h0 = (int64_t)blockIdx.y * 64;
-    const T *from = blockIdx.z ? a.up : a.gate;
-    const int64_t stride = blockIdx.z ? a.up_stride : a.gate_stride;
+    uint32_t block = blockIdx.x;
+    if (block >= a.blocks) {
+        block -= a.blocks;
+        const uint32_t which = block / a.stage_blocks;
+        product_stage<T>(stage, which, block - which * a.stage_blocks, a.stage_blocks);
+        return;
+    }
+    const bool up = block >= a.blocks / 2;
+    if (up) block -= a.blocks / 2;
+    const int64_t c0 = (int64_t)(block % a.tiles_c) * 64, h0 = (int64_t)(block / a.tiles_c) * 64;
+    const T *from = (const T *)(up ? a.up : a.gate);
+    const int64_t stride = up ? a.up_stride : a.gate_stride;
 #pragma unroll
     for (int j = 0; j < 64 * 64 / kThreads; ++j) {
         const int i = threadIdx.x + j * kThreads;
@@ -264,7 +276,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void gated_turn_ker
         const AttnFrag<TERMS> f = attn_split<TERMS, TERMS == 3>(x);
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
-            *(pccnn_u32x4 *)(a.to + (t * a.channels + c) * 2 * a.padded + blockIdx.z * a.padded + h) =
+            *(pccnn_u32x4 *)(a.to + (t * a.channels + c) * 2 * a.padded + (up ? a.padded : 0) + h) =
                 __builtin_bit_cast(pccnn_u32x4, f.t[t]);
     }
 }
@@ -590,9 +602,10 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     plan.splits = (int)pccnn_ceil_div(steps, per);
     return plan;
 }
-// Operands of the products: the tensors themselves, or their rows laid out anew in the workspace.
+// Operands of the products: the tensors themselves, or their rows laid out anew in the workspace.  `turned` (nullable): where the
+// turned weights go.
 int gated_operands(const char *name, const pccnn_gated *p, const GatedPlan &plan, PccnnArena &arena, ProductRows (&r)[3],
-                   hipStream_t s)
+                   uint16_t *turned, hipStream_t s)
 {
     StageArgs a = {};
     a.width = p->channels;
@@ -611,14 +624,25 @@ int gated_operands(const char *name, const pccnn_gated *p, const GatedPlan &plan
         a.s[count++] = {plan.p[i], plan.stride[i], plan.rows[i], wide_of(plan.p[i], plan.stride[i], p->channels, p->type), to};
         most = std::max(most, plan.rows[i] * plan.units);
     }
-    if (count == 0) return PCCNN_OK;
-    const dim3 grid((unsigned)std::min<int64_t>(pccnn_ceil_div(most, 256), 8192), (unsigned)count);
-    if (p->type == PCCNN_TYPE_F32)
-        product_stage_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (p->type == PCCNN_TYPE_BF16)
-        product_stage_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
-    else
-        product_stage_kernel<int8_t><<<grid, 256, 0, s>>>(a);
+    if (turned != nullptr) {
+        TurnArgs t = {p->gate, p->up, p->gate_stride, p->up_stride, p->hidden, p->channels, plan.padded, turned};
+        t.tiles_c = (uint32_t)pccnn_ceil_div(p->channels, 64);
+        t.blocks = 2 * t.tiles_c * (uint32_t)pccnn_ceil_div(plan.padded, 64);
+        t.stage_blocks = product_stage_blocks(most);
+        const unsigned blocks = t.blocks + t.stage_blocks * count;
+        if (p->type == PCCNN_TYPE_F32)
+            gated_prepare_kernel<float><<<blocks, kThreads, 0, s>>>(t, a);
+        else
+            gated_prepare_kernel<uint16_t><<<blocks, kThreads, 0, s>>>(t, a);
+    } else if (count > 0) {
+        const dim3 grid(product_stage_blocks(most), (unsigned)count);
+        if (p->type == PCCNN_TYPE_F32)
+            product_stage_kernel<float><<<grid, 256, 0, s>>>(a);
+        else if (p->type == PCCNN_TYPE_BF16)
+            product_stage_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
+        else
+            product_stage_kernel<int8_t><<<grid, 256, 0, s>>>(a);
+    }
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
 }
@@ -739,7 +763,7 @@ extern "C" int pccnn_gated_forward(const pccnn_gated *p, void *out, int out_type
     }
     PccnnArena arena(workspace, workspace_bytes);
     ProductRows r[3];
-    rc = gated_operands(name, p, plan, arena, r, s);
+    rc = gated_operands(name, p, plan, arena, r, nullptr, s);
     if (rc != PCCNN_OK) return rc;
     GatedArgs a = {};
     a.x = r[0], a.gate = r[1], a.up = r[2];
@@ -779,7 +803,7 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
     float *part = arena.take<float>(bytes.part / sizeof(float));
     PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
     if (p->n > 0) {
-        rc = gated_operands(name, p, plan, arena, r, s);
+        rc = gated_operands(name, p, plan, arena, r, d_feats != nullptr ? turned : nullptr, s);
         if (rc != PCCNN_OK) return rc;
         GatedArgs a = {};
         a.x = r[0], a.gate = r[1], a.up = r[2];
@@ -791,18 +815,6 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         if (rc != PCCNN_OK) return rc;
     }
     if (d_feats != nullptr && p->n > 0) {
-        auto turn = [&](auto zero) {
-            using T = decltype(zero);
-            const TurnArgs<T> t = {(const T *)p->gate, (const T *)p->up, p->gate_stride, p->up_stride, p->hidden, p->channels,
-                                   plan.padded, turned};
-            const dim3 grid((unsigned)pccnn_ceil_div(p->channels, 64), (unsigned)pccnn_ceil_div(plan.padded, 64), 2);
-            gated_turn_kernel<T><<<grid, kThreads, 0, s>>>(t);
-        };
-        if (f32)
-            turn(0.0f);
-        else
-            turn((uint16_t)0);
-        PCCNN_LAUNCH_CHECK();
         BackArgs a = {};
         a.x = d;
         a.w = {turned, 4 * plan.padded, p->channels, p->channels * 4 * plan.padded};

@@ -10,6 +10,7 @@
 #pragma once
 #include "attention_tiles.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #ifdef __HIPCC__
@@ -539,18 +540,23 @@ struct StageArgs {
     int64_t width;
     int units;
 };
-template <typename T> static __global__ __launch_bounds__(256) void product_stage_kernel(StageArgs a)
+template <typename T> __device__ __forceinline__ void product_stage(const StageArgs &a, uint32_t which, uint32_t block, uint32_t blocks)
 {
     constexpr int UNIT = FewStep<T>::UNIT, TERMS = FewStep<T>::TERMS;
-    const StageSource s = blockIdx.y == 0 ? a.s[0] : blockIdx.y == 1 ? a.s[1] : a.s[2];
+    const StageSource s = which == 0 ? a.s[0] : which == 1 ? a.s[1] : a.s[2];
     const int64_t count = s.rows * a.units;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < count; i += (int64_t)blocks * 256) {
         const int64_t row = i / a.units;
         const FewFrag<TERMS> f = few_load<T>((const T *)s.p + row * s.stride, (i - row * a.units) * UNIT, a.width, s.wide);
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) ((pccnn_u32x4 *)s.to)[t * count + i] = f.t[t];
     }
 }
+template <typename T> static __global__ __launch_bounds__(256) void product_stage_kernel(StageArgs a)
+{
+    product_stage<T>(a, blockIdx.y, blockIdx.x, gridDim.x);
+}
+static inline unsigned product_stage_blocks(int64_t units) { return (unsigned)std::min<int64_t>(pccnn_ceil_div(units, 256), 8192); }
 
 // ---------------------------------------------------------------------------------------------- launches
 //
