@@ -465,7 +465,7 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int j = 0; j < MT; ++j) acc[i][j] = E::mma(fa[kk & 1][i], fb[kk & 1][j], acc[i][j]);
+                for (int j = 0; j < MT; ++j) acc[i][j] = E::mma(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);
                 if (i == 0 && kk < 2) {
                     __builtin_amdgcn_sched_barrier(0x6);
                     if (more) fetch(kk, there);
@@ -481,25 +481,21 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
         walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
     }
     float *part = a.part + split * a.cols_d * a.channels;
+    // columns of x in the lanes: a store is of whole lines (gradients 4000 x 256 -> 704 bf16 53 us, with columns of (dG | dU) there,
+    // 16 bytes of 32 rows to a store, 61)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int64_t d = d0 + 32 * (MT * wd + j) + (lane & 31);
-        if (d >= a.cols_d) continue;
+    for (int i = 0; i < 2; ++i) {
+        const int64_t c = x0 + 64 * wx + 32 * i + (lane & 31);
+        if (c >= a.channels) continue;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < MT; ++j) {
+            const int64_t d = d0 + 32 * (MT * wd + j) + 4 * half;
+            float *to = part + d * a.channels + c;
+            const int rows_d = (int)min(a.cols_d - d, (int64_t)32);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t c = x0 + 64 * wx + 32 * i + 8 * q + 4 * half;
-                if (a.channels % 4 == 0) {
-                    if (c < a.channels)
-                        *(float4 *)(part + d * a.channels + c) =
-                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c + e < a.channels) part[d * a.channels + c + e] = acc[i][j][4 * q + e];
-                }
-            }
+            for (int e = 0; e < 16; ++e)
+                if (8 * (e / 4) + e % 4 < rows_d) to[(8 * (e / 4) + e % 4) * a.channels] = acc[i][j][e];
+        }
     }
 }
 // Sum of the parts, in their order, into the two gradients, VEC values to a thread.
