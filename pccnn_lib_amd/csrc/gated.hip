@@ -284,26 +284,38 @@ template <typename T> __global__ __launch_bounds__(kThreads) void gated_prepare_
 template <typename T> struct ProductOf { typedef ProductBf16 type; };
 template <> struct ProductOf<float> { typedef ProductF32 type; };
 
-// dx: rows of (dG | dU) times the turned weights.
+// dx: rows of (dG | dU) times the turned weights.  Where its tiles leave compute units without work, the sums over hidden channels
+// are cut into parts that are added afterwards in their order (gradients 300 x 512 -> 1408 f32 101 -> 77 us, bf16 54 -> 50).
 struct BackArgs {
     ProductRows x, w;
     int64_t n, cols;
-    int units;
+    int units;                               // of a part
+    int all_units, splits;
     ProductGrid grid;
-    void *out;
+    void *out;                               // [n, cols], f32 [split][n, cols] of parts
 };
-template <typename T, int BM, int BN, int WM, int WN>
+// OUT: result, f32 for parts.
+template <typename T, typename OUT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a)
 {
     typedef ProductNT<typename ProductOf<T>::type, BM, BN, WM, WN, false> Product;
-    typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
+    typedef ProductStage<OUT, BM, BN, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
-    uint32_t row_tile, col_tile;
+    uint32_t row_tile, col_tile, split = 0;
     if (!product_tile(a.grid, row_tile, col_tile)) return;
+    ProductRows x = a.x, w = a.w;
+    int units = a.units;
+    if (a.splits > 1) {                      // (parts are whole pieces of 128 bytes)
+        split = product_split(col_tile, a.splits);
+        const int first = (int)split * a.units;
+        x.p = (const char *)x.p + first / 8 * x.step;
+        w.p = (const char *)w.p + first / 8 * w.step;
+        units = min(units, a.all_units - first);
+    }
     const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
-    p.run(a.x, row0, a.w, a.w, col0, a.units, lds);
-    const Stage stage = {(T *)lds};
+    p.run(x, row0, w, w, col0, units, lds);
+    const Stage stage = {(OUT *)lds};
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m)
 #pragma unroll
@@ -316,7 +328,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a
                 stage.put(p.row_of(m), p.col_of(n) + 8 * q + 4 * p.half, v);
             }
     __syncthreads();
-    stage.out(DenseRow<T>{(T *)a.out, a.cols}, row0, a.n, col0, a.cols);
+    stage.out(DenseRow<OUT>{(OUT *)a.out + split * a.n * a.cols, a.cols}, row0, a.n, col0, a.cols);
 }
 
 // dWg and dWu: columns of (dG | dU) times columns of x, the inner dimension over the rows, which are cut into parts whose sums
@@ -498,16 +510,14 @@ __global__ __launch_bounds__(weights_threads(DP, XP, XT, MT)) void gated_weights
         }
     }
 }
-// Sum of the parts, in their order, into the two gradients, VEC values to a thread.
+// Sum of parts, `step` values apart, in their order, VEC values to a thread; blockIdx.y = 1: of those from `second` on.
 template <typename T, int VEC>
-__global__ __launch_bounds__(kThreads) void gated_weights_sum_kernel(const float *__restrict__ part, int splits, int64_t hidden,
-                                                                    int64_t padded, int64_t channels, T *__restrict__ d_gate,
-                                                                    T *__restrict__ d_up)
+__global__ __launch_bounds__(kThreads) void gated_sum_kernel(const float *__restrict__ part, int splits, int64_t step, int64_t count,
+                                                            int64_t second, T *__restrict__ to, T *__restrict__ to_second)
 {
     const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VEC;
-    if (i >= hidden * channels) return;
-    const float *from = part + (blockIdx.y ? padded * channels : 0) + i;
-    const int64_t step = 2 * padded * channels;
+    if (i >= count) return;
+    const float *from = part + (blockIdx.y ? second : 0) + i;
     float sum[VEC] = {};
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) {
@@ -516,7 +526,7 @@ __global__ __launch_bounds__(kThreads) void gated_weights_sum_kernel(const float
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum[e] += v[e];
     }
-    pccnn_store<VEC>((blockIdx.y ? d_up : d_gate) + i, sum);
+    pccnn_store<VEC>((blockIdx.y ? to_second : to) + i, sum);
 }
 
 // ------------------------------------------------------------------------------------------- host
@@ -550,6 +560,7 @@ struct GatedPlan {
     int64_t padded, pieces;                  // hidden channels in whole units; 64 columns of (dG | dU) each
     int tiles_x, tiles_d, splits;            // weights' gradients
     int64_t per_split;
+    int dx_units, dx_splits;                 // dx: units of a part, parts
 };
 int gated_check(const char *name, const pccnn_gated *p)
 {
@@ -596,6 +607,12 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     const int64_t per = std::max<int64_t>(std::min<int64_t>(4, steps), pccnn_ceil_div(steps, want));
     plan.per_split = per * rows;
     plan.splits = (int)pccnn_ceil_div(steps, per);
+    // dx: parts of eight pieces of 128 bytes at least, no more than fill the chip
+    const int64_t tiles = pccnn_ceil_div(p->n, 64) * pccnn_ceil_div(p->channels, 64), pieces = plan.pieces;
+    int64_t parts = 1;
+    if (p->n > 0 && product_small(p->n, p->channels)) parts = std::max<int64_t>(1, std::min(256 / tiles, pieces / 8));
+    plan.dx_units = (int)(parts > 1 ? pccnn_ceil_div(pieces, parts) * 8 : 2 * plan.padded / 8);
+    plan.dx_splits = (int)pccnn_ceil_div(2 * plan.padded / 8, plan.dx_units);
     return plan;
 }
 // Operands of the products: the tensors themselves, or their rows laid out anew in the workspace.  `turned` (nullable): where the
@@ -662,15 +679,35 @@ template <class E, typename T, bool BACK> int gated_launch(const char *name, Gat
         return gated_launch_tile<E, T, BACK, 128, 128, 2, 2>(name, a, s);
     }
 }
-template <typename T, int BM, int BN, int WM, int WN> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+template <typename T, int BM, int BN, int WM, int WN, typename OUT = T> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
 {
     typedef ProductNT<typename ProductOf<T>::type, BM, BN, WM, WN, false> Product;
-    const size_t lds = std::max(Product::lds_bytes(a.units), (size_t)BM * BN * sizeof(T));
-    return product_launch(name, gated_dx_kernel<T, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
-                          pccnn_ceil_div(a.cols, BN), s);
+    const size_t lds = std::max(Product::lds_bytes(a.units), (size_t)BM * BN * sizeof(OUT));
+    return product_launch(name, gated_dx_kernel<T, OUT, BM, BN, WM, WN>, lds, Product::THREADS, a, pccnn_ceil_div(a.n, BM),
+                          pccnn_ceil_div(a.cols, BN) * a.splits, s);
 }
-template <typename T> int dx_launch(const char *name, BackArgs &a, hipStream_t s)
+// `count` sums (and as many of the parts from `second` on, if there is a second result).
+template <typename T>
+int sum_launch(const float *part, int splits, int64_t step, int64_t count, int64_t second, bool wide, void *to, void *to_second, hipStream_t s)
 {
+    const int vec = wide ? 4 : 1;
+    const dim3 grid((unsigned)pccnn_ceil_div(count, kThreads * vec), to_second != nullptr ? 2 : 1);
+    if (wide)
+        gated_sum_kernel<T, 4><<<grid, kThreads, 0, s>>>(part, splits, step, count, second, (T *)to, (T *)to_second);
+    else
+        gated_sum_kernel<T, 1><<<grid, kThreads, 0, s>>>(part, splits, step, count, second, (T *)to, (T *)to_second);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+template <typename T> int dx_launch(const char *name, BackArgs &a, float *part, hipStream_t s)
+{
+    if (a.splits > 1) {
+        void *out = a.out;
+        a.out = part;
+        const int rc = dx_launch<T, 64, 64, 2, 2, float>(name, a, s);
+        if (rc != PCCNN_OK) return rc;
+        return sum_launch<T>(part, a.splits, a.n * a.cols, a.n * a.cols, 0, a.n * a.cols % 4 == 0, out, nullptr, s);
+    }
     if (product_small(a.n, a.cols)) return dx_launch<T, 64, 64, 2, 2>(name, a, s);
     if constexpr (std::is_same<T, float>::value) {
         return a.cols <= 64 ? dx_launch<T, 128, 64, 4, 2>(name, a, s) : dx_launch<T, 128, 128, 4, 2>(name, a, s);
@@ -717,7 +754,9 @@ BackBytes back_bytes(const pccnn_gated *p, const GatedPlan &plan)
     BackBytes b;
     b.d_pre = (size_t)plan.planes * p->n * plan.pieces * 128;
     b.turned = (size_t)plan.planes * p->channels * 2 * plan.padded * 2;
-    b.part = (size_t)plan.splits * 2 * plan.padded * p->channels * sizeof(float);
+    // (dx's parts are added before the weights' are there)
+    b.part = std::max((size_t)plan.splits * 2 * plan.padded, plan.dx_splits > 1 ? (size_t)plan.dx_splits * p->n : 0) * p->channels *
+             sizeof(float);
     return b;
 }
 
@@ -814,8 +853,9 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
         BackArgs a = {};
         a.x = d;
         a.w = {turned, 4 * plan.padded, p->channels, p->channels * 4 * plan.padded};
-        a.n = p->n, a.cols = p->channels, a.units = (int)(2 * plan.padded / 8), a.out = d_feats;
-        rc = f32 ? dx_launch<float>(name, a, s) : dx_launch<uint16_t>(name, a, s);
+        a.n = p->n, a.cols = p->channels, a.out = d_feats;
+        a.units = plan.dx_units, a.all_units = (int)(2 * plan.padded / 8), a.splits = plan.dx_splits;
+        rc = f32 ? dx_launch<float>(name, a, part, s) : dx_launch<uint16_t>(name, a, part, s);
         if (rc != PCCNN_OK) return rc;
     }
     if (d_gate != nullptr) {
@@ -834,19 +874,10 @@ extern "C" int pccnn_gated_backward(const pccnn_gated *p, const void *in_grads, 
                                           : weights_launch<ProductBf16, 4, 2, 128, 4>(a, s);
             if (rc != PCCNN_OK) return rc;
         }
-        auto sum = [&](auto zero, auto vec) {
-            using T = decltype(zero);
-            constexpr int VEC = decltype(vec)::value;
-            const dim3 grid((unsigned)pccnn_ceil_div(p->hidden * p->channels, kThreads * VEC), 2);
-            gated_weights_sum_kernel<T, VEC><<<grid, kThreads, 0, s>>>(part, splits, p->hidden, plan.padded, p->channels,
-                                                                      (T *)d_gate, (T *)d_up);
-        };
+        const int64_t count = p->hidden * p->channels, second = plan.padded * p->channels;
         const bool wide = p->channels % 4 == 0;
-        if (f32)
-            wide ? sum(0.0f, std::integral_constant<int, 4>()) : sum(0.0f, std::integral_constant<int, 1>());
-        else
-            wide ? sum((uint16_t)0, std::integral_constant<int, 4>()) : sum((uint16_t)0, std::integral_constant<int, 1>());
-        PCCNN_LAUNCH_CHECK();
+        return f32 ? sum_launch<float>(part, splits, 2 * second, count, second, wide, d_gate, d_up, s)
+                   : sum_launch<uint16_t>(part, splits, 2 * second, count, second, wide, d_gate, d_up, s);
     }
     return PCCNN_OK;
 }

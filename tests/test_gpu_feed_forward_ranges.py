@@ -37,6 +37,17 @@ def test_gated_by_every_tile(ops, type, rows, channels, hidden):
     _check_gated(ops, x, gate, up, "gelu" if channels % 3 else "silu", g)
 
 
+# dx in parts of the hidden channels: two of unequal length, five, many, and one whose last 128 bytes are not full
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,channels,hidden", [(300, 72, 600), (300, 512, 1408), (1, 9, 4100), (65, 33, 2051)])
+def test_gated_gradients_of_few_rows_and_many_hidden_channels(ops, type, rows, channels, hidden):
+    dtype, gen = TYPES[type], _gen(rows + hidden)
+    x, g = _normal(gen, rows, channels).to(dtype).to(DEV), _normal(gen, rows, hidden).to(dtype).to(DEV)
+    gate, up = ((_normal(gen, hidden, channels) * (k / channels ** 0.5)).to(dtype).to(DEV) for k in (1.5, 1.0))
+    got = _check_gated(ops, x, gate, up, "silu", g)
+    assert torch.equal(got[1], ops.gated_linear_grads(x, gate, up, g, "silu", grad_mask=ops.GRAD_FEATS)[0])
+
+
 @pytest.mark.parametrize("rows,channels,hidden", TILES)
 def test_8bit_products_by_every_tile(ops, rows, channels, hidden):
     gen = _gen(rows + 1)
@@ -148,7 +159,7 @@ class Guarded:
 
 
 @pytest.mark.parametrize("type", [0, 1])
-@pytest.mark.parametrize("rows,channels,hidden", [(5, 24, 40), (70, 61, 33), (300, 130, 65), (3000, 250, 264)])
+@pytest.mark.parametrize("rows,channels,hidden", [(5, 24, 40), (70, 61, 33), (300, 130, 65), (3000, 250, 264), (70, 24, 2056)])
 def test_nothing_is_written_beside_results_and_workspaces(lib, type, rows, channels, hidden):
     from pccnn_lib_amd import _lib
     gen, dtype, bytes = _gen(rows), (torch.float32, torch.bfloat16)[type], (4, 2)[type]
