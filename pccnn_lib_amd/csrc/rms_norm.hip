@@ -8,6 +8,10 @@
 // it is read once.  Rows longer than that (8192 values, 2048 to 4096 where rows only allow narrow loads) are read again from
 // the caches.  The row's factor is common to t and a, so no code depends on a rounding of it; t, a and the quotient are 64 bits
 // wide, so codes are the nearest integers, whichever way the row is laid over lanes.
+//
+// Bound by memory: bf16 65536 x 256 with a residual, forward 25 us and backward 25 + 4 (134 MB each, 5.4 TB/s where a copy of
+// 1 GiB has 5.2); 800000 x 128 with a residual to 8 bits 146 us (4.9 TB/s, vector ALU 70 % with the 64-bit quotients); rows of
+// 1365 that allow single loads only, 1037 of them, 5.4 us; eight rows 2 us, which is a launch.
 #include "elements.h"
 
 #include <algorithm>
