@@ -258,8 +258,11 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
         }
     }
     // Rows from `row` of `x`, rows from `col` of `one` (and `two`); `units`: 16-byte units of every row, at least one.
-    __device__ __forceinline__ void run(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two,
-                                        int64_t col, int units, uint16_t *lds)
+    // `last(there)` is called among the products of the last tile, when nothing is asked for any more: `there` is a tile's room in LDS
+    // that nobody uses, and what is asked for into it is there on return.  Returns that room.
+    template <typename LAST>
+    __device__ __forceinline__ uint16_t *run(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two,
+                                             int64_t col, int units, uint16_t *lds, LAST last)
     {
         FeedM fm;
         FeedN f1, f2;
@@ -288,9 +291,12 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             }
         // `here` holds what is worked on, `there` is where the next tile goes.  That the two do not overlap is what lets the reads go
         // on while the tile is on its way.
-        auto walk = [&](auto begin, const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more) {
+        auto walk = [&](auto begin, const uint16_t *__restrict__ here, uint16_t *__restrict__ there, bool more, bool end) {
             multiply<decltype(begin)::value>(here, [&](int part) {
-                if (more) fetch(part, there);
+                if (more)
+                    fetch(part, there);
+                else if (end && part == 0)
+                    last(there);
             });
         };
         // the tile that is worked on next; `newer`: tiles behind it that have been asked for
@@ -300,15 +306,21 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
             product_landed();
         };
         landed(min(total, STAGES - 1) - 1);
-        walk(std::true_type(), lds, lds + (STAGES - 1) * STAGE, total >= STAGES);
-        int slot = 0;
+        int slot = 0, free = total == 1 ? 1 : STAGES - 1;
+        walk(std::true_type(), lds, lds + free * STAGE, total >= STAGES, total == 1);
         for (int step = 1; step < total; ++step) {
             landed(min(total - step, STAGES - 1) - 1);
-            const int free = slot;                                    // the tile of the step before
+            free = slot;                                              // the tile of the step before
             slot = slot + 1 < STAGES ? slot + 1 : 0;
-            walk(std::false_type(), lds + slot * STAGE, lds + free * STAGE, step + STAGES <= total);
+            walk(std::false_type(), lds + slot * STAGE, lds + free * STAGE, step + STAGES <= total, step + 1 == total);
         }
         product_landed();                                             // LDS is free for the results
+        return lds + free * STAGE;
+    }
+    __device__ __forceinline__ void run(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two,
+                                        int64_t col, int units, uint16_t *lds)
+    {
+        run(x, row, one, two, col, units, lds, [](uint16_t *) {});
     }
 };
 
@@ -326,34 +338,32 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
     // Columns col .. col + 3 (col a multiple of four) of a row.
     __device__ __forceinline__ void put(int row, int col, const float (&v)[4]) const { pccnn_store<4>(at(row, col), v); }
     __device__ __forceinline__ void get(int row, int col, float (&v)[4]) const { pccnn_load<4>(at(row, col), v); }
-    // Rows row0 .. of `from`, columns col0 .. , zeros past `rows` and `width`.  Needs a barrier behind it; `wide` as attn_load has
-    // it.  Rows that are whole 16-byte units land by attn_landed().
-    __device__ __forceinline__ void bring(const T *from, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width,
-                                          int wide) const
+    // Rows row0 .. of `from`, columns col0 .. , zeros past `rows` and `width`.  Rows that are whole 16-byte units: lands by the next
+    // wait for vector memory.
+    __device__ __forceinline__ void bring(const T *from, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
     {
         constexpr int COUNT = BM * UNITS / THREADS;
         static_assert(COUNT * THREADS == BM * UNITS && THREADS % (8 * UNITS) == 0, "the same unit in every round");
-        const int r0 = (int)threadIdx.x / UNITS;
-        if (wide == 2) {
-            const int unit = place(r0, (int)threadIdx.x % UNITS);
-            const int64_t col = col0 + unit * PER;
-            const __amdgpu_buffer_rsrc_t window = product_window(from + row0 * stride + col0);
-            const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
+        const int r0 = (int)threadIdx.x / UNITS, unit = place(r0, (int)threadIdx.x % UNITS);
+        const int64_t col = col0 + unit * PER;
+        const __amdgpu_buffer_rsrc_t window = product_window(from + row0 * stride + col0);
+        const int wave_unit = __builtin_amdgcn_readfirstlane(threadIdx.x & ~(PCCNN_WAVE - 1));
 #pragma unroll
-            for (int j = 0; j < COUNT; ++j) {
-                const int r = r0 + j * (THREADS / UNITS);
-                attn_bring(window, row0 + r < rows && col < width ? (uint32_t)((r * stride + unit * PER) * sizeof(T)) : kAttnNowhere,
-                           base + PER * (j * THREADS + wave_unit));
-            }
-        } else {
-            for (int j = 0; j < COUNT; ++j) {
-                const int r = r0 + j * (THREADS / UNITS), unit = (int)threadIdx.x % UNITS;
+        for (int j = 0; j < COUNT; ++j) {
+            const int r = r0 + j * (THREADS / UNITS);
+            attn_bring(window, row0 + r < rows && col < width ? (uint32_t)((r * stride + unit * PER) * sizeof(T)) : kAttnNowhere,
+                       base + PER * (j * THREADS + wave_unit));
+        }
+    }
+    // The same of rows that are not; needs a barrier behind it.
+    __device__ __forceinline__ void copy(const T *from, int64_t stride, int64_t row0, int64_t rows, int64_t col0, int64_t width) const
+    {
+        for (int i = threadIdx.x; i < BM * UNITS; i += THREADS) {
+            const int r = i / UNITS, unit = i % UNITS;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int64_t col = col0 + unit * PER + i;
-                    base[r * COLS + PER * place(r, unit) + i] =
-                        row0 + r < rows && col < width ? from[(row0 + r) * stride + col] : (T)0;
-                }
+            for (int e = 0; e < PER; ++e) {
+                const int64_t col = col0 + unit * PER + e;
+                base[r * COLS + PER * place(r, unit) + e] = row0 + r < rows && col < width ? from[(row0 + r) * stride + col] : (T)0;
             }
         }
     }
