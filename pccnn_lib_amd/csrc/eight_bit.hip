@@ -32,7 +32,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void linear_i8_kernel(LinearArg
     typedef ProductStage<T, BM, BN, Product::THREADS> Stage;
     extern __shared__ __align__(16) uint16_t lds[];
     uint32_t row_tile, col_tile;
-    if (!product_tile(a.grid, row_tile, col_tile)) return;
+    if (!product_tile(a.grid, blockIdx.x, row_tile, col_tile)) return;
     const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
     float x_scale[Product::MT];

@@ -49,11 +49,11 @@ static inline uint32_t product_workgroups(const ProductGrid &g)
 }
 
 #ifdef __HIPCC__
-// The tile of the workgroup, in scalar registers; false: it has none.
-__device__ __forceinline__ bool product_tile(const ProductGrid &g, uint32_t &row_tile, uint32_t &col_tile)
+// The tile of workgroup `at`, in scalar registers; false: it has none.
+__device__ __forceinline__ bool product_tile(const ProductGrid &g, uint32_t at, uint32_t &row_tile, uint32_t &col_tile)
 {
-    const uint32_t within = blockIdx.x & ((PCCNN_XCDS << g.run_log2) - 1);
-    const uint32_t block = blockIdx.x - within + ((within % PCCNN_XCDS) << g.run_log2) + within / PCCNN_XCDS;
+    const uint32_t within = at & ((PCCNN_XCDS << g.run_log2) - 1);
+    const uint32_t block = at - within + ((within % PCCNN_XCDS) << g.run_log2) + within / PCCNN_XCDS;
     if (block >= g.blocks) return false;
     row_tile = (uint32_t)(((uint64_t)block * g.magic) >> g.shift);
     col_tile = block - row_tile * g.tiles;

@@ -37,7 +37,7 @@ def test_gated_by_every_tile(ops, type, rows, channels, hidden):
     _check_gated(ops, x, gate, up, "gelu" if channels % 3 else "silu", g)
 
 
-# dx in parts of the hidden channels: two of unequal length, five, many, and one whose last 128 bytes are not full
+# dx in parts of the hidden channels: two of unequal length, several, many, and one whose last 128 bytes are not full
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,channels,hidden", [(300, 72, 600), (300, 512, 1408), (1, 9, 4100), (65, 33, 2051)])
 def test_gated_gradients_of_few_rows_and_many_hidden_channels(ops, type, rows, channels, hidden):
