@@ -5,13 +5,13 @@
 //   8 bits: t = s gamma   a = max |t|   code = nearest integer of 127 t / a (ties to even)   scale = a rstd / 127
 //
 // A row lives in the registers of LANES lanes: 8 to 64 of a wavefront (64 / LANES rows at a time), or the 256 of a workgroup;
-// it is read once.  Rows longer than that (8192 values, 2048 to 4096 where rows only allow narrow loads) are read again from
-// the caches.  The row's factor is common to t and a, so no code depends on a rounding of it; t, a and the quotient are 64 bits
+// it is read once, 16 bytes to a load wherever the row starts.  Rows of more than 8192 values are read again from the
+// caches.  The row's factor is common to t and a, so no code depends on a rounding of it; t, a and the quotient are 64 bits
 // wide, so codes are the nearest integers, whichever way the row is laid over lanes.
 //
 // Bound by memory: bf16 65536 x 256 with a residual, forward 25 us and backward 25 + 4 (134 MB each, 5.4 TB/s where a copy of
-// 1 GiB has 5.2); 800000 x 128 with a residual to 8 bits 146 us (4.9 TB/s, vector ALU 70 % with the 64-bit quotients); rows of
-// 1365 that allow single loads only, 1037 of them, 5.4 us; eight rows 2 us, which is a launch.
+// 1 GiB has 5.2); 800000 x 128 with a residual to 8 bits 146 us (4.9 TB/s, vector ALU 70 % with the 64-bit quotients); 1037
+// rows of 1365 5.5 us; eight rows 2 us, which is a launch.
 #include "elements.h"
 
 #include <algorithm>
@@ -25,7 +25,7 @@ constexpr int kWaves = kThreads / PCCNN_WAVE;
 // (800000 x 128 in 8 bits 153 us, with 2048 171; 65536 x 512 46 and 51).
 constexpr int kMaxBlocks = 1536;
 constexpr int kBackBlocks = 512;
-constexpr int kMostValues = 32, kMostLoads = 16;       // of a lane: values of a row, loads they take
+constexpr int kMostValues = 32;              // of a row, in a lane
 
 // Sum and largest over the LANES lanes that share a row; LANES = 256: over the workgroup, all of whose threads take part.
 template <int LANES> __device__ __forceinline__ float row_sum(float v, float *scratch)
@@ -80,22 +80,70 @@ __device__ __forceinline__ int code_of(double t, double a, double inv_a)
     const double u = 127.0 * t, y = u * inv_a;
     return (int)rint(fma(fma(-a, y, u), inv_a, y));
 }
-template <int COUNT> __device__ __forceinline__ void store_codes(int8_t *p, const int (&q)[COUNT])
+
+// VEC values (16 bytes) of a row; single values instead took up to twice as long (training 20000 x 333 f32 74 us, 44 so; bf16 88 and 43;
+// 8 bits 36 and 20; only bf16 inference of 20000 x 99 7.3 and 8.5).  WHOLE (65536 x 256 bf16 backward 6 us less): every row starts at a multiple of 16 bytes and has whole units; else at any address a value
+// may have, and of the last ones only the `left` that exist, zeros behind them.  Their addresses are kept from the compiler, which
+// would make one access of what both branches have, and two of a whole unit.
+template <typename T> __device__ __forceinline__ __attribute__((address_space(1))) T *row_end(T *p)
 {
-    if constexpr (COUNT == 1) {
-        *p = (int8_t)q[0];
-    } else if constexpr (COUNT == 2) {
-        *(uint16_t *)p = (uint16_t)((q[0] & 255) | (q[1] & 255) << 8);
+    uint64_t at = (uint64_t)p;
+    asm("" : "+v"(at));
+    return (__attribute__((address_space(1))) T *)at;
+}
+template <bool WHOLE, int VEC, typename T> __device__ __forceinline__ void row_load(const T *p, int left, float (&v)[VEC])
+{
+    static_assert(VEC * sizeof(T) == 16, "16 bytes");
+    if constexpr (WHOLE) {
+        pccnn_load<VEC>(p, v);
     } else {
-        uint32_t w[COUNT / 4];
+        T t[VEC];
+        if (left >= VEC) {
+            __builtin_memcpy(t, p, 16);
+        } else {
+            const auto end = row_end(p);
 #pragma unroll
-        for (int i = 0; i < COUNT / 4; ++i)
+            for (int i = 0; i < VEC; ++i) t[i] = i < left ? end[i] : (T)0;
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if constexpr (std::is_same<T, float>::value)
+                v[i] = t[i];
+            else
+                v[i] = pccnn_bf16_value(t[i]);
+    }
+}
+template <bool WHOLE, int VEC, typename T> __device__ __forceinline__ void row_store(T *p, int left, const float (&v)[VEC])
+{
+    if constexpr (WHOLE) {
+        pccnn_store<VEC>(p, v);
+    } else {
+        alignas(16) T t[VEC];
+        pccnn_store<VEC>(t, v);
+        if (left >= VEC) {
+            __builtin_memcpy(p, t, 16);
+        } else {
+            const auto end = row_end(p);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i < left) end[i] = t[i];
+        }
+    }
+}
+template <bool WHOLE, int VEC> __device__ __forceinline__ void row_store_codes(int8_t *p, int left, const int (&q)[VEC])
+{
+    if (WHOLE || left >= VEC) {
+        alignas(8) uint32_t w[VEC / 4];
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i)
             w[i] = (uint32_t)(q[4 * i] & 255) | (uint32_t)(q[4 * i + 1] & 255) << 8 | (uint32_t)(q[4 * i + 2] & 255) << 16 |
                    (uint32_t)q[4 * i + 3] << 24;
-        if constexpr (COUNT == 4)
-            *(uint32_t *)p = w[0];
-        else
-            *(uint2 *)p = make_uint2(w[0], w[1]);
+        __builtin_memcpy(WHOLE ? __builtin_assume_aligned(p, VEC) : p, w, VEC);
+    } else {
+        const auto end = row_end(p);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < left) end[i] = (int8_t)q[i];
     }
 }
 
@@ -113,7 +161,7 @@ struct RmsArgs {
 };
 
 // CODES: the result in 8 bits.
-template <typename T, bool CODES, int VEC, int LANES, int CHUNKS>
+template <typename T, bool CODES, bool WHOLE, int VEC, int LANES, int CHUNKS>
 __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
 {
     constexpr int ROWS = LANES <= PCCNN_WAVE ? kThreads / LANES : 1;                 // of a workgroup at a time
@@ -137,21 +185,21 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
             const int col = (k * LANES + lane) * VEC;
             const bool in = live && col < c;
             if (in) {
-                pccnn_load<VEC>((const T *)a.feats + row * a.stride + col, x[k]);
+                row_load<WHOLE, VEC>((const T *)a.feats + row * a.stride + col, c - col, x[k]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) x[k][i] = 0.0f;
             }
             if (a.residual != nullptr && in) {
                 float r[VEC];
-                pccnn_load<VEC>((const T *)a.residual + row * a.residual_stride + col, r);
+                row_load<WHOLE, VEC>((const T *)a.residual + row * a.residual_stride + col, c - col, r);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) x[k][i] += r[i];
                 if constexpr (!std::is_same<T, float>::value) {                      // the stream as it is stored
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) x[k][i] = pccnn_bf16_value((uint16_t)pccnn_bf16_pair(x[k][i], x[k][i]));
                 }
-                pccnn_store<VEC>((T *)a.total + row * a.c + col, x[k]);
+                row_store<WHOLE, VEC>((T *)a.total + row * a.c + col, c - col, x[k]);
             }
 #pragma unroll
             for (int i = 0; i < VEC; ++i) squares = fmaf(x[k][i], x[k][i], squares);
@@ -192,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
                 int q[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) q[i] = fine ? code_of((double)x[k][i] * (double)g[k][i], most, inv) : 0;
-                store_codes<VEC>(a.codes + row * a.c + col, q);
+                row_store_codes<WHOLE, VEC>(a.codes + row * a.c + col, c - col, q);
             }
         } else {
             if (!live) continue;
@@ -203,7 +251,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
                 float y[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) y[i] = x[k][i] * rstd * g[k][i];
-                pccnn_store<VEC>((T *)a.out + row * a.c + col, y);
+                row_store<WHOLE, VEC>((T *)a.out + row * a.c + col, c - col, y);
             }
         }
     }
@@ -277,7 +325,7 @@ struct RmsBackArgs {
     void *d_feats;                           // nullable
     float *sums;                             // nullable: a row of column sums for each workgroup
 };
-template <typename T, int VEC, int LANES, int CHUNKS>
+template <typename T, bool WHOLE, int VEC, int LANES, int CHUNKS>
 __global__ __launch_bounds__(kThreads) void rms_bwd_kernel(RmsBackArgs a)
 {
     constexpr int ROWS = LANES <= PCCNN_WAVE ? kThreads / LANES : 1, COLUMNS = LANES * CHUNKS * VEC;
@@ -303,8 +351,8 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_kernel(RmsBackArgs a)
         for (int k = 0; k < CHUNKS; ++k) {
             const int col = (k * LANES + lane) * VEC;
             if (live && col < c) {
-                pccnn_load<VEC>((const T *)a.total + row * a.stride + col, x[k]);
-                pccnn_load<VEC>((const T *)a.grads + row * a.grads_stride + col, g[k]);
+                row_load<WHOLE, VEC>((const T *)a.total + row * a.stride + col, c - col, x[k]);
+                row_load<WHOLE, VEC>((const T *)a.grads + row * a.grads_stride + col, c - col, g[k]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) x[k][i] = g[k][i] = 0.0f;
@@ -331,11 +379,11 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_kernel(RmsBackArgs a)
             for (int i = 0; i < VEC; ++i) d[i] = rstd * (g[k][i] - x[k][i] * dot);
             if (a.total_grads != nullptr) {
                 float t[VEC];
-                pccnn_load<VEC>((const T *)a.total_grads + row * a.total_grads_stride + col, t);
+                row_load<WHOLE, VEC>((const T *)a.total_grads + row * a.total_grads_stride + col, c - col, t);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) d[i] += t[i];
             }
-            pccnn_store<VEC>((T *)a.d_feats + row * a.c + col, d);
+            row_store<WHOLE, VEC>((T *)a.d_feats + row * a.c + col, c - col, d);
         }
     }
     if (a.sums == nullptr) return;
@@ -429,19 +477,18 @@ __global__ __launch_bounds__(kReduceThreads) void rms_reduce_kernel(const float 
 
 // ------------------------------------------------------------------------------------------- host
 
-// How a row of c values is laid over lanes: VEC values per load (16 bytes when every row allows it), the fewest lanes of 8 .. 64
-// that hold the row in one load each, then more loads per lane, then the lanes of a workgroup.  chunks 0: not in registers.
+// How a row of c values is laid over lanes: 16 bytes a load, the fewest lanes of 8 .. 64 that hold the row in one load each, then
+// more loads per lane, then the lanes of a workgroup.  chunks 0: not in registers.
 struct RmsShape {
-    int vec, lanes, chunks;
+    int lanes, chunks;
 };
-RmsShape rms_shape(int64_t c, int type, int align)
+RmsShape rms_shape(int64_t c, int type)
 {
-    const int full = 16 / pccnn_type_bytes(type);
-    RmsShape s = {align == 16 && c % full == 0 ? full : (type == PCCNN_TYPE_BF16 && align >= 4 && c % 2 == 0 ? 2 : 1), 8, 1};
-    const int64_t units = pccnn_ceil_div(c, s.vec);
+    const int vec = 16 / pccnn_type_bytes(type), most = kMostValues / vec;
+    const int64_t units = pccnn_ceil_div(c, vec);
+    RmsShape s = {8, 1};
     while (s.lanes < PCCNN_WAVE && s.lanes < units) s.lanes *= 2;
-    const int most = std::min(kMostValues / s.vec, kMostLoads);
-    if (units > (int64_t)PCCNN_WAVE * std::min(most, 4)) s.lanes = kThreads;
+    if (units > (int64_t)PCCNN_WAVE * 4) s.lanes = kThreads;
     while ((int64_t)s.lanes * s.chunks < units && s.chunks <= most) s.chunks *= 2;
     if (s.chunks > most) s.chunks = 0;
     return s;
@@ -450,15 +497,12 @@ struct RmsRows {
     const void *p;
     int64_t stride;
 };
-// The widest alignment (16, 4 or 1 bytes) that every row of a call's tensors has.
-int rms_align(int type, std::initializer_list<RmsRows> tensors)
+// Whether every row of a call's tensors has whole 16-byte units at multiples of 16 bytes.
+bool rms_whole(int64_t c, int type, std::initializer_list<RmsRows> tensors)
 {
-    for (int bytes = 16; bytes > 1; bytes /= 4) {
-        bool all = true;
-        for (const RmsRows &t : tensors) all = all && (t.p == nullptr || pccnn_rows_aligned(t.p, t.stride, type, bytes));
-        if (all) return bytes;
-    }
-    return 1;
+    bool all = c * pccnn_type_bytes(type) % 16 == 0;
+    for (const RmsRows &t : tensors) all = all && (t.p == nullptr || pccnn_rows_aligned(t.p, t.stride, type, 16));
+    return all;
 }
 int64_t rms_blocks(int64_t n, int lanes, int most)
 {
@@ -471,47 +515,41 @@ int64_t rms_wide_parts(int64_t n, int64_t c)
 }
 int64_t rms_most_parts(int64_t n, int64_t c) { return c <= kThreads * kMostValues ? std::min<int64_t>(n, kBackBlocks) : rms_wide_parts(n, c); }
 
-template <typename T, int VEC, typename CALL> void rms_launch_shape(const RmsShape &s, const CALL &call)
+template <typename T, bool WHOLE, int VEC, typename CALL> void rms_launch_shape(const RmsShape &s, const CALL &call)
 {
-    if (s.lanes == 8) return call.template launch<T, VEC, 8, 1>();
-    if (s.lanes == 16) return call.template launch<T, VEC, 16, 1>();
-    if (s.lanes == 32) return call.template launch<T, VEC, 32, 1>();
+    if (s.lanes == 8) return call.template launch<T, WHOLE, VEC, 8, 1>();
+    if (s.lanes == 16) return call.template launch<T, WHOLE, VEC, 16, 1>();
+    if (s.lanes == 32) return call.template launch<T, WHOLE, VEC, 32, 1>();
     if (s.lanes == 64) {
-        if (s.chunks == 1) return call.template launch<T, VEC, 64, 1>();
-        if (s.chunks == 2) return call.template launch<T, VEC, 64, 2>();
-        return call.template launch<T, VEC, 64, 4>();
+        if (s.chunks == 1) return call.template launch<T, WHOLE, VEC, 64, 1>();
+        if (s.chunks == 2) return call.template launch<T, WHOLE, VEC, 64, 2>();
+        return call.template launch<T, WHOLE, VEC, 64, 4>();
     }
-    if (s.chunks <= 2) return call.template launch<T, VEC, 256, 2>();
-    if (s.chunks == 4) return call.template launch<T, VEC, 256, 4>();
-    if constexpr (VEC <= 4) {
-        if (s.chunks == 8) return call.template launch<T, VEC, 256, 8>();
-        if constexpr (VEC <= 2) return call.template launch<T, VEC, 256, 16>();
-    }
+    if (s.chunks <= 2) return call.template launch<T, WHOLE, VEC, 256, 2>();
+    if (s.chunks == 4) return call.template launch<T, WHOLE, VEC, 256, 4>();
+    if constexpr (VEC == 4) return call.template launch<T, WHOLE, VEC, 256, 8>();
 }
-template <typename CALL> void rms_launch(const RmsShape &s, int type, const CALL &call)
+template <typename CALL> void rms_launch(const RmsShape &s, int type, bool whole, const CALL &call)
 {
-    if (type == PCCNN_TYPE_F32) {
-        if (s.vec == 4) return rms_launch_shape<float, 4>(s, call);
-        return rms_launch_shape<float, 1>(s, call);
-    }
-    if (s.vec == 8) return rms_launch_shape<uint16_t, 8>(s, call);
-    if (s.vec == 2) return rms_launch_shape<uint16_t, 2>(s, call);
-    return rms_launch_shape<uint16_t, 1>(s, call);
+    if (type == PCCNN_TYPE_F32)
+        whole ? rms_launch_shape<float, true, 4>(s, call) : rms_launch_shape<float, false, 4>(s, call);
+    else
+        whole ? rms_launch_shape<uint16_t, true, 8>(s, call) : rms_launch_shape<uint16_t, false, 8>(s, call);
 }
 template <bool CODES> struct RmsForward {
     const RmsArgs &a;
     hipStream_t stream;
-    template <typename T, int VEC, int LANES, int CHUNKS> void launch() const
+    template <typename T, bool WHOLE, int VEC, int LANES, int CHUNKS> void launch() const
     {
-        rms_fwd_kernel<T, CODES, VEC, LANES, CHUNKS><<<(unsigned)rms_blocks(a.n, LANES, kMaxBlocks), kThreads, 0, stream>>>(a);
+        rms_fwd_kernel<T, CODES, WHOLE, VEC, LANES, CHUNKS><<<(unsigned)rms_blocks(a.n, LANES, kMaxBlocks), kThreads, 0, stream>>>(a);
     }
 };
 struct RmsBackward {
     const RmsBackArgs &a;
     hipStream_t stream;
-    template <typename T, int VEC, int LANES, int CHUNKS> void launch() const
+    template <typename T, bool WHOLE, int VEC, int LANES, int CHUNKS> void launch() const
     {
-        rms_bwd_kernel<T, VEC, LANES, CHUNKS><<<(unsigned)rms_blocks(a.n, LANES, kBackBlocks), kThreads, 0, stream>>>(a);
+        rms_bwd_kernel<T, WHOLE, VEC, LANES, CHUNKS><<<(unsigned)rms_blocks(a.n, LANES, kBackBlocks), kThreads, 0, stream>>>(a);
     }
 };
 
@@ -526,10 +564,10 @@ int rms_check(const char *name, int type, int weight_type, int64_t n, int64_t c,
 template <bool CODES> int rms_run(const RmsArgs &a, int type, void *stream)
 {
     const hipStream_t s = (hipStream_t)stream;
-    int align = rms_align(type, {{a.feats, a.stride}, {a.residual, a.residual_stride}, {a.out, a.c}, {a.total, a.c}});
-    const RmsShape shape = rms_shape(a.c, type, align);
+    const RmsShape shape = rms_shape(a.c, type);
     if (shape.chunks > 0) {
-        rms_launch(shape, type, RmsForward<CODES>{a, s});
+        rms_launch(shape, type, rms_whole(a.c, type, {{a.feats, a.stride}, {a.residual, a.residual_stride}, {a.out, a.c}, {a.total, a.c}}),
+                   RmsForward<CODES>{a, s});
     } else {
         const unsigned blocks = (unsigned)std::min<int64_t>(a.n, 16384);
         if (type == PCCNN_TYPE_F32)
@@ -616,12 +654,13 @@ extern "C" int pccnn_rms_norm_backward(const void *total, int type, int64_t row_
             a.sums = arena.take<float>((size_t)rms_most_parts(n, channels) * (size_t)channels);
             PCCNN_REQUIRE(arena.ok(), PCCNN_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", name, workspace_bytes);
         }
-        const int align = rms_align(type, {{total, row_stride}, {in_grads, grads_stride}, {total_grads, total_grads_stride},
-                                           {d_feats, channels}});
-        const RmsShape shape = rms_shape(channels, type, align);
+        const RmsShape shape = rms_shape(channels, type);
         if (shape.chunks > 0) {
             parts = (int)rms_blocks(n, shape.lanes, kBackBlocks);
-            rms_launch(shape, type, RmsBackward{a, s});
+            rms_launch(shape, type,
+                       rms_whole(channels, type, {{total, row_stride}, {in_grads, grads_stride}, {total_grads, total_grads_stride},
+                                                  {d_feats, channels}}),
+                       RmsBackward{a, s});
         } else {
             const unsigned blocks = (unsigned)std::min<int64_t>(n, 16384);
             parts = (int)rms_wide_parts(n, channels);
