@@ -609,9 +609,11 @@ int pccnn_attention_backward(const pccnn_attention *problem, const void *out, co
 
 /* s = feats (+ residual, nullable: rounded to the type and written to total_out [n,channels]); out[n,channels] =
  * s gamma / sqrt(avg(s^2) + eps) per row.  gamma [channels] of weight_type.  rstd_out (nullable) f32[n] = 1 / sqrt(..), which the
- * backward call takes.  pccnn_rms_norm_8bit: the same result as codes_out i8[n,channels] and scales_out f32[n]: scale = largest
- * magnitude / 127, codes the nearest integers (ties to even; the row's factor cancels, so they are decided on s gamma, in 64 bits).
- * A row of zeros has scale 0, a row that holds an infinity or NaN has codes 0 and scale NaN.  pccnn_quantize_rows: feats as they are.
+ * backward call takes.  eps >= 0; with 0 a row of zeros is 0 / 0, and a row whose 1 / sqrt(..) leaves f32 (an average below 2^-256)
+ * has rstd infinity, so its norm but no gradients.  pccnn_rms_norm_8bit: the same result as codes_out i8[n,channels] and scales_out
+ * f32[n]: scale = largest magnitude / 127, codes the nearest integers (ties to even; the row's factor cancels, so they are decided on
+ * s gamma, in 64 bits).  A row of zeros has scale 0, a row that holds an infinity or NaN has codes 0 and scale NaN.
+ * pccnn_quantize_rows: feats as they are.
  * Backward, from s (feats, or total_out where there was a residual): d_feats (nullable) [n,channels] = the gradient of s along
  * the norm plus total_grads (nullable, the gradient of total_out): of feats and of residual alike; d_gamma (nullable) [channels]
  * of weight_type, summed in a fixed order; the workspace is only needed for it. */

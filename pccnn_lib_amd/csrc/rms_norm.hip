@@ -62,15 +62,29 @@ template <int LANES> __device__ __forceinline__ double row_most(double v, double
     return __longlong_as_double(bits);
 }
 
-// 1 / sqrt(avg + eps) from the sum of squares; squares that leave f32 (values beyond 10^19) are summed again, scaled, by `again`.
-constexpr float kShrink = 0x1p-80f;
-template <typename AGAIN> __device__ __forceinline__ float rstd_of(float squares, float inv_c, float eps, AGAIN again)
+// 1 / sqrt(avg + eps) from the sum of squares is `lift` times the result.  lift is 1 but for rows whose squares leave f32: values
+// beyond 10^19, or below 10^-19 under an eps below the smallest normal f32 (from which on eps covers what small squares lose: at
+// most 2^-150 each).  Their squares are summed again, scaled, by `again`, and the caller takes its values times lift, so that neither
+// they nor the result leave f32.
+constexpr float kShrink = 0x1p-80f, kGrow = 0x1p100f;
+template <typename AGAIN> __device__ __forceinline__ float rstd_of(float squares, float inv_c, float eps, float &lift, AGAIN again)
 {
-    if (__any(!(squares <= FLT_MAX))) {
-        const float scaled = again();
-        if (!(squares <= FLT_MAX)) return scaled <= FLT_MAX ? kShrink / sqrtf(scaled * inv_c) : scaled != scaled ? scaled : 0.0f;
+    const float most = squares * inv_c + eps;
+    const bool high = !(squares <= FLT_MAX), low = most < FLT_MIN;
+    lift = 1.0f;
+    if (__any(high || low)) {
+        const float scale = high ? kShrink : low ? kGrow : 1.0f;
+        const float scaled = again(scale) * inv_c + eps * scale * scale;
+        if (high) {
+            lift = 0x1p-8f;
+            return kShrink / lift / sqrtf(scaled);
+        }
+        if (low) {
+            lift = kGrow;
+            return 1.0f / sqrtf(scaled);
+        }
     }
-    return 1.0f / sqrtf(squares * inv_c + eps);
+    return 1.0f / sqrtf(most);
 }
 
 // COUNT codes of 127 t / a: a's reciprocal, the quotient and what it leaves corrected once, which is the correctly rounded
@@ -207,15 +221,22 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
         float rstd = 1.0f;
         if (!CODES || a.gamma != nullptr) {
             squares = row_sum<LANES>(squares, (float *)scratch);
-            rstd = rstd_of(squares, inv_c, a.eps, [&]() {
+            float lift;
+            rstd = rstd_of(squares, inv_c, a.eps, lift, [&](float scale) {
                 float again = 0.0f;
 #pragma unroll
                 for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) again = fmaf(x[k][i] * kShrink, x[k][i] * kShrink, again);
+                    for (int i = 0; i < VEC; ++i) again = fmaf(x[k][i] * scale, x[k][i] * scale, again);
                 return row_sum<LANES>(again, (float *)scratch);
             });
-            if (a.rstd != nullptr && live && lane == 0) a.rstd[row] = rstd;
+            if (a.rstd != nullptr && live && lane == 0) a.rstd[row] = rstd * lift;
+            if (lift != 1.0f) {
+#pragma unroll
+                for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) x[k][i] *= lift;
+            }
         }
         if constexpr (CODES) {
             double most = 0.0;
@@ -232,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_kernel(RmsArgs a)
             const bool fine = most > 0.0 && most <= DBL_MAX;
             const double inv = fine ? 1.0 / most : 0.0;
             if (!live) continue;
-            if (lane == 0) a.scales[row] = most != most ? NAN : (float)(most * (double)rstd / 127.0);
+            if (lane == 0) a.scales[row] = fine ? (float)(most * (double)rstd / 127.0) : most == 0.0 ? 0.0f : NAN;
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k) {
                 const int col = (k * LANES + lane) * VEC;
@@ -283,31 +304,31 @@ template <typename T, bool CODES> __global__ __launch_bounds__(kThreads) void rm
             }
         }
         const T *s = a.residual != nullptr ? (const T *)a.total + row * a.c : x;     // (a thread reads what it wrote)
-        float rstd = 1.0f;
+        float rstd = 1.0f, lift = 1.0f;
         if (!CODES || a.gamma != nullptr) {
             squares = row_sum<kThreads>(squares, (float *)scratch);
-            rstd = rstd_of(squares, 1.0f / (float)a.c, a.eps, [&]() {
+            rstd = rstd_of(squares, 1.0f / (float)a.c, a.eps, lift, [&](float scale) {
                 float again = 0.0f;
                 for (int64_t col = threadIdx.x; col < a.c; col += kThreads) {
                     pccnn_load<1>(s + col, v);
-                    again = fmaf(v[0] * kShrink, v[0] * kShrink, again);
+                    again = fmaf(v[0] * scale, v[0] * scale, again);
                 }
                 return row_sum<kThreads>(again, (float *)scratch);
             });
-            if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
+            if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd * lift;
         }
-        if constexpr (CODES) {
-            most = row_most<kThreads>(odd ? NAN : most, scratch + kWaves);
-            if (threadIdx.x == 0) a.scales[row] = most != most ? NAN : (float)(most * (double)rstd / 127.0);
-        }
+        if constexpr (CODES) most = row_most<kThreads>(odd ? NAN : most, scratch + kWaves);
         const bool fine = most > 0.0 && most <= DBL_MAX;
+        if constexpr (CODES) {
+            if (threadIdx.x == 0) a.scales[row] = fine ? (float)(most * (double)lift * (double)rstd / 127.0) : most == 0.0 ? 0.0f : NAN;
+        }
         const double inv = fine ? 1.0 / most : 0.0;
         for (int64_t col = threadIdx.x; col < a.c; col += kThreads) {
             pccnn_load<1>(s + col, v);
             if constexpr (CODES) {
                 a.codes[row * a.c + col] = (int8_t)(fine ? code_of((double)v[0] * (double)weight(col), most, inv) : 0);
             } else {
-                v[0] = v[0] * rstd * weight(col);
+                v[0] = v[0] * lift * rstd * weight(col);
                 pccnn_store<1>((T *)a.out + row * a.c + col, v);
             }
         }

@@ -1,0 +1,74 @@
+"""The feed-forward operators at the ends of their values on the GPU: rows that no eps covers, products that leave f32, activations
+far from zero.  Tolerances as in test_gpu_feed_forward.py; where results are far apart in size they are relative, value by value."""
+import pytest
+import torch
+
+from .test_gpu_feed_forward import DEV, F, TYPES, UNIT, _chain, _codes, _gen, _norm_exact, _normal, _within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from pccnn_lib_amd import pccnn_lib_ops
+    return pccnn_lib_ops
+
+
+# ------------------------------------------------------------------------------------------------------- rows without eps
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60, 1e-42])                     # (the second is zero in f32)
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [24, 700, 9100])
+def test_norm_of_tiny_rows_without_eps(ops, type, channels, eps):
+    # squares of 1e-20 have a few bits in f32, those of 1e-25 none; 1e-39 has no 1 / rms in f32, but a norm
+    dtype, gen = TYPES[type], _gen(channels)
+    x, g = _normal(gen, 7, channels), _normal(gen, 7, channels).to(dtype)
+    for row, size in enumerate((1.0, 1e-18, 1e-20, 1e-25, 1e-35, 1e-39, 1e30)):
+        x[row] *= size
+    x, w = x.to(dtype), (1.0 + 0.3 * _normal(gen, channels)).to(DEV)
+    small = float(torch.tensor(eps, dtype=torch.float32))
+    y, dx, _, xhat, exact = _norm_exact(x, w.cpu(), small, g, None)
+    f = F * (_chain(channels) / 2 + 8)
+    out, rstd = ops.rms_norm(x.to(DEV), w, eps=eps, return_stats=True)
+    # (2^-149: results that are themselves below the smallest normal value)
+    _within(out, y, (UNIT[dtype] + f) * y.abs() + (2.0 ** -134 if type == "bf16" else 2.0 ** -149), "out")
+    inside = (exact.squeeze(1) < 3e38)
+    _within(rstd[inside.to(DEV)], exact.squeeze(1)[inside], f * exact.squeeze(1)[inside] + 2.0 ** -149, "rstd")
+    assert bool(rstd[~inside.to(DEV)].isinf().all())
+    # the gradients of rows whose 1 / rms squared is far inside f32
+    use = slice(0, 3)
+    d_feats, _ = ops.rms_norm_grads(x[use].to(DEV), w, rstd[use], g[use].to(DEV))
+    scaled = (g.double() * w.cpu().double()).abs()
+    size = exact * (scaled + xhat.abs() * (scaled * xhat.abs()).mean(1, keepdim=True))
+    _within(d_feats, dx[use], UNIT[dtype] * dx[use].abs() + 4 * f * size[use], "dx")
+    codes, scales = ops.rms_norm_8bit(x.to(DEV), w, eps=eps)
+    want = y.abs().amax(1) / 127.0
+    assert torch.equal(codes.cpu(), _codes(x, w.cpu()))
+    _within(scales, want, F * (_chain(channels) / 2 + 9) * want, "scales")
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [24, 700, 9100])
+def test_rows_of_zeros_have_scale_zero_without_eps(ops, type, channels):
+    gen = _gen(channels)
+    x = _normal(gen, 5, channels).to(TYPES[type])
+    x[0], x[3] = 0.0, -0.0
+    gamma = torch.ones(channels, device=DEV)
+    codes, scales = ops.rms_norm_8bit(x.to(DEV), gamma, eps=0.0)
+    assert torch.equal(codes.cpu(), _codes(x)) and float(scales[0]) == float(scales[3]) == 0.0 and bool((scales[[1, 2, 4]] > 0).all())
+    codes, scales, total = ops.rms_norm_8bit(x.to(DEV), gamma, (-x).to(DEV), eps=0.0)
+    assert not bool(total.any()) and not bool(codes.any()) and not bool(scales.any())
+    out, rstd = ops.rms_norm(x.to(DEV), gamma, eps=0.0, return_stats=True)
+    assert bool(out[[0, 3]].isnan().all()) and bool(rstd[[0, 3]].isinf().all())           # 0 / 0, 1 / 0
+    assert bool(torch.isfinite(out[[1, 2, 4]]).all())
+
+
+@pytest.mark.parametrize("channels", [24, 700, 9100])
+def test_norm_of_huge_rows_keeps_eps(ops, channels):
+    # squares that leave f32 beside an eps that weighs as much as they do
+    x = _normal(_gen(channels), 3, channels) * 1e19
+    y, _, _, _, exact = _norm_exact(x, torch.ones(channels), 1e38, torch.ones_like(x), None)
+    out, rstd = ops.rms_norm(x.to(DEV), torch.ones(channels, device=DEV), eps=1e38, return_stats=True)
+    f = F * (_chain(channels) / 2 + 8)
+    _within(rstd, exact.squeeze(1), f * exact.squeeze(1), "rstd")
+    _within(out, y, 2 * f * y.abs(), "out")
