@@ -69,13 +69,15 @@ template <bool EXACT, bool SLOPE, int which> __device__ __forceinline__ float ac
         // max(g, 0) - |g| Phi(-|g|); `shrunk` is zero from 64 on, but not times infinity (a NaN is in it)
         return fmaf(-__builtin_amdgcn_fmed3f(fabsf(g), 0.0f, 64.0f) * shrunk, p, __int_as_float(max(__float_as_int(g), 0)));
     }
-    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
-    if constexpr (which == PCCNN_ACT_SIGMOID) {
-        if (SLOPE) slope = s * (1.0f - s);
-        return s;
+    if constexpr (SLOPE) {                   // s and 1 - s from exp(-|g|), so that neither is what the other leaves of one
+        const float e = EXACT ? expf(-fabsf(g)) : __builtin_amdgcn_exp2f(fabsf(g) * -1.4426950408889634f);
+        const float r = EXACT ? 1.0f / (1.0f + e) : __builtin_amdgcn_rcpf(1.0f + e), q = e * r;
+        const float s = g < 0.0f ? q : r, rest = g < 0.0f ? r : q;
+        slope = which == PCCNN_ACT_SIGMOID ? r * q : s * fmaf(g, rest, 1.0f);
+        return which == PCCNN_ACT_SIGMOID ? s : g * s;
     }
-    if (SLOPE) slope = s * fmaf(g, 1.0f - s, 1.0f);
-    return g * s;
+    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+    return which == PCCNN_ACT_SIGMOID ? s : g * s;
 }
 // `call` with the activation as a constant: one branch for a tile, not one for a value.
 template <typename CALL> __device__ __forceinline__ void by_activation(int which, CALL call)

@@ -72,3 +72,33 @@ def test_norm_of_huge_rows_keeps_eps(ops, channels):
     f = F * (_chain(channels) / 2 + 8)
     _within(rstd, exact.squeeze(1), f * exact.squeeze(1), "rstd")
     _within(out, y, 2 * f * y.abs(), "out")
+
+
+# ------------------------------------------------------------------------------------------------ activations far from zero
+
+def _one_hot(gates, dtype, rows):
+    """Features and weights whose projections are `gates` (values of the type) for every row, and one: one channel each."""
+    x = torch.zeros(rows, 8)
+    x[:, 0] = x[:, 1] = 1.0
+    gate, up = torch.zeros(len(gates), 8), torch.zeros(len(gates), 8)
+    gate[:, 0], up[:, 1] = gates, 1.0
+    return [t.to(dtype).to(DEV) for t in (x, gate, up)]
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_slopes_of_open_and_closed_gates(ops, type):
+    # the gradients of the weights' first channel are sums over equal rows of the slope: of gates up to 80 each keeps its value,
+    # on both sides of zero.  exp, reciprocal: 2^-20 as elsewhere and, of exp(-|g|), what a rounding of the exponent's argument brings
+    dtype, rows = TYPES[type], 64
+    gates = torch.tensor([s * v for v in (0.5, 4.0, 8.0, 12.0, 14.0, 17.0, 20.0, 40.0, 80.0) for s in (1.0, -1.0)], dtype=torch.float64)
+    x, gate, up = _one_hot(gates, dtype, rows)
+    g = torch.ones(rows, len(gates), dtype=dtype, device=DEV)
+    error = 2.0 ** -20 + 2 * F * gates.abs()
+    s, rest = torch.sigmoid(gates), torch.sigmoid(-gates)
+    for name, act, slope, size in (("sigmoid", s, s * rest, s * rest),
+                                   ("silu", gates * s, s * (1 + gates * rest), s * (1 + gates.abs() * rest))):
+        d_gate, d_up = (d.cpu().double() for d in ops.gated_linear_grads(x, gate, up, g, name)[1:])
+        # dG and dU are rounded as operands, and the sum as a result
+        u = 2 * UNIT[dtype] + rows * F
+        _within(d_gate[:, 0], rows * slope, rows * (u * slope.abs() + error * size), name + " slope")
+        _within(d_up[:, 1], rows * act, rows * (u + error) * act.abs(), name)
