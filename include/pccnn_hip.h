@@ -641,8 +641,8 @@ int pccnn_linear_8bit(const int8_t *codes, const float *scales, const int8_t *we
 /* h[n,hidden] = act(feats gate^T) * (feats up^T): feats [n,channels], gate and up [hidden,channels], `type` f32 or bf16 for all
  * three (h likewise), or PCCNN_TYPE_I8: codes with their scales [n], [hidden], [hidden] (h f32 or bf16, out_type).  channels and
  * hidden <= 2^20.  Backward (f32, bf16; channels * hidden < 2^31) from the inputs and in_grads [n,hidden]: d_feats (nullable)
- * [n,channels], d_gate and d_up (both or neither) [hidden,channels].  Products of f32 keep f32 accuracy; infinities in f32
- * operands give NaN.  bf16: both projections stay in f32, the gradients of the projections are rounded to bf16 for the products
+ * [n,channels], d_gate and d_up (both or neither) [hidden,channels].  Products of f32 keep f32 accuracy; results
+ * that are not finite are what f32 arithmetic gives.  bf16: both projections stay in f32, the gradients of the projections are rounded to bf16 for the products
  * that they enter, so that the three gradients are off by 0.0023 to 0.0025 of themselves in the 2-norm, where their last rounding
  * alone is 0.0017. */
 typedef struct pccnn_gated {

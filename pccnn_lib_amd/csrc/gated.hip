@@ -136,6 +136,7 @@ __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_kernel(GatedArgs a)
         if constexpr (BACK)
             if (a.grads_wide == 2) Stage{(T *)there}.bring((const T *)a.grads, a.grads_stride, row0, a.n, col0, a.hidden);
     });
+    p.settle(a.x, row0, a.gate, a.up, col0, a.units);
     const Stage stage = {BACK ? (T *)room : (T *)lds}, second = {(T *)(room == lds ? lds + Product::STAGE : lds)};
     if constexpr (BACK) {
         static_assert(Stage::BYTES <= Product::STAGE * sizeof(uint16_t), "results in the tiles' rooms");
@@ -331,6 +332,7 @@ __device__ __forceinline__ void dx_tile(const BackArgs &a, uint32_t block, uint1
     const int64_t row0 = (int64_t)row_tile * BM, col0 = (int64_t)col_tile * BN;
     Product p;
     p.run(x, row0, w, w, col0, units, lds);
+    p.settle(x, row0, w, w, col0, units);
     const Stage stage = {(OUT *)lds};
 #pragma unroll
     for (int m = 0; m < Product::MT; ++m)
@@ -512,6 +514,32 @@ __device__ __forceinline__ void weights_tile(const WeightsArgs &a, uint32_t at, 
         product_landed();
         const int stage = step & 1;
         walk(lds + stage * STAGE, lds + (stage ^ 1) * STAGE, step + 1 < total);
+    }
+    if constexpr (TERMS == 3) {              // (as ProductNT::settle has it: one row of the part for each half of the wavefront)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                if (!product_unsettled(product_most<16>(acc[i][j]))) continue;
+                const int64_t col_x = x0 + 64 * wx + 32 * i + (lane & 31), col_d = d0 + 32 * (MT * wd + j) + (lane & 31);
+                const char *at_x = (const char *)a.x.p + first * a.x.stride + col_x / 64 * a.x.step + col_x % 64 * 2;
+                const char *at_d = (const char *)a.d.p + first * a.d.stride + col_d / 64 * a.d.step + col_d % 64 * 2;
+                auto value = [&](const char *at, const ProductRows &s, int row, bool there) {
+                    float t[3] = {0.0f, 0.0f, 0.0f};
+                    if (there && row < rows)
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) t[e] = pccnn_bf16_value(*(const uint16_t *)(at + row * s.stride + e * s.plane));
+                    return product_value(t[0], t[1], t[2]);
+                };
+                pccnn_f32x16 again = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+                for (int row = 0; row < rows; row += 2)
+                    again = __builtin_amdgcn_mfma_f32_32x32x2f32(value(at_d, a.d, row + half, col_d < a.cols_d),
+                                                                 value(at_x, a.x, row + half, col_x < a.cols_x), again, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(fabsf(acc[i][j][e]) <= FLT_MAX)) acc[i][j][e] = again[e];
+            }
     }
     float *part = a.part + split * a.cols_d * a.channels;
     // columns of x in the lanes: a store is of whole lines (gradients 4000 x 256 -> 704 bf16 53 us, with columns of (dG | dU) there,

@@ -6,11 +6,14 @@
 // Operands are bf16 or 8-bit integers whose rows start at multiples of 16 bytes and have whole 16-byte units (zeros behind the
 // last element); whatever is not like that is laid out so first (product_stage_kernel), f32 as three planes of bf16 terms, whose
 // tiles lie in LDS together: a product of f32 operands is the sum of the six products of planes whose indices add up to at most 2,
-// smallest first.
+// smallest first.  Where a product leaves f32 its terms' products are infinities of both signs, and an infinite operand's second
+// term is infinite, its third NaN: f32 results that are not finite are formed again by the f32 matrix instructions (settle), a block
+// of 32 x 32 at a time, and are then what f32 arithmetic gives.
 #pragma once
 #include "attention_tiles.h"
 
 #include <algorithm>
+#include <float.h>
 #include <type_traits>
 
 #ifdef __HIPCC__
@@ -109,6 +112,34 @@ __device__ __forceinline__ uint32_t product_split(uint32_t &block, uint32_t by)
     block = quotient;
     return rest;
 }
+
+// f32 values from their terms (attn_split): the terms' sum is exact.
+__device__ __forceinline__ float product_value(float t0, float t1, float t2) { return fabsf(t1) <= FLT_MAX ? t2 + t1 + t0 : t1; }
+// Unit `unit` of an operand row of three planes; zeros from `units` on.
+__device__ __forceinline__ void product_values(const ProductRows &s, int64_t row, int unit, int units, float (&v)[8])
+{
+    float t[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[0][i] = t[1][i] = t[2][i] = 0.0f;
+    if (unit < units) {
+        const char *at = (const char *)s.p + row * s.stride + unit / 8 * s.step + unit % 8 * 16;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) pccnn_load<8>((const uint16_t *)(at + i * s.plane), t[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = product_value(t[0][i], t[1][i], t[2][i]);
+}
+// The largest magnitude of a block's results; NaN if there is one.  An instruction for two of them (inference 400000 x 64 -> 176
+// 245 us, unsettled 235, with a comparison for each 253).
+template <int COUNT, typename ACC> __device__ __forceinline__ float product_most(const ACC &acc)
+{
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < COUNT; e += 2)
+        most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, fabsf(acc[e])), fabsf(acc[e + 1]));
+    return most;
+}
+__device__ __forceinline__ bool product_unsettled(float most) { return __any(!(most <= FLT_MAX)); }
 
 // Brings tile after tile of ROWS operand rows, UNITS units of 16 bytes of each, into LDS: the inner dimension lies along the rows.
 // TERMS tiles, one of each plane, one behind the other.
@@ -321,6 +352,41 @@ template <class E, int BM, int BN, int WM, int WN, bool PAIR> struct ProductNT {
                                         int64_t col, int units, uint16_t *lds)
     {
         run(x, row, one, two, col, units, lds, [](uint16_t *) {});
+    }
+    // Behind `run`, with the same arguments: f32 results that are not finite, again.  (Rows and channels that do not exist take the
+    // last one's values.)  32000 x 512 -> 1408: 0.61 to 0.66 ms, with one infinite weight no more, with a column of them 1.53.
+    __device__ __forceinline__ void settle(const ProductRows &x, int64_t row, const ProductRows &one, const ProductRows &two, int64_t col,
+                                           int units)
+    {
+        if constexpr (TERMS == 3) {
+            float most = 0.0f;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) most = __builtin_elementwise_maximum(most, product_most<16>(acc[m][n]));
+            if (!product_unsettled(most)) return;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (!product_unsettled(product_most<16>(acc[m][n]))) continue;
+                    const ProductRows &w = PAIR && n >= NT / 2 ? two : one;
+                    const int64_t x_row = min(row + row_of(m), x.rows - 1);
+                    const int64_t w_row = min(col + col_of(n) % PART + (lane & 31), w.rows - 1);
+                    pccnn_f32x16 again = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+                    for (int unit = 0; unit < units; unit += 2) {     // a unit for each half of the wavefront
+                        float a[8], b[8];
+                        product_values(w, w_row, unit + half, units, a);
+                        product_values(x, x_row, unit + half, units, b);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) again = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], again, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (!(fabsf(acc[m][n][e]) <= FLT_MAX)) acc[m][n][e] = again[e];
+                }
+        }
     }
 };
 
@@ -548,7 +614,48 @@ template <typename T, int OUTS, int RT, int WAVES> struct FewProduct {
 #pragma unroll
                 for (int o = 0; o < OUTS; ++o)
                     acc[r][o] += __builtin_bit_cast(typename S::Acc, lds[v][r * OUTS + o][lane]);
+        if constexpr (std::is_same<T, float>::value) settle(x, rows, w, col, cols, inner, lds[0]);
         return true;
+    }
+    // As ProductNT::settle has it; one block after the other, in `lds`, so that the sums' registers are all that it adds to the way of
+    // the others.
+    __device__ __forceinline__ void settle(const FewRows &x, int64_t rows, const FewRows (&w)[OUTS], int64_t col, int64_t cols,
+                                           int64_t inner, pccnn_u32x4 (*lds)[PCCNN_WAVE])
+    {
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int o = 0; o < OUTS; ++o) most = __builtin_elementwise_maximum(most, product_most<4>(acc[r][o]));
+        if (!product_unsettled(most)) return;
+        const int lane = threadIdx.x % PCCNN_WAVE, line = lane & 15, quarter = lane >> 4;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int o = 0; o < OUTS; ++o) lds[r * OUTS + o][lane] = __builtin_bit_cast(pccnn_u32x4, acc[r][o]);
+#pragma unroll 1
+        for (int block = 0; block < RT * OUTS; ++block) {
+            pccnn_f32x4 c = __builtin_bit_cast(pccnn_f32x4, lds[block][lane]), again = {0, 0, 0, 0};
+            const FewRows &one = w[block % OUTS];
+            const float *xr = (const float *)x.p + min((int64_t)(16 * (block / OUTS) + line), rows - 1) * x.stride;
+            const float *wr = (const float *)one.p + min(col + line, cols - 1) * one.stride;
+#pragma unroll 1
+            for (int k = 0; k < (int)inner; k += 4 * S::UNIT) {
+                AttnChunk<float> a, b;
+                attn_load(a, wr, k + quarter * S::UNIT, (int)inner, one.wide);
+                attn_load(b, xr, k + quarter * S::UNIT, (int)inner, x.wide);
+#pragma unroll
+                for (int i = 0; i < S::UNIT; ++i) again = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], again, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(fabsf(c[e]) <= FLT_MAX)) c[e] = again[e];
+            lds[block][lane] = __builtin_bit_cast(pccnn_u32x4, c);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int o = 0; o < OUTS; ++o) acc[r][o] = __builtin_bit_cast(typename S::Acc, lds[r * OUTS + o][lane]);
     }
 };
 

@@ -1808,8 +1808,8 @@ def _gated_forward(p, out):
 def gated_linear(feats, gate, up, activation="silu"):
     """act(feats gate^T) * (feats up^T), element by element: both projections, the activation and their product in one kernel.
     feats [N, C], gate and up [H, C] (the weights of linear maps; rows may be a view's), all float32 or all bfloat16;
-    ``activation``: "silu", "gelu" (x Phi(x)), "sigmoid" or "relu".  -> [N, H].  float32 keeps float32 accuracy (infinities give
-    NaN); bfloat16 keeps both projections in fp32 and rounds the result once."""
+    ``activation``: "silu", "gelu" (x Phi(x)), "sigmoid" or "relu".  -> [N, H].  float32 keeps float32 accuracy (and gives what
+    float32 arithmetic gives where values leave it); bfloat16 keeps both projections in fp32 and rounds the result once."""
     p = _gated_args("gated_linear", feats, gate, up, activation)
     return _gated_forward(p, torch.empty((p.n, p.hidden), dtype=feats.dtype, device=feats.device))
 

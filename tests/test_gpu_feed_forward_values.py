@@ -102,3 +102,66 @@ def test_slopes_of_open_and_closed_gates(ops, type):
         u = 2 * UNIT[dtype] + rows * F
         _within(d_gate[:, 0], rows * slope, rows * (u * slope.abs() + error * size), name + " slope")
         _within(d_up[:, 1], rows * act, rows * (u + error) * act.abs(), name)
+
+
+# --------------------------------------------------------------------------------------------------- products that leave f32
+
+def _gated_64(x, gate, up, name, g):
+    """The formula in 64 bits, for sigmoid with its gradients.  (The slope is s(g) s(-g): s (1 - s) is zero from g = 37 on in 64
+    bits too, and infinity times zero is not infinity.)"""
+    x, gate, up, g = (t.cpu().double() for t in (x, gate, up, g))
+    G, U = x @ gate.t(), x @ up.t()
+    if name == "relu":
+        return [torch.relu(G) * U]
+    s = torch.sigmoid(G)
+    dG, dU = g * U * s * torch.sigmoid(-G), g * s
+    return [s * U, dG @ gate + dU @ up, dG.t() @ x, dU.t() @ x]
+
+
+# Rows: without tiles (16, 32 and 64 of them); tiles of 64 x 64, with the weights' gradients and in parts; of 128 x 128; dx of 128 x 64
+PAST = [(6, 40, 72), (20, 33, 17), (60, 40, 24), (300, 40, 72), (300, 72, 600), (20500, 40, 72), (10300, 200, 72)]
+
+
+@pytest.mark.parametrize("rows,channels,hidden", PAST)
+def test_gated_f32_of_finite_values_whose_products_leave_f32(ops, rows, channels, hidden):
+    gen = _gen(rows + channels)
+    x, gate, up, g = (_normal(gen, *s) for s in ((rows, channels), (hidden, channels), (hidden, channels), (rows, hidden)))
+    gate, up = gate / channels ** 0.5, up / channels ** 0.5
+    x[1, 3], gate[5, 3], gate[6, 3] = 2.5e25, 1e30, -1e30           # two projections of 2.5e55, whose sigmoid is one and zero
+    x[:, 2], up[7, 2], g[2, 7] = 0.0, 1e30, 1e20                    # a term of 1e50 / 2 in dx
+    x[4, 6], gate[9, 6], g[4, 9] = 1e25, 1.0, 1e20                  # a term of 1e45 in the gradient of up
+    args = [t.to(DEV) for t in (x, gate, up)]
+    got = [ops.gated_linear(*args, "sigmoid"), *ops.gated_linear_grads(*args, g.to(DEV), "sigmoid")]
+    want = _gated_64(x, gate, up, "sigmoid", g)
+    # the terms' magnitudes
+    s, U = torch.sigmoid(x.double() @ gate.double().t()), (x.double() @ up.double().t()).abs()
+    dG, dU = g.double().abs() * U * s * (1 - s), g.double().abs() * s
+    U = x.double().abs() @ up.double().abs().t()
+    sizes = [s * U, dG @ gate.double().abs() + dU @ up.double().abs(), dG.t() @ x.double().abs(), dU.t() @ x.double().abs()]
+    left = 0
+    for a, b, size, what in zip(got, want, sizes, ("h", "dx", "dgate", "dup")):
+        a, inside = a.cpu(), b.abs() <= torch.finfo(torch.float32).max
+        left += int((~inside).sum())
+        assert torch.equal(a[~inside], b[~inside].float()), what
+        _within(a[inside], b[inside], 2.0 ** -18 * size[inside] + 2.0 ** -100, what)
+    assert left == 2                                                # dx[2, 2] and dup[9, 6]
+    h, b = ops.gated_linear(*args, "relu").cpu(), _gated_64(x, gate, up, "relu", g)[0].float()
+    assert float(b[1, 5].abs()) == float("inf")
+    assert torch.equal(h[~torch.isfinite(b)], b[~torch.isfinite(b)]) and torch.equal(torch.isfinite(h), torch.isfinite(b))
+
+
+@pytest.mark.parametrize("rows,channels,hidden", PAST)
+def test_gated_f32_of_infinite_operands_is_what_f32_arithmetic_gives(ops, rows, channels, hidden):
+    gen = _gen(rows + channels + 1)
+    x, gate, up, g = (_normal(gen, *s) for s in ((rows, channels), (hidden, channels), (hidden, channels), (rows, hidden)))
+    inf = float("inf")
+    x[1, 3], x[rows - 1, 0], gate[5, 4], up[hidden - 1, channels - 1] = inf, -inf, -inf, inf
+    gate[8, 3] = 0.0                                                # infinity times zero
+    args = [t.to(DEV) for t in (x, gate, up)]
+    h, d_feats = ops.gated_linear(*args, "sigmoid"), ops.gated_linear_grads(*args, g.to(DEV), "sigmoid")[0]
+    want = [*_gated_64(x, gate, up, "sigmoid", g)[:2], _gated_64(x, gate, up, "relu", g)[0]]
+    for a, b in zip((h, d_feats, ops.gated_linear(*args, "relu")), want):
+        a, b = a.cpu(), b.float()
+        assert bool(b.isnan().any()) and bool(b.isinf().any())
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[b.isinf()], b[b.isinf()])
+        assert torch.equal(torch.isfinite(a), torch.isfinite(b))
