@@ -104,6 +104,69 @@ def test_slopes_of_open_and_closed_gates(ops, type):
         _within(d_up[:, 1], rows * act, rows * (u + error) * act.abs(), name)
 
 
+def _act_64(g, name):
+    """Activation, slope, and the magnitude that the slope's terms have, in 64 bits."""
+    if name == "relu":
+        return g.clamp(min=0), (g > 0).double(), (g > 0).double()
+    if name == "gelu":
+        phi, flow = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5), g * torch.exp(-0.5 * g * g) * (0.5 / torch.pi) ** 0.5
+        return g * phi, phi + flow, phi + flow.abs()
+    s, rest = torch.sigmoid(g), torch.sigmoid(-g)
+    if name == "sigmoid":
+        return s, s * rest, s * rest
+    return g * s, s * (1 + g * rest), s * (1 + g.abs() * rest)
+
+
+def _act_error(g, name, exact):
+    """Of an activation relative to itself, of a slope relative to its terms.  f32 results: half a dozen operations of at most
+    2^-23 each, and the arguments' roundings, which an exponential of -g^2 / 2 multiplies by g^2.  bf16 results: exponentials by
+    their base-2 instruction, whose argument is rounded twice; the normal distribution to 2^-13.5."""
+    if name == "relu":
+        return torch.zeros_like(g)
+    if name == "gelu":
+        return (12 + 2 * g * g) * F + (0.0 if exact else 2.0 ** -13.5)
+    return (12 + (0.0 if exact else 4 * g.abs())) * F
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("name", ["silu", "gelu", "sigmoid", "relu"])
+def test_activations_keep_their_value_far_from_zero(ops, type, rows, name):
+    dtype, exact = TYPES[type], type == "f32"
+    far = 12.5 if name == "gelu" else 80.0                             # (Phi(-13) is below the smallest normal value)
+    gates = torch.cat([torch.linspace(-far, far, 333), torch.linspace(-2.0, 2.0, 67)]).to(dtype)
+    x, gate, up = _one_hot(gates.float(), dtype, rows)
+    g = gates.double()
+    act, slope, size = _act_64(g, name)
+    error, u = _act_error(g, name, exact), UNIT[dtype]
+    h = ops.gated_linear(x, gate, up, name)
+    _within(h, act.expand(rows, -1), (u + error) * act.abs(), name)
+    # one row: the gradients of the weights' channels are dG and dU, rounded as operands and as results
+    upstream = torch.zeros(rows, len(gates), dtype=dtype, device=DEV)
+    upstream[0] = 1.0
+    d_gate, d_up = ops.gated_linear_grads(x, gate, up, upstream, name)[1:]
+    twice = 2 * u * (1 + u)
+    _within(d_gate[:, 0], slope, twice * slope.abs() + (1 + twice) * error * size, name + " slope")
+    _within(d_up[:, 1], act, (twice + (1 + twice) * error) * act.abs(), name)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("name", ["silu", "gelu", "sigmoid", "relu"])
+def test_activations_of_8bit_operands_keep_their_value_far_from_zero(ops, rows, name):
+    codes = torch.arange(-127, 128).to(torch.int8)
+    x, gate, up = (torch.zeros(n, 16, dtype=torch.int8) for n in (rows, len(codes), len(codes)))
+    x[:, 0] = x[:, 1] = up[:, 1] = 1
+    gate[:, 0] = codes
+    scales = [torch.ones(rows), torch.full((len(codes),), 0.0977), torch.ones(len(codes))]           # gates up to 12.4
+    g = codes.double() * scales[1].double()
+    args = [t.to(DEV) for pair in zip((x, gate, up), scales) for t in pair]
+    act, _, _ = _act_64(g, name)
+    for dtype, u in UNIT.items():
+        # (the scale's product rounds the gate once: as an argument's rounding)
+        error = _act_error(g, name, dtype == torch.float32) + (0 if name == "relu" else (2 * g.abs() + 2 * g * g) * F) + F
+        _within(ops.gated_linear_8bit(*args, name, dtype), act.expand(rows, -1), (u + error) * act.abs(), name)
+
+
 # --------------------------------------------------------------------------------------------------- products that leave f32
 
 def _gated_64(x, gate, up, name, g):
