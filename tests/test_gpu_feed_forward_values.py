@@ -228,3 +228,28 @@ def test_gated_f32_of_infinite_operands_is_what_f32_arithmetic_gives(ops, rows, 
         assert bool(b.isnan().any()) and bool(b.isinf().any())
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[b.isinf()], b[b.isinf()])
         assert torch.equal(torch.isfinite(a), torch.isfinite(b))
+
+
+# ------------------------------------------------------------------------------------------------------------ in the 2-norm
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ["silu", "gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("rows,channels,hidden", [(40, 96, 80), (300, 96, 256), (5000, 128, 200)])
+def test_results_and_gradients_in_the_2_norm(ops, type, name, rows, channels, hidden):
+    # A rounding to bf16 is evenly spread over a step of 2^-7 of the value's power of two: 2^-7 / sqrt(12) of the value at most in the
+    # root mean square.  Results have one, gradients another one of the gradients of the projections, independent of it.  f32: as
+    # test_gated_f32_keeps_f32_accuracy has it.
+    dtype, gen = TYPES[type], _gen(rows)
+    x, gate, up, g = (_normal(gen, *s) for s in ((rows, channels), (hidden, channels), (hidden, channels), (rows, hidden)))
+    x, gate, up, g = (t.to(dtype) for t in (x, 1.5 * gate / channels ** 0.5, up / channels ** 0.5, g))
+    args = [t.to(DEV) for t in (x, gate, up)]
+    got = [ops.gated_linear(*args, name), *ops.gated_linear_grads(*args, g.to(DEV), name)]
+    x, gate, up, g = (t.double() for t in (x, gate, up, g))
+    G, U = x @ gate.t(), x @ up.t()
+    act, slope, _ = _act_64(G, name)
+    dG, dU = g * U * slope, g * act
+    want = [act * U, dG @ gate + dU @ up, dG.t() @ x, dU.t() @ x]
+    one = 2.0 ** -20 if type == "f32" else 2.0 ** -7 / 12 ** 0.5
+    for a, b, roundings, what in zip(got, want, (1, 2, 2, 2), ("h", "dx", "dgate", "dup")):
+        off = float((a.cpu().double() - b).norm() / b.norm())
+        assert off <= one * roundings ** 0.5, "%s: off by %g" % (what, off)
