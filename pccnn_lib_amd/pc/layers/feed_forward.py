@@ -4,7 +4,7 @@ import torch
 
 from ... import pccnn_lib_ops as _ops
 from ...op_wrappers import ComputeGatedLinear
-from .norm import RMSNormalization
+from .norm import RMSNormalization, of_one_type
 
 
 class GatedFeedForward(torch.nn.Module):
@@ -15,7 +15,8 @@ class GatedFeedForward(torch.nn.Module):
     with x [N, p_num_features] and ``p_update`` [N, p_num_features] what the layer before adds to them (the addition is part of the
     norm's kernel).  ``p_hidden``: hidden channels, by default 8/3 of the features in whole eights, which makes three maps as large
     as two of four times the features.  ``p_activation``: "silu", "gelu", "sigmoid" or "relu".  Sub-modules ``norm_``
-    (``RMSNormalization``), ``gate_``, ``up_``, ``down_`` (linear maps).  float32 or bfloat16 (``.to(torch.bfloat16)``)."""
+    (``RMSNormalization``), ``gate_``, ``up_``, ``down_`` (linear maps).  float32 or bfloat16 (``.to(torch.bfloat16)``); under
+    autocast to bfloat16 the norm's result and the weights of all three maps are bfloat16, like those of any linear map."""
 
     def __init__(self, p_num_features, p_hidden=None, p_activation="silu", p_eps=1e-6):
         super(GatedFeedForward, self).__init__()
@@ -35,7 +36,10 @@ class GatedFeedForward(torch.nn.Module):
             normed, total = self.norm_(p_feats), p_feats
         else:
             normed, total = self.norm_(p_feats, p_update)
-        return total + self.down_(ComputeGatedLinear.apply(normed, self.gate_.weight, self.up_.weight, self.activation_))
+        gate, up = self.gate_.weight, self.up_.weight
+        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+            normed, gate, up = normed.to(torch.bfloat16), gate.to(torch.bfloat16), up.to(torch.bfloat16)
+        return total + self.down_(ComputeGatedLinear.apply(normed, gate, up, self.activation_))
 
 
 class GatedFeedForward8Bit(torch.nn.Module):
@@ -70,6 +74,7 @@ class GatedFeedForward8Bit(torch.nn.Module):
     def forward(self, p_feats, p_update=None):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (p_feats, p_update)):
             raise RuntimeError("GatedFeedForward8Bit: no gradients (call it under torch.no_grad())")
+        p_feats, p_update = of_one_type(p_feats, p_update)
         got = _ops.rms_norm_8bit(p_feats, self.gamma_, p_update, self.eps_)
         total = p_feats if p_update is None else got[2]
         hidden = _ops.gated_linear_8bit(got[0], got[1], self.gate_codes_, self.gate_scales_, self.up_codes_, self.up_scales_,

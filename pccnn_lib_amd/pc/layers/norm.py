@@ -59,6 +59,15 @@ class LayerNormalization(torch.nn.Module):
         return ComputeLayerNorm.apply(p_feats, self.gamma_.reshape(-1), self.betas_.reshape(-1), self.eps_)
 
 
+def of_one_type(p_feats, p_update):
+    """Under autocast features and their update may be of two types (a linear map gives bfloat16 beside a float32 stream): both
+    in the wider one, as their sum has it."""
+    if p_update is not None and p_update.dtype != p_feats.dtype and torch.is_autocast_enabled("cuda"):
+        wider = torch.promote_types(p_feats.dtype, p_update.dtype)
+        return p_feats.to(wider), p_update.to(wider)
+    return p_feats, p_update
+
+
 class RMSNormalization(torch.nn.Module):
     """Root-mean-square norm of every point's features, parameter ``gamma_`` [1, F] (no counterpart in the reference).  Features
     float32, or bfloat16 under a parameter of either type.  With ``p_residual`` (the update that the features get first) the sum
@@ -70,4 +79,5 @@ class RMSNormalization(torch.nn.Module):
         self.gamma_ = torch.nn.Parameter(torch.ones(1, p_num_features))
 
     def forward(self, p_feats, p_residual=None):
+        p_feats, p_residual = of_one_type(p_feats, p_residual)
         return ComputeRMSNorm.apply(p_feats, self.gamma_.reshape(-1), p_residual, self.eps_)
