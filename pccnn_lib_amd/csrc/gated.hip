@@ -349,7 +349,7 @@ __device__ __forceinline__ void dx_tile(const BackArgs &a, uint32_t block, uint1
                 stage.put(p.row_of(m), p.col_of(n) + 8 * q + 4 * p.half, v);
             }
     __syncthreads();
-    stage.out(DenseRow<OUT>{(OUT *)a.out + split * a.n * a.cols, a.cols}, row0, a.n, col0, a.cols);
+    stage.out(DenseRow<OUT>{(OUT *)a.out + split * a.n * a.cols, a.cols, a.splits > 1}, row0, a.n, col0, a.cols);
 }
 template <typename T, typename OUT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN *PCCNN_WAVE) void gated_dx_kernel(BackArgs a)

@@ -466,15 +466,17 @@ template <typename T, int BM, int COLS, int THREADS> struct ProductStage {
 };
 // Where a unit of a result lies, and whether it goes past the caches.  Results whose rows are whole lines do (800000 x 64 -> 256
 // 159 -> 144 us, 34123 x 512 -> 1408 in 8 bits 86 -> 79); partial lines do not (34123 x 1000 f32 49 -> 54), nor does what the next
-// kernels read (training 8192 x 512 -> 1408 174 -> 182, 400000 x 64 -> 176 341 -> 368; 65536 x 512 -> 1408 832 -> 823).
+// kernels read (training 8192 x 512 -> 1408 174 -> 182, 400000 x 64 -> 176 341 -> 368; 65536 x 512 -> 1408 832 -> 823; dx in parts,
+// 300 x 512 -> 1408 f32 70.0 -> 70.8, bf16 41.9 -> 42.1).
 // Rows of `stride` elements; or pieces of 64 columns of all rows, one behind the other, so that what a tile of rows takes of one
 // piece lies together (65536 x 2816 x 512: 167 us, with rows in one piece 196; 65536 x 512 under 2816 columns, the inner
 // dimension over the rows, 191 and 219).
 template <typename T> struct DenseRow {
     T *p;
     int64_t stride;
+    bool read_next = false;                  // by the call's next kernel
     __device__ __forceinline__ bool whole() const { return stride * (int)sizeof(T) % 16 == 0; }
-    __device__ __forceinline__ bool lines() const { return stride * (int)sizeof(T) % 128 == 0; }
+    __device__ __forceinline__ bool lines() const { return !read_next && stride * (int)sizeof(T) % 128 == 0; }
     __device__ __forceinline__ int64_t row_step() const { return stride; }
     __device__ __forceinline__ T *at(int64_t row, int64_t col) const { return p + row * stride + col; }
 };
