@@ -20,9 +20,18 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMostWidth = 1 << 20;      // channels and hidden channels: a tile's rows stay within 32-bit offsets
-// Rows that need no tiles: up to 32 (512 -> 1408 in bf16, 17, 32, 33 and 64 rows 5.3, 5.5, 6.9 and 7.5 us, in tiles 5.6; in 8 bits
-// 5.2, 5.5, 6.8 and 8.0 against 5.0), up to 64 of f32, whose operands are laid out for tiles (8.5 to 12.4 against 22).
-constexpr int few_rows(int type) { return type == PCCNN_TYPE_F32 ? 64 : 32; }
+// Rows that need no tiles: up to 32 of bf16 (512 -> 1408, 17, 32, 33 and 64 rows 5.3, 5.5, 6.9 and 7.5 us, in tiles 5.6), up to 64 of
+// f32, whose operands are laid out for tiles (8.5 to 12.4 against 22).  8 bits, by how wide all three operands' rows can be loaded
+// (wide_of), us without tiles : in tiles.  Whole 16 bytes: 16 and 17 rows of 512 -> 1408 3.6 : 4.2 and 4.5 : 4.2, from 1024
+// channels on 32 (1024 -> 2736 17 and 32 rows 5.3 : 5.5 and 5.7 : 5.5, 1280 -> 2048 5.7 : 6.0 and 6.1 : 6.1).  Whole 4 bytes, which
+// tiles lay out first: 32 (500 -> 1408 5.7 : 7.2, 1000 -> 2736 8.7 : 11.5).  Single bytes: 16 up to 512 channels (333 -> 900 6.9 : 7.5,
+// 17 rows 8.8 : 7.5; one row of 501 -> 2048 7.7 : 8.6, of 701 -> 700 11.8 : 8.5, of 1365 -> 512 19 : 10).
+constexpr int64_t few_rows(int type, int64_t channels, int wide)
+{
+    if (type != PCCNN_TYPE_I8) return type == PCCNN_TYPE_F32 ? 64 : 32;
+    if (wide == 0) return channels <= 512 ? 16 : 0;
+    return wide == 1 || channels >= 1024 ? 32 : 16;
+}
 
 // ------------------------------------------------------------------------------------------- activations
 
@@ -675,9 +684,11 @@ GatedPlan gated_plan(const pccnn_gated *p, bool backward)
     const int64_t unit = unit_of(p->type);
     plan.units = pccnn_ceil_div(p->channels, unit);
     plan.planes = p->type == PCCNN_TYPE_F32 ? 3 : 1;
-    plan.few = !backward && p->n <= few_rows(p->type);
     plan.p[0] = p->feats, plan.p[1] = p->gate, plan.p[2] = p->up;
     plan.stride[0] = p->feats_stride, plan.stride[1] = p->gate_stride, plan.stride[2] = p->up_stride;
+    int wide = 2;
+    for (int i = 0; i < 3; ++i) wide = std::min(wide, wide_of(plan.p[i], plan.stride[i], p->channels, p->type));
+    plan.few = !backward && p->n <= few_rows(p->type, p->channels, wide);
     plan.rows[0] = p->n, plan.rows[1] = plan.rows[2] = p->hidden;
     for (int i = 0; i < 3; ++i) {
         plan.stage[i] = !plan.few && !as_they_are(plan.p[i], plan.stride[i], p->channels, p->type);

@@ -3,6 +3,7 @@ far from zero.  Tolerances as in test_gpu_feed_forward.py; where results are far
 import pytest
 import torch
 
+from . import test_gpu_feed_forward as base
 from .test_gpu_feed_forward import DEV, F, TYPES, UNIT, _chain, _codes, _gen, _norm_exact, _normal, _within
 
 pytestmark = pytest.mark.gpu
@@ -253,3 +254,11 @@ def test_results_and_gradients_in_the_2_norm(ops, type, name, rows, channels, hi
     for a, b, roundings, what in zip(got, want, (1, 2, 2, 2), ("h", "dx", "dgate", "dup")):
         off = float((a.cpu().double() - b).norm() / b.norm())
         assert off <= one * roundings ** 0.5, "%s: off by %g" % (what, off)
+
+
+# ------------------------------------------------------------------------------------- few rows in 8 bits, by every load width
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33])
+@pytest.mark.parametrize("channels", [48, 512, 1040, 100, 1028, 33, 511, 513, 1031])
+def test_gated_of_few_8bit_rows(ops, rows, channels):
+    base.test_gated_8bit_against_exact_sums(ops, rows, channels, 40 + channels % 3)
