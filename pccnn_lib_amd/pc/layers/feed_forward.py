@@ -12,8 +12,8 @@ class GatedFeedForward(torch.nn.Module):
 
         s + down(act(gate(norm(s))) * up(norm(s))),   s = x, or x + update
 
-    with x [N, p_num_features] and ``p_update`` [N, p_num_features] what the layer before adds to them (the addition is part of the
-    norm's kernel).  ``p_hidden``: hidden channels, by default 8/3 of the features in whole eights, which makes three maps as large
+    with x [N, p_num_features] and ``p_update`` [N, p_num_features] what the layer before adds to them, where it has not yet (the
+    addition is part of the norm's kernel; ``CrossAttention``'s result is its features with the update added: x as it is).  ``p_hidden``: hidden channels, by default 8/3 of the features in whole eights, which makes three maps as large
     as two of four times the features.  ``p_activation``: "silu", "gelu", "sigmoid" or "relu".  Sub-modules ``norm_``
     (``RMSNormalization``), ``gate_``, ``up_``, ``down_`` (linear maps).  float32 or bfloat16 (``.to(torch.bfloat16)``); under
     autocast to bfloat16 the norm's result and the weights of all three maps are bfloat16, like those of any linear map."""
