@@ -262,3 +262,41 @@ def test_results_and_gradients_in_the_2_norm(ops, type, name, rows, channels, hi
 @pytest.mark.parametrize("channels", [48, 512, 1040, 100, 1028, 33, 511, 513, 1031])
 def test_gated_of_few_8bit_rows(ops, rows, channels):
     base.test_gated_8bit_against_exact_sums(ops, rows, channels, 40 + channels % 3)
+
+
+# -------------------------------------------------------------------------------------- what a workspace held before a call
+
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("rows,channels,hidden", [(5, 24, 40), (70, 61, 33), (300, 130, 65), (70, 24, 2056), (3000, 250, 264), (0, 24, 40)])
+def test_what_a_workspace_held_has_no_effect(ops, type, rows, channels, hidden):
+    import ctypes
+    from pccnn_lib_amd import _lib
+    lib, gen, dtype = _lib.load(), _gen(rows), (torch.float32, torch.bfloat16)[type]
+    x, gate, up, g = (_normal(gen, *s).to(dtype).to(DEV) for s in ((rows, channels), (hidden, channels), (hidden, channels), (rows, hidden)))
+    want = [ops.gated_linear(x, gate, up), *ops.gated_linear_grads(x, gate, up, g)]
+    p = _lib.Gated()
+    p.feats, p.gate, p.up = x.data_ptr(), gate.data_ptr(), up.data_ptr()
+    p.feats_stride = p.gate_stride = p.up_stride = channels
+    p.n, p.channels, p.hidden, p.type, p.activation = rows, channels, hidden, type, 0
+    stream = torch.cuda.current_stream().cuda_stream
+    gamma = torch.ones(channels, device=DEV)
+    out, rstd = ops.rms_norm(x, gamma, return_stats=True)
+    want += [ops.rms_norm_grads(x, gamma, rstd, x)[1]]
+    codes, scales = ops.quantize_rows(x)
+    weights, weight_scales = ops.quantize_rows(gate)
+    want += [ops.linear_8bit(codes, scales, weights, weight_scales, dtype=dtype)]
+    for fill in (0xFF, 0x7F):                                              # NaN, and the largest codes and values
+        got = [torch.empty_like(t) for t in want]
+        space = lambda size: torch.full((size,), fill, dtype=torch.uint8, device=DEV)  # noqa: E731
+        work = space(lib.pccnn_gated_workspace_bytes(ctypes.byref(p), 0))
+        assert lib.pccnn_gated_forward(ctypes.byref(p), got[0].data_ptr(), type, work.data_ptr(), work.numel(), stream) == 0
+        back = space(lib.pccnn_gated_workspace_bytes(ctypes.byref(p), 1))
+        assert lib.pccnn_gated_backward(ctypes.byref(p), g.data_ptr(), hidden, got[1].data_ptr(), got[2].data_ptr(), got[3].data_ptr(),
+                                        back.data_ptr(), back.numel(), stream) == 0
+        sums = space(lib.pccnn_rms_norm_workspace_bytes(rows, channels))
+        assert lib.pccnn_rms_norm_backward(x.data_ptr(), type, channels, gamma.data_ptr(), 0, rstd.data_ptr(), x.data_ptr(), channels,
+                                           None, 0, rows, channels, None, got[4].data_ptr(), sums.data_ptr(), sums.numel(), stream) == 0
+        rows8 = space(lib.pccnn_linear_8bit_workspace_bytes(codes.data_ptr(), weights.data_ptr(), rows, channels, hidden))
+        assert lib.pccnn_linear_8bit(codes.data_ptr(), scales.data_ptr(), weights.data_ptr(), weight_scales.data_ptr(), None, rows,
+                                     channels, hidden, got[5].data_ptr(), type, rows8.data_ptr(), rows8.numel(), stream) == 0
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
