@@ -632,7 +632,8 @@ int pccnn_quantize_rows(const void *feats, int type, int64_t row_stride, int64_t
                         float *scales_out, void *stream);
 
 /* out[n,outer] (f32 or bf16) = (sum_k codes[n,k] weights[outer,k]) scales[n] weight_scales[outer] + bias[outer] (nullable);
- * codes and weights dense rows of `inner` <= PCCNN_MAX_INNER_8BIT.  The sums are exact. */
+ * codes and weights dense rows of `inner` <= PCCNN_MAX_INNER_8BIT.  The sums are exact; the two scales are multiplied first, in f32,
+ * here and in the gated map: products of scales outside 2^-126 .. 2^127 lose bits or are infinite. */
 size_t pccnn_linear_8bit_workspace_bytes(const int8_t *codes, const int8_t *weights, int64_t n, int64_t inner, int64_t outer);
 int pccnn_linear_8bit(const int8_t *codes, const float *scales, const int8_t *weights, const float *weight_scales,
                       const float *bias, int64_t n, int64_t inner, int64_t outer, void *out, int out_type, void *workspace,
@@ -641,8 +642,9 @@ int pccnn_linear_8bit(const int8_t *codes, const float *scales, const int8_t *we
 /* h[n,hidden] = act(feats gate^T) * (feats up^T): feats [n,channels], gate and up [hidden,channels], `type` f32 or bf16 for all
  * three (h likewise), or PCCNN_TYPE_I8: codes with their scales [n], [hidden], [hidden] (h f32 or bf16, out_type).  channels and
  * hidden <= 2^20.  Backward (f32, bf16; channels * hidden < 2^31) from the inputs and in_grads [n,hidden]: d_feats (nullable)
- * [n,channels], d_gate and d_up (both or neither) [hidden,channels].  Products of f32 keep f32 accuracy; results
- * that are not finite are what f32 arithmetic gives.  bf16: both projections stay in f32, the gradients of the projections are rounded to bf16 for the products
+ * [n,channels], d_gate and d_up (both or neither) [hidden,channels].  Products of f32 keep f32 accuracy
+ * (operands below 2^-110 an absolute one: they are multiples of 2^-133 there); results that are not finite are what f32 arithmetic
+ * gives.  bf16: both projections stay in f32, the gradients of the projections are rounded to bf16 for the products
  * that they enter, so that the three gradients are off by 0.0023 to 0.0025 of themselves in the 2-norm, where their last rounding
  * alone is 0.0017. */
 typedef struct pccnn_gated {

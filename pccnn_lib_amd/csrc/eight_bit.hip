@@ -3,7 +3,7 @@
 // The sums are whole numbers of 32 bits, exact in any order; what is rounded is their conversion to f32 (from 2^24 on), the
 // product with the scales and the result.
 //
-// 65536 x 1408 x 512 to bf16: 57 us, 1.66 POP/s, matrix pipe 44 % of the cycles (tiles of 256 x 256, eleven steps each, and what
+// 65536 x 1408 x 512 to bf16: 57 us, 1.66 POP/s, matrix pipe 45 % of the cycles (tiles of 256 x 256, eleven steps each, and what
 // fills and empties them); 34123 x 200 x 1000 to f32: rows laid out 7 us, product 38, bound by its 136 MB of results (3.6 TB/s);
 // one row of 1408 x 512: 4 us, a launch and two trips to memory.
 #include "product_tiles.h"

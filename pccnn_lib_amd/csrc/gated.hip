@@ -7,10 +7,16 @@
 // would be 740 MB of f32 for 65536 x 512 -> 1408, written and read again (143 us each); the products are 119 us at the rate of a large
 // one.
 //
-// bf16 65536 x 512 -> 1408 (189 GFLOP a product): forward 205 to 238 us, dG and dU 278 to 313, dx 165 to 188, weights 188 + 11, by
-// machine: 0.8 to 1.15 PFLOP/s at 1.8 to 2.0 GHz, which is power, matrix pipe 46, 33, 58 and 62 % of the cycles; between the products
-// of a tile of 256 x 256 and the next nothing multiplies, since one workgroup fills a compute unit's LDS.  800000 x 64 -> 256, gelu:
-// 149 us, vector ALU 100 %: 205 million results.
+// bf16 65536 x 512 -> 1408 (189 GFLOP a product), by machine: forward 205 to 245 us, dG and dU 267 to 321, dx 165 to 193, weights 178 to
+// 208 and 11 for their sum: 0.59 to 1.15 PFLOP/s.  The matrix pipe works 47, 35, 62 and 63 % of the busy cycles, at 1.7 GHz: while a
+// tile of 256 x 256 is filled, activated and stored nothing multiplies, since one workgroup fills a compute unit's LDS.  f32
+// 32000 x 512 -> 1408, six products of terms (554 GFLOP): forward 559 to 583 us, matrix pipe 51 % at 1.9 GHz, for the same reason
+// (tiles of 128 x 128 in three planes, one workgroup to a compute unit).  800000 x 64 -> 256, gelu: 150 to 171 us, vector ALU 100 %:
+// 205 million results.
+//
+// bf16: dG and dU are rounded to bf16, since they are operands of the next products; the three gradients are then off by 0.0023 to
+// 0.0025 in the 2-norm, the plain formula's by 0.0017, which is their last rounding.  Two terms of each instead would double both
+// products and the 370 MB that hold them.
 #include "product_tiles.h"
 
 #include <algorithm>

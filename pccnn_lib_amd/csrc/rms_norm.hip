@@ -11,7 +11,9 @@
 //
 // Bound by memory: bf16 65536 x 256 with a residual, forward 25 us and backward 25 + 4 (134 MB each, 5.4 TB/s where a copy of
 // 1 GiB has 5.2); 800000 x 128 with a residual to 8 bits 146 us (4.9 TB/s, vector ALU 70 % with the 64-bit quotients); 1037
-// rows of 1365 5.5 us; eight rows 2 us, which is a launch.
+// rows of 1365 5.5 us; eight rows 2 us, which is a launch.  bf16 rows that are not whole units take longer than their bytes:
+// 20000 x 333 with a residual 17 us forward and 25 backward for 10 each (two wavefronts to a SIMD in the backward kernel, each with one
+// row on its way, whose end comes in single loads; f32, twice the bytes, 19 and 22), 1000 x 8191 26 and 33 + 8 for 13 each.
 #include "elements.h"
 
 #include <algorithm>
@@ -95,10 +97,11 @@ __device__ __forceinline__ int code_of(double t, double a, double inv_a)
     return (int)rint(fma(fma(-a, y, u), inv_a, y));
 }
 
-// VEC values (16 bytes) of a row; single values instead took up to twice as long (training 20000 x 333 f32 74 us, 44 so; bf16 88 and 43;
-// 8 bits 36 and 20; only bf16 inference of 20000 x 99 7.3 and 8.5).  WHOLE (65536 x 256 bf16 backward 6 us less): every row starts at a multiple of 16 bytes and has whole units; else at any address a value
-// may have, and of the last ones only the `left` that exist, zeros behind them.  Their addresses are kept from the compiler, which
-// would make one access of what both branches have, and two of a whole unit.
+// VEC values (16 bytes) of a row; single values instead took up to twice as long (training 20000 x 333 f32 74 us, 44 so; bf16 88 and
+// 43; 8 bits 36 and 20; only bf16 inference of 20000 x 99 7.3 and 8.5).  WHOLE (65536 x 256 bf16 backward 6 us less): every row starts
+// at a multiple of 16 bytes and has whole units; else at any address a value may have, and of the last ones only the `left` that
+// exist, zeros behind them.  Their addresses are kept from the compiler, which would make one access of what both branches have, and
+// two of a whole unit.
 template <typename T> __device__ __forceinline__ __attribute__((address_space(1))) T *row_end(T *p)
 {
     uint64_t at = (uint64_t)p;
@@ -534,7 +537,10 @@ int64_t rms_wide_parts(int64_t n, int64_t c)
 {
     return std::min(n, std::max<int64_t>(1, 1024 / pccnn_ceil_div(c, kThreads)));
 }
-int64_t rms_most_parts(int64_t n, int64_t c) { return c <= kThreads * kMostValues ? std::min<int64_t>(n, kBackBlocks) : rms_wide_parts(n, c); }
+int64_t rms_most_parts(int64_t n, int64_t c)
+{
+    return c <= kThreads * kMostValues ? std::min<int64_t>(n, kBackBlocks) : rms_wide_parts(n, c);
+}
 
 template <typename T, bool WHOLE, int VEC, typename CALL> void rms_launch_shape(const RmsShape &s, const CALL &call)
 {

@@ -71,7 +71,7 @@ def of_one_type(p_feats, p_update):
 class RMSNormalization(torch.nn.Module):
     """Root-mean-square norm of every point's features, parameter ``gamma_`` [1, F] (no counterpart in the reference).  Features
     float32, or bfloat16 under a parameter of either type.  With ``p_residual`` (the update that the features get first) the sum
-    comes back too: (norm of the sum, the sum)."""
+    comes back too: (norm of the sum, the sum); under autocast the two may be of two types."""
 
     def __init__(self, p_num_features, p_eps=1e-6):
         super(RMSNormalization, self).__init__()

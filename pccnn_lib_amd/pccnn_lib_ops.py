@@ -1761,7 +1761,7 @@ def _codes_args(name, label, codes, scales, device=None):
 def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None, dtype=None):
     """Linear map of 8-bit rows: (codes weight_codes^T) * scales[:, None] * weight_scales (+ bias).  codes int8 [N, C], scales
     f32 [N], weight_codes int8 [O, C], weight_scales f32 [O], bias f32 [O] -> [N, O], bfloat16 or what ``dtype`` says (float32).
-    The sums are exact (C <= 131071)."""
+    The sums are exact (C <= 131071); the two scales are multiplied first, in float32."""
     name = "linear_8bit"
     _codes_args(name, "codes", codes, scales)
     _codes_args(name, "weight_codes", weight_codes, weight_scales, codes.device)
